@@ -74,6 +74,14 @@ def _spread(rng, lo, hi):
 
 def draw(rng):
     op = rng.choice(["route", "rows", "q4"])
+    most = [max(work(c)[what] for c in listed() if c["op"] == op) for what in ("bytes", "flops")]
+    while True:
+        c = _drawn(rng, op)
+        if work(c)["bytes"] <= most[0] and work(c)["flops"] <= most[1]:
+            return c
+
+
+def _drawn(rng, op):
     if op == "route":
         experts = _spread(rng, 8, 256)
         c = _route("", tokens=_spread(rng, 1, 131072), experts=experts, top_k=rng.randint(1, 8),
@@ -82,8 +90,7 @@ def draw(rng):
     elif op == "rows":
         top_k = rng.randint(1, 8)
         width = _spread(rng, 64, 8192)
-        most = min(65536, 8192 * 2 * 4096 // (top_k * width))
-        c = _rows("", tokens=_spread(rng, 1, most), top_k=top_k, width=width, dtype=rng.choice(list(DTYPES)),
+        c = _rows("", tokens=_spread(rng, 1, 65536), top_k=top_k, width=width, dtype=rng.choice(list(DTYPES)),
                   unrouted=rng.choice([0.0, 0.0, 0.2]), train=rng.random() < 0.6)
     else:
         most = 8 * 14336 * 4096
