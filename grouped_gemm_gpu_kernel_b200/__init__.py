@@ -20,6 +20,7 @@ from dataclasses import dataclass, field
 from typing import List, Optional, Sequence
 
 from . import capi
+from .moe import MoeRouter, Q4Plan, moe_combine, moe_combine_backward, moe_dispatch
 
 __all__ = [
     "SortMode", "ProblemDesc", "KernelConfig", "PreparedProblemSet", "OccupancyInfo", "GroupedGemmExecutor",
@@ -28,6 +29,7 @@ __all__ = [
     "NATIVE_CONFIGS", "REFERENCE_CONFIGS", "PAIR_CONFIGS", "selftest_wait_timeout", "capi", "MoePlan",
     "selftest_wait_timeout_word", "baseline_status", "noalloc_status", "DevicePlan",
     "InputType", "OutputType", "Activation", "Layout", "TileClasses",
+    "MoeRouter", "moe_dispatch", "moe_combine", "moe_combine_backward", "Q4Plan",
 ]
 
 

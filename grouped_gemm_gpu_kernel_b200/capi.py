@@ -26,10 +26,16 @@ EXPORTED_SYMBOLS = (
     "gg_ipc_export", "gg_ipc_open", "gg_ipc_close",
     "gg_device_plan_create", "gg_device_plan_run", "gg_device_plan_status", "gg_device_plan_prepared",
     "gg_device_plan_destroy",
+    "gg_router_create", "gg_router_run", "gg_router_backward", "gg_router_destroy",
+    "gg_moe_dispatch", "gg_moe_combine", "gg_moe_combine_backward",
+    "gg_q4_plan_create", "gg_q4_plan_run", "gg_q4_plan_status", "gg_q4_plan_destroy",
 )
 GG_STATUS_BAD_ROWS = 0x100
 GG_STATUS_BAD_PROBLEMS = 0x200
 GG_DEVICE_PLAN_MAX_PROBLEMS = 4096
+GG_ROUTER_MAX_EXPERTS = 1024
+GG_ROUTER_MAX_TOP_K = 32
+GG_Q4_MAX_EXPERTS = 1024
 GG_INPUT_F16 = 0
 GG_INPUT_BF16 = 1
 GG_INPUT_E4M3 = 2
@@ -109,6 +115,28 @@ class GGIpcHandle(ctypes.Structure):
     _fields_ = [("handle", ctypes.c_ubyte * 64), ("offset", ctypes.c_ulonglong), ("bytes", ctypes.c_ulonglong)]
 
 
+class GGRouterConfig(ctypes.Structure):
+    _fields_ = [("experts", ctypes.c_int), ("top_k", ctypes.c_int), ("capacity_tokens", ctypes.c_int),
+                ("logit_type", ctypes.c_int), ("normalize", ctypes.c_int)]
+
+
+class GGRoute(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "logits", "token_mask", "indices", "weights", "positions", "rows", "losses", "row_tokens", "lse",
+        "prob_mean")] + [("tokens", ctypes.c_int), ("ld", ctypes.c_int)]
+
+
+class GGRouteGradient(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "logits", "indices", "weights", "rows", "losses", "lse", "grad_weights", "grad_losses",
+        "grad_logits")] + [("tokens", ctypes.c_int), ("ld", ctypes.c_int), ("ld_grad", ctypes.c_int)]
+
+
+class GGQ4Problem(ctypes.Structure):
+    _fields_ = [(name, ctypes.POINTER(ctypes.c_void_p)) for name in ("q", "scales", "zeros", "bias")] + [
+        (name, ctypes.c_int) for name in ("experts", "n", "k", "group", "ldq", "input_type", "output_type", "activation")]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -163,6 +191,20 @@ def load() -> ctypes.CDLL:
         "gg_device_plan_status": ([vp, i32p, i32p], ctypes.c_int),
         "gg_device_plan_prepared": ([vp, i32p, i32p, ctypes.c_int], ctypes.c_int),
         "gg_device_plan_destroy": ([vp], None),
+        "gg_router_create": ([P(GGRouterConfig), P(vp)], ctypes.c_int),
+        "gg_router_run": ([vp, P(GGRoute), vp], ctypes.c_int),
+        "gg_router_backward": ([vp, P(GGRouteGradient), vp], ctypes.c_int),
+        "gg_router_destroy": ([vp], None),
+        "gg_moe_dispatch": ([vp, ctypes.c_int, vp] + [ctypes.c_int] * 4 + [vp, ctypes.c_int, ctypes.c_int, vp],
+                            ctypes.c_int),
+        "gg_moe_combine": ([vp] + [ctypes.c_int] * 3 + [vp, vp] + [ctypes.c_int] * 3 + [vp, ctypes.c_int, ctypes.c_int,
+                                                                                       vp], ctypes.c_int),
+        "gg_moe_combine_backward": ([vp, ctypes.c_int, ctypes.c_int, vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, vp, vp,
+                                     ctypes.c_int, ctypes.c_int, ctypes.c_int, vp, ctypes.c_int, vp, vp], ctypes.c_int),
+        "gg_q4_plan_create": ([P(GGQ4Problem), vp, P(vp)], ctypes.c_int),
+        "gg_q4_plan_run": ([vp, vp, ctypes.c_int, ctypes.c_int, vp, vp, vp, ctypes.c_int, ctypes.c_int, vp], ctypes.c_int),
+        "gg_q4_plan_status": ([vp, i32p], ctypes.c_int),
+        "gg_q4_plan_destroy": ([vp], None),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

@@ -1,0 +1,631 @@
+// gg_router.cu -- the mixture-of-experts router: top-k experts of every token, their weights, the
+// row counts, the places of the rows in packed order, the balance and z losses, and the gradient of
+// all of them with respect to the logits.
+//
+// Forward. A group of G lanes holds one token's logits, V consecutive experts a lane (G * V >=
+// experts), so a warp works on 32 / G tokens at once. Choosing is on the logits themselves, through
+// an integer key that orders like the value, so equal logits tie exactly and rounding of exp() never
+// decides. Every warp owns a contiguous range of tokens and counts its choices per expert as it
+// goes; a slot's rank among its warp's earlier slots of the same expert is its place up to an offset
+// that only depends on (expert, warp). Those offsets need the counts of all warps, so a second
+// kernel adds them (for few tokens one block does both in one launch). No atomics: ranks and sums
+// have a fixed order, and the same inputs give the same bits.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <new>
+
+#include "gg_epilogue_ops.cuh"
+#include "grouped_gemm_b200.h"
+
+namespace gg {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kMaxBlocks = 148;  // one forward block per SM at most
+
+struct RouterShape {
+  int experts, top_k, normalize;
+};
+
+// What a forward pass leaves per block and warp for the second kernel.
+struct RouterWork {
+  int* warp_before;   // [blocks][warps][experts] rows of the block's earlier warps
+  int* block_count;   // [blocks][experts]
+  float* block_prob;  // [blocks][experts] sums of p
+  float* block_z;     // [blocks][2]: sum of lse^2, valid tokens
+};
+
+// Orders like the float it comes from, 0 below all: -0 equals +0, a NaN is above +infinity, and
+// -infinity (an expert that cannot be taken) gives 0.
+__device__ __forceinline__ unsigned order_key(float v) {
+  if (isnan(v)) return 0xffffffffu;
+  if (v == -INFINITY) return 0u;
+  const unsigned b = __float_as_uint(v + 0.0f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+__device__ __forceinline__ float key_value(unsigned k) {
+  if (k == 0xffffffffu) return __uint_as_float(0x7fffffffu);
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+
+template <int G>
+__device__ __forceinline__ unsigned group_max(unsigned v) {
+  if constexpr (G == 32) {
+    return __reduce_max_sync(kFull, v);
+  } else {
+#pragma unroll
+    for (int d = G / 2; d > 0; d >>= 1) v = max(v, __shfl_xor_sync(kFull, v, d));
+    return v;
+  }
+}
+
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int d = G / 2; d > 0; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
+  return v;
+}
+
+// V consecutive elements from p (element count `have` of them exist; the rest read as `fill`).
+template <int F, int V>
+__device__ __forceinline__ void load_row(const void* base, int64_t at, int have, bool vec, float fill, float (&v)[V]) {
+  if (vec && have >= V) {
+    if constexpr (F == kOutF32) {
+      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i) {
+        const float4 q = __ldg(p + i);
+        v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
+      }
+    } else {
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(base) + at);
+#pragma unroll
+      for (int i = 0; i < V / 8; ++i) {
+        const uint4 q = __ldg(p + i);
+        const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const float2 f = unpack2<F>(w[h]);
+          v[8 * i + 2 * h] = f.x, v[8 * i + 2 * h + 1] = f.y;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = i < have ? load_out<F>(base, at + i) : fill;
+  }
+}
+
+__host__ __device__ constexpr int router_warps(int V) { return V <= 8 ? 16 : 8; }
+
+// Shared memory of a forward block, in 4-byte words: counts [warps][experts], sums of p
+// [warps][experts], slots (index and value) [warps][tokens a warp takes at once][top_k], the factor
+// of the weights per such token, and z and valid tokens per warp; then the second phase's tables.
+size_t forward_smem(int G, int V, int experts, int top_k) {
+  const int warps = router_warps(V), at_once = 32 / G;
+  return 4ull * (2ull * warps * experts + warps * at_once * (2ull * top_k + 2) + 2ull * warps);
+}
+
+constexpr int kPlaceParts = 8;  // most parts the blocks' counts are summed in
+size_t place_smem(int threads, int experts) {
+  const int parts = std::max(1, std::min(kPlaceParts, threads / std::max(1, experts)));
+  return 4ull * ((2ull * parts + 2) * experts + 64);
+}
+
+struct PlaceArgs {
+  RouterShape shape;
+  RouterWork work;
+  int tokens, tokens_per_warp, blocks;
+  const int* indices;
+  int* positions;
+  int* rows;
+  int* row_tokens;
+  float* prob_mean;
+  float* losses;
+};
+
+__device__ __forceinline__ float block_sum(float v, float* s_warp) {
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) s_warp[threadIdx.x / 32] = v;
+  __syncthreads();
+  float s = 0.0f;
+  for (int i = 0; i < static_cast<int>(blockDim.x) / 32; ++i) s += s_warp[i];
+  return s;
+}
+
+// Turns the ranks of this block's slots into packed rows. smem: place_smem bytes.
+__device__ void place_block(const PlaceArgs& a, int block, unsigned char* smem) {
+  const int E = a.shape.experts, K = a.shape.top_k;
+  const int tid = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
+  const int parts = max(1, min(kPlaceParts, threads / E));
+  int* s_before = reinterpret_cast<int*>(smem);  // [parts][E], then part 0 holds the sums
+  int* s_total = s_before + parts * E;
+  int* s_base = s_total + parts * E;
+  int* s_sum = s_base + E;  // [E] totals again, kept while s_total is scanned
+  float* s_warp = reinterpret_cast<float*>(s_sum + E);
+  for (int i = tid; i < parts * E; i += threads) {
+    const int part = i / E, e = i - part * E;
+    int before = 0, total = 0;
+    for (int b = part; b < a.blocks; b += parts) {
+      const int c = a.work.block_count[static_cast<int64_t>(b) * E + e];
+      total += c;
+      before += b < block ? c : 0;
+    }
+    s_before[i] = before;
+    s_total[i] = total;
+  }
+  __syncthreads();
+  for (int e = tid; e < E; e += threads) {
+    int before = 0, total = 0;
+    for (int p = 0; p < parts; ++p) before += s_before[p * E + e], total += s_total[p * E + e];
+    s_base[e] = before;
+    s_sum[e] = total;
+  }
+  __syncthreads();
+  if (tid < 32) {  // the experts' offsets: an exclusive scan of the totals
+    int run = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + tid;
+      const int c = e < E ? s_sum[e] : 0;
+      int inc = c;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(kFull, inc, d);
+        if (tid >= d) inc += up;
+      }
+      if (e < E) s_base[e] += run + inc - c;
+      run += __shfl_sync(kFull, inc, 31);
+    }
+    if (tid == 0) s_warp[32] = __int_as_float(run);
+  }
+  __syncthreads();
+  const int routed = __float_as_int(s_warp[32]);
+
+  const int warps = threads / 32, warp = tid / 32, lane = tid % 32;
+  const int64_t unit = static_cast<int64_t>(block) * warps + warp;
+  const int64_t t0 = min(static_cast<int64_t>(a.tokens), unit * a.tokens_per_warp);
+  const int64_t t1 = min(static_cast<int64_t>(a.tokens), t0 + a.tokens_per_warp);
+  const int* before = a.work.warp_before + unit * E;
+  for (int64_t s = t0 * K + lane; s < t1 * K; s += 32) {
+    const int e = a.indices[s];
+    int p = -1;
+    if (e >= 0) {
+      p = s_base[e] + before[e] + a.positions[s];
+      if (a.row_tokens) a.row_tokens[p] = static_cast<int>(s / K);
+    }
+    a.positions[s] = p;
+  }
+  if (a.row_tokens) {
+    const int64_t slots = static_cast<int64_t>(a.tokens) * K;
+    for (int64_t s = routed + static_cast<int64_t>(block) * threads + tid; s < slots;
+         s += static_cast<int64_t>(a.blocks) * threads)
+      a.row_tokens[s] = -1;
+  }
+  if (block != 0) return;
+
+  // block 0: counts, means and losses
+  float z = 0.0f, n = 0.0f;
+  for (int b = tid; b < a.blocks; b += threads) z += a.work.block_z[2 * b], n += a.work.block_z[2 * b + 1];
+  z = block_sum(z, s_warp);
+  n = block_sum(n, s_warp);
+  const float inv_n = 1.0f / fmaxf(n, 1.0f);
+  const float inv_routed = 1.0f / static_cast<float>(max(routed, 1));
+  __syncthreads();
+  float* s_prob = reinterpret_cast<float*>(s_before);  // [parts][E]
+  for (int i = tid; i < parts * E; i += threads) {
+    const int part = i / E, e = i - part * E;
+    float sum = 0.0f;
+    for (int b = part; b < a.blocks; b += parts) sum += a.work.block_prob[static_cast<int64_t>(b) * E + e];
+    s_prob[i] = sum;
+  }
+  __syncthreads();
+  float balance = 0.0f;
+  for (int e = tid; e < E; e += threads) {
+    float sum = 0.0f;
+    for (int p = 0; p < parts; ++p) sum += s_prob[p * E + e];
+    const float mean = sum * inv_n;
+    if (a.prob_mean) a.prob_mean[e] = mean;
+    a.rows[e] = s_sum[e];
+    balance = fmaf(static_cast<float>(s_sum[e]) * inv_routed, mean, balance);
+  }
+  balance = block_sum(balance, s_warp);
+  if (tid == 0) {
+    a.losses[0] = static_cast<float>(E) * balance;
+    a.losses[1] = z * inv_n;
+    a.losses[2] = n;
+  }
+}
+
+struct ForwardArgs {
+  const void* logits;
+  const unsigned char* mask;
+  int* indices;
+  float* weights;
+  float* lse;
+  int64_t ld;
+  int vec;  // rows can be read 16 bytes at a time
+  PlaceArgs place;
+};
+
+template <int F, int G, int V>
+__global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(ForwardArgs a) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int kWarps = router_warps(V), kAtOnce = 32 / G;
+  const int E = a.place.shape.experts, K = a.place.shape.top_k, T = a.place.tokens;
+  const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
+  const int group = lane / G, gl = lane % G;
+  int* s_count = reinterpret_cast<int*>(smem);
+  float* s_prob = reinterpret_cast<float*>(s_count + kWarps * E);
+  int* s_slot = reinterpret_cast<int*>(s_prob + kWarps * E) + warp * kAtOnce * (2 * K + 2);
+  float* s_value = reinterpret_cast<float*>(s_slot + kAtOnce * K);
+  float* s_factor = s_value + kAtOnce * K;  // [kAtOnce] factor, then [kAtOnce] largest logit
+  float* s_z = s_prob + kWarps * E + kWarps * kAtOnce * (2 * K + 2);
+  int* count = s_count + warp * E;
+  for (int e = lane; e < E; e += 32) count[e] = 0;
+  __syncwarp();
+
+  const int per_warp = a.place.tokens_per_warp;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  const int64_t t0 = min(static_cast<int64_t>(T), unit * per_warp);
+  const int64_t t1 = min(static_cast<int64_t>(T), t0 + per_warp);
+  const int e0 = gl * V, have = max(0, min(V, E - e0));
+  float prob[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) prob[i] = 0.0f;
+  float z = 0.0f, n = 0.0f;
+
+  for (int64_t tb = t0; tb < t1; tb += kAtOnce) {
+    const int64_t t = tb + group;
+    const bool live = t < t1 && (a.mask == nullptr || a.mask[t] != 0);
+    float v[V];
+    unsigned key[V];
+    load_row<F, V>(a.logits, t * a.ld + e0, live ? have : 0, a.vec != 0, -INFINITY, v);
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = order_key(v[i]);
+    float top = -INFINITY, chosen = 0.0f;
+    bool valid = false;
+    for (int j = 0; j < K; ++j) {
+      unsigned mine = key[0];
+#pragma unroll
+      for (int i = 1; i < V; ++i) mine = max(mine, key[i]);
+      const unsigned best = group_max<G>(mine);
+      const unsigned holders = __ballot_sync(kFull, mine == best);
+      const unsigned of_group = G == 32 ? holders : (holders >> (group * G)) & ((1u << (G & 31)) - 1u);
+      const int owner = __ffs(of_group) - 1;  // experts are in lane order: the lowest lane has the lowest expert
+      const float value = key_value(best);
+      if (j == 0) top = value, valid = best != 0u;
+      if (best != 0u) chosen += __expf(value - top);
+      if (gl == owner) {
+        int at = 0;
+#pragma unroll
+        for (int i = V - 1; i >= 0; --i) at = key[i] == best ? i : at;
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = i == at ? 0u : key[i];
+        s_slot[group * K + j] = best != 0u ? e0 + at : -1;
+        s_value[group * K + j] = value;
+      }
+    }
+    float sum = 0.0f;
+    float ex[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      ex[i] = i < have && valid ? __expf(v[i] - top) : 0.0f;
+      sum += ex[i];
+    }
+    sum = group_sum<G>(sum);
+    const float inv = valid ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) prob[i] = fmaf(ex[i], inv, prob[i]);
+    const float lse = valid ? top + logf(sum) : 0.0f;
+    if (gl == 0) {
+      z = fmaf(lse, lse, z);
+      n += valid ? 1.0f : 0.0f;
+      if (a.lse && t < t1) a.lse[t] = lse;
+      s_factor[group] = a.place.shape.normalize ? 1.0f / chosen : inv;
+      s_factor[kAtOnce + group] = top;
+    }
+    __syncwarp();
+    // the slots of these tokens, in order: 32 at a time
+    const int slots = static_cast<int>(min(static_cast<int64_t>(kAtOnce), t1 - tb)) * K;
+    for (int s0 = 0; s0 < slots; s0 += 32) {
+      const int s = s0 + lane;
+      const int e = s < slots ? s_slot[s] : -1;
+      const unsigned same = __match_any_sync(kFull, e);
+      const int seen = e >= 0 ? count[e] : 0;
+      __syncwarp();
+      if (e >= 0 && lane == 31 - __clz(same)) count[e] = seen + __popc(same);
+      __syncwarp();
+      if (s < slots) {
+        const int g = s / K;
+        const int64_t at = tb * K + s;
+        a.indices[at] = e;
+        a.weights[at] = e >= 0 ? __expf(s_value[s] - s_factor[kAtOnce + g]) * s_factor[g] : 0.0f;
+        a.place.positions[at] = seen + __popc(same & ((1u << lane) - 1u));
+      }
+    }
+    __syncwarp();
+  }
+
+  // the block's sums: over the groups of a warp, then over the warps
+#pragma unroll
+  for (int d = G; d < 32; d <<= 1) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) prob[i] += __shfl_xor_sync(kFull, prob[i], d);
+    z += __shfl_xor_sync(kFull, z, d);
+    n += __shfl_xor_sync(kFull, n, d);
+  }
+  if (group == 0)
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < have) s_prob[warp * E + e0 + i] = prob[i];
+  if (lane == 0) s_z[2 * warp] = z, s_z[2 * warp + 1] = n;
+  __syncthreads();
+  const RouterWork& w = a.place.work;
+  for (int e = tid; e < E; e += 32 * kWarps) {
+    int run = 0;
+    float p = 0.0f;
+    for (int i = 0; i < kWarps; ++i) {
+      w.warp_before[(static_cast<int64_t>(blockIdx.x) * kWarps + i) * E + e] = run;
+      run += s_count[i * E + e];
+      p += s_prob[i * E + e];
+    }
+    w.block_count[static_cast<int64_t>(blockIdx.x) * E + e] = run;
+    w.block_prob[static_cast<int64_t>(blockIdx.x) * E + e] = p;
+  }
+  if (tid < 2) {
+    float sum = 0.0f;
+    for (int i = 0; i < kWarps; ++i) sum += s_z[2 * i + tid];
+    w.block_z[2 * blockIdx.x + tid] = sum;
+  }
+  if (gridDim.x == 1) {
+    __syncthreads();
+    place_block(a.place, 0, smem);
+  }
+}
+
+__global__ void router_place_kernel(PlaceArgs a) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  place_block(a, static_cast<int>(blockIdx.x), smem);
+}
+
+struct BackwardArgs {
+  RouterShape shape;
+  const void* logits;
+  const int* indices;
+  const float* weights;
+  const int* rows;
+  const float* losses;
+  const float* lse;
+  const float* grad_weights;
+  const float* grad_losses;
+  void* grad;
+  int tokens;
+  int64_t ld, ldg;
+  int vec, vec_grad;
+};
+
+// dl = p (c_e - <c, p> + 2 g1 lse / n) + the weights' part, with c_e = g0 E f(e) / n.
+template <int F, int G, int V>
+__global__ void __launch_bounds__(32 * router_warps(V)) router_backward_kernel(BackwardArgs a) {
+  constexpr int kWarps = router_warps(V), kAtOnce = 32 / G;
+  __shared__ float s_part[kWarps][kAtOnce * G * V];  // the weights' part of each token's gradient
+  __shared__ float s_sum[kWarps];
+  const int E = a.shape.experts, K = a.shape.top_k;
+  const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
+  const int group = lane / G, gl = lane % G;
+  const int e0 = gl * V, have = max(0, min(V, E - e0));
+  const float n = a.losses[2];
+  const float inv_n = n > 0.0f ? 1.0f / n : 0.0f;
+  const float g0 = a.grad_losses ? a.grad_losses[0] : 0.0f, g1 = a.grad_losses ? a.grad_losses[1] : 0.0f;
+  float routed = 0.0f;
+  for (int e = tid; e < E; e += 32 * kWarps) routed += static_cast<float>(a.rows[e]);
+  routed = block_sum(routed, s_sum);
+  const float scale = routed > 0.0f ? g0 * static_cast<float>(E) * inv_n / routed : 0.0f;
+  float c[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) c[i] = i < have ? scale * static_cast<float>(a.rows[e0 + i]) : 0.0f;
+  float* part = s_part[warp] + group * G * V;
+#pragma unroll
+  for (int i = 0; i < V; ++i) part[e0 + i] = 0.0f;
+  __syncwarp();
+
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps * kAtOnce;
+  for (int64_t tb = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * kAtOnce; tb < a.tokens; tb += step) {
+    const int64_t t = tb + group;
+    const bool live = t < a.tokens && a.indices[t * K] >= 0;
+    // the weights' part: slot j by lane j of the group
+    float lane_sum = 0.0f;
+    for (int j = gl; j < K; j += G) {
+      const int e = live ? a.indices[t * K + j] : -1;
+      if (e >= 0 && a.grad_weights) lane_sum = fmaf(a.weights[t * K + j], a.grad_weights[t * K + j], lane_sum);
+    }
+    const float dot_w = group_sum<G>(lane_sum);
+    for (int j = gl; j < K; j += G) {
+      const int e = live ? a.indices[t * K + j] : -1;
+      if (e >= 0 && e < E && a.grad_weights) {
+        const float w = a.weights[t * K + j];
+        part[e] = w * (a.grad_weights[t * K + j] - (a.shape.normalize ? dot_w : 0.0f));
+      }
+    }
+    float v[V];
+    load_row<F, V>(a.logits, t * a.ld + e0, live ? have : 0, a.vec != 0, -INFINITY, v);
+    const float lse = live ? a.lse[t] : 0.0f;
+    float dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      v[i] = i < have && live ? __expf(v[i] - lse) : 0.0f;
+      dot = fmaf(c[i], v[i], dot);
+    }
+    dot = group_sum<G>(dot);
+    const float common = 2.0f * g1 * inv_n * lse - dot - (a.shape.normalize ? 0.0f : dot_w);
+    __syncwarp();
+    if (t < a.tokens) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = live ? fmaf(v[i], c[i] + common, part[e0 + i]) : 0.0f;
+      const int64_t at = t * a.ldg + e0;
+      if (a.vec_grad && have == V) {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+          const float4 o = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          if constexpr (F == kOutF32) store_out4<F>(static_cast<float*>(a.grad) + at + 4 * i, o);
+          else store_out4<F>(static_cast<unsigned short*>(a.grad) + at + 4 * i, o);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (i < have) store_out<F>(a.grad, at + i, v[i]);
+      }
+    }
+    __syncwarp();
+    for (int j = gl; j < K; j += G) {
+      const int e = live ? a.indices[t * K + j] : -1;
+      if (e >= 0 && e < E) part[e] = 0.0f;
+    }
+    __syncwarp();
+  }
+}
+
+// The lane layout for a number of experts: G lanes a token, V experts a lane.
+template <typename Fn>
+void with_layout(int experts, Fn f) {
+  using std::integral_constant;
+  if (experts <= 32) f(integral_constant<int, 4>(), integral_constant<int, 8>());
+  else if (experts <= 64) f(integral_constant<int, 8>(), integral_constant<int, 8>());
+  else if (experts <= 128) f(integral_constant<int, 16>(), integral_constant<int, 8>());
+  else if (experts <= 256) f(integral_constant<int, 32>(), integral_constant<int, 8>());
+  else if (experts <= 512) f(integral_constant<int, 32>(), integral_constant<int, 16>());
+  else f(integral_constant<int, 32>(), integral_constant<int, 32>());
+}
+
+template <typename Fn>
+void with_logits(int type, Fn f) {
+  if (type == GG_OUTPUT_F32) f(std::integral_constant<int, kOutF32>());
+  else if (type == GG_OUTPUT_F16) f(std::integral_constant<int, kOutF16>());
+  else f(std::integral_constant<int, kOutBF16>());
+}
+
+int type_bytes(int type) { return type == GG_OUTPUT_F32 ? 4 : 2; }
+
+// Rows of `ld` elements from `p` whose every element at a multiple of 8 is 16-byte aligned.
+bool rows_aligned(const void* p, int64_t ld, int type) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * type_bytes(type)) % 16 == 0;
+}
+
+}  // namespace
+}  // namespace gg
+
+struct gg_router {
+  gg_router_config config{};
+  void* block = nullptr;
+  gg::RouterWork work{};
+};
+
+extern "C" {
+
+int gg_router_create(const gg_router_config* config, gg_router** out) {
+  if (!out) return cudaErrorInvalidValue;
+  *out = nullptr;
+  if (!config) return cudaErrorInvalidValue;
+  const gg_router_config& c = *config;
+  if (c.experts < 1 || c.experts > GG_ROUTER_MAX_EXPERTS || c.top_k < 1 || c.top_k > GG_ROUTER_MAX_TOP_K ||
+      c.capacity_tokens < 0 || static_cast<int64_t>(c.capacity_tokens) * c.top_k > INT32_MAX ||
+      (c.logit_type != GG_OUTPUT_F32 && c.logit_type != GG_OUTPUT_F16 && c.logit_type != GG_OUTPUT_BF16))
+    return cudaErrorInvalidValue;
+  gg_router* r = new (std::nothrow) gg_router();
+  if (!r) return cudaErrorMemoryAllocation;
+  r->config = c;
+  size_t warps = 0;
+  gg::with_layout(c.experts, [&](auto, auto v) { warps = gg::router_warps(v()); });
+  const size_t E = static_cast<size_t>(c.experts), B = gg::kMaxBlocks;
+  const size_t words = B * warps * E + 2 * B * E + 2 * B;
+  cudaError_t st = cudaMalloc(&r->block, words * 4);
+  if (st != cudaSuccess) {
+    delete r;
+    return st;
+  }
+  r->work.warp_before = static_cast<int*>(r->block);
+  r->work.block_count = r->work.warp_before + B * warps * E;
+  r->work.block_prob = reinterpret_cast<float*>(r->work.block_count + B * E);
+  r->work.block_z = r->work.block_prob + B * E;
+  *out = r;
+  return cudaSuccess;
+}
+
+int gg_router_run(gg_router* router, const gg_route* route, void* stream) {
+  if (!router || !router->block) return cudaErrorInvalidDevicePointer;
+  if (!route) return cudaErrorInvalidValue;
+  const gg_router_config& c = router->config;
+  const gg_route& q = *route;
+  if (q.tokens < 0 || q.tokens > c.capacity_tokens || q.ld < c.experts || !q.rows || !q.losses) return cudaErrorInvalidValue;
+  if (q.tokens > 0 && (!q.logits || !q.indices || !q.weights || !q.positions)) return cudaErrorInvalidValue;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t st = cudaSuccess;
+  gg::with_logits(c.logit_type, [&](auto f) {
+    gg::with_layout(c.experts, [&](auto g, auto v) {
+      constexpr int G = g(), V = v();
+      constexpr int warps = gg::router_warps(V), at_once = 32 / G;
+      // tokens a warp: whole turns, as few as fill the blocks
+      const int64_t share = (static_cast<int64_t>(q.tokens) + gg::kMaxBlocks * warps - 1) / (gg::kMaxBlocks * warps);
+      const int64_t per_warp = std::max<int64_t>(1, (share + at_once - 1) / at_once) * at_once;
+      const int blocks = static_cast<int>(std::max<int64_t>(1, (q.tokens + per_warp * warps - 1) / (per_warp * warps)));
+      gg::ForwardArgs a{};
+      a.logits = q.logits;
+      a.mask = q.token_mask;
+      a.indices = q.indices;
+      a.weights = q.weights;
+      a.lse = q.lse;
+      a.ld = q.ld;
+      a.vec = gg::rows_aligned(q.logits, q.ld, c.logit_type);
+      a.place = {{c.experts, c.top_k, c.normalize != 0}, router->work, q.tokens, static_cast<int>(per_warp), blocks,
+                 q.indices, q.positions, q.rows, q.row_tokens, q.prob_mean, q.losses};
+      const size_t place = gg::place_smem(32 * warps, c.experts);
+      const size_t smem = std::max(gg::forward_smem(G, V, c.experts, c.top_k), blocks == 1 ? place : 0);
+      auto kernel = gg::router_forward_kernel<f(), G, V>;
+      if (smem > 48 * 1024) {
+        st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (st != cudaSuccess) return;
+      }
+      kernel<<<blocks, 32 * warps, smem, s>>>(a);
+      if (blocks > 1) gg::router_place_kernel<<<blocks, 32 * warps, place, s>>>(a.place);
+      st = cudaGetLastError();
+    });
+  });
+  return st;
+}
+
+int gg_router_backward(const gg_router* router, const gg_route_gradient* gradient, void* stream) {
+  if (!router) return cudaErrorInvalidDevicePointer;
+  if (!gradient) return cudaErrorInvalidValue;
+  const gg_router_config& c = router->config;
+  const gg_route_gradient& q = *gradient;
+  if (q.tokens < 0 || q.tokens > c.capacity_tokens || q.ld < c.experts || q.ld_grad < c.experts) return cudaErrorInvalidValue;
+  if (q.tokens == 0) return cudaSuccess;
+  if (!q.logits || !q.indices || !q.weights || !q.rows || !q.losses || !q.lse || !q.grad_logits) return cudaErrorInvalidValue;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  gg::with_logits(c.logit_type, [&](auto f) {
+    gg::with_layout(c.experts, [&](auto g, auto v) {
+      constexpr int G = g(), V = v();
+      constexpr int warps = gg::router_warps(V), at_once = 32 / G;
+      gg::BackwardArgs a{{c.experts, c.top_k, c.normalize != 0}, q.logits, q.indices, q.weights, q.rows, q.losses, q.lse,
+                         q.grad_weights, q.grad_losses, q.grad_logits, q.tokens, q.ld, q.ld_grad,
+                         gg::rows_aligned(q.logits, q.ld, c.logit_type),
+                         gg::rows_aligned(q.grad_logits, q.ld_grad, c.logit_type)};
+      const int64_t blocks = (static_cast<int64_t>(q.tokens) + warps * at_once - 1) / (warps * at_once);
+      gg::router_backward_kernel<f(), G, V>
+          <<<static_cast<int>(std::min<int64_t>(blocks, 4 * gg::kMaxBlocks)), 32 * warps, 0, s>>>(a);
+    });
+  });
+  return cudaGetLastError();
+}
+
+void gg_router_destroy(gg_router* router) {
+  if (!router) return;
+  if (router->block) cudaFree(router->block);
+  delete router;
+}
+
+}  // extern "C"

@@ -372,6 +372,160 @@ int gg_moe_plan_run(gg_moe_plan* plan, const int* rows, void* stream);
 int gg_moe_plan_status(gg_moe_plan* plan, int* status, int* total_tiles);
 void gg_moe_plan_destroy(gg_moe_plan* plan);
 
+/* ---- mixture-of-experts router ----------------------------------------------------------------
+ * No counterpart in the reference. From the router's logits (tokens x experts) to what the grouped
+ * product needs: the experts of every token with their weights, the row counts per expert (the
+ * `rows` of gg_moe_plan_run) and the places of the tokens' rows in packed order; with the balance
+ * loss, the z loss, and the gradient of all of them with respect to the logits.
+ *
+ * For token t with logits l(t, e):
+ *   valid(t)   token_mask is NULL or token_mask[t] != 0, and some l(t, e) is not -infinity. A
+ *              token that is not valid goes to no expert, whatever its logits hold (NaN included),
+ *              and counts in no mean.
+ *   S(t)       the top_k largest logits, the lower expert first where two are equal (-0 equals 0,
+ *              a NaN is above +infinity and all NaNs are equal). An expert at -infinity is never
+ *              taken; where fewer than top_k are left, the slots over hold index -1, weight 0,
+ *              position -1.
+ *   p(t, .)    softmax over all experts; lse(t) the logarithm of its denominator.
+ *   weights    with normalize the softmax over S(t), else p at S(t).
+ *   rows[e]    tokens with e in S(t).
+ *   positions  the packed rows are the taken (token, expert) pairs ordered by expert, then token;
+ *              positions[t * top_k + j] is the packed row of slot j of token t.
+ *   row_tokens the token of every packed row; -1 past the last.
+ *   losses     [0] balance: experts * sum_e f(e) prob_mean(e), with f(e) = rows[e] / sum of rows and
+ *              prob_mean(e) the mean of p(t, e) over valid tokens (1 when both are uniform);
+ *              [1] z: the mean of lse(t)^2 over valid tokens; [2] the number of valid tokens.
+ * Everything but the logits is held in FP32 or 32-bit integers. Sums over tokens are taken in a fixed
+ * order: the same inputs give the same bits. The logits are read as FP32, FP16 or BF16
+ * (GG_OUTPUT_F32 / F16 / BF16). */
+#define GG_ROUTER_MAX_EXPERTS 1024
+#define GG_ROUTER_MAX_TOP_K 32
+typedef struct gg_router_config {
+  int experts;         /* 1..GG_ROUTER_MAX_EXPERTS */
+  int top_k;           /* 1..GG_ROUTER_MAX_TOP_K; may exceed experts (slots over hold -1) */
+  int capacity_tokens; /* most tokens of a run; capacity_tokens * top_k must fit an int */
+  int logit_type;      /* GG_OUTPUT_F32, GG_OUTPUT_F16 or GG_OUTPUT_BF16: logits and their gradient */
+  int normalize;       /* weights sum to 1 over the chosen experts */
+} gg_router_config;
+
+/* One forward pass. All pointers are device memory; t runs over tokens, j over top_k. */
+typedef struct gg_route {
+  const void* logits;              /* tokens x experts, row pitch ld elements */
+  const unsigned char* token_mask; /* tokens bytes, 0: not routed; NULL: all are */
+  int* indices;                    /* tokens x top_k */
+  float* weights;                  /* tokens x top_k */
+  int* positions;                  /* tokens x top_k */
+  int* rows;                       /* experts */
+  float* losses;                   /* 3 */
+  int* row_tokens;                 /* optional: tokens * top_k */
+  float* lse;                      /* optional (needed by the backward pass): tokens, 0 for a token not valid */
+  float* prob_mean;                /* optional: experts */
+  int tokens;                      /* 0..capacity_tokens */
+  int ld;                          /* >= experts */
+} gg_route;
+
+/* The gradient with respect to the logits, from the forward pass's inputs and outputs:
+ *   grad_weights (tokens x top_k, NULL: zeros; the entry of a slot without an expert is not read),
+ *   grad_losses (2 values: of losses[0] and losses[1]; NULL: zeros).
+ * The choice S(t) and the counts carry no gradient. Rows of tokens not valid get zeros. */
+typedef struct gg_route_gradient {
+  const void* logits;
+  const int* indices;
+  const float* weights;
+  const int* rows;
+  const float* losses;
+  const float* lse;
+  const float* grad_weights;
+  const float* grad_losses;
+  void* grad_logits; /* tokens x experts, row pitch ld_grad, of the logits' type */
+  int tokens;
+  int ld;
+  int ld_grad;
+} gg_route_gradient;
+
+typedef struct gg_router gg_router;
+/* Allocates the router's workspace (per-block counts and sums). Sizes out of range or an unknown
+ * logit_type -> cudaErrorInvalidValue before any device work. */
+int gg_router_create(const gg_router_config* config, gg_router** out);
+/* Enqueues on `stream`, without host synchronisation. tokens == 0 writes zero rows and losses.
+ * Runs of one router on two streams at once race on its workspace: one router per concurrent stream. */
+int gg_router_run(gg_router* router, const gg_route* route, void* stream);
+/* One launch on `stream`; uses no workspace. */
+int gg_router_backward(const gg_router* router, const gg_route_gradient* gradient, void* stream);
+void gg_router_destroy(gg_router* router);
+
+/* ---- rows into expert order and back ----------------------------------------------------------
+ * No counterpart in the reference. The moves between a layer's tokens and the packed rows of the
+ * grouped product, by the router's positions (tokens x top_k; an entry outside
+ * [0, packed_rows) goes nowhere and reads nothing). Each is one launch on `stream`. */
+
+/* packed[positions[t][j], :] = x[t, :]. Elements of elem_bytes (1, 2 or 4) bytes, copied as they are;
+ * ldx and ldp in elements. Packed rows that no position names are not written. */
+int gg_moe_dispatch(const void* x, int ldx, const int* positions, int tokens, int top_k, int width, int elem_bytes,
+                    void* packed, int packed_rows, int ldp, void* stream);
+
+/* out[t, :] = sum_j weights[t][j] * packed[positions[t][j], :], j in order, in FP32, rounded once to
+ * out_type; weights NULL: 1 (the gradient of gg_moe_dispatch). A token without rows gets zeros.
+ * packed_type and out_type: GG_OUTPUT_*. out must not overlap packed. */
+int gg_moe_combine(const void* packed, int packed_type, int packed_rows, int ldp, const int* positions,
+                   const float* weights, int tokens, int top_k, int width, void* out, int out_type, int ldo,
+                   void* stream);
+
+/* The gradient of gg_moe_combine with weights:
+ *   grad_packed[positions[t][j], :] = weights[t][j] * grad_out[t, :]   (packed_type, pitch ldgp)
+ *   grad_weights[t][j] = <grad_out[t, :], packed[positions[t][j], :]>  (FP32; 0 where nothing was routed)
+ * grad_out has out_type. Packed rows that no position names are not written. grad_packed may be packed
+ * itself (each element is read before it is written, by the same thread). */
+int gg_moe_combine_backward(const void* grad_out, int out_type, int ldo, const void* packed, int packed_type,
+                            int packed_rows, int ldp, const int* positions, const float* weights, int tokens,
+                            int top_k, int width, void* grad_packed, int ldgp, float* grad_weights, void* stream);
+
+/* ---- experts with 4-bit weights ----------------------------------------------------------------
+ * No counterpart in the reference. The decoding form of the mixture-of-experts plan: the few rows
+ * of every expert against its weights held in 4 bits with a scale per output and group of k:
+ *   D[r, o] = act(sum_k A[r, k] * scale(o, k / group) * (q(o, k) - zero(o, k / group)) + bias(o))
+ * for the rows r of expert e, which are packed as in gg_moe_plan_run (expert 0's rows first) with
+ * the counts in device memory. The differences q - zero are exact, products and sums are FP32,
+ * D is rounded once. With experts = 1 it is a matrix-vector product with one 4-bit matrix.
+ * gg_q4_plan_create lays the weights out once for the kernel (the caller's copies may be freed
+ * after it returns). */
+typedef struct gg_q4_problem {
+  const unsigned char* const* q;  /* host array of `experts` device pointers: n rows of ceil(k / 2) bytes, row
+                                     pitch ldq bytes; byte b of a row holds k = 2b in its low 4 bits and
+                                     k = 2b + 1 in its high 4 bits, as unsigned numbers */
+  const void* const* scales;      /* host array of device pointers: n x ceil(k / group), packed, of the input type */
+  const unsigned char* const* zeros; /* optional host array of device pointers: n x ceil(k / group) bytes of 0..15
+                                     (the low 4 bits count); NULL: all 8 */
+  const float* const* bias;       /* optional host array of device pointers (NULL entries: none): n FP32 values */
+  int experts;                    /* 1..GG_Q4_MAX_EXPERTS */
+  int n;                          /* outputs, >= 1 */
+  int k;                          /* inputs, >= 1 */
+  int group;                      /* 32, 64 or a multiple of 128 */
+  int ldq;
+  int input_type;                 /* GG_INPUT_F16 or GG_INPUT_BF16: type of A and the scales */
+  int output_type;                /* GG_OUTPUT_*: type of D */
+  int activation;                 /* GG_ACT_* (GELU in its tanh form) */
+} gg_q4_problem;
+#define GG_Q4_MAX_EXPERTS 1024
+typedef struct gg_q4_plan gg_q4_plan;
+/* Allocates the plan's copy of the weights, fills it in order on `stream` and synchronises that
+ * stream. Errors: sizes or types out of range, null pointers -> cudaErrorInvalidValue before any
+ * device work; CUDA errors passed through. */
+int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** out);
+/* a: rows of the input type, pitch lda (>= k); packed row r reads row r of a, or row row_tokens[r]
+ *   when row_tokens (device) is given (the gather of a dispatch done by the product itself; an entry
+ *   outside [0, a_rows) reads zeros); a_rows: rows of a.
+ * rows: `experts` counts in device memory; NULL with experts == 1: all capacity_rows rows.
+ * d: capacity_rows x n of the output type, pitch ldd (>= n); rows past the counts' sum are not written.
+ * One launch on `stream`. Counts that are negative or sum to more than capacity_rows (or than
+ * a_rows without row_tokens) compute nothing and raise GG_STATUS_BAD_ROWS. Runs of one plan may
+ * overlap on several streams. */
+int gg_q4_plan_run(gg_q4_plan* plan, const void* a, int lda, int a_rows, const int* row_tokens, const int* rows,
+                   void* d, int ldd, int capacity_rows, void* stream);
+/* Synchronises; returns (then clears) the GG_STATUS_* bits of the plan's runs. */
+int gg_q4_plan_status(gg_q4_plan* plan, int* status);
+void gg_q4_plan_destroy(gg_q4_plan* plan);
+
 /* ---- grouped GEMM prepared on the device ----------------------------------------------------
  * No counterpart in the reference, whose problem set is prepared on the host
  * (src/grouped_gemm.cu:967-1022 prepare_problem_set, 1132-1239 build). Here the problem
