@@ -37,22 +37,20 @@ struct RouterWork {
   float* block_z;     // [blocks][2]: sum of lse^2, valid tokens
 };
 
-// Orders like the float it comes from, 0 below all: -0 equals +0, a NaN is above +infinity, and
-// -infinity (an expert that cannot be taken) gives 0.
-__device__ __forceinline__ unsigned order_key(float v) {
-  if (isnan(v)) return 0xffffffffu;
-  if (v == -INFINITY) return 0u;
-  const unsigned b = __float_as_uint(v + 0.0f);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+constexpr int kTaken = INT32_MIN;             // below every key
+constexpr int kClosed = static_cast<int>(0x807fffffu);  // the key of -infinity: an expert that cannot be taken
+
+// A signed integer that orders like the float: adding 0 turns -0 into +0 and every NaN into the
+// positive one, which is above +infinity; negative numbers order backwards in their low 31 bits.
+__device__ __forceinline__ int order_key(float v) {
+  const int b = __float_as_int(v + 0.0f);
+  return b ^ ((b >> 31) & 0x7fffffff);
 }
 
-__device__ __forceinline__ float key_value(unsigned k) {
-  if (k == 0xffffffffu) return __uint_as_float(0x7fffffffu);
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
+__device__ __forceinline__ float key_value(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
 
 template <int G>
-__device__ __forceinline__ unsigned group_max(unsigned v) {
+__device__ __forceinline__ int group_max(int v) {
   if constexpr (G == 32) {
     return __reduce_max_sync(kFull, v);
   } else {
@@ -99,20 +97,30 @@ __device__ __forceinline__ void load_row(const void* base, int64_t at, int have,
   }
 }
 
-__host__ __device__ constexpr int router_warps(int V) { return V <= 8 ? 16 : 8; }
+// Warps of a forward block (one block an SM): as many as the registers of V experts a lane allow.
+__host__ __device__ constexpr int router_warps(int V) { return V <= 8 ? 32 : V <= 16 ? 16 : 8; }
+constexpr int kBackwardWarps = 8;
+
+constexpr int kForwardSmemMost = 160 * 1024;
+constexpr int kCandidates = 64;  // see choose_of_candidates
 
 // Shared memory of a forward block, in 4-byte words: counts [warps][experts], sums of p
-// [warps][experts], slots (index and value) [warps][tokens a warp takes at once][top_k], the factor
-// of the weights per such token, and z and valid tokens per warp; then the second phase's tables.
+// [warps][experts], slots (index and key) [warps][tokens a warp takes at once][top_k], the factor
+// of the weights and the largest logit per such token, and z and valid tokens per warp; where a
+// warp takes one token at once, its candidates (key and expert).
 size_t forward_smem(int G, int V, int experts, int top_k) {
   const int warps = router_warps(V), at_once = 32 / G;
-  return 4ull * (2ull * warps * experts + warps * at_once * (2ull * top_k + 2) + 2ull * warps);
+  return 4ull * (2ull * warps * experts + warps * at_once * (2ull * top_k + 2) + 2ull * warps +
+                 (G == 32 ? 2ull * warps * kCandidates : 0));
 }
 
-constexpr int kPlaceParts = 8;  // most parts the blocks' counts are summed in
+// Parts the blocks' counts are summed in: what the threads allow, so that each sums few rows.
+__host__ __device__ __forceinline__ int place_parts(int threads, int experts) {
+  const int p = threads / experts;
+  return p < 1 ? 1 : p > 16 ? 16 : p;
+}
 size_t place_smem(int threads, int experts) {
-  const int parts = std::max(1, std::min(kPlaceParts, threads / std::max(1, experts)));
-  return 4ull * ((2ull * parts + 2) * experts + 64);
+  return 4ull * ((3ull * place_parts(threads, experts) + 2) * experts + 64);
 }
 
 struct PlaceArgs {
@@ -137,26 +145,49 @@ __device__ __forceinline__ float block_sum(float v, float* s_warp) {
   return s;
 }
 
-// Turns the ranks of this block's slots into packed rows. smem: place_smem bytes.
+// Sums of rows b0, b0 + step, ... < rows of a [rows][E] table at column e, eight loads in flight (one
+// after the other, they would cost a trip to L2 each). `split`: also the sum of the rows below it.
+template <typename T>
+__device__ __forceinline__ T column_sum(const T* table, int E, int e, int b0, int step, int rows, int split, T* below) {
+  T total = 0, lower = 0;
+  for (int b = b0; b < rows; b += 8 * step) {
+    T c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = b + i * step < rows ? table[static_cast<int64_t>(b + i * step) * E + e] : T(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      total += c[i];
+      lower += b + i * step < split ? c[i] : T(0);
+    }
+  }
+  *below = lower;
+  return total;
+}
+
+// Turns the ranks of this block's slots into packed rows. smem: place_smem bytes. Block 0 also sums what
+// the blocks left behind into the counts, means and losses.
 __device__ void place_block(const PlaceArgs& a, int block, unsigned char* smem) {
   const int E = a.shape.experts, K = a.shape.top_k;
   const int tid = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
-  const int parts = max(1, min(kPlaceParts, threads / E));
-  int* s_before = reinterpret_cast<int*>(smem);  // [parts][E], then part 0 holds the sums
-  int* s_total = s_before + parts * E;
-  int* s_base = s_total + parts * E;
-  int* s_sum = s_base + E;  // [E] totals again, kept while s_total is scanned
+  const int parts = place_parts(threads, E);
+  int* s_before = reinterpret_cast<int*>(smem);  // [parts][E]
+  int* s_total = s_before + parts * E;           // [parts][E]
+  float* s_prob = reinterpret_cast<float*>(s_total + parts * E);  // [parts][E]
+  int* s_base = reinterpret_cast<int*>(s_prob + parts * E);       // [E]
+  int* s_sum = s_base + E;                                        // [E]
   float* s_warp = reinterpret_cast<float*>(s_sum + E);
+  float z = 0.0f, n = 0.0f;
+  if (block == 0)
+    for (int b = tid; b < a.blocks; b += threads) z += a.work.block_z[2 * b], n += a.work.block_z[2 * b + 1];
   for (int i = tid; i < parts * E; i += threads) {
     const int part = i / E, e = i - part * E;
-    int before = 0, total = 0;
-    for (int b = part; b < a.blocks; b += parts) {
-      const int c = a.work.block_count[static_cast<int64_t>(b) * E + e];
-      total += c;
-      before += b < block ? c : 0;
-    }
+    int before;
+    s_total[i] = column_sum(a.work.block_count, E, e, part, parts, a.blocks, block, &before);
     s_before[i] = before;
-    s_total[i] = total;
+    if (block == 0) {
+      float none;
+      s_prob[i] = column_sum(a.work.block_prob, E, e, part, parts, a.blocks, 0, &none);
+    }
   }
   __syncthreads();
   for (int e = tid; e < E; e += threads) {
@@ -190,6 +221,7 @@ __device__ void place_block(const PlaceArgs& a, int block, unsigned char* smem) 
   const int64_t t0 = min(static_cast<int64_t>(a.tokens), unit * a.tokens_per_warp);
   const int64_t t1 = min(static_cast<int64_t>(a.tokens), t0 + a.tokens_per_warp);
   const int* before = a.work.warp_before + unit * E;
+#pragma unroll 4
   for (int64_t s = t0 * K + lane; s < t1 * K; s += 32) {
     const int e = a.indices[s];
     int p = -1;
@@ -207,22 +239,10 @@ __device__ void place_block(const PlaceArgs& a, int block, unsigned char* smem) 
   }
   if (block != 0) return;
 
-  // block 0: counts, means and losses
-  float z = 0.0f, n = 0.0f;
-  for (int b = tid; b < a.blocks; b += threads) z += a.work.block_z[2 * b], n += a.work.block_z[2 * b + 1];
   z = block_sum(z, s_warp);
   n = block_sum(n, s_warp);
   const float inv_n = 1.0f / fmaxf(n, 1.0f);
   const float inv_routed = 1.0f / static_cast<float>(max(routed, 1));
-  __syncthreads();
-  float* s_prob = reinterpret_cast<float*>(s_before);  // [parts][E]
-  for (int i = tid; i < parts * E; i += threads) {
-    const int part = i / E, e = i - part * E;
-    float sum = 0.0f;
-    for (int b = part; b < a.blocks; b += parts) sum += a.work.block_prob[static_cast<int64_t>(b) * E + e];
-    s_prob[i] = sum;
-  }
-  __syncthreads();
   float balance = 0.0f;
   for (int e = tid; e < E; e += threads) {
     float sum = 0.0f;
@@ -251,6 +271,45 @@ struct ForwardArgs {
   PlaceArgs place;
 };
 
+// The top_k largest keys of a token that a whole warp holds, V consecutive experts a lane, when
+// top_k <= 8: the smallest of the maxima of eight groups of four lanes bounds the 8th largest key from below,
+// so only keys from it on are candidates. On random logits that leaves about 22 (the draws until
+// every group was hit). They are gathered, two a lane at most, and then each round compares two keys
+// a lane instead of V: measured 1.9x over the rounds on all keys at 256 experts, top 8. Lane j gets the expert
+// and key of slot j (expert -1: none). False: more candidates than fit, nothing is chosen.
+template <int V>
+__device__ __forceinline__ bool choose_of_candidates(const int (&key)[V], int mine, int e0, int K, int2* s_candidates, int lane,
+                                                     int* slot_expert, int* slot_key) {
+  int bound = max(mine, __shfl_xor_sync(kFull, mine, 1));
+  bound = max(bound, __shfl_xor_sync(kFull, bound, 2));
+  bound = max(__reduce_min_sync(kFull, bound), kClosed + 1);
+  int n = 0;
+  const unsigned lower = (1u << lane) - 1u;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const bool in = key[i] >= bound;
+    const unsigned who = __ballot_sync(kFull, in);
+    const int at = n + __popc(who & lower);
+    if (in && at < kCandidates) s_candidates[at] = make_int2(key[i], e0 + i);
+    n += __popc(who);
+  }
+  if (n > kCandidates) return false;
+  __syncwarp();
+  int2 a = make_int2(kTaken, INT32_MAX), b = a;
+  if (lane < n) a = s_candidates[lane];
+  if (lane + 32 < n) b = s_candidates[lane + 32];
+  for (int j = 0; j < K; ++j) {
+    const int best = __reduce_max_sync(kFull, max(a.x, b.x));
+    // the lowest expert of those that hold it (the candidates are in no order of experts)
+    const int e = best == kTaken ? -1
+                                 : __reduce_min_sync(kFull, min(a.x == best ? a.y : INT32_MAX, b.x == best ? b.y : INT32_MAX));
+    if (lane == j) *slot_expert = e, *slot_key = best;
+    if (a.y == e) a.x = kTaken;
+    if (b.y == e) b.x = kTaken;
+  }
+  return true;
+}
+
 template <int F, int G, int V>
 __global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(ForwardArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -258,11 +317,12 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(Fo
   const int E = a.place.shape.experts, K = a.place.shape.top_k, T = a.place.tokens;
   const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
   const int group = lane / G, gl = lane % G;
-  int* s_count = reinterpret_cast<int*>(smem);
+  int2* s_candidates = reinterpret_cast<int2*>(smem) + warp * kCandidates;
+  int* s_count = reinterpret_cast<int*>(smem + (G == 32 ? 8 * kWarps * kCandidates : 0));
   float* s_prob = reinterpret_cast<float*>(s_count + kWarps * E);
   int* s_slot = reinterpret_cast<int*>(s_prob + kWarps * E) + warp * kAtOnce * (2 * K + 2);
-  float* s_value = reinterpret_cast<float*>(s_slot + kAtOnce * K);
-  float* s_factor = s_value + kAtOnce * K;  // [kAtOnce] factor, then [kAtOnce] largest logit
+  int* s_key = s_slot + kAtOnce * K;
+  float* s_factor = reinterpret_cast<float*>(s_key + kAtOnce * K);  // [kAtOnce] factor, then [kAtOnce] largest logit
   float* s_z = s_prob + kWarps * E + kWarps * kAtOnce * (2 * K + 2);
   int* count = s_count + warp * E;
   for (int e = lane; e < E; e += 32) count[e] = 0;
@@ -282,31 +342,49 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(Fo
     const int64_t t = tb + group;
     const bool live = t < t1 && (a.mask == nullptr || a.mask[t] != 0);
     float v[V];
-    unsigned key[V];
+    int key[V];
     load_row<F, V>(a.logits, t * a.ld + e0, live ? have : 0, a.vec != 0, -INFINITY, v);
 #pragma unroll
     for (int i = 0; i < V; ++i) key[i] = order_key(v[i]);
-    float top = -INFINITY, chosen = 0.0f;
-    bool valid = false;
-    for (int j = 0; j < K; ++j) {
-      unsigned mine = key[0];
+    int mine = key[0];
 #pragma unroll
-      for (int i = 1; i < V; ++i) mine = max(mine, key[i]);
-      const unsigned best = group_max<G>(mine);
-      const unsigned holders = __ballot_sync(kFull, mine == best);
-      const unsigned of_group = G == 32 ? holders : (holders >> (group * G)) & ((1u << (G & 31)) - 1u);
-      const int owner = __ffs(of_group) - 1;  // experts are in lane order: the lowest lane has the lowest expert
-      const float value = key_value(best);
-      if (j == 0) top = value, valid = best != 0u;
-      if (best != 0u) chosen += __expf(value - top);
-      if (gl == owner) {
-        int at = 0;
+    for (int i = 1; i < V; ++i) mine = max(mine, key[i]);
+    const int largest = group_max<G>(mine);
+    const bool valid = largest > kClosed;
+    const float top = key_value(largest);
+    float chosen = 0.0f;
+    bool done = false;
+    if constexpr (G == 32) {
+      if (K >= 4 && K <= 8) {
+        int slot_expert = -1, slot_key = kTaken;
+        done = choose_of_candidates<V>(key, mine, e0, K, s_candidates, lane, &slot_expert, &slot_key);
+        if (done) {
+          if (lane < K) s_slot[lane] = slot_expert, s_key[lane] = slot_key;
+          chosen = group_sum<32>(slot_expert >= 0 ? __expf(key_value(slot_key) - top) : 0.0f);
+        }
+      }
+    }
+    if (!done) {
+      int best = largest;
+      for (int j = 0; j < K; ++j) {
+        const unsigned holders = __ballot_sync(kFull, mine == best);
+        const unsigned of_group = G == 32 ? holders : (holders >> (group * G)) & ((1u << (G & 31)) - 1u);
+        const int owner = __ffs(of_group) - 1;  // experts are in lane order: the lowest lane has the lowest expert
+        if (best > kClosed) chosen += __expf(key_value(best) - top);
+        if (gl == owner) {
+          int at = 0;
 #pragma unroll
-        for (int i = V - 1; i >= 0; --i) at = key[i] == best ? i : at;
+          for (int i = V - 1; i >= 0; --i) at = key[i] == best ? i : at;
 #pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = i == at ? 0u : key[i];
-        s_slot[group * K + j] = best != 0u ? e0 + at : -1;
-        s_value[group * K + j] = value;
+          for (int i = 0; i < V; ++i) key[i] = i == at ? kTaken : key[i];
+          s_slot[group * K + j] = best > kClosed ? e0 + at : -1;
+          s_key[group * K + j] = best;
+        }
+        if (j + 1 == K) break;
+        mine = key[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) mine = max(mine, key[i]);
+        best = group_max<G>(mine);
       }
     }
     float sum = 0.0f;
@@ -343,7 +421,7 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(Fo
         const int g = s / K;
         const int64_t at = tb * K + s;
         a.indices[at] = e;
-        a.weights[at] = e >= 0 ? __expf(s_value[s] - s_factor[kAtOnce + g]) * s_factor[g] : 0.0f;
+        a.weights[at] = e >= 0 ? __expf(key_value(s_key[s]) - s_factor[kAtOnce + g]) * s_factor[g] : 0.0f;
         a.place.positions[at] = seen + __popc(same & ((1u << lane) - 1u));
       }
     }
@@ -408,11 +486,14 @@ struct BackwardArgs {
   int vec, vec_grad;
 };
 
-// dl = p (c_e - <c, p> + 2 g1 lse / n) + the weights' part, with c_e = g0 E f(e) / n.
+// dl = p (c_e - <c, p> + 2 g1 lse / n) + the weights' part, with c_e = g0 E f(e) / n. One pass: a
+// group of lanes reads its token's logits once and writes the gradient once; all loads of a turn are
+// issued before the first is used.
 template <int F, int G, int V>
-__global__ void __launch_bounds__(32 * router_warps(V)) router_backward_kernel(BackwardArgs a) {
-  constexpr int kWarps = router_warps(V), kAtOnce = 32 / G;
-  __shared__ float s_part[kWarps][kAtOnce * G * V];  // the weights' part of each token's gradient
+__global__ void __launch_bounds__(32 * kBackwardWarps) router_backward_kernel(BackwardArgs a) {
+  constexpr int kWarps = kBackwardWarps, kAtOnce = 32 / G;
+  constexpr int kSlotTurns = (GG_ROUTER_MAX_TOP_K + G - 1) / G;
+  __shared__ __align__(16) float s_part[kWarps][kAtOnce * G * V];  // the weights' part of each token's gradient
   __shared__ float s_sum[kWarps];
   const int E = a.shape.experts, K = a.shape.top_k;
   const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
@@ -436,24 +517,35 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_backward_kernel(B
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps * kAtOnce;
   for (int64_t tb = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * kAtOnce; tb < a.tokens; tb += step) {
     const int64_t t = tb + group;
-    const bool live = t < a.tokens && a.indices[t * K] >= 0;
-    // the weights' part: slot j by lane j of the group
-    float lane_sum = 0.0f;
-    for (int j = gl; j < K; j += G) {
-      const int e = live ? a.indices[t * K + j] : -1;
-      if (e >= 0 && a.grad_weights) lane_sum = fmaf(a.weights[t * K + j], a.grad_weights[t * K + j], lane_sum);
-    }
-    const float dot_w = group_sum<G>(lane_sum);
-    for (int j = gl; j < K; j += G) {
-      const int e = live ? a.indices[t * K + j] : -1;
-      if (e >= 0 && e < E && a.grad_weights) {
-        const float w = a.weights[t * K + j];
-        part[e] = w * (a.grad_weights[t * K + j] - (a.shape.normalize ? dot_w : 0.0f));
-      }
-    }
+    const bool in = t < a.tokens;
     float v[V];
-    load_row<F, V>(a.logits, t * a.ld + e0, live ? have : 0, a.vec != 0, -INFINITY, v);
-    const float lse = live ? a.lse[t] : 0.0f;
+    load_row<F, V>(a.logits, t * a.ld + e0, in ? have : 0, a.vec != 0, -INFINITY, v);
+    // slot j of a token by lane j of its group (and j + G, ... where top_k is larger)
+    int e[kSlotTurns];
+    float w[kSlotTurns], gw[kSlotTurns];
+#pragma unroll
+    for (int i = 0; i < kSlotTurns; ++i) {
+      const int j = gl + i * G;
+      const bool slot = in && j < K;
+      e[i] = slot ? a.indices[t * K + j] : -1;
+      w[i] = slot ? a.weights[t * K + j] : 0.0f;
+      gw[i] = slot && a.grad_weights ? a.grad_weights[t * K + j] : 0.0f;
+      if (i * G + G >= K) break;
+    }
+    const float lse = in ? a.lse[t] : 0.0f;
+    const bool live = __shfl_sync(kFull, e[0], group * G) >= 0;  // a token that was routed has a first slot
+    float dot_w = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSlotTurns; ++i) {
+      if (e[i] >= 0) dot_w = fmaf(w[i], gw[i], dot_w);
+      if (i * G + G >= K) break;
+    }
+    dot_w = group_sum<G>(dot_w);
+#pragma unroll
+    for (int i = 0; i < kSlotTurns; ++i) {
+      if (e[i] >= 0 && e[i] < E) part[e[i]] = w[i] * (gw[i] - (a.shape.normalize ? dot_w : 0.0f));
+      if (i * G + G >= K) break;
+    }
     float dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -463,16 +555,22 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_backward_kernel(B
     dot = group_sum<G>(dot);
     const float common = 2.0f * g1 * inv_n * lse - dot - (a.shape.normalize ? 0.0f : dot_w);
     __syncwarp();
-    if (t < a.tokens) {
+    if (in) {
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = live ? fmaf(v[i], c[i] + common, part[e0 + i]) : 0.0f;
       const int64_t at = t * a.ldg + e0;
       if (a.vec_grad && have == V) {
+        if constexpr (F == kOutF32) {
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i) {
-          const float4 o = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-          if constexpr (F == kOutF32) store_out4<F>(static_cast<float*>(a.grad) + at + 4 * i, o);
-          else store_out4<F>(static_cast<unsigned short*>(a.grad) + at + 4 * i, o);
+          for (int i = 0; i < V / 4; ++i)
+            store_out4<F>(static_cast<float*>(a.grad) + at + 4 * i,
+                          make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < V / 8; ++i)
+            *reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.grad) + at + 8 * i) =
+                make_uint4(pack2<F>(v[8 * i], v[8 * i + 1]), pack2<F>(v[8 * i + 2], v[8 * i + 3]),
+                           pack2<F>(v[8 * i + 4], v[8 * i + 5]), pack2<F>(v[8 * i + 6], v[8 * i + 7]));
         }
       } else {
 #pragma unroll
@@ -481,9 +579,10 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_backward_kernel(B
       }
     }
     __syncwarp();
-    for (int j = gl; j < K; j += G) {
-      const int e = live ? a.indices[t * K + j] : -1;
-      if (e >= 0 && e < E) part[e] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSlotTurns; ++i) {
+      if (e[i] >= 0 && e[i] < E) part[e[i]] = 0.0f;
+      if (i * G + G >= K) break;
     }
     __syncwarp();
   }
@@ -539,10 +638,22 @@ int gg_router_create(const gg_router_config* config, gg_router** out) {
   if (!r) return cudaErrorMemoryAllocation;
   r->config = c;
   size_t warps = 0;
-  gg::with_layout(c.experts, [&](auto, auto v) { warps = gg::router_warps(v()); });
+  cudaError_t st = cudaSuccess;
+  gg::with_logits(c.logit_type, [&](auto f) {
+    gg::with_layout(c.experts, [&](auto g, auto v) {
+      warps = gg::router_warps(v());
+      // the most any router of this kernel takes: the attribute is the kernel's, not the router's
+      st = cudaFuncSetAttribute(gg::router_forward_kernel<f(), g(), v()>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                gg::kForwardSmemMost);
+    });
+  });
+  if (st != cudaSuccess) {
+    delete r;
+    return st;
+  }
   const size_t E = static_cast<size_t>(c.experts), B = gg::kMaxBlocks;
   const size_t words = B * warps * E + 2 * B * E + 2 * B;
-  cudaError_t st = cudaMalloc(&r->block, words * 4);
+  st = cudaMalloc(&r->block, words * 4);
   if (st != cudaSuccess) {
     delete r;
     return st;
@@ -585,10 +696,6 @@ int gg_router_run(gg_router* router, const gg_route* route, void* stream) {
       const size_t place = gg::place_smem(32 * warps, c.experts);
       const size_t smem = std::max(gg::forward_smem(G, V, c.experts, c.top_k), blocks == 1 ? place : 0);
       auto kernel = gg::router_forward_kernel<f(), G, V>;
-      if (smem > 48 * 1024) {
-        st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (st != cudaSuccess) return;
-      }
       kernel<<<blocks, 32 * warps, smem, s>>>(a);
       if (blocks > 1) gg::router_place_kernel<<<blocks, 32 * warps, place, s>>>(a.place);
       st = cudaGetLastError();
@@ -609,14 +716,14 @@ int gg_router_backward(const gg_router* router, const gg_route_gradient* gradien
   gg::with_logits(c.logit_type, [&](auto f) {
     gg::with_layout(c.experts, [&](auto g, auto v) {
       constexpr int G = g(), V = v();
-      constexpr int warps = gg::router_warps(V), at_once = 32 / G;
+      constexpr int warps = gg::kBackwardWarps, at_once = 32 / G;
       gg::BackwardArgs a{{c.experts, c.top_k, c.normalize != 0}, q.logits, q.indices, q.weights, q.rows, q.losses, q.lse,
                          q.grad_weights, q.grad_losses, q.grad_logits, q.tokens, q.ld, q.ld_grad,
                          gg::rows_aligned(q.logits, q.ld, c.logit_type),
                          gg::rows_aligned(q.grad_logits, q.ld_grad, c.logit_type)};
       const int64_t blocks = (static_cast<int64_t>(q.tokens) + warps * at_once - 1) / (warps * at_once);
       gg::router_backward_kernel<f(), G, V>
-          <<<static_cast<int>(std::min<int64_t>(blocks, 4 * gg::kMaxBlocks)), 32 * warps, 0, s>>>(a);
+          <<<static_cast<int>(std::min<int64_t>(blocks, 8 * gg::kMaxBlocks)), 32 * warps, 0, s>>>(a);
     });
   });
   return cudaGetLastError();

@@ -15,26 +15,33 @@ constructors and tensor mismatches raise ValueError.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Sequence
 
 from . import capi
 
 _types = {}  # torch dtype -> GG_OUTPUT_*
-_ints = None
+_f32 = _i32 = None
+_masks = ()
+
+# The checks below run before every launch, which a decoding step makes some ten of: each reads an attribute of a
+# tensor once (some 50 to 100 ns apiece), and the C structs are filled by one struct.pack.
+_ROUTE = struct.Struct("@10P2i")
+_ROUTE_GRADIENT = struct.Struct("@9P3i4x")
 
 
 def _load_types():
-    global _ints
+    global _f32, _i32, _masks
     import torch
 
     _types[torch.float32] = capi.GG_OUTPUT_F32
     _types[torch.float16] = capi.GG_OUTPUT_F16
     _types[torch.bfloat16] = capi.GG_OUTPUT_BF16
-    _ints = (torch.float32, torch.int32, torch.uint8, torch.bool)
+    _f32, _i32, _masks = torch.float32, torch.int32, (torch.uint8, torch.bool)
 
 
 def _type_of(t, name: str) -> int:
-    if not _types:
+    if _f32 is None:
         _load_types()
     v = _types.get(t.dtype)
     if v is None:
@@ -50,26 +57,27 @@ def _stream(stream) -> Optional[int]:
     return getattr(stream, "cuda_stream", None) or None
 
 
-def _rows_of(t, rows: int, cols: int, name: str) -> int:
+def _shape(t, name: str):
+    s = t.shape
+    if len(s) != 2:
+        raise ValueError(f"{name}: two dimensions expected, got {tuple(s)}")
+    return s
+
+
+def _pitch(t, rows: int, cols: int, name: str) -> int:
     """The row pitch of a rows x cols device tensor with contiguous columns."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+    if t.shape != (rows, cols):
         raise ValueError(f"{name}: shape ({rows}, {cols}) expected, got {tuple(t.shape)}")
     r, c = t.stride()
-    if cols > 1 and c != 1:
-        raise ValueError(f"{name}: columns must be contiguous")
-    if rows > 1 and r < cols:
-        raise ValueError(f"{name}: rows overlap")
-    if not t.is_cuda:
-        raise ValueError(f"{name}: a CUDA tensor expected")
+    if (c != 1 and cols > 1) or (r < cols and rows > 1) or not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor with contiguous columns and rows that do not overlap expected")
     return r if r >= cols and r > 0 else max(1, cols)
 
 
-def _packed(t, count: int, kind: int, name: str) -> int:
-    """The address of a contiguous device tensor of `count` elements of the given kind (0 float32, 1 int32)."""
-    if _ints is None:
-        _load_types()
-    if t.dtype is not _ints[kind] or t.numel() != count or not t.is_contiguous() or not t.is_cuda:
-        raise ValueError(f"{name}: a contiguous CUDA {_ints[kind]} tensor of {count} elements expected, got "
+def _packed(t, count: int, dtype, name: str) -> int:
+    """The address of a contiguous device tensor of `count` elements."""
+    if t.dtype is not dtype or t.numel() != count or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError(f"{name}: a contiguous CUDA {dtype} tensor of {count} elements expected, got "
                          f"{t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
@@ -103,23 +111,23 @@ class MoeRouter:
         (tokens), zero where a token is not routed."""
         if not self._h:
             return capi.CUDA_ERROR_INVALID_DEVICE_POINTER
-        t, e = logits.shape[0], self.experts
-        slots = t * self.top_k
         if _type_of(logits, "logits") != self.logit_type:
             raise ValueError(f"logits: the router was made for another type than {logits.dtype}")
-        ld = _rows_of(logits, t, e, "logits")
-        mask = None
+        t, e = _shape(logits, "logits")[0], self.experts
+        slots = t * self.top_k
+        ld = _pitch(logits, t, e, "logits")
+        mask = 0
         if token_mask is not None:
-            if token_mask.dtype not in _ints[2:] or token_mask.numel() != t or not token_mask.is_contiguous() or not token_mask.is_cuda:
+            if token_mask.dtype not in _masks or token_mask.numel() != t or not token_mask.is_contiguous() or not token_mask.is_cuda:
                 raise ValueError("token_mask: one contiguous CUDA uint8 or bool per token expected")
             mask = token_mask.data_ptr()
-        q = capi.GGRoute(logits.data_ptr(), mask, _packed(indices, slots, 1, "indices"),
-                         _packed(weights, slots, 0, "weights"), _packed(positions, slots, 1, "positions"),
-                         _packed(rows, e, 1, "rows"), _packed(losses, 3, 0, "losses"),
-                         None if row_tokens is None else _packed(row_tokens, slots, 1, "row_tokens"),
-                         None if lse is None else _packed(lse, t, 0, "lse"),
-                         None if prob_mean is None else _packed(prob_mean, e, 0, "prob_mean"), t, ld)
-        return self._lib.gg_router_run(self._h, ctypes.byref(q), _stream(stream))
+        q = _ROUTE.pack(logits.data_ptr(), mask, _packed(indices, slots, _i32, "indices"),
+                        _packed(weights, slots, _f32, "weights"), _packed(positions, slots, _i32, "positions"),
+                        _packed(rows, e, _i32, "rows"), _packed(losses, 3, _f32, "losses"),
+                        0 if row_tokens is None else _packed(row_tokens, slots, _i32, "row_tokens"),
+                        0 if lse is None else _packed(lse, t, _f32, "lse"),
+                        0 if prob_mean is None else _packed(prob_mean, e, _f32, "prob_mean"), t, ld)
+        return self._lib.gg_router_run(self._h, q, _stream(stream))
 
     def backward(self, logits, indices, weights, rows, losses, lse, grad_weights, grad_losses, grad_logits,
                  stream=None) -> int:
@@ -127,19 +135,18 @@ class MoeRouter:
         top_k, or None) and of losses[0] and losses[1] (float32, 2, or None)."""
         if not self._h:
             return capi.CUDA_ERROR_INVALID_DEVICE_POINTER
-        t, e = logits.shape[0], self.experts
-        slots = t * self.top_k
         if _type_of(logits, "logits") != self.logit_type or grad_logits.dtype is not logits.dtype:
             raise ValueError("logits, grad_logits: the router's type expected")
-        ld = _rows_of(logits, t, e, "logits")
-        ldg = _rows_of(grad_logits, t, e, "grad_logits")
-        q = capi.GGRouteGradient(logits.data_ptr(), _packed(indices, slots, 1, "indices"),
-                                 _packed(weights, slots, 0, "weights"), _packed(rows, e, 1, "rows"),
-                                 _packed(losses, 3, 0, "losses"), _packed(lse, t, 0, "lse"),
-                                 None if grad_weights is None else _packed(grad_weights, slots, 0, "grad_weights"),
-                                 None if grad_losses is None else _packed(grad_losses, 2, 0, "grad_losses"),
+        t, e = _shape(logits, "logits")[0], self.experts
+        slots = t * self.top_k
+        ld, ldg = _pitch(logits, t, e, "logits"), _pitch(grad_logits, t, e, "grad_logits")
+        q = _ROUTE_GRADIENT.pack(logits.data_ptr(), _packed(indices, slots, _i32, "indices"),
+                                 _packed(weights, slots, _f32, "weights"), _packed(rows, e, _i32, "rows"),
+                                 _packed(losses, 3, _f32, "losses"), _packed(lse, t, _f32, "lse"),
+                                 0 if grad_weights is None else _packed(grad_weights, slots, _f32, "grad_weights"),
+                                 0 if grad_losses is None else _packed(grad_losses, 2, _f32, "grad_losses"),
                                  grad_logits.data_ptr(), t, ld, ldg)
-        return self._lib.gg_router_backward(self._h, ctypes.byref(q), _stream(stream))
+        return self._lib.gg_router_backward(self._h, q, _stream(stream))
 
     def close(self):
         if self._h:
@@ -154,53 +161,55 @@ class MoeRouter:
 
 
 def _slots(positions, tokens: int) -> int:
-    if positions.dim() != 2 or positions.shape[0] != tokens:
-        raise ValueError(f"positions: ({tokens}, top_k) expected, got {tuple(positions.shape)}")
-    return positions.shape[1]
+    t, k = _shape(positions, "positions")
+    if t != tokens:
+        raise ValueError(f"positions: ({tokens}, top_k) expected, got ({t}, {k})")
+    return k
 
 
 def moe_dispatch(x, positions, packed, stream=None) -> int:
     """packed[positions[t, j]] = x[t]: x (tokens, width), packed (rows, width), of one dtype of 1, 2 or 4
     bytes; positions (tokens, top_k) int32, entries outside packed's rows go nowhere."""
-    t, w = x.shape
+    if _f32 is None:
+        _load_types()
+    t, w = _shape(x, "x")
     k = _slots(positions, t)
     if packed.dtype is not x.dtype:
         raise ValueError("x, packed: one dtype expected")
-    pos = _packed(positions, t * k, 1, "positions")
-    r = packed.shape[0]
-    ldx, ldp = _rows_of(x, t, w, "x"), _rows_of(packed, r, w, "packed")
-    return capi.load().gg_moe_dispatch(x.data_ptr(), ldx, pos, t, k, w, x.element_size(), packed.data_ptr(), r, ldp,
-                                       _stream(stream))
+    r = _shape(packed, "packed")[0]
+    ldx, ldp = _pitch(x, t, w, "x"), _pitch(packed, r, w, "packed")
+    return capi.load().gg_moe_dispatch(x.data_ptr(), ldx, _packed(positions, t * k, _i32, "positions"), t, k, w,
+                                       x.element_size(), packed.data_ptr(), r, ldp, _stream(stream))
 
 
 def moe_combine(packed, positions, out, weights=None, stream=None) -> int:
     """out[t] = sum over j of weights[t, j] * packed[positions[t, j]] (weights None: 1, the gradient of
     moe_dispatch); weights float32 (tokens, top_k)."""
-    t, w = out.shape
+    pt, ot = _type_of(packed, "packed"), _type_of(out, "out")
+    t, w = _shape(out, "out")
     k = _slots(positions, t)
-    pos = _packed(positions, t * k, 1, "positions")
-    wts = None if weights is None else _packed(weights, t * k, 0, "weights")
-    r = packed.shape[0]
-    ldp, ldo = _rows_of(packed, r, w, "packed"), _rows_of(out, t, w, "out")
-    return capi.load().gg_moe_combine(packed.data_ptr(), _type_of(packed, "packed"), r, ldp, pos, wts, t, k, w,
-                                      out.data_ptr(), _type_of(out, "out"), ldo, _stream(stream))
+    r = _shape(packed, "packed")[0]
+    ldp, ldo = _pitch(packed, r, w, "packed"), _pitch(out, t, w, "out")
+    return capi.load().gg_moe_combine(packed.data_ptr(), pt, r, ldp, _packed(positions, t * k, _i32, "positions"),
+                                      None if weights is None else _packed(weights, t * k, _f32, "weights"), t, k, w,
+                                      out.data_ptr(), ot, ldo, _stream(stream))
 
 
 def moe_combine_backward(grad_out, packed, positions, weights, grad_packed, grad_weights, stream=None) -> int:
     """The gradients of moe_combine with weights: grad_packed (like packed) and grad_weights (float32,
     tokens x top_k)."""
-    t, w = grad_out.shape
+    ot, pt = _type_of(grad_out, "grad_out"), _type_of(packed, "packed")
+    t, w = _shape(grad_out, "grad_out")
     k = _slots(positions, t)
-    pos = _packed(positions, t * k, 1, "positions")
-    r = packed.shape[0]
+    r = _shape(packed, "packed")[0]
     if grad_packed.dtype is not packed.dtype:
         raise ValueError("packed, grad_packed: one dtype expected")
-    ldo, ldp = _rows_of(grad_out, t, w, "grad_out"), _rows_of(packed, r, w, "packed")
-    ldgp = _rows_of(grad_packed, r, w, "grad_packed")
+    ldo, ldp, ldgp = (_pitch(grad_out, t, w, "grad_out"), _pitch(packed, r, w, "packed"),
+                      _pitch(grad_packed, r, w, "grad_packed"))
     return capi.load().gg_moe_combine_backward(
-        grad_out.data_ptr(), _type_of(grad_out, "grad_out"), ldo, packed.data_ptr(), _type_of(packed, "packed"), r, ldp,
-        pos, _packed(weights, t * k, 0, "weights"), t, k, w, grad_packed.data_ptr(), ldgp,
-        _packed(grad_weights, t * k, 0, "grad_weights"), _stream(stream))
+        grad_out.data_ptr(), ot, ldo, packed.data_ptr(), pt, r, ldp, _packed(positions, t * k, _i32, "positions"),
+        _packed(weights, t * k, _f32, "weights"), t, k, w, grad_packed.data_ptr(), ldgp,
+        _packed(grad_weights, t * k, _f32, "grad_weights"), _stream(stream))
 
 
 class Q4Plan:
@@ -247,11 +256,11 @@ class Q4Plan:
             raise ValueError(f"a: the plan was made for another type than {a.dtype}")
         if _type_of(d, "d") != self.output_type:
             raise ValueError(f"d: the plan was made for another type than {d.dtype}")
-        ar, cap = a.shape[0], d.shape[0]
-        lda, ldd = _rows_of(a, ar, self.k, "a"), _rows_of(d, cap, self.n, "d")
+        ar, cap = _shape(a, "a")[0], _shape(d, "d")[0]
+        lda, ldd = _pitch(a, ar, self.k, "a"), _pitch(d, cap, self.n, "d")
         return self._lib.gg_q4_plan_run(
-            self._h, a.data_ptr(), lda, ar, None if row_tokens is None else _packed(row_tokens, cap, 1, "row_tokens"),
-            None if rows is None else _packed(rows, self.experts, 1, "rows"), d.data_ptr(), ldd, cap, _stream(stream))
+            self._h, a.data_ptr(), lda, ar, None if row_tokens is None else _packed(row_tokens, cap, _i32, "row_tokens"),
+            None if rows is None else _packed(rows, self.experts, _i32, "rows"), d.data_ptr(), ldd, cap, _stream(stream))
 
     def status(self) -> int:
         """Synchronises; returns (then clears) the GG_STATUS_* bits of the plan's runs."""
