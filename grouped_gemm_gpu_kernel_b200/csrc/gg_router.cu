@@ -60,6 +60,15 @@ __device__ __forceinline__ int group_max(int v) {
   }
 }
 
+// exp(x) for x <= 0: 2^-22 + |x| 2^-24 relative (the exponential unit, and the scaled argument's
+// rounding), and 0 below 2^-126. expf() costs four times the instructions for 2^-23, which a softmax
+// over logits rounded to 16 or 24 bits has no use for.
+__device__ __forceinline__ float exp_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
@@ -99,18 +108,25 @@ __device__ __forceinline__ void load_row(const void* base, int64_t at, int have,
 
 // Warps of a forward block (one block an SM): as many as the registers of V experts a lane allow.
 __host__ __device__ constexpr int router_warps(int V) { return V <= 8 ? 32 : V <= 16 ? 16 : 8; }
+constexpr int kFewWarps = 4;  // of a forward block that takes few tokens
 constexpr int kBackwardWarps = 8;
+constexpr int kBackwardBlocks = 4;  // of them an SM: the grid is one wave, and a warp walks its tokens
 
 constexpr int kForwardSmemMost = 160 * 1024;
 constexpr int kCandidates = 64;  // see choose_of_candidates
 
+// Slots a warp gathers before it places them: 32 (one a lane) or, where its tokens of one turn have more,
+// theirs. At least one turn, at most 32 tokens.
+__host__ __device__ __forceinline__ int slots_held(int at_once, int top_k) {
+  return at_once * top_k > 32 ? at_once * top_k : 32;
+}
+
 // Shared memory of a forward block, in 4-byte words: counts [warps][experts], sums of p
-// [warps][experts], slots (index and key) [warps][tokens a warp takes at once][top_k], the factor
-// of the weights and the largest logit per such token, and z and valid tokens per warp; where a
-// warp takes one token at once, its candidates (key and expert).
-size_t forward_smem(int G, int V, int experts, int top_k) {
-  const int warps = router_warps(V), at_once = 32 / G;
-  return 4ull * (2ull * warps * experts + warps * at_once * (2ull * top_k + 2) + 2ull * warps +
+// [warps][experts], per warp the held slots (index and key) and the factor of the weights and the
+// largest logit of their tokens (32 at most), z and valid tokens per warp; where a warp takes one
+// token at once, its candidates (key and expert).
+size_t forward_smem(int G, int warps, int experts, int top_k) {
+  return 4ull * (2ull * warps * experts + warps * (2ull * slots_held(32 / G, top_k) + 64) + 2ull * warps +
                  (G == 32 ? 2ull * warps * kCandidates : 0));
 }
 
@@ -120,7 +136,7 @@ __host__ __device__ __forceinline__ int place_parts(int threads, int experts) {
   return p < 1 ? 1 : p > 16 ? 16 : p;
 }
 size_t place_smem(int threads, int experts) {
-  return 4ull * ((3ull * place_parts(threads, experts) + 2) * experts + 64);
+  return 4ull * ((3ull * place_parts(threads, experts) + 2 + threads / 32) * experts + 64);
 }
 
 struct PlaceArgs {
@@ -220,16 +236,29 @@ __device__ void place_block(const PlaceArgs& a, int block, unsigned char* smem) 
   const int64_t unit = static_cast<int64_t>(block) * warps + warp;
   const int64_t t0 = min(static_cast<int64_t>(a.tokens), unit * a.tokens_per_warp);
   const int64_t t1 = min(static_cast<int64_t>(a.tokens), t0 + a.tokens_per_warp);
-  const int* before = a.work.warp_before + unit * E;
-#pragma unroll 4
-  for (int64_t s = t0 * K + lane; s < t1 * K; s += 32) {
-    const int e = a.indices[s];
-    int p = -1;
-    if (e >= 0) {
-      p = s_base[e] + before[e] + a.positions[s];
-      if (a.row_tokens) a.row_tokens[p] = static_cast<int>(s / K);
+  int* first = reinterpret_cast<int*>(s_warp + 64) + warp * E;  // of every expert, the first row of this warp
+  for (int e = lane; e < E; e += 32) first[e] = s_base[e] + a.work.warp_before[unit * E + e];
+  __syncwarp();
+  constexpr int kBatch = 8;  // slots a lane loads before it stores the first
+  for (int64_t s0 = t0 * K + lane; s0 < t1 * K; s0 += 32 * kBatch) {
+    int e[kBatch], rank[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int64_t s = s0 + 32 * i;
+      e[i] = s < t1 * K ? a.indices[s] : -1;
+      rank[i] = s < t1 * K ? a.positions[s] : 0;
     }
-    a.positions[s] = p;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int64_t s = s0 + 32 * i;
+      if (s >= t1 * K) break;
+      int p = -1;
+      if (e[i] >= 0) {
+        p = first[e[i]] + rank[i];
+        if (a.row_tokens) a.row_tokens[p] = static_cast<int>(static_cast<unsigned>(s) / static_cast<unsigned>(K));
+      }
+      a.positions[s] = p;
+    }
   }
   if (a.row_tokens) {
     const int64_t slots = static_cast<int64_t>(a.tokens) * K;
@@ -283,17 +312,21 @@ __device__ __forceinline__ bool choose_of_candidates(const int (&key)[V], int mi
   int bound = max(mine, __shfl_xor_sync(kFull, mine, 1));
   bound = max(bound, __shfl_xor_sync(kFull, bound, 2));
   bound = max(__reduce_min_sync(kFull, bound), kClosed + 1);
-  int n = 0;
-  const unsigned lower = (1u << lane) - 1u;
+  unsigned in = 0;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const bool in = key[i] >= bound;
-    const unsigned who = __ballot_sync(kFull, in);
-    const int at = n + __popc(who & lower);
-    if (in && at < kCandidates) s_candidates[at] = make_int2(key[i], e0 + i);
-    n += __popc(who);
+  for (int i = 0; i < V; ++i) in |= key[i] >= bound ? 1u << i : 0u;
+  int upto = __popc(in);
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(kFull, upto, d);
+    upto += lane >= d ? up : 0;
   }
+  const int n = __shfl_sync(kFull, upto, 31);
   if (n > kCandidates) return false;
+  int2* to = s_candidates + upto - __popc(in);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (in >> i & 1u) *to++ = make_int2(key[i], e0 + i);
   __syncwarp();
   int2 a = make_int2(kTaken, INT32_MAX), b = a;
   if (lane < n) a = s_candidates[lane];
@@ -310,20 +343,21 @@ __device__ __forceinline__ bool choose_of_candidates(const int (&key)[V], int mi
   return true;
 }
 
-template <int F, int G, int V>
-__global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(ForwardArgs a) {
+template <int F, int G, int V, int W>
+__global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
-  constexpr int kWarps = router_warps(V), kAtOnce = 32 / G;
+  constexpr int kWarps = W, kAtOnce = 32 / G;
   const int E = a.place.shape.experts, K = a.place.shape.top_k, T = a.place.tokens;
   const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
   const int group = lane / G, gl = lane % G;
   int2* s_candidates = reinterpret_cast<int2*>(smem) + warp * kCandidates;
   int* s_count = reinterpret_cast<int*>(smem + (G == 32 ? 8 * kWarps * kCandidates : 0));
   float* s_prob = reinterpret_cast<float*>(s_count + kWarps * E);
-  int* s_slot = reinterpret_cast<int*>(s_prob + kWarps * E) + warp * kAtOnce * (2 * K + 2);
-  int* s_key = s_slot + kAtOnce * K;
-  float* s_factor = reinterpret_cast<float*>(s_key + kAtOnce * K);  // [kAtOnce] factor, then [kAtOnce] largest logit
-  float* s_z = s_prob + kWarps * E + kWarps * kAtOnce * (2 * K + 2);
+  const int held = slots_held(kAtOnce, K);  // slots a warp keeps until it places them together
+  int* s_slot = reinterpret_cast<int*>(s_prob + kWarps * E) + warp * (2 * held + 64);
+  int* s_key = s_slot + held;
+  float* s_factor = reinterpret_cast<float*>(s_key + held);  // [32] factors of the weights, then [32] largest logits
+  float* s_z = s_prob + kWarps * E + kWarps * (2 * held + 64);
   int* count = s_count + warp * E;
   for (int e = lane; e < E; e += 32) count[e] = 0;
   __syncwarp();
@@ -338,8 +372,14 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(Fo
   for (int i = 0; i < V; ++i) prob[i] = 0.0f;
   float z = 0.0f, n = 0.0f;
 
+  // Tokens held at a time: as many whole turns as fill the lanes with slots. The first of them is th.
+  const int turns = max(1, 32 / (kAtOnce * K));
+  const int lane_token = lane / K;  // the held token of this lane's slot among the first 32
+  int turn = 0;
+  int64_t th = t0;
   for (int64_t tb = t0; tb < t1; tb += kAtOnce) {
     const int64_t t = tb + group;
+    const int slot0 = (turn * kAtOnce + group) * K;
     const bool live = t < t1 && (a.mask == nullptr || a.mask[t] != 0);
     float v[V];
     int key[V];
@@ -359,8 +399,8 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(Fo
         int slot_expert = -1, slot_key = kTaken;
         done = choose_of_candidates<V>(key, mine, e0, K, s_candidates, lane, &slot_expert, &slot_key);
         if (done) {
-          if (lane < K) s_slot[lane] = slot_expert, s_key[lane] = slot_key;
-          chosen = group_sum<32>(slot_expert >= 0 ? __expf(key_value(slot_key) - top) : 0.0f);
+          if (lane < K) s_slot[slot0 + lane] = slot_expert, s_key[slot0 + lane] = slot_key;
+          chosen = group_sum<32>(slot_expert >= 0 ? exp_fast(key_value(slot_key) - top) : 0.0f);
         }
       }
     }
@@ -370,15 +410,15 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(Fo
         const unsigned holders = __ballot_sync(kFull, mine == best);
         const unsigned of_group = G == 32 ? holders : (holders >> (group * G)) & ((1u << (G & 31)) - 1u);
         const int owner = __ffs(of_group) - 1;  // experts are in lane order: the lowest lane has the lowest expert
-        if (best > kClosed) chosen += __expf(key_value(best) - top);
+        if (best > kClosed) chosen += exp_fast(key_value(best) - top);
         if (gl == owner) {
           int at = 0;
 #pragma unroll
           for (int i = V - 1; i >= 0; --i) at = key[i] == best ? i : at;
 #pragma unroll
           for (int i = 0; i < V; ++i) key[i] = i == at ? kTaken : key[i];
-          s_slot[group * K + j] = best > kClosed ? e0 + at : -1;
-          s_key[group * K + j] = best;
+          s_slot[slot0 + j] = best > kClosed ? e0 + at : -1;
+          s_key[slot0 + j] = best;
         }
         if (j + 1 == K) break;
         mine = key[0];
@@ -391,24 +431,25 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(Fo
     float ex[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      ex[i] = i < have && valid ? __expf(v[i] - top) : 0.0f;
+      ex[i] = i < have && valid ? exp_fast(v[i] - top) : 0.0f;
       sum += ex[i];
     }
     sum = group_sum<G>(sum);
-    const float inv = valid ? 1.0f / sum : 0.0f;
+    const float inv = valid ? __fdividef(1.0f, sum) : 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) prob[i] = fmaf(ex[i], inv, prob[i]);
-    const float lse = valid ? top + logf(sum) : 0.0f;
+    const float lse = valid ? top + __logf(sum) : 0.0f;
     if (gl == 0) {
       z = fmaf(lse, lse, z);
       n += valid ? 1.0f : 0.0f;
       if (a.lse && t < t1) a.lse[t] = lse;
-      s_factor[group] = a.place.shape.normalize ? 1.0f / chosen : inv;
-      s_factor[kAtOnce + group] = top;
+      s_factor[turn * kAtOnce + group] = a.place.shape.normalize ? __fdividef(1.0f, chosen) : inv;
+      s_factor[32 + turn * kAtOnce + group] = top;
     }
     __syncwarp();
-    // the slots of these tokens, in order: 32 at a time
-    const int slots = static_cast<int>(min(static_cast<int64_t>(kAtOnce), t1 - tb)) * K;
+    if (++turn < turns && tb + kAtOnce < t1) continue;
+    // the slots of the held tokens, in order, 32 at a time
+    const int slots = static_cast<int>(min(t1, tb + kAtOnce) - th) * K;
     for (int s0 = 0; s0 < slots; s0 += 32) {
       const int s = s0 + lane;
       const int e = s < slots ? s_slot[s] : -1;
@@ -418,14 +459,16 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(Fo
       if (e >= 0 && lane == 31 - __clz(same)) count[e] = seen + __popc(same);
       __syncwarp();
       if (s < slots) {
-        const int g = s / K;
-        const int64_t at = tb * K + s;
+        const int h = s0 == 0 ? lane_token : s / K;
+        const int64_t at = th * K + s;
         a.indices[at] = e;
-        a.weights[at] = e >= 0 ? __expf(key_value(s_key[s]) - s_factor[kAtOnce + g]) * s_factor[g] : 0.0f;
+        a.weights[at] = e >= 0 ? exp_fast(key_value(s_key[s]) - s_factor[32 + h]) * s_factor[h] : 0.0f;
         a.place.positions[at] = seen + __popc(same & ((1u << lane) - 1u));
       }
     }
     __syncwarp();
+    turn = 0;
+    th = tb + kAtOnce;
   }
 
   // the block's sums: over the groups of a warp, then over the warps
@@ -442,6 +485,7 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(Fo
       if (i < have) s_prob[warp * E + e0 + i] = prob[i];
   if (lane == 0) s_z[2 * warp] = z, s_z[2 * warp + 1] = n;
   __syncthreads();
+  cudaTriggerProgrammaticLaunchCompletion();
   const RouterWork& w = a.place.work;
   for (int e = tid; e < E; e += 32 * kWarps) {
     int run = 0;
@@ -465,8 +509,11 @@ __global__ void __launch_bounds__(32 * router_warps(V)) router_forward_kernel(Fo
   }
 }
 
-__global__ void router_place_kernel(PlaceArgs a) {
+// Launched so that its blocks may be set up while the forward kernel ends; nothing is read before the
+// forward kernel's writes are there.
+__global__ void __launch_bounds__(1024) router_place_kernel(PlaceArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
+  cudaGridDependencySynchronize();
   place_block(a, static_cast<int>(blockIdx.x), smem);
 }
 
@@ -490,10 +537,12 @@ struct BackwardArgs {
 // group of lanes reads its token's logits once and writes the gradient once; all loads of a turn are
 // issued before the first is used.
 template <int F, int G, int V>
-__global__ void __launch_bounds__(32 * kBackwardWarps) router_backward_kernel(BackwardArgs a) {
+__global__ void __launch_bounds__(32 * kBackwardWarps, V == 8 ? kBackwardBlocks : 1) router_backward_kernel(BackwardArgs a) {
   constexpr int kWarps = kBackwardWarps, kAtOnce = 32 / G;
   constexpr int kSlotTurns = (GG_ROUTER_MAX_TOP_K + G - 1) / G;
-  __shared__ __align__(16) float s_part[kWarps][kAtOnce * G * V];  // the weights' part of each token's gradient
+  // the weights' part of each token's gradient: expert v of a lane at [v / 4][lane][v % 4], so that a lane
+  // reads its experts four at a time and no two lanes of a quarter warp meet in a bank
+  __shared__ float4 s_part[kWarps][V / 4][32];
   __shared__ float s_sum[kWarps];
   const int E = a.shape.experts, K = a.shape.top_k;
   const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
@@ -509,17 +558,22 @@ __global__ void __launch_bounds__(32 * kBackwardWarps) router_backward_kernel(Ba
   float c[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) c[i] = i < have ? scale * static_cast<float>(a.rows[e0 + i]) : 0.0f;
-  float* part = s_part[warp] + group * G * V;
+  float* part = reinterpret_cast<float*>(s_part[warp]);
+  const auto place = [&](int e) { return (e % V / 4 * 32 + group * G + e / V) * 4 + e % 4; };
 #pragma unroll
-  for (int i = 0; i < V; ++i) part[e0 + i] = 0.0f;
+  for (int i = 0; i < V / 4; ++i) s_part[warp][i][lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   __syncwarp();
 
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps * kAtOnce;
-  for (int64_t tb = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * kAtOnce; tb < a.tokens; tb += step) {
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * kAtOnce;
+  float next[V];
+  load_row<F, V>(a.logits, (first + group) * a.ld + e0, first + group < a.tokens ? have : 0, a.vec != 0, -INFINITY, next);
+  for (int64_t tb = first; tb < a.tokens; tb += step) {
     const int64_t t = tb + group;
     const bool in = t < a.tokens;
     float v[V];
-    load_row<F, V>(a.logits, t * a.ld + e0, in ? have : 0, a.vec != 0, -INFINITY, v);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = next[i];
     // slot j of a token by lane j of its group (and j + G, ... where top_k is larger)
     int e[kSlotTurns];
     float w[kSlotTurns], gw[kSlotTurns];
@@ -533,6 +587,7 @@ __global__ void __launch_bounds__(32 * kBackwardWarps) router_backward_kernel(Ba
       if (i * G + G >= K) break;
     }
     const float lse = in ? a.lse[t] : 0.0f;
+    load_row<F, V>(a.logits, (t + step) * a.ld + e0, t + step < a.tokens ? have : 0, a.vec != 0, -INFINITY, next);
     const bool live = __shfl_sync(kFull, e[0], group * G) >= 0;  // a token that was routed has a first slot
     float dot_w = 0.0f;
 #pragma unroll
@@ -543,13 +598,13 @@ __global__ void __launch_bounds__(32 * kBackwardWarps) router_backward_kernel(Ba
     dot_w = group_sum<G>(dot_w);
 #pragma unroll
     for (int i = 0; i < kSlotTurns; ++i) {
-      if (e[i] >= 0 && e[i] < E) part[e[i]] = w[i] * (gw[i] - (a.shape.normalize ? dot_w : 0.0f));
+      if (e[i] >= 0 && e[i] < E) part[place(e[i])] = w[i] * (gw[i] - (a.shape.normalize ? dot_w : 0.0f));
       if (i * G + G >= K) break;
     }
     float dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      v[i] = i < have && live ? __expf(v[i] - lse) : 0.0f;
+      v[i] = i < have && live ? exp_fast(v[i] - lse) : 0.0f;
       dot = fmaf(c[i], v[i], dot);
     }
     dot = group_sum<G>(dot);
@@ -557,7 +612,12 @@ __global__ void __launch_bounds__(32 * kBackwardWarps) router_backward_kernel(Ba
     __syncwarp();
     if (in) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = live ? fmaf(v[i], c[i] + common, part[e0 + i]) : 0.0f;
+      for (int i = 0; i < V / 4; ++i) {
+        const float4 p = s_part[warp][i][lane];
+        const float q[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[4 * i + x] = live ? fmaf(v[4 * i + x], c[4 * i + x] + common, q[x]) : 0.0f;
+      }
       const int64_t at = t * a.ldg + e0;
       if (a.vec_grad && have == V) {
         if constexpr (F == kOutF32) {
@@ -581,7 +641,7 @@ __global__ void __launch_bounds__(32 * kBackwardWarps) router_backward_kernel(Ba
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < kSlotTurns; ++i) {
-      if (e[i] >= 0 && e[i] < E) part[e[i]] = 0.0f;
+      if (e[i] >= 0 && e[i] < E) part[place(e[i])] = 0.0f;
       if (i * G + G >= K) break;
     }
     __syncwarp();
@@ -641,12 +701,15 @@ int gg_router_create(const gg_router_config* config, gg_router** out) {
   cudaError_t st = cudaSuccess;
   gg::with_logits(c.logit_type, [&](auto f) {
     gg::with_layout(c.experts, [&](auto g, auto v) {
-      warps = gg::router_warps(v());
+      constexpr int W = gg::router_warps(v());
+      warps = W;
       // the most any router of this kernel takes: the attribute is the kernel's, not the router's
-      st = cudaFuncSetAttribute(gg::router_forward_kernel<f(), g(), v()>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      st = cudaFuncSetAttribute(gg::router_forward_kernel<f(), g(), v(), W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 gg::kForwardSmemMost);
     });
   });
+  if (st == cudaSuccess)
+    st = cudaFuncSetAttribute(gg::router_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gg::kForwardSmemMost);
   if (st != cudaSuccess) {
     delete r;
     return st;
@@ -677,28 +740,45 @@ int gg_router_run(gg_router* router, const gg_route* route, void* stream) {
   cudaError_t st = cudaSuccess;
   gg::with_logits(c.logit_type, [&](auto f) {
     gg::with_layout(c.experts, [&](auto g, auto v) {
-      constexpr int G = g(), V = v();
-      constexpr int warps = gg::router_warps(V), at_once = 32 / G;
-      // tokens a warp: whole turns, as few as fill the blocks
-      const int64_t share = (static_cast<int64_t>(q.tokens) + gg::kMaxBlocks * warps - 1) / (gg::kMaxBlocks * warps);
-      const int64_t per_warp = std::max<int64_t>(1, (share + at_once - 1) / at_once) * at_once;
-      const int blocks = static_cast<int>(std::max<int64_t>(1, (q.tokens + per_warp * warps - 1) / (per_warp * warps)));
-      gg::ForwardArgs a{};
-      a.logits = q.logits;
-      a.mask = q.token_mask;
-      a.indices = q.indices;
-      a.weights = q.weights;
-      a.lse = q.lse;
-      a.ld = q.ld;
-      a.vec = gg::rows_aligned(q.logits, q.ld, c.logit_type);
-      a.place = {{c.experts, c.top_k, c.normalize != 0}, router->work, q.tokens, static_cast<int>(per_warp), blocks,
-                 q.indices, q.positions, q.rows, q.row_tokens, q.prob_mean, q.losses};
-      const size_t place = gg::place_smem(32 * warps, c.experts);
-      const size_t smem = std::max(gg::forward_smem(G, V, c.experts, c.top_k), blocks == 1 ? place : 0);
-      auto kernel = gg::router_forward_kernel<f(), G, V>;
-      kernel<<<blocks, 32 * warps, smem, s>>>(a);
-      if (blocks > 1) gg::router_place_kernel<<<blocks, 32 * warps, place, s>>>(a.place);
-      st = cudaGetLastError();
+      constexpr int G = g(), V = v(), at_once = 32 / G;
+      const auto launch = [&](auto warps_c) {
+        constexpr int warps = warps_c();
+        // tokens a warp: whole turns, as few as fill the blocks
+        const int64_t share = (static_cast<int64_t>(q.tokens) + gg::kMaxBlocks * warps - 1) / (gg::kMaxBlocks * warps);
+        const int64_t per_warp = std::max<int64_t>(1, (share + at_once - 1) / at_once) * at_once;
+        const int blocks = static_cast<int>(std::max<int64_t>(1, (q.tokens + per_warp * warps - 1) / (per_warp * warps)));
+        gg::ForwardArgs a{};
+        a.logits = q.logits;
+        a.mask = q.token_mask;
+        a.indices = q.indices;
+        a.weights = q.weights;
+        a.lse = q.lse;
+        a.ld = q.ld;
+        a.vec = gg::rows_aligned(q.logits, q.ld, c.logit_type);
+        a.place = {{c.experts, c.top_k, c.normalize != 0}, router->work, q.tokens, static_cast<int>(per_warp), blocks,
+                   q.indices, q.positions, q.rows, q.row_tokens, q.prob_mean, q.losses};
+        const size_t place = gg::place_smem(32 * warps, c.experts);
+        const size_t forward = gg::forward_smem(G, warps, c.experts, c.top_k);
+        gg::router_forward_kernel<f(), G, V, warps>
+            <<<blocks, 32 * warps, blocks == 1 ? std::max(place, forward) : forward, s>>>(a);
+        st = cudaGetLastError();
+        if (st != cudaSuccess || blocks == 1) return;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+        cfg.blockDim = dim3(32 * warps);
+        cfg.dynamicSmemBytes = place;
+        cfg.stream = s;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        st = cudaLaunchKernelEx(&cfg, gg::router_place_kernel, a.place);
+      };
+      // A decoding step's few tokens: one block of a few warps, whose sums and scans are as much shorter
+      // (4 tokens of 64 experts, top 2: XX us against YY us with the full block).
+      if (V == 8 && q.tokens <= gg::kFewWarps * at_once) launch(std::integral_constant<int, V == 8 ? gg::kFewWarps : gg::router_warps(V)>());
+      else launch(std::integral_constant<int, gg::router_warps(V)>());
     });
   });
   return st;
@@ -723,7 +803,7 @@ int gg_router_backward(const gg_router* router, const gg_route_gradient* gradien
                          gg::rows_aligned(q.grad_logits, q.ld_grad, c.logit_type)};
       const int64_t blocks = (static_cast<int64_t>(q.tokens) + warps * at_once - 1) / (warps * at_once);
       gg::router_backward_kernel<f(), G, V>
-          <<<static_cast<int>(std::min<int64_t>(blocks, 8 * gg::kMaxBlocks)), 32 * warps, 0, s>>>(a);
+          <<<static_cast<int>(std::min<int64_t>(blocks, gg::kBackwardBlocks * gg::kMaxBlocks)), 32 * warps, 0, s>>>(a);
     });
   });
   return cudaGetLastError();
