@@ -10,17 +10,19 @@
 // or tensor memory, a detour that costs more than the matrix work of 8 columns; a fragment in
 // registers is fed from the unpacking directly.
 //
-// Weights are laid out once (gg_q4_plan_create), per expert as blocks of 16 outputs x 128 k, 1 KB:
-//   [half h][lane][4 words]: lane l, word i, half h hold output 16 tile + 8 h + l / 4 and
-//   k = 128 block + 32 i + 8 (l % 4) + 0..7, the eight values in the nibbles (0, 4, 1, 5, 2, 6, 3, 7)
-//   from the low end, so that one mask gives the pair (x, x + 1) in the two halves of a register
-// and per block the scales as [l / 4][group of the block][half], the zeros alike.
+// Weights are laid out once (gg_q4_plan_create), per expert as blocks of 16 outputs x 128 k, tile by tile
+// and along k in a tile. A block is what one step of a warp reads, in one piece:
+//   1024 bytes of weights [half h][lane][4 words]: lane l, word i, half h hold output 16 tile + 8 h + l / 4
+//   and k = 128 block + 32 i + 8 (l % 4) + 0..7, the eight values in the nibbles (0, 4, 1, 5, 2, 6, 3, 7)
+//   from the low end, so that one mask gives the pair (x, x + 1) in the two halves of a register;
+//   its scales [l / 4][group of the block][half], 16 bits each; the zeros alike, 8 bits each (if any).
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "gg_epilogue_ops.cuh"
@@ -35,13 +37,16 @@ constexpr int kTileN = 16;   // outputs a block of weights covers
 constexpr int kBlockK = 128; // k values a block covers
 constexpr int kBlockBytes = kTileN * kBlockK / 2;
 
+// Bytes of a block with `per` groups along its k.
+__host__ __device__ constexpr int record_bytes(int per, bool zeros) {
+  return kBlockBytes + kTileN * per * 2 + (zeros ? kTileN * per : 0);
+}
+
 struct Q4Params {
-  const unsigned char* q;       // [experts][n_tiles][k_blocks][1024]
-  const unsigned short* scales; // [experts][n_tiles][k_blocks][8][groups of a block][2]
-  const unsigned char* zeros;   // the same, bytes; NULL: all 8
+  const unsigned char* blocks;  // [experts][n_tiles][k_blocks][record_bytes]
   const float* const* bias;     // [experts]; NULL: none
   int* status;
-  int experts, n, k, n_tiles, k_blocks, output_type, activation;
+  int experts, n, k, n_tiles, k_blocks, output_type, activation, sms;
   // of a run
   const void* a;
   const int* row_tokens;
@@ -49,21 +54,19 @@ struct Q4Params {
   void* d;
   int64_t lda, ldd;
   int a_rows, capacity_rows;
-  int vec_a;
+  const unsigned short* no_row; // k zeros, for a gathered row that does not exist
 };
 
 struct Q4PackParams {
   const unsigned char* const* q;
   const void* const* scales;
-  const unsigned char* const* zeros;
-  unsigned char* out_q;
-  unsigned short* out_scales;
-  unsigned char* out_zeros;
-  int experts, n, k, group, n_tiles, k_blocks, per_block;
+  const unsigned char* const* zeros;  // its entries are NULL without zeros
+  unsigned char* out;
+  int experts, n, k, group, n_tiles, k_blocks, per_block, record, with_zeros;
   int64_t ldq;
 };
 
-// One thread per 16-byte piece (expert, tile, block, half, lane), and one per scale.
+// One thread per 16-byte piece of the weights (block, half, lane), and one per scale and zero.
 __global__ void __launch_bounds__(kQ4Threads) q4_pack_kernel(Q4PackParams p) {
   const int64_t blocks = static_cast<int64_t>(p.experts) * p.n_tiles * p.k_blocks;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kQ4Threads;
@@ -86,10 +89,10 @@ __global__ void __launch_bounds__(kQ4Threads) q4_pack_kernel(Q4PackParams p) {
       }
       w[x] = word;
     }
-    reinterpret_cast<uint4*>(p.out_q)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(p.out + b * p.record)[i % 64] = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  const int per = 16 * p.per_block;
-  const int groups = (p.k + p.group - 1) / p.group;
+  const int per = kTileN * p.per_block;
+  const int groups = (p.k - 1) / p.group + 1;
   for (int64_t i = first; i < blocks * per; i += stride) {
     const int64_t b = i / per;
     const int in = static_cast<int>(i % per);
@@ -100,8 +103,10 @@ __global__ void __launch_bounds__(kQ4Threads) q4_pack_kernel(Q4PackParams p) {
     const int k = kBlockK * kb + kBlockK / p.per_block * sub;
     const bool in_range = o < p.n && k < p.k;
     const int64_t at = static_cast<int64_t>(o) * groups + k / p.group;
-    p.out_scales[i] = in_range ? static_cast<const unsigned short*>(p.scales[e])[at] : static_cast<unsigned short>(0);
-    if (p.out_zeros) p.out_zeros[i] = in_range ? p.zeros[e][at] & 15 : 8;
+    unsigned char* record = p.out + b * p.record + kBlockBytes;
+    reinterpret_cast<unsigned short*>(record)[in] =
+        in_range ? static_cast<const unsigned short*>(p.scales[e])[at] : static_cast<unsigned short>(0);
+    if (p.with_zeros) record[2 * per + in] = in_range ? p.zeros[e][at] & 15 : 8;
   }
 }
 
@@ -118,25 +123,69 @@ struct Q4Type<true> {
   static constexpr unsigned kMagic = 0x43004300u;  // 128
 };
 
-// (a - b) of two pairs of 16-bit numbers; exact here (whole numbers below 2048, below 256 in BF16).
-template <bool kBf16>
-__device__ __forceinline__ unsigned sub2(unsigned a, unsigned b) {
+// What is taken from the unpacked pairs, in both halves: the magic number plus the zero; and for the
+// nibbles left four bits up in FP16 the same of (1024 + 16 q) / 16, -(64 + zero). `zeros`: the zeros of
+// outputs l / 4 (low byte) and l / 4 + 8.
+template <bool kBf16, int kHalf>
+struct Q4Zero {
+  unsigned ones, sixteens;
+  __device__ __forceinline__ explicit Q4Zero(unsigned zeros) {
+    ones = __byte_perm(zeros, kBf16 ? 0x43434343u : 0x64646464u, kHalf ? 0x4141 : 0x4040);
+    sixteens = __byte_perm(zeros << 4, 0xd4d4d4d4u, kHalf ? 0x4141 : 0x4040);  // a step of 1 is 16 units in the last place
+  }
+};
+
+// The eight nibbles of a word as four pairs q - zero, exact (whole numbers below 2048, below 256 in
+// BF16). FP16's ten mantissa bits leave room to take two of the four pairs without a shift.
+__device__ __forceinline__ unsigned and_or(unsigned x, unsigned mask, unsigned add) {  // (x & mask) | add
   unsigned d;
-  if constexpr (kBf16) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(mask), "r"(add));
   return d;
 }
 
+template <bool kBf16, typename Zero>
+__device__ __forceinline__ void unpack8(unsigned w, const Zero& z, unsigned (&f)[4]) {
+  constexpr unsigned kMagic = Q4Type<kBf16>::kMagic;
+  if constexpr (kBf16) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const unsigned x = and_or(w >> (4 * v), 0x000f000fu, kMagic);
+      asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(f[v]) : "r"(x), "r"(z.ones));
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < 4; v += 2) {
+      const unsigned u = v == 0 ? w : w >> 8;
+      const unsigned x = and_or(u, 0x000f000fu, kMagic), y = and_or(u, 0x00f000f0u, kMagic);
+      asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(f[v]) : "r"(x), "r"(z.ones));
+      asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(f[v + 1]) : "r"(y), "r"(0x2c002c00u), "r"(z.sixteens));
+    }
+  }
+}
+
+// c = a b (first) or c += a b; `first` is known at compile time.
 template <bool kBf16>
-__device__ __forceinline__ void mma16816(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-  if constexpr (kBf16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma16816(float (&c)[4], bool first, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                         unsigned b1) {
+  if constexpr (kBf16) {
+    if (first)
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                   : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                   : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                   : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                   : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    if (first)
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                   : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                   : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                   : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                   : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
 }
 
 __device__ __forceinline__ float q4_activate(float x, int act) {
@@ -145,138 +194,396 @@ __device__ __forceinline__ float q4_activate(float x, int act) {
   return x;
 }
 
-// Eight activations from k on of row `row` (elements past k are zero), as four packed pairs.
-__device__ __forceinline__ uint4 load_a(const Q4Params& p, int64_t row, int k) {
-  const unsigned short* at = static_cast<const unsigned short*>(p.a) + row * p.lda + k;
-  if (p.vec_a && k + 8 <= p.k) return __ldg(reinterpret_cast<const uint4*>(at));
+// Eight activations from `at` on, of which `have` exist (the others are zero), as four packed pairs.
+__device__ __forceinline__ uint4 load_pairs(const unsigned short* at, int have) {
   unsigned v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = k + i < p.k ? __ldg(at + i) : 0u;
+  for (int i = 0; i < 8; ++i) v[i] = i < have ? __ldg(at + i) : 0u;
   return make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
 }
 
-// kPer: groups per 128-k block (1, 2 or 4).
-template <bool kBf16, int kPer, bool kZeros>
-__global__ void __launch_bounds__(kQ4Threads) q4_kernel(Q4Params p) {
-  __shared__ int s_row0[GG_Q4_MAX_EXPERTS];   // first packed row of each busy expert
-  __shared__ int s_rows[GG_Q4_MAX_EXPERTS];
-  __shared__ int s_item[GG_Q4_MAX_EXPERTS + 1];  // first item of each busy expert
-  __shared__ int s_expert[GG_Q4_MAX_EXPERTS];
-  __shared__ int s_busy, s_bad;
-  __shared__ float s_sum[kQ4Warps][kTileN * 8];
-  using Type = Q4Type<kBf16>;
-  const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
-  const int g = lane / 4, t = lane % 4;
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(to))), "l"(from)
+               : "memory");
+}
 
-  if (warp == 0) {  // the busy experts, in order
-    int busy = 0, item = 0;
-    int64_t row = 0;
-    bool bad = false;
-    for (int e0 = 0; e0 < p.experts; e0 += 32) {
-      const int e = e0 + lane;
-      const int rows = e >= p.experts ? 0 : p.rows ? p.rows[e] : p.capacity_rows;
-      bad |= rows < 0;
-      // sums clamped per expert, so that no count overflows before it is refused
-      const int64_t mine = max(0, rows);
-      int64_t upto = mine;
+// The kernel's work is cut into tasks: a tile (16 outputs) of a busy expert against a chunk of up to 8 kNT of
+// its rows. A group of `splits` warps of a block takes a contiguous range of the tasks, two tiles of one
+// chunk together where it has them (the activations are read once for both); its warps take
+// every splits-th 128-k step and add their sums up in shared memory, in order. Ranges differ by at
+// most one task, and the blocks that share an SM have neighbouring ones.
+constexpr int kPairTiles = 2;
+constexpr int kPairN = kPairTiles * kTileN;
+constexpr int kTasksPerGroup = 3;
+constexpr int kStages = 4;     // steps a warp has in flight
+constexpr int kSumPitch = 36;  // floats per row of the warps' sums: no two lanes meet in a bank
+
+// The busy experts, found from the counts by every block for itself.
+struct Q4Work {
+  int* expert;  // busy experts, in order
+  int* row0;    // their first packed row
+  int* rows;
+  int* chunk0;  // their first chunk; one more entry: all chunks
+  int splits, tasks;
+};
+
+// A place in the sequence of tasks: within an expert pair by pair of tiles, in a pair chunk by chunk (those
+// after the first find the weights in L2), then the pair's tiles.
+struct Q4Place {
+  int cur, pair, chunk, in;  // busy expert, pair's first tile, chunk, tile in the pair
+  int left;                  // tasks left of the range, this one included
+};
+
+__device__ __forceinline__ Q4Place place_of(const Q4Work& w, int n_tiles, int task, int end) {
+  Q4Place c{0, 0, 0, 0, end - task};
+  if (c.left <= 0) return c;
+  while (w.chunk0[c.cur + 1] * n_tiles <= task) ++c.cur;
+  const int chunks = w.chunk0[c.cur + 1] - w.chunk0[c.cur], in = task - w.chunk0[c.cur] * n_tiles;
+  c.pair = in / (kPairTiles * chunks) * kPairTiles;
+  const int width = min(kPairTiles, n_tiles - c.pair), rest = in - c.pair * chunks;
+  c.chunk = rest / width;
+  c.in = rest - c.chunk * width;
+  return c;
+}
+
+// Tiles that the place's step takes together.
+__device__ __forceinline__ int tiles_at(const Q4Place& c, int n_tiles) {
+  return min(min(kPairTiles, n_tiles - c.pair) - c.in, c.left);
+}
+
+__device__ __forceinline__ void advance(const Q4Work& w, int n_tiles, Q4Place& c) {
+  const int took = tiles_at(c, n_tiles);
+  c.left -= took;
+  c.in += took;
+  if (c.in < min(kPairTiles, n_tiles - c.pair)) return;
+  c.in = 0;
+  if (++c.chunk < w.chunk0[c.cur + 1] - w.chunk0[c.cur]) return;
+  c.chunk = 0;
+  c.pair += kPairTiles;
+  if (c.pair < n_tiles) return;
+  c.pair = 0;
+  ++c.cur;
+}
+
+template <bool kBf16, int kPer, bool kZeros, int kNT, bool kVec>
+struct Q4Warp {
+  static constexpr int kRecord = record_bytes(kPer, kZeros);
+  struct Stage {  // a step's blocks in shared memory
+    unsigned char tile[kPairTiles][kRecord];
+  };
+  const Q4Params& p;
+  const Q4Work& work;
+  Stage* ring;
+  int warp, lane, share;  // share: which of the group's steps are this warp's
+
+  // The copies run ahead of the arithmetic with a place of their own.
+  struct Ahead {
+    Q4Place place;
+    int kb, tiles;
+    const unsigned char* from;
+  };
+  __device__ __forceinline__ void enter(Ahead& c) const {
+    c.kb = share;
+    c.tiles = tiles_at(c.place, p.n_tiles);
+    if (c.place.left > 0)
+      c.from = p.blocks + ((static_cast<int64_t>(work.expert[c.place.cur]) * p.n_tiles + c.place.pair + c.place.in) * p.k_blocks + share) * kRecord +
+               16 * lane;
+  }
+  // Starts the copy of a step into a stage and moves on.
+  __device__ __forceinline__ void fetch(Ahead& c, Stage& to) const {
+    if (c.place.left > 0) {
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += up;
-      }
-      const unsigned has = __ballot_sync(0xffffffffu, mine > 0);
-      const int at = busy + __popc(has & ((1u << lane) - 1u));
-      if (mine > 0) {
-        s_expert[at] = e;
-        s_rows[at] = static_cast<int>(mine);
-        s_row0[at] = static_cast<int>(min(static_cast<int64_t>(p.capacity_rows), row + upto - mine));
-      }
-      busy += __popc(has);
-      row += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    bad = __any_sync(0xffffffffu, bad) || row > p.capacity_rows || (p.row_tokens == nullptr && row > p.a_rows);
-    __syncwarp();
-    if (lane == 0) {
-      if (!bad)
-        for (int i = 0; i < busy; ++i) {
-          s_item[i] = item;
-          item += (s_rows[i] + 7) / 8 * p.n_tiles;
+      for (int t = 0; t < kPairTiles; ++t)
+        if (t < c.tiles) {
+          const unsigned char* q = c.from + static_cast<int64_t>(t) * p.k_blocks * kRecord;
+          unsigned char* at = to.tile[t] + 16 * lane;
+          copy16(at, q);
+          copy16(at + 512, q + 512);
+          if (16 * lane < kRecord - kBlockBytes) copy16(at + kBlockBytes, q + kBlockBytes);
         }
-      s_item[busy] = item;
-      s_busy = busy;
-      s_bad = bad;
-      if (bad && blockIdx.x == 0) atomicOr(p.status, GG_STATUS_BAD_ROWS);
+      c.from += work.splits * kRecord;
+      c.kb += work.splits;
+      if (c.kb >= p.k_blocks) {
+        advance(work, p.n_tiles, c.place);
+        enter(c);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  __device__ __forceinline__ uint4 weights(const Stage& st, int t, int half) const {
+    return reinterpret_cast<const uint4*>(st.tile[t])[lane + 32 * half];
+  }
+  __device__ __forceinline__ float2 scale(const Stage& st, int t, int sub) const {
+    return unpack2<Q4Type<kBf16>::kOut>(reinterpret_cast<const unsigned*>(st.tile[t] + kBlockBytes)[lane / 4 * kPer + sub]);
+  }
+  __device__ __forceinline__ unsigned zeros(const Stage& st, int t, int sub) const {
+    if constexpr (kZeros)
+      return reinterpret_cast<const unsigned short*>(st.tile[t] + kBlockBytes + 32 * kPer)[lane / 4 * kPer + sub];
+    else
+      return 0x0808u;
+  }
+
+  // 16 outputs x 32 k (word i of the lane's pieces) against 8 rows: two products.
+  static __device__ __forceinline__ unsigned word(const uint4& q, int i) {  // i is known at compile time
+    return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w;
+  }
+  static __device__ __forceinline__ void multiply(float (&part)[4], bool first, const unsigned (&f0)[4], const unsigned (&f1)[4],
+                                                  const uint4& x) {
+    mma16816<kBf16>(part, first, f0[0], f1[0], f0[1], f1[1], x.x, x.y);
+    mma16816<kBf16>(part, false, f0[2], f1[2], f0[3], f1[3], x.z, x.w);
+  }
+  static __device__ __forceinline__ void scale_add(float (&acc)[4], const float2& s, const float (&part)[4]) {
+    acc[0] = fmaf(s.x, part[0], acc[0]);
+    acc[1] = fmaf(s.x, part[1], acc[1]);
+    acc[2] = fmaf(s.y, part[2], acc[2]);
+    acc[3] = fmaf(s.y, part[3], acc[3]);
+  }
+
+  // One tile of a step, 16 outputs x 128 k, against NT x 8 rows. load(i, j): the lane's activations of 32-k
+  // word i and rows 8 j.
+  template <int NT, typename Load>
+  __device__ __forceinline__ void step(const Stage& st, int t, const Load& load, float (&acc)[NT][4]) const {
+    const uint4 q0 = weights(st, t, 0), q1 = weights(st, t, 1);
+#pragma unroll
+    for (int sub = 0; sub < kPer; ++sub) {
+      const unsigned zz = zeros(st, t, sub);
+      const Q4Zero<kBf16, 0> z0(zz);
+      const Q4Zero<kBf16, 1> z1(zz);
+      float part[NT][4];
+#pragma unroll
+      for (int i = sub * (4 / kPer); i < (sub + 1) * (4 / kPer); ++i) {
+        unsigned f0[4], f1[4];
+        unpack8<kBf16>(word(q0, i), z0, f0);
+        unpack8<kBf16>(word(q1, i), z1, f1);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) multiply(part[j], i == sub * (4 / kPer), f0, f1, load(i, j));
+      }
+      const float2 s = scale(st, t, sub);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) scale_add(acc[j], s, part[j]);
+    }
+  }
+
+  // The rows of the activations that this lane feeds, column lane / 4 of each 8; they change with the
+  // expert and the chunk, not with the outputs.
+  struct Rows {
+    int row0 = -1;
+    int index[kNT];
+  };
+  __device__ __forceinline__ void find_rows(int row0, int count, Rows& r) const {
+    if (row0 == r.row0) return;
+    r.row0 = row0;
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) {
+      // a column past the chunk's rows is computed and not stored: it reads the first row again
+      const int at = row0 + (8 * j + lane / 4 < count ? 8 * j + lane / 4 : 0);
+      r.index[j] = p.row_tokens ? __ldg(p.row_tokens + at) : at;
+    }
+  }
+
+  // This warp's steps of one task or pair of tasks, then the group's sums and the outputs.
+  template <int NT>
+  __device__ __forceinline__ void run(int e, int tile, int tiles, int count, const Rows& r, Ahead& ahead, int& stage, float* sums,
+                                      int& flip) const {
+    const int g = lane / 4, t4 = lane % 4;
+    float acc[kPairTiles][NT][4];
+#pragma unroll
+    for (int t = 0; t < kPairTiles; ++t)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) acc[t][j][v] = 0.0f;
+    const unsigned short* rows[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      rows[j] = (r.index[j] >= 0 && r.index[j] < p.a_rows ? static_cast<const unsigned short*>(p.a) + r.index[j] * p.lda : p.no_row) + 8 * t4;
+    // eight activations of 32-k word i of block kb; past k they are zeros
+    const auto from_memory = [&](int kb, int i, int j) {
+      const int k = kBlockK * kb + 32 * i;
+      if constexpr (kVec) return __ldg(reinterpret_cast<const uint4*>(k + 8 * t4 < p.k ? rows[j] + k : p.no_row));
+      else return load_pairs(rows[j] + k, p.k - k - 8 * t4);
+    };
+    // Up to 16 rows the registers hold a step's activations, so that they are on their way while the next
+    // stage is waited for; more are read word by word, again for each tile (from L1).
+    constexpr bool kHeld = NT <= 2;
+    uint4 x[4][kHeld ? NT : 1];
+    const auto hold = [&](int kb) {
+      if constexpr (kHeld) {
+        if (kVec && kBlockK * (kb + 1) <= p.k) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const unsigned short* at = rows[j] + kBlockK * kb;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i][j] = __ldg(reinterpret_cast<const uint4*>(at + 32 * i));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i][j] = from_memory(kb, i, j);
+        }
+      }
+    };
+    int kb = share;
+    hold(kb);
+    while (true) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp();  // every lane's copies of this stage are there, and all are done with the one refilled now
+      fetch(ahead, ring[(stage + kStages - 1) % kStages]);
+      const Stage& st = ring[stage];
+#pragma unroll
+      for (int t = 0; t < kPairTiles; ++t)
+        if (t < tiles) {
+          if constexpr (kHeld) step<NT>(st, t, [&](int i, int j) { return x[i][j]; }, acc[t]);
+          else step<NT>(st, t, [&](int i, int j) { return from_memory(kb, i, j); }, acc[t]);
+        }
+      stage = (stage + 1) % kStages;
+      kb += work.splits;
+      if (kb >= p.k_blocks) break;
+      hold(kb);
+    }
+    const int first = warp - share, id = 32 * share + lane;  // the group's first warp; the thread in the group
+    const float* bias = p.bias ? p.bias[e] : nullptr;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      if (8 * j >= count) break;  // the same for the whole group
+      // [warp][row][output], in two buffers: a thread may still read the last one when another writes
+      float* mine = sums + (flip * kQ4Warps + warp) * 8 * kSumPitch;
+#pragma unroll
+      for (int t = 0; t < kPairTiles; ++t)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) mine[(2 * t4 + v % 2) * kSumPitch + kTileN * t + g + 8 * (v / 2)] = acc[t][j][v];
+      if (work.splits > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + first / work.splits), "r"(32 * work.splits) : "memory");
+      else __syncwarp();
+      for (int i = id; i < 8 * kPairN; i += 32 * work.splits) {
+        const int row = i / kPairN, o = kTileN * tile + i % kPairN;
+        if (8 * j + row >= count || i % kPairN >= kTileN * tiles || o >= p.n) continue;
+        const float* from = sums + ((flip * kQ4Warps + first) * 8 + row) * kSumPitch + i % kPairN;
+        float sum = 0.0f;
+        for (int w = 0; w < work.splits; ++w) sum += from[w * 8 * kSumPitch];
+        if (bias) sum += __ldg(bias + o);
+        store_out_rt(p.output_type, p.d, static_cast<int64_t>(r.row0 + 8 * j + row) * p.ldd + o, q4_activate(sum, p.activation));
+      }
+      flip ^= 1;
+    }
+  }
+};
+
+// The busy experts and the split, by one warp. False: the counts are not valid.
+__device__ __forceinline__ bool find_work(const Q4Params& p, Q4Work& w, int most_rows, int lane) {
+  int busy = 0, chunks = 0;
+  int64_t row = 0;
+  bool bad = false;
+  for (int e0 = 0; e0 < p.experts; e0 += 32) {
+    const int e = e0 + lane;
+    const int rows = e >= p.experts ? 0 : p.rows ? p.rows[e] : p.capacity_rows;
+    bad |= rows < 0;
+    const int mine = max(0, rows);
+    int64_t upto = mine;
+    int chunk = (min(mine, p.capacity_rows) + most_rows - 1) / most_rows;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, upto, d);
+      const int cu = __shfl_up_sync(0xffffffffu, chunk, d);
+      if (lane >= d) upto += up, chunk += cu;
+    }
+    const unsigned has = __ballot_sync(0xffffffffu, mine > 0);
+    const int at = busy + __popc(has & ((1u << lane) - 1u));
+    if (mine > 0) {
+      w.expert[at] = e;
+      w.rows[at] = mine;
+      w.row0[at] = static_cast<int>(min(static_cast<int64_t>(p.capacity_rows), row + upto - mine));
+      w.chunk0[at + 1] = chunks + chunk;
+    }
+    busy += __popc(has);
+    row += __shfl_sync(0xffffffffu, upto, 31);
+    chunks += __shfl_sync(0xffffffffu, chunk, 31);
+    // a sum past the rows there are is refused below; stopping here keeps the sums from overflowing
+    if (row > p.capacity_rows) break;
+  }
+  if (lane == 0) w.chunk0[0] = 0;
+  bad = __any_sync(0xffffffffu, bad) || row > p.capacity_rows || (p.row_tokens == nullptr && row > p.a_rows);
+  w.tasks = bad ? 0 : chunks * p.n_tiles;
+  // Split k until a group has fewer than kTasksPerGroup tasks: fewer shares mean longer runs between two sums,
+  // more shares even work over the SMs; and never into shares of nothing.
+  w.splits = 1;
+  while (w.splits < kQ4Warps && 2 * w.splits <= p.k_blocks &&
+         static_cast<int64_t>(w.tasks) * w.splits < static_cast<int64_t>(kTasksPerGroup) * kQ4Warps * gridDim.x)
+    w.splits *= 2;
+  return !bad;
+}
+
+// kPer: groups per 128-k block (1, 2 or 4). kNT: most rows of an expert worked on together, in eights. kVec:
+// the activations are read 16 bytes at a time (aligned rows, k a multiple of 8).
+template <bool kBf16, int kPer, bool kZeros, int kNT, bool kVec>
+__global__ void __launch_bounds__(kQ4Threads, 2) q4_kernel(const __grid_constant__ Q4Params p) {
+  using Warp = Q4Warp<kBf16, kPer, kZeros, kNT, kVec>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ int s_plan[2];
+  const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
+  auto* rings = reinterpret_cast<typename Warp::Stage*>(smem);
+  float* sums = reinterpret_cast<float*>(rings + kQ4Warps * kStages);
+  Q4Work work;
+  work.expert = reinterpret_cast<int*>(sums + 2 * kQ4Warps * 8 * kSumPitch);
+  work.row0 = work.expert + p.experts;
+  work.rows = work.row0 + p.experts;
+  work.chunk0 = work.rows + p.experts;
+  if (warp == 0) {
+    const bool good = find_work(p, work, 8 * kNT, lane);
+    if (lane == 0) {
+      s_plan[0] = work.splits, s_plan[1] = work.tasks;
+      if (!good && blockIdx.x == 0) atomicOr(p.status, GG_STATUS_BAD_ROWS);
     }
   }
   __syncthreads();
-  if (s_bad) return;
-  const int items = s_item[s_busy];
-  int cur = 0;
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    while (s_item[cur + 1] <= item) ++cur;
-    const int in = item - s_item[cur];
-    const int tile = in % p.n_tiles, chunk = in / p.n_tiles;
-    const int e = s_expert[cur];
-    const int row0 = s_row0[cur] + 8 * chunk, count = min(8, s_rows[cur] - 8 * chunk);
-    // this lane's row of the activations: column g of the product
-    int64_t arow = -1;
-    if (g < count) {
-      arow = p.row_tokens ? p.row_tokens[row0 + g] : row0 + g;
-      if (arow >= p.a_rows) arow = -1;
-    }
-    const int64_t blk0 = (static_cast<int64_t>(e) * p.n_tiles + tile) * p.k_blocks;
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int kb = warp; kb < p.k_blocks; kb += kQ4Warps) {
-      const uint4* wq = reinterpret_cast<const uint4*>(p.q + (blk0 + kb) * kBlockBytes) + lane;
-      const uint4 w0 = __ldg(wq), w1 = __ldg(wq + 32);
-      const unsigned lo[4] = {w0.x, w0.y, w0.z, w0.w}, hi[4] = {w1.x, w1.y, w1.z, w1.w};
-      const int64_t meta = ((blk0 + kb) * 8 + g) * kPer * 2;
-#pragma unroll
-      for (int sub = 0; sub < kPer; ++sub) {
-        const unsigned sc = __ldg(reinterpret_cast<const unsigned*>(p.scales + meta) + sub);
-        const float2 s = unpack2<Type::kOut>(sc);
-        unsigned z0 = 8, z1 = 8;
-        if constexpr (kZeros) z0 = __ldg(p.zeros + meta + 2 * sub), z1 = __ldg(p.zeros + meta + 2 * sub + 1);
-        const unsigned b0 = Type::kMagic + z0 * 0x10001u, b1 = Type::kMagic + z1 * 0x10001u;
-        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = sub * (4 / kPer); i < (sub + 1) * (4 / kPer); ++i) {
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (arow >= 0) x = load_a(p, arow, kBlockK * kb + 32 * i + 8 * t);
-          unsigned f0[4], f1[4];
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            f0[v] = sub2<kBf16>(((lo[i] >> (4 * v)) & 0x000f000fu) | Type::kMagic, b0);
-            f1[v] = sub2<kBf16>(((hi[i] >> (4 * v)) & 0x000f000fu) | Type::kMagic, b1);
-          }
-          const unsigned a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
-          mma16816<kBf16>(part, a0, x.x, x.y);
-          mma16816<kBf16>(part, a1, x.z, x.w);
-        }
-        acc[0] = fmaf(s.x, part[0], acc[0]);
-        acc[1] = fmaf(s.x, part[1], acc[1]);
-        acc[2] = fmaf(s.y, part[2], acc[2]);
-        acc[3] = fmaf(s.y, part[3], acc[3]);
-      }
-    }
-    // sums of the warps, in warp order: [row of the activations][output]
-    __syncthreads();
-    s_sum[warp][(2 * t) * kTileN + g] = acc[0];
-    s_sum[warp][(2 * t + 1) * kTileN + g] = acc[1];
-    s_sum[warp][(2 * t) * kTileN + g + 8] = acc[2];
-    s_sum[warp][(2 * t + 1) * kTileN + g + 8] = acc[3];
-    __syncthreads();
-    if (tid < kTileN * 8) {
-      const int r = tid / kTileN, o = kTileN * tile + tid % kTileN;
-      if (r < count && o < p.n) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kQ4Warps; ++w) sum += s_sum[w][tid];
-        if (p.bias && p.bias[e]) sum += p.bias[e][o];
-        store_out_rt(p.output_type, p.d, (row0 + r) * p.ldd + o, q4_activate(sum, p.activation));
-      }
-    }
+  work.splits = s_plan[0], work.tasks = s_plan[1];
+
+  // the group's range: blocks b, b + SMs, ... (which share an SM) are neighbours
+  const int per_sm = gridDim.x % p.sms == 0 ? gridDim.x / p.sms : 0;
+  const int rank = per_sm ? blockIdx.x % p.sms * per_sm + blockIdx.x / p.sms : blockIdx.x;
+  const int64_t groups = static_cast<int64_t>(gridDim.x) * (kQ4Warps / work.splits);
+  const int64_t group = static_cast<int64_t>(rank) * (kQ4Warps / work.splits) + warp / work.splits;
+  Q4Place place = place_of(work, p.n_tiles, static_cast<int>(group * work.tasks / groups),
+                           static_cast<int>((group + 1) * work.tasks / groups));
+
+  const Warp w{p, work, rings + warp * kStages, warp, lane, warp % work.splits};
+  typename Warp::Ahead ahead{place, 0, 0, nullptr};
+  w.enter(ahead);
+  for (int i = 0; i < kStages - 1; ++i) w.fetch(ahead, w.ring[i]);
+  int stage = 0, flip = 0;
+  typename Warp::Rows rows;
+  for (; place.left > 0; advance(work, p.n_tiles, place)) {
+    const int most = 8 * kNT, row0 = work.row0[place.cur] + most * place.chunk;
+    const int count = min(most, work.rows[place.cur] - most * place.chunk);
+    const int e = work.expert[place.cur], tile = place.pair + place.in, tiles = tiles_at(place, p.n_tiles);
+    w.find_rows(row0, count, rows);
+    if (kNT == 1 || count <= 8) w.template run<1>(e, tile, tiles, count, rows, ahead, stage, sums, flip);
+    else if (kNT == 2 || count <= 16) w.template run<kNT < 2 ? 1 : 2>(e, tile, tiles, count, rows, ahead, stage, sums, flip);
+    else w.template run<kNT < 4 ? 1 : 4>(e, tile, tiles, count, rows, ahead, stage, sums, flip);
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <int kPer, bool kZeros>
+size_t q4_smem(int experts) {
+  return static_cast<size_t>(kQ4Warps) * kStages * kPairTiles * record_bytes(kPer, kZeros) + 2 * kQ4Warps * 8 * kSumPitch * sizeof(float) +
+         (4 * static_cast<size_t>(experts) + 1) * sizeof(int);
+}
+
+// The variants of a run: one for activations that are not read 16 bytes at a time, and for those that are,
+// by the most rows any expert can have: 8, 16, or more (the registers that 32 rows take cost the
+// smaller ones).
+enum Q4Variant { kQ4Narrow, kQ4Rows8, kQ4Rows16, kQ4Rows32, kQ4Variants };
+
+template <typename F>
+void with_variant(int v, F f) {
+  using std::bool_constant;
+  using std::integral_constant;
+  if (v == kQ4Narrow) f(integral_constant<int, 1>(), bool_constant<false>());
+  else if (v == kQ4Rows8) f(integral_constant<int, 1>(), bool_constant<true>());
+  else if (v == kQ4Rows16) f(integral_constant<int, 2>(), bool_constant<true>());
+  else f(integral_constant<int, 4>(), bool_constant<true>());
 }
 
 template <typename F>
@@ -300,11 +607,12 @@ void with_q4(bool bf16, int per_block, bool zeros, F f) {
 }  // namespace gg
 
 struct gg_q4_plan {
-  void* block = nullptr;  // weights | scales | zeros | bias table | status
+  void* block = nullptr;  // blocks of weights | bias table | status | a row of zeros | the caller's pointers
   gg::Q4Params params{};
-  bool bf16 = false;
+  bool bf16 = false, zeros = false;
   int per_block = 1;
-  int grid = 0;
+  int grid[gg::kQ4Variants] = {};  // resident blocks of each variant
+  size_t smem = 0;
 };
 
 extern "C" {
@@ -326,11 +634,11 @@ int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** o
   const int per_block = q.group >= gg::kBlockK ? 1 : gg::kBlockK / q.group;
   const size_t blocks = E * n_tiles * k_blocks;
   const auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  const size_t scales_at = up(blocks * gg::kBlockBytes);
-  const size_t zeros_at = up(scales_at + blocks * 16 * per_block * 2);
-  const size_t bias_at = up(zeros_at + (q.zeros ? blocks * 16 * per_block : 0));
+  const int record = gg::record_bytes(per_block, q.zeros != nullptr);
+  const size_t bias_at = up(blocks * record);
   const size_t status_at = up(bias_at + E * sizeof(void*));
-  const size_t tables_at = up(status_at + sizeof(int));  // the caller's pointers, read once
+  const size_t no_row_at = up(status_at + sizeof(int));
+  const size_t tables_at = up(no_row_at + static_cast<size_t>(q.k) * 2);  // the caller's pointers, read once
   const size_t bytes = tables_at + 3 * E * sizeof(void*);
 
   gg_q4_plan* plan = new (std::nothrow) gg_q4_plan();
@@ -342,12 +650,20 @@ int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** o
     tables[E + e] = q.scales[e];
     tables[2 * E + e] = q.zeros ? q.zeros[e] : nullptr;
   }
-  int device = 0, sms = 0, per_sm = 0;
+  int device = 0, sms = 0, per_sm[gg::kQ4Variants] = {};
+  size_t smem = 0;
   cudaError_t st = cudaGetDevice(&device);
   if (st == cudaSuccess) st = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
   if (st == cudaSuccess)
     gg::with_q4(q.input_type == GG_INPUT_BF16, per_block, q.zeros != nullptr, [&](auto b, auto n, auto z) {
-      st = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, gg::q4_kernel<b(), n(), z()>, gg::kQ4Threads, 0);
+      smem = gg::q4_smem<n(), z()>(q.experts);
+      for (int v = 0; v < gg::kQ4Variants && st == cudaSuccess; ++v)
+        gg::with_variant(v, [&](auto nt, auto vec) {
+          const auto kernel = gg::q4_kernel<b(), n(), z(), nt(), vec()>;
+          st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(gg::q4_smem<n(), z()>(GG_Q4_MAX_EXPERTS)));
+          if (st == cudaSuccess) st = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm[v], kernel, gg::kQ4Threads, smem);
+        });
     });
   if (st == cudaSuccess) st = cudaMalloc(&plan->block, bytes);
   if (st != cudaSuccess) {
@@ -358,23 +674,11 @@ int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** o
   st = cudaMemcpyAsync(base + tables_at, tables.data(), tables.size() * sizeof(void*), cudaMemcpyHostToDevice, s);
   if (st == cudaSuccess && q.bias)
     st = cudaMemcpyAsync(base + bias_at, q.bias, E * sizeof(void*), cudaMemcpyHostToDevice, s);
-  if (st == cudaSuccess) st = cudaMemsetAsync(base + status_at, 0, sizeof(int), s);
+  if (st == cudaSuccess) st = cudaMemsetAsync(base + status_at, 0, tables_at - status_at, s);
   if (st == cudaSuccess) {
     const unsigned char* const* table = reinterpret_cast<const unsigned char* const*>(base + tables_at);
-    gg::Q4PackParams pk{table,
-                        reinterpret_cast<const void* const*>(table + E),
-                        table + 2 * E,
-                        base,
-                        reinterpret_cast<unsigned short*>(base + scales_at),
-                        q.zeros ? base + zeros_at : nullptr,
-                        q.experts,
-                        q.n,
-                        q.k,
-                        q.group,
-                        n_tiles,
-                        k_blocks,
-                        per_block,
-                        q.ldq};
+    gg::Q4PackParams pk{table,   reinterpret_cast<const void* const*>(table + E), table + 2 * E, base,   q.experts, q.n,
+                        q.k,     q.group, n_tiles, k_blocks, per_block, record, q.zeros != nullptr, q.ldq};
     const size_t want = (blocks * 64 + gg::kQ4Threads - 1) / gg::kQ4Threads;
     gg::q4_pack_kernel<<<static_cast<unsigned>(std::min<size_t>(want, 1u << 16)), gg::kQ4Threads, 0, s>>>(pk);
     st = cudaGetLastError();
@@ -386,11 +690,11 @@ int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** o
     return st;
   }
   gg::Q4Params& p = plan->params;
-  p.q = base;
-  p.scales = reinterpret_cast<const unsigned short*>(base + scales_at);
-  p.zeros = q.zeros ? base + zeros_at : nullptr;
+  p.blocks = base;
+  p.sms = sms;
   p.bias = q.bias ? reinterpret_cast<const float* const*>(base + bias_at) : nullptr;
   p.status = reinterpret_cast<int*>(base + status_at);
+  p.no_row = reinterpret_cast<const unsigned short*>(base + no_row_at);
   p.experts = q.experts;
   p.n = q.n;
   p.k = q.k;
@@ -399,8 +703,10 @@ int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** o
   p.output_type = q.output_type;
   p.activation = q.activation;
   plan->bf16 = q.input_type == GG_INPUT_BF16;
+  plan->zeros = q.zeros != nullptr;
   plan->per_block = per_block;
-  plan->grid = std::max(1, sms * per_sm);
+  for (int v = 0; v < gg::kQ4Variants; ++v) plan->grid[v] = std::max(1, sms * per_sm[v]);
+  plan->smem = smem;
   *out = plan;
   return cudaSuccess;
 }
@@ -412,8 +718,6 @@ int gg_q4_plan_run(gg_q4_plan* plan, const void* a, int lda, int a_rows, const i
   if (capacity_rows < 0 || a_rows < 0 || lda < p.k || ldd < p.n || (!rows && p.experts != 1)) return cudaErrorInvalidValue;
   if (capacity_rows == 0 && !rows) return cudaSuccess;
   if ((capacity_rows > 0 && !d) || (a_rows > 0 && !a)) return cudaErrorInvalidValue;
-  // items are counted in an int: (rows / 8 + experts) tiles of 16 outputs
-  if ((static_cast<int64_t>(capacity_rows) / 8 + p.experts) * p.n_tiles > INT32_MAX) return cudaErrorInvalidValue;
   p.a = a;
   p.lda = lda;
   p.a_rows = a_rows;
@@ -422,13 +726,24 @@ int gg_q4_plan_run(gg_q4_plan* plan, const void* a, int lda, int a_rows, const i
   p.d = d;
   p.ldd = ldd;
   p.capacity_rows = capacity_rows;
-  p.vec_a = (reinterpret_cast<uintptr_t>(a) & 15u) == 0 && lda % 8 == 0;
-  const int64_t most = (static_cast<int64_t>(capacity_rows) / 8 + std::min(capacity_rows, p.experts)) * p.n_tiles;
-  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(plan->grid, most)));
+  const bool vec = (reinterpret_cast<uintptr_t>(a) & 15u) == 0 && lda % 8 == 0 && p.k % 8 == 0;
+  const int variant = !vec ? gg::kQ4Narrow : capacity_rows <= 8 ? gg::kQ4Rows8 : capacity_rows <= 16 ? gg::kQ4Rows16 : gg::kQ4Rows32;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  gg::with_q4(plan->bf16, plan->per_block, p.zeros != nullptr, [&](auto b, auto n, auto z) {
-    gg::q4_kernel<b(), n(), z()><<<grid, gg::kQ4Threads, 0, s>>>(p);
+  cudaError_t st = cudaSuccess;
+  gg::with_variant(variant, [&](auto nt, auto vec_c) {
+    // tasks are counted in an int: one per tile of each chunk of rows, chunks at most this
+    const int64_t chunks = std::min<int64_t>(capacity_rows, static_cast<int64_t>(capacity_rows) / (8 * nt()) + p.experts);
+    const int64_t most = chunks * p.n_tiles;
+    if (most > INT32_MAX) {
+      st = cudaErrorInvalidValue;
+      return;
+    }
+    const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(plan->grid[variant], most)));
+    gg::with_q4(plan->bf16, plan->per_block, plan->zeros, [&](auto b, auto n, auto z) {
+      gg::q4_kernel<b(), n(), z(), nt(), vec_c()><<<grid, gg::kQ4Threads, plan->smem, s>>>(p);
+    });
   });
+  if (st != cudaSuccess) return st;
   return cudaGetLastError();
 }
 
