@@ -376,6 +376,9 @@ cudaError_t take_status(int* word, int* bits) {
 }
 
 }  // namespace
+
+unsigned long long wait_limit_ns() { return wait_timeout_ns(); }
+
 }  // namespace gg
 
 // ---- the executor ------------------------------------------------------------------------------

@@ -44,6 +44,9 @@ cudaError_t kernel_occupancy(Variant v, int* active_blocks_per_sm, cudaFuncAttri
 cudaError_t kernel_resident_ctas(Variant v, int* ctas);
 cudaError_t launch_wait_selftest(int* status, unsigned long long timeout_ns, cudaStream_t stream);
 
+// The limit of every wait inside a kernel (GG_WAIT_TIMEOUT_MS, 2 s by default).
+unsigned long long wait_limit_ns();
+
 // Count of IPC mappings opened or closed in this process (gg_ipc.cu); a cached answer about which
 // GPU owns an address is stale once it changes.
 unsigned ipc_mapping_generation();

@@ -26,6 +26,8 @@
 #include <vector>
 
 #include "gg_epilogue_ops.cuh"
+#include "gg_internal.h"
+#include "gg_ptx.cuh"
 #include "grouped_gemm_b200.h"
 
 namespace gg {
@@ -47,6 +49,7 @@ struct Q4Params {
   const float* const* bias;     // [experts]; NULL: none
   int* status;
   int experts, n, k, n_tiles, k_blocks, output_type, activation, sms;
+  unsigned long long timeout_ns;
   // of a run
   const void* a;
   const int* row_tokens;
@@ -169,20 +172,20 @@ __device__ __forceinline__ void mma16816(float (&c)[4], bool first, unsigned a0,
                                          unsigned b1) {
   if constexpr (kBf16) {
     if (first)
-      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                    : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                    : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
     else
-      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                    : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                    : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   } else {
     if (first)
-      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                    : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                    : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
     else
-      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                    : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                    : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
@@ -202,21 +205,35 @@ __device__ __forceinline__ uint4 load_pairs(const unsigned short* at, int have) 
   return make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
 }
 
-__device__ __forceinline__ void copy16(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(to))), "l"(from)
+// `bytes` (a multiple of 16) from global to shared memory, counted on the mbarrier.
+__device__ __forceinline__ void copy_bulk(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from),
+               "r"(bytes), "r"(bar)
                : "memory");
 }
 
+// Waits for a phase, at most timeout_ns: a wait that runs out raises GG_STATUS_TIMEOUT_PRODUCER, and the
+// kernel goes on with what is in the stage, so that its barriers stay matched and it ends.
+__device__ __forceinline__ void wait_bounded(uint32_t bar, uint32_t parity, unsigned long long timeout_ns, int* status) {
+  if (ptx::mbar_try_wait(bar, parity)) return;
+  const uint64_t start = ptx::global_timer_ns();
+  for (unsigned i = 0; !ptx::mbar_try_wait_sleep(bar, parity, 1000u); ++i)
+    if (ptx::global_timer_ns() - start > timeout_ns || i > 0x40000000u) {
+      atomicOr(status, GG_STATUS_TIMEOUT_PRODUCER);
+      return;
+    }
+}
+
 // The kernel's work is cut into tasks: a tile (16 outputs) of a busy expert against a chunk of up to 8 kNT of
-// its rows. A group of `splits` warps of a block takes a contiguous range of the tasks, two tiles of one
-// chunk together where it has them (the activations are read once for both); its warps take
-// every splits-th 128-k step and add their sums up in shared memory, in order. Ranges differ by at
-// most one task, and the blocks that share an SM have neighbouring ones.
-constexpr int kPairTiles = 2;
-constexpr int kPairN = kPairTiles * kTileN;
-constexpr int kTasksPerGroup = 3;
-constexpr int kStages = 4;     // steps a warp has in flight
-constexpr int kSumPitch = 36;  // floats per row of the warps' sums: no two lanes meet in a bank
+// its rows. A group of `splits` warps of a block takes a contiguous range of the tasks; each of its
+// warps has a contiguous share of k, and they add their sums up in shared memory, in order. Ranges differ by
+// at most one task, and the blocks that share an SM have neighbouring ones. A warp's blocks of a tile
+// lie one after the other: it keeps two stages of up to kStageBlocks of them coming, one bulk copy each,
+// started by its first lane as soon as the warp is through with a stage, whatever task comes next.
+constexpr int kTaskCost = 2;
+constexpr int kStageBlocks = 4;
+constexpr int kStages = 2;
+constexpr int kSumPitch = 20;  // floats per row of the warps' sums: no two lanes meet in a bank
 
 // The busy experts, found from the counts by every block for itself.
 struct Q4Work {
@@ -227,101 +244,73 @@ struct Q4Work {
   int splits, tasks;
 };
 
-// A place in the sequence of tasks: within an expert pair by pair of tiles, in a pair chunk by chunk (those
-// after the first find the weights in L2), then the pair's tiles.
+// A place in the sequence of tasks: expert by expert, tile by tile, in a tile chunk by chunk (those after the
+// first find the weights in L2).
 struct Q4Place {
-  int cur, pair, chunk, in;  // busy expert, pair's first tile, chunk, tile in the pair
-  int left;                  // tasks left of the range, this one included
+  int cur, tile, chunk, chunks;  // busy expert, tile, chunk of the expert's chunks
+  int left;                      // tasks left of the range, this one included
 };
 
 __device__ __forceinline__ Q4Place place_of(const Q4Work& w, int n_tiles, int task, int end) {
-  Q4Place c{0, 0, 0, 0, end - task};
+  Q4Place c{0, 0, 0, 1, end - task};
   if (c.left <= 0) return c;
   while (w.chunk0[c.cur + 1] * n_tiles <= task) ++c.cur;
-  const int chunks = w.chunk0[c.cur + 1] - w.chunk0[c.cur], in = task - w.chunk0[c.cur] * n_tiles;
-  c.pair = in / (kPairTiles * chunks) * kPairTiles;
-  const int width = min(kPairTiles, n_tiles - c.pair), rest = in - c.pair * chunks;
-  c.chunk = rest / width;
-  c.in = rest - c.chunk * width;
+  c.chunks = w.chunk0[c.cur + 1] - w.chunk0[c.cur];
+  const int in = task - w.chunk0[c.cur] * n_tiles;
+  c.tile = in / c.chunks;
+  c.chunk = in - c.tile * c.chunks;
   return c;
 }
 
-// Tiles that the place's step takes together.
-__device__ __forceinline__ int tiles_at(const Q4Place& c, int n_tiles) {
-  return min(min(kPairTiles, n_tiles - c.pair) - c.in, c.left);
-}
-
-__device__ __forceinline__ void advance(const Q4Work& w, int n_tiles, Q4Place& c) {
-  const int took = tiles_at(c, n_tiles);
-  c.left -= took;
-  c.in += took;
-  if (c.in < min(kPairTiles, n_tiles - c.pair)) return;
-  c.in = 0;
-  if (++c.chunk < w.chunk0[c.cur + 1] - w.chunk0[c.cur]) return;
+// To the next task; true where that is of another tile.
+__device__ __forceinline__ bool advance(const Q4Work& w, int n_tiles, Q4Place& c) {
+  if (--c.left <= 0) return false;
+  if (++c.chunk < c.chunks) return false;
   c.chunk = 0;
-  c.pair += kPairTiles;
-  if (c.pair < n_tiles) return;
-  c.pair = 0;
-  ++c.cur;
+  if (++c.tile == n_tiles) {
+    c.tile = 0;
+    ++c.cur;
+    c.chunks = w.chunk0[c.cur + 1] - w.chunk0[c.cur];
+  }
+  return true;
 }
 
 template <bool kBf16, int kPer, bool kZeros, int kNT, bool kVec>
 struct Q4Warp {
   static constexpr int kRecord = record_bytes(kPer, kZeros);
-  struct Stage {  // a step's blocks in shared memory
-    unsigned char tile[kPairTiles][kRecord];
-  };
+  static constexpr int kStageBytes = kStageBlocks * kRecord;
   const Q4Params& p;
   const Q4Work& work;
-  Stage* ring;
-  int warp, lane, share;  // share: which of the group's steps are this warp's
+  const unsigned char* ring;  // this lane's 16 bytes of the first stage
+  uint32_t ring_address, bars;  // the first stage and the stages' barriers as shared addresses
+  int warp, lane;
+  int share, kb0, run;  // the warp's share of k: blocks [kb0, kb0 + run)
 
   // The copies run ahead of the arithmetic with a place of their own.
   struct Ahead {
     Q4Place place;
-    int kb, tiles;
-    const unsigned char* from;
+    int left;                   // blocks of the task that are not under way
+    const unsigned char* from;  // the next of them
   };
   __device__ __forceinline__ void enter(Ahead& c) const {
-    c.kb = share;
-    c.tiles = tiles_at(c.place, p.n_tiles);
-    if (c.place.left > 0)
-      c.from = p.blocks + ((static_cast<int64_t>(work.expert[c.place.cur]) * p.n_tiles + c.place.pair + c.place.in) * p.k_blocks + share) * kRecord +
-               16 * lane;
+    c.left = c.place.left > 0 ? run : 0;
+    if (c.left > 0)
+      c.from = p.blocks + ((static_cast<int64_t>(work.expert[c.place.cur]) * p.n_tiles + c.place.tile) * p.k_blocks + kb0) * kRecord;
   }
-  // Starts the copy of a step into a stage and moves on.
-  __device__ __forceinline__ void fetch(Ahead& c, Stage& to) const {
-    if (c.place.left > 0) {
-#pragma unroll
-      for (int t = 0; t < kPairTiles; ++t)
-        if (t < c.tiles) {
-          const unsigned char* q = c.from + static_cast<int64_t>(t) * p.k_blocks * kRecord;
-          unsigned char* at = to.tile[t] + 16 * lane;
-          copy16(at, q);
-          copy16(at + 512, q + 512);
-          if (16 * lane < kRecord - kBlockBytes) copy16(at + kBlockBytes, q + kBlockBytes);
-        }
-      c.from += work.splits * kRecord;
-      c.kb += work.splits;
-      if (c.kb >= p.k_blocks) {
-        advance(work, p.n_tiles, c.place);
-        enter(c);
-      }
+  // Starts the copy of the next blocks into a stage.
+  __device__ __forceinline__ void fetch(Ahead& c, int stage) const {
+    if (c.left <= 0) return;
+    const int blocks = min(kStageBlocks, c.left);
+    if (lane == 0) {
+      ptx::mbar_arrive_expect_tx(bars + 8 * stage, blocks * kRecord);
+      copy_bulk(ring_address + stage * kStageBytes, c.from, blocks * kRecord, bars + 8 * stage);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
-
-  __device__ __forceinline__ uint4 weights(const Stage& st, int t, int half) const {
-    return reinterpret_cast<const uint4*>(st.tile[t])[lane + 32 * half];
-  }
-  __device__ __forceinline__ float2 scale(const Stage& st, int t, int sub) const {
-    return unpack2<Q4Type<kBf16>::kOut>(reinterpret_cast<const unsigned*>(st.tile[t] + kBlockBytes)[lane / 4 * kPer + sub]);
-  }
-  __device__ __forceinline__ unsigned zeros(const Stage& st, int t, int sub) const {
-    if constexpr (kZeros)
-      return reinterpret_cast<const unsigned short*>(st.tile[t] + kBlockBytes + 32 * kPer)[lane / 4 * kPer + sub];
-    else
-      return 0x0808u;
+    c.from += blocks * kRecord;
+    c.left -= blocks;
+    if (c.left == 0) {
+      advance(work, p.n_tiles, c.place);
+      enter(c);
+    }
   }
 
   // 16 outputs x 32 k (word i of the lane's pieces) against 8 rows: two products.
@@ -340,14 +329,18 @@ struct Q4Warp {
     acc[3] = fmaf(s.y, part[3], acc[3]);
   }
 
-  // One tile of a step, 16 outputs x 128 k, against NT x 8 rows. load(i, j): the lane's activations of 32-k
-  // word i and rows 8 j.
-  template <int NT, typename Load>
-  __device__ __forceinline__ void step(const Stage& st, int t, const Load& load, float (&acc)[NT][4]) const {
-    const uint4 q0 = weights(st, t, 0), q1 = weights(st, t, 1);
+  // One block, 16 outputs x 128 k, against NT x 8 rows. at: this lane's first 16 bytes of the block; x: the
+  // lane's activations of its four words; reload(i): called when word i is used.
+  template <int NT, typename Reload>
+  __device__ __forceinline__ void multiply_block(const unsigned char* at, const uint4 (&x)[4][NT], float (&acc)[NT][4],
+                                                 const Reload& reload) const {
+    const uint4 q0 = *reinterpret_cast<const uint4*>(at), q1 = *reinterpret_cast<const uint4*>(at + 512);
+    const unsigned char* meta = at - 16 * lane + kBlockBytes;
+    const int first = lane / 4 * kPer;
 #pragma unroll
     for (int sub = 0; sub < kPer; ++sub) {
-      const unsigned zz = zeros(st, t, sub);
+      unsigned zz = 0x0808u;
+      if constexpr (kZeros) zz = reinterpret_cast<const unsigned short*>(meta + 32 * kPer)[first + sub];
       const Q4Zero<kBf16, 0> z0(zz);
       const Q4Zero<kBf16, 1> z1(zz);
       float part[NT][4];
@@ -357,19 +350,20 @@ struct Q4Warp {
         unpack8<kBf16>(word(q0, i), z0, f0);
         unpack8<kBf16>(word(q1, i), z1, f1);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) multiply(part[j], i == sub * (4 / kPer), f0, f1, load(i, j));
+        for (int j = 0; j < NT; ++j) multiply(part[j], i == sub * (4 / kPer), f0, f1, x[i][j]);
+        reload(i);
       }
-      const float2 s = scale(st, t, sub);
+      const float2 s = unpack2<Q4Type<kBf16>::kOut>(reinterpret_cast<const unsigned*>(meta)[first + sub]);
 #pragma unroll
       for (int j = 0; j < NT; ++j) scale_add(acc[j], s, part[j]);
     }
   }
 
-  // The rows of the activations that this lane feeds, column lane / 4 of each 8; they change with the
-  // expert and the chunk, not with the outputs.
+  // Where this lane's activations start, of column lane / 4 of each 8 rows and the warp's share of k; they
+  // change with the expert and the chunk, not with the outputs.
   struct Rows {
     int row0 = -1;
-    int index[kNT];
+    const unsigned short* at[kNT];
   };
   __device__ __forceinline__ void find_rows(int row0, int count, Rows& r) const {
     if (row0 == r.row0) return;
@@ -377,71 +371,70 @@ struct Q4Warp {
 #pragma unroll
     for (int j = 0; j < kNT; ++j) {
       // a column past the chunk's rows is computed and not stored: it reads the first row again
-      const int at = row0 + (8 * j + lane / 4 < count ? 8 * j + lane / 4 : 0);
-      r.index[j] = p.row_tokens ? __ldg(p.row_tokens + at) : at;
+      int64_t row = row0 + (8 * j + lane / 4 < count ? 8 * j + lane / 4 : 0);
+      if (p.row_tokens) row = __ldg(p.row_tokens + row);
+      r.at[j] = (row >= 0 && row < p.a_rows ? static_cast<const unsigned short*>(p.a) + row * p.lda : p.no_row) + kBlockK * kb0 +
+                8 * (lane % 4);
     }
   }
 
-  // This warp's steps of one task or pair of tasks, then the group's sums and the outputs.
+  // This warp's share of one task, then the group's sums and the outputs. `stage`, `parity`: of the next stage.
   template <int NT>
-  __device__ __forceinline__ void run(int e, int tile, int tiles, int count, const Rows& r, Ahead& ahead, int& stage, float* sums,
-                                      int& flip) const {
+  __device__ __forceinline__ void compute(int e, int tile, int count, const Rows& r, Ahead& ahead, int& stage, uint32_t& parity,
+                                          float* sums, int& flip) const {
     const int g = lane / 4, t4 = lane % 4;
-    float acc[kPairTiles][NT][4];
-#pragma unroll
-    for (int t = 0; t < kPairTiles; ++t)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) acc[t][j][v] = 0.0f;
-    const unsigned short* rows[NT];
+    float acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
-      rows[j] = (r.index[j] >= 0 && r.index[j] < p.a_rows ? static_cast<const unsigned short*>(p.a) + r.index[j] * p.lda : p.no_row) + 8 * t4;
-    // eight activations of 32-k word i of block kb; past k they are zeros
-    const auto from_memory = [&](int kb, int i, int j) {
-      const int k = kBlockK * kb + 32 * i;
-      if constexpr (kVec) return __ldg(reinterpret_cast<const uint4*>(k + 8 * t4 < p.k ? rows[j] + k : p.no_row));
-      else return load_pairs(rows[j] + k, p.k - k - 8 * t4);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) acc[j][v] = 0.0f;
+    const unsigned short* rows[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) rows[j] = r.at[j];
+    int k_left = p.k - kBlockK * kb0;  // activations of a row from the block on
+    // Eight activations of 32-k word i from rows[j] on; past k (checked where a word may reach it) zeros.
+    const auto load = [&](int i, int j, auto check) {
+      if constexpr (!kVec) return load_pairs(rows[j] + 32 * i, k_left - 32 * i - 8 * t4);
+      else if constexpr (check()) return __ldg(reinterpret_cast<const uint4*>(k_left > 32 * i + 8 * t4 ? rows[j] + 32 * i : p.no_row));
+      else return __ldg(reinterpret_cast<const uint4*>(rows[j] + 32 * i));
     };
-    // Up to 16 rows the registers hold a step's activations, so that they are on their way while the next
-    // stage is waited for; more are read word by word, again for each tile (from L1).
-    constexpr bool kHeld = NT <= 2;
-    uint4 x[4][kHeld ? NT : 1];
-    const auto hold = [&](int kb) {
-      if constexpr (kHeld) {
-        if (kVec && kBlockK * (kb + 1) <= p.k) {
+    // A block's words in registers, each read again, of the next block, as soon as it is used.
+    uint4 x[4][NT];
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const unsigned short* at = rows[j] + kBlockK * kb;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i][j] = __ldg(reinterpret_cast<const uint4*>(at + 32 * i));
-          }
-        } else {
+      for (int j = 0; j < NT; ++j) x[i][j] = load(i, j, std::true_type());
+    // Blocks [b, b + count) of the stage, as one piece of code: their addresses are constants from two bases.
+    const auto blocks_of = [&](const unsigned char* at, auto count, auto check) {
+      constexpr int kCount = count();
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
+      for (int b = 0; b < kCount; ++b)
+        multiply_block<NT>(at + b * kRecord, x, acc, [&](int i) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i][j] = from_memory(kb, i, j);
-        }
+          for (int j = 0; j < NT; ++j) x[i][j] = load(4 * b + i + 4, j, check);
+        });
+      k_left -= kCount * kBlockK;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) rows[j] += kCount * kBlockK;
+    };
+    constexpr int kTogether = kVec ? 2 : 1;
+    for (int left = run; left > 0; left -= kStageBlocks) {
+      wait_bounded(bars + 8 * stage, parity, p.timeout_ns, p.status);
+      const unsigned char* at = ring + stage * kStageBytes;
+      int blocks = min(kStageBlocks, left);
+      // The words ahead are of these blocks and the next: within k for all lanes, or else looked at (past the
+      // warp's last block they may be another share's: not used).
+      if constexpr (kVec) {
+#pragma unroll 1
+        for (; blocks >= kTogether && k_left >= (kTogether + 1) * kBlockK; blocks -= kTogether, at += kTogether * kRecord)
+          blocks_of(at, std::integral_constant<int, kTogether>(), std::false_type());
       }
-    };
-    int kb = share;
-    hold(kb);
-    while (true) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-      __syncwarp();  // every lane's copies of this stage are there, and all are done with the one refilled now
-      fetch(ahead, ring[(stage + kStages - 1) % kStages]);
-      const Stage& st = ring[stage];
-#pragma unroll
-      for (int t = 0; t < kPairTiles; ++t)
-        if (t < tiles) {
-          if constexpr (kHeld) step<NT>(st, t, [&](int i, int j) { return x[i][j]; }, acc[t]);
-          else step<NT>(st, t, [&](int i, int j) { return from_memory(kb, i, j); }, acc[t]);
-        }
-      stage = (stage + 1) % kStages;
-      kb += work.splits;
-      if (kb >= p.k_blocks) break;
-      hold(kb);
+#pragma unroll 1
+      for (; blocks > 0; --blocks, at += kRecord) blocks_of(at, std::integral_constant<int, 1>(), std::true_type());
+      __syncwarp();  // all lanes are through with the stage
+      fetch(ahead, stage);
+      stage ^= 1;
+      parity ^= stage == 0;
     }
     const int first = warp - share, id = 32 * share + lane;  // the group's first warp; the thread in the group
     const float* bias = p.bias ? p.bias[e] : nullptr;
@@ -449,17 +442,17 @@ struct Q4Warp {
     for (int j = 0; j < NT; ++j) {
       if (8 * j >= count) break;  // the same for the whole group
       // [warp][row][output], in two buffers: a thread may still read the last one when another writes
-      float* mine = sums + (flip * kQ4Warps + warp) * 8 * kSumPitch;
-#pragma unroll
-      for (int t = 0; t < kPairTiles; ++t)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) mine[(2 * t4 + v % 2) * kSumPitch + kTileN * t + g + 8 * (v / 2)] = acc[t][j][v];
+      float* mine = sums + (flip * kQ4Warps + warp) * 8 * kSumPitch + 2 * t4 * kSumPitch + g;
+      mine[0] = acc[j][0];
+      mine[kSumPitch] = acc[j][1];
+      mine[8] = acc[j][2];
+      mine[kSumPitch + 8] = acc[j][3];
       if (work.splits > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + first / work.splits), "r"(32 * work.splits) : "memory");
       else __syncwarp();
-      for (int i = id; i < 8 * kPairN; i += 32 * work.splits) {
-        const int row = i / kPairN, o = kTileN * tile + i % kPairN;
-        if (8 * j + row >= count || i % kPairN >= kTileN * tiles || o >= p.n) continue;
-        const float* from = sums + ((flip * kQ4Warps + first) * 8 + row) * kSumPitch + i % kPairN;
+      for (int i = id; i < 8 * kTileN; i += 32 * work.splits) {
+        const int row = i / kTileN, o = kTileN * tile + i % kTileN;
+        if (8 * j + row >= count || o >= p.n) continue;
+        const float* from = sums + ((flip * kQ4Warps + first) * 8 + row) * kSumPitch + i % kTileN;
         float sum = 0.0f;
         for (int w = 0; w < work.splits; ++w) sum += from[w * 8 * kSumPitch];
         if (bias) sum += __ldg(bias + o);
@@ -505,12 +498,18 @@ __device__ __forceinline__ bool find_work(const Q4Params& p, Q4Work& w, int most
   if (lane == 0) w.chunk0[0] = 0;
   bad = __any_sync(0xffffffffu, bad) || row > p.capacity_rows || (p.row_tokens == nullptr && row > p.a_rows);
   w.tasks = bad ? 0 : chunks * p.n_tiles;
-  // Split k until a group has fewer than kTasksPerGroup tasks: fewer shares mean longer runs between two sums,
-  // more shares even work over the SMs; and never into shares of nothing.
+  // The split whose longest group is done first: its tasks times a share's blocks and what a task costs besides
+  // (its sums and outputs, about kTaskCost blocks). One warp takes about as long for a block whether all or
+  // half of an SM's warps are busy, so few whole shares beat many with a short last round: 1792 tasks of 32
+  // blocks, XX us in one share against YY in four.
+  const float warps = static_cast<float>(kQ4Warps * gridDim.x);
+  float least = INFINITY;
   w.splits = 1;
-  while (w.splits < kQ4Warps && 2 * w.splits <= p.k_blocks &&
-         static_cast<int64_t>(w.tasks) * w.splits < static_cast<int64_t>(kTasksPerGroup) * kQ4Warps * gridDim.x)
-    w.splits *= 2;
+  for (int splits = 1; splits <= kQ4Warps && splits <= p.k_blocks; splits *= 2) {
+    const float longest = ceilf(__fdividef(static_cast<float>(w.tasks) * splits, warps));
+    const float cost = longest * (static_cast<float>((p.k_blocks + splits - 1) / splits) + kTaskCost);
+    if (cost < least) least = cost, w.splits = splits;
+  }
   return !bad;
 }
 
@@ -522,13 +521,17 @@ __global__ void __launch_bounds__(kQ4Threads, 2) q4_kernel(const __grid_constant
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int s_plan[2];
   const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
-  auto* rings = reinterpret_cast<typename Warp::Stage*>(smem);
-  float* sums = reinterpret_cast<float*>(rings + kQ4Warps * kStages);
+  float* sums = reinterpret_cast<float*>(smem + kQ4Warps * kStages * Warp::kStageBytes);
+  __shared__ uint64_t s_bars[kQ4Warps][kStages];
   Q4Work work;
   work.expert = reinterpret_cast<int*>(sums + 2 * kQ4Warps * 8 * kSumPitch);
   work.row0 = work.expert + p.experts;
   work.rows = work.row0 + p.experts;
   work.chunk0 = work.rows + p.experts;
+  if (tid < kQ4Warps * kStages) {
+    ptx::mbar_init(ptx::smem_addr(&s_bars[0][0] + tid), 1);
+    ptx::fence_mbar_init();
+  }
   if (warp == 0) {
     const bool good = find_work(p, work, 8 * kNT, lane);
     if (lane == 0) {
@@ -542,39 +545,42 @@ __global__ void __launch_bounds__(kQ4Threads, 2) q4_kernel(const __grid_constant
   // the group's range: blocks b, b + SMs, ... (which share an SM) are neighbours
   const int per_sm = gridDim.x % p.sms == 0 ? gridDim.x / p.sms : 0;
   const int rank = per_sm ? blockIdx.x % p.sms * per_sm + blockIdx.x / p.sms : blockIdx.x;
-  const int64_t groups = static_cast<int64_t>(gridDim.x) * (kQ4Warps / work.splits);
-  const int64_t group = static_cast<int64_t>(rank) * (kQ4Warps / work.splits) + warp / work.splits;
-  Q4Place place = place_of(work, p.n_tiles, static_cast<int>(group * work.tasks / groups),
-                           static_cast<int>((group + 1) * work.tasks / groups));
+  const int groups = gridDim.x * (kQ4Warps / work.splits), group = rank * (kQ4Warps / work.splits) + warp / work.splits;
+  // rounded alike for the end of one range and the start of the next; the last ends with the tasks
+  const float share_of = __fdividef(static_cast<float>(work.tasks), static_cast<float>(groups));
+  const auto start = [&](int g) { return g == groups ? work.tasks : min(work.tasks, __float2int_rz(g * share_of)); };
+  Q4Place place = place_of(work, p.n_tiles, start(group), start(group + 1));
 
-  const Warp w{p, work, rings + warp * kStages, warp, lane, warp % work.splits};
-  typename Warp::Ahead ahead{place, 0, 0, nullptr};
+  const int share = warp % work.splits, kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * share / work.splits);
+  const unsigned char* ring = smem + warp * kStages * Warp::kStageBytes;
+  const Warp w{p, work, ring + 16 * lane, ptx::smem_addr(ring), ptx::smem_addr(s_bars[warp]), warp, lane, share, kb0,
+               static_cast<int>(static_cast<int64_t>(p.k_blocks) * (share + 1) / work.splits) - kb0};
+  typename Warp::Ahead ahead{place, 0, nullptr};
   w.enter(ahead);
-  for (int i = 0; i < kStages - 1; ++i) w.fetch(ahead, w.ring[i]);
+  for (int i = 0; i < kStages; ++i) w.fetch(ahead, i);
   int stage = 0, flip = 0;
+  uint32_t parity = 0;
   typename Warp::Rows rows;
   for (; place.left > 0; advance(work, p.n_tiles, place)) {
     const int most = 8 * kNT, row0 = work.row0[place.cur] + most * place.chunk;
     const int count = min(most, work.rows[place.cur] - most * place.chunk);
-    const int e = work.expert[place.cur], tile = place.pair + place.in, tiles = tiles_at(place, p.n_tiles);
+    const int e = work.expert[place.cur];
     w.find_rows(row0, count, rows);
-    if (kNT == 1 || count <= 8) w.template run<1>(e, tile, tiles, count, rows, ahead, stage, sums, flip);
-    else if (kNT == 2 || count <= 16) w.template run<kNT < 2 ? 1 : 2>(e, tile, tiles, count, rows, ahead, stage, sums, flip);
-    else w.template run<kNT < 4 ? 1 : 4>(e, tile, tiles, count, rows, ahead, stage, sums, flip);
+    if (kNT == 1 || count <= 8) w.template compute<1>(e, place.tile, count, rows, ahead, stage, parity, sums, flip);
+    else w.template compute<kNT>(e, place.tile, count, rows, ahead, stage, parity, sums, flip);
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 template <int kPer, bool kZeros>
 size_t q4_smem(int experts) {
-  return static_cast<size_t>(kQ4Warps) * kStages * kPairTiles * record_bytes(kPer, kZeros) + 2 * kQ4Warps * 8 * kSumPitch * sizeof(float) +
+  return static_cast<size_t>(kQ4Warps) * kStages * kStageBlocks * record_bytes(kPer, kZeros) + 2 * kQ4Warps * 8 * kSumPitch * sizeof(float) +
          (4 * static_cast<size_t>(experts) + 1) * sizeof(int);
 }
 
-// The variants of a run: one for activations that are not read 16 bytes at a time, and for those that are,
-// by the most rows any expert can have: 8, 16, or more (the registers that 32 rows take cost the
-// smaller ones).
-enum Q4Variant { kQ4Narrow, kQ4Rows8, kQ4Rows16, kQ4Rows32, kQ4Variants };
+// The variants of a run: one for activations that are not read 16 bytes at a time, and two for those that
+// are: 8 rows at most, whose registers let the compiler order the block more freely, and 16 at a time (32 at a
+// time, in spilled registers, took 34 us where two chunks of 16, the second from L2, take 30).
+enum Q4Variant { kQ4Narrow, kQ4Rows8, kQ4Rows16, kQ4Variants };
 
 template <typename F>
 void with_variant(int v, F f) {
@@ -582,8 +588,7 @@ void with_variant(int v, F f) {
   using std::integral_constant;
   if (v == kQ4Narrow) f(integral_constant<int, 1>(), bool_constant<false>());
   else if (v == kQ4Rows8) f(integral_constant<int, 1>(), bool_constant<true>());
-  else if (v == kQ4Rows16) f(integral_constant<int, 2>(), bool_constant<true>());
-  else f(integral_constant<int, 4>(), bool_constant<true>());
+  else f(integral_constant<int, 2>(), bool_constant<true>());
 }
 
 template <typename F>
@@ -700,6 +705,7 @@ int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** o
   p.k = q.k;
   p.n_tiles = n_tiles;
   p.k_blocks = k_blocks;
+  p.timeout_ns = gg::wait_limit_ns();
   p.output_type = q.output_type;
   p.activation = q.activation;
   plan->bf16 = q.input_type == GG_INPUT_BF16;
@@ -727,7 +733,7 @@ int gg_q4_plan_run(gg_q4_plan* plan, const void* a, int lda, int a_rows, const i
   p.ldd = ldd;
   p.capacity_rows = capacity_rows;
   const bool vec = (reinterpret_cast<uintptr_t>(a) & 15u) == 0 && lda % 8 == 0 && p.k % 8 == 0;
-  const int variant = !vec ? gg::kQ4Narrow : capacity_rows <= 8 ? gg::kQ4Rows8 : capacity_rows <= 16 ? gg::kQ4Rows16 : gg::kQ4Rows32;
+  const int variant = !vec ? gg::kQ4Narrow : capacity_rows <= 8 ? gg::kQ4Rows8 : gg::kQ4Rows16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t st = cudaSuccess;
   gg::with_variant(variant, [&](auto nt, auto vec_c) {
