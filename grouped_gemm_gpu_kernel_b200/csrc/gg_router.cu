@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <cstring>
 #include <new>
 
 #include "gg_epilogue_ops.cuh"
@@ -63,11 +64,13 @@ __device__ __forceinline__ int group_max(int v) {
 // exp(x) for x <= 0: 2^-22 + |x| 2^-24 relative (the exponential unit, and the scaled argument's
 // rounding), and 0 below 2^-126. expf() costs four times the instructions for 2^-23, which a softmax
 // over logits rounded to 16 or 24 bits has no use for.
-__device__ __forceinline__ float exp_fast(float x) {
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_fast(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float exp_fast(float x) { return exp2_fast(x * kLog2e); }
 
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
@@ -114,7 +117,6 @@ constexpr int kBackwardBlocks = 4;  // of them an SM: the grid is one wave, and 
 
 constexpr int kForwardSmemMost = 160 * 1024;
 constexpr int kCandidates = 64;  // see choose_of_candidates
-
 // Slots a warp gathers before it places them: 32 (one a lane) or, where its tokens of one turn have more,
 // theirs. At least one turn, at most 32 tokens.
 __host__ __device__ __forceinline__ int slots_held(int at_once, int top_k) {
@@ -124,15 +126,15 @@ __host__ __device__ __forceinline__ int slots_held(int at_once, int top_k) {
 // Shared memory of a forward block, in 4-byte words: counts [warps][experts], sums of p
 // [warps][experts], per warp the held slots (index and key) and the factor of the weights and the
 // largest logit of their tokens (32 at most), z and valid tokens per warp; where a warp takes one
-// token at once, its candidates (key and expert).
+// token at once, its candidates (keys, then experts).
 size_t forward_smem(int G, int warps, int experts, int top_k) {
   return 4ull * (2ull * warps * experts + warps * (2ull * slots_held(32 / G, top_k) + 64) + 2ull * warps +
-                 (G == 32 ? 2ull * warps * kCandidates : 0));
+                 (G == 32 ? 2ull * kCandidates * warps : 0));
 }
 
 // Parts the blocks' counts are summed in: what the threads allow, so that each sums few rows.
 __host__ __device__ __forceinline__ int place_parts(int threads, int experts) {
-  const int p = threads / experts;
+  const int p = threads / (experts % 4 == 0 ? experts / 4 : experts);
   return p < 1 ? 1 : p > 16 ? 16 : p;
 }
 size_t place_smem(int threads, int experts) {
@@ -161,49 +163,89 @@ __device__ __forceinline__ float block_sum(float v, float* s_warp) {
   return s;
 }
 
-// Sums of rows b0, b0 + step, ... < rows of a [rows][E] table at column e, eight loads in flight (one
-// after the other, they would cost a trip to L2 each). `split`: also the sum of the rows below it.
-template <typename T>
-__device__ __forceinline__ T column_sum(const T* table, int E, int e, int b0, int step, int rows, int split, T* below) {
-  T total = 0, lower = 0;
-  for (int b = b0; b < rows; b += 8 * step) {
-    T c[8];
+// Sums over the rows of a [rows][E] table, N columns (1 or 4) and one of `parts` of the rows a thread, eight rows
+// loaded before the first is added (one after the other, they would cost a trip to L2 each). total and, where
+// given, below (the rows before `split`) become [parts][E] partial sums.
+template <int N, typename T>
+__device__ __forceinline__ void sum_rows(const T* table, int E, int rows, int parts, int split, T* total, T* below) {
+  const int columns = E / N;
+  for (int i = threadIdx.x; i < parts * columns; i += blockDim.x) {
+    const int part = i / columns, e = (i - part * columns) * N;
+    T all[N], low[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = b + i * step < rows ? table[static_cast<int64_t>(b + i * step) * E + e] : T(0);
+    for (int x = 0; x < N; ++x) all[x] = low[x] = T(0);
+    for (int b = part; b < rows; b += 8 * parts) {
+      T c[8][N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      total += c[i];
-      lower += b + i * step < split ? c[i] : T(0);
+      for (int r = 0; r < 8; ++r) {
+        const int at = b + r * parts;
+        const T* from = table + static_cast<int64_t>(at) * E + e;
+        if constexpr (N == 4) {
+          int4 q = make_int4(0, 0, 0, 0);
+          if (at < rows) q = *reinterpret_cast<const int4*>(from);
+          memcpy(c[r], &q, sizeof(q));
+        } else {
+          c[r][0] = at < rows ? *from : T(0);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+          all[x] += c[r][x];
+          low[x] += b + r * parts < split ? c[r][x] : T(0);
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      total[part * E + e + x] = all[x];
+      if (below) below[part * E + e + x] = low[x];
     }
   }
-  *below = lower;
-  return total;
 }
 
-// Turns the ranks of this block's slots into packed rows. smem: place_smem bytes. Block 0 also sums what
-// the blocks left behind into the counts, means and losses.
-__device__ void place_block(const PlaceArgs& a, int block, unsigned char* smem) {
+// Turns the ranks of a block's slots into packed rows (slots), and what the blocks left behind into the
+// counts, means and losses (losses). smem: place_smem bytes.
+__device__ void place_block(const PlaceArgs& a, int block, bool slots, bool losses, unsigned char* smem) {
   const int E = a.shape.experts, K = a.shape.top_k;
   const int tid = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
+  const int warps = threads / 32, warp = tid / 32, lane = tid % 32;
   const int parts = place_parts(threads, E);
-  int* s_before = reinterpret_cast<int*>(smem);  // [parts][E]
-  int* s_total = s_before + parts * E;           // [parts][E]
+  int* s_before = reinterpret_cast<int*>(smem);                   // [parts][E]
+  int* s_total = s_before + parts * E;                            // [parts][E]
   float* s_prob = reinterpret_cast<float*>(s_total + parts * E);  // [parts][E]
   int* s_base = reinterpret_cast<int*>(s_prob + parts * E);       // [E]
   int* s_sum = s_base + E;                                        // [E]
-  float* s_warp = reinterpret_cast<float*>(s_sum + E);
-  float z = 0.0f, n = 0.0f;
-  if (block == 0)
-    for (int b = tid; b < a.blocks; b += threads) z += a.work.block_z[2 * b], n += a.work.block_z[2 * b + 1];
-  for (int i = tid; i < parts * E; i += threads) {
-    const int part = i / E, e = i - part * E;
-    int before;
-    s_total[i] = column_sum(a.work.block_count, E, e, part, parts, a.blocks, block, &before);
-    s_before[i] = before;
-    if (block == 0) {
-      float none;
-      s_prob[i] = column_sum(a.work.block_prob, E, e, part, parts, a.blocks, 0, &none);
+  float* s_warp = reinterpret_cast<float*>(s_sum + E);            // [64]
+  int* first = reinterpret_cast<int*>(s_warp + 64) + warp * E;    // of every expert, the first row of this warp
+
+  // this warp's first slots and its experts' earlier rows, on their way during the sums
+  const int unit = block * warps + warp;
+  const int t0 = static_cast<int>(min(static_cast<int64_t>(a.tokens), static_cast<int64_t>(unit) * a.tokens_per_warp));
+  const int s_end = (a.tokens - t0 > a.tokens_per_warp ? t0 + a.tokens_per_warp : a.tokens) * K;
+  constexpr int kBatch = 4;  // slots a lane loads before it stores the first
+  int e_of[kBatch], rank[kBatch];
+  const auto load_slots = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const bool in = s_end - s0 > 32 * i;
+      e_of[i] = in ? a.indices[s0 + 32 * i] : -1;
+      rank[i] = in ? a.positions[s0 + 32 * i] : 0;
     }
+  };
+  if (slots) {
+    load_slots(t0 * K + lane);
+    for (int e = lane; e < E; e += 32) first[e] = a.work.warp_before[static_cast<int64_t>(unit) * E + e];
+  }
+  float z = 0.0f, n = 0.0f;
+  if (losses)
+    for (int b = tid; b < a.blocks; b += threads) z += a.work.block_z[2 * b], n += a.work.block_z[2 * b + 1];
+  if (E % 4 == 0) {
+    sum_rows<4>(a.work.block_count, E, a.blocks, parts, block, s_total, s_before);
+    if (losses) sum_rows<4>(a.work.block_prob, E, a.blocks, parts, 0, s_prob, static_cast<float*>(nullptr));
+  } else {
+    sum_rows<1>(a.work.block_count, E, a.blocks, parts, block, s_total, s_before);
+    if (losses) sum_rows<1>(a.work.block_prob, E, a.blocks, parts, 0, s_prob, static_cast<float*>(nullptr));
   }
   __syncthreads();
   for (int e = tid; e < E; e += threads) {
@@ -232,41 +274,28 @@ __device__ void place_block(const PlaceArgs& a, int block, unsigned char* smem) 
   __syncthreads();
   const int routed = __float_as_int(s_warp[32]);
 
-  const int warps = threads / 32, warp = tid / 32, lane = tid % 32;
-  const int64_t unit = static_cast<int64_t>(block) * warps + warp;
-  const int64_t t0 = min(static_cast<int64_t>(a.tokens), unit * a.tokens_per_warp);
-  const int64_t t1 = min(static_cast<int64_t>(a.tokens), t0 + a.tokens_per_warp);
-  int* first = reinterpret_cast<int*>(s_warp + 64) + warp * E;  // of every expert, the first row of this warp
-  for (int e = lane; e < E; e += 32) first[e] = s_base[e] + a.work.warp_before[unit * E + e];
-  __syncwarp();
-  constexpr int kBatch = 8;  // slots a lane loads before it stores the first
-  for (int64_t s0 = t0 * K + lane; s0 < t1 * K; s0 += 32 * kBatch) {
-    int e[kBatch], rank[kBatch];
+  if (slots) {
+    for (int s0 = t0 * K + lane; s0 < s_end; s0 += 32 * kBatch) {
+      if (s0 != t0 * K + lane) load_slots(s0);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int64_t s = s0 + 32 * i;
-      e[i] = s < t1 * K ? a.indices[s] : -1;
-      rank[i] = s < t1 * K ? a.positions[s] : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int64_t s = s0 + 32 * i;
-      if (s >= t1 * K) break;
-      int p = -1;
-      if (e[i] >= 0) {
-        p = first[e[i]] + rank[i];
-        if (a.row_tokens) a.row_tokens[p] = static_cast<int>(static_cast<unsigned>(s) / static_cast<unsigned>(K));
+      for (int i = 0; i < kBatch; ++i) {
+        const int s = s0 + 32 * i, e = e_of[i];
+        if (s_end - s0 <= 32 * i) break;
+        int p = -1;
+        if (e >= 0) {
+          p = s_base[e] + first[e] + rank[i];
+          if (a.row_tokens) a.row_tokens[p] = static_cast<int>(static_cast<unsigned>(s) / static_cast<unsigned>(K));
+        }
+        a.positions[s] = p;
       }
-      a.positions[s] = p;
+      if (s_end - s0 <= 32 * kBatch) break;
     }
+    if (a.row_tokens)
+      for (int64_t s = routed + static_cast<int64_t>(block) * threads + tid; s < static_cast<int64_t>(a.tokens) * K;
+           s += static_cast<int64_t>(a.blocks) * threads)
+        a.row_tokens[s] = -1;
   }
-  if (a.row_tokens) {
-    const int64_t slots = static_cast<int64_t>(a.tokens) * K;
-    for (int64_t s = routed + static_cast<int64_t>(block) * threads + tid; s < slots;
-         s += static_cast<int64_t>(a.blocks) * threads)
-      a.row_tokens[s] = -1;
-  }
-  if (block != 0) return;
+  if (!losses) return;
 
   z = block_sum(z, s_warp);
   n = block_sum(n, s_warp);
@@ -303,44 +332,81 @@ struct ForwardArgs {
 // The top_k largest keys of a token that a whole warp holds, V consecutive experts a lane, when
 // top_k <= 8: the smallest of the maxima of eight groups of four lanes bounds the 8th largest key from below,
 // so only keys from it on are candidates. On random logits that leaves about 22 (the draws until
-// every group was hit). They are gathered, two a lane at most, and then each round compares two keys
-// a lane instead of V: measured 1.9x over the rounds on all keys at 256 experts, top 8. Lane j gets the expert
-// and key of slot j (expert -1: none). False: more candidates than fit, nothing is chosen.
+// every group was hit). They are gathered in shared memory in the order of experts, one a lane (two where they are
+// more than 32), and each lane counts the keys above its own: that is its slot. The counts depend on no
+// other lane's, unlike rounds that take one maximum after the other (131072 tokens of 256 experts, top 8, forward:
+// XX us against 105 us with such rounds on the candidates). Equal keys give a slot twice, and leave one empty unless it is the last; then, and
+// only then, the keys before a lane's own are counted from its own on. Writes the slots and returns the
+// lane's part of the sum of exp(key - top); fits: false where there are more than kCandidates, and nothing is written.
+// The keys in list[0, n) (a multiple of 8 is read; those past n are kTaken) above `own`, which is at `at`; with
+// `ties` the equal ones before it as well.
+__device__ __forceinline__ int keys_above(const int* list, int n, int own, int at, bool ties) {
+  int rank = 0;
+  if (!ties) {
+    for (int c = 0; c < n; c += 8) {
+      const int4 x = *reinterpret_cast<const int4*>(list + c), y = *reinterpret_cast<const int4*>(list + c + 4);
+      const int k[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        asm("{ .reg .pred p; setp.gt.s32 p, %1, %2; @p add.s32 %0, %0, 1; }" : "+r"(rank) : "r"(k[i]), "r"(own));
+    }
+  } else {
+    for (int c = 0; c < n; ++c) rank += list[c] > (c < at ? own - 1 : own);
+  }
+  return rank;
+}
+
 template <int V>
-__device__ __forceinline__ bool choose_of_candidates(const int (&key)[V], int mine, int e0, int K, int2* s_candidates, int lane,
-                                                     int* slot_expert, int* slot_key) {
+__device__ __forceinline__ float choose_of_candidates(const int (&key)[V], int mine, int e0, int K, int* s_list, unsigned list, int lane,
+                                                      int* s_slot, int* s_key, float top, bool* fits) {
   int bound = max(mine, __shfl_xor_sync(kFull, mine, 1));
   bound = max(bound, __shfl_xor_sync(kFull, bound, 2));
   bound = max(__reduce_min_sync(kFull, bound), kClosed + 1);
-  unsigned in = 0;
-#pragma unroll
-  for (int i = 0; i < V; ++i) in |= key[i] >= bound ? 1u << i : 0u;
-  int upto = __popc(in);
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int up = __shfl_up_sync(kFull, upto, d);
-    upto += lane >= d ? up : 0;
-  }
-  const int n = __shfl_sync(kFull, upto, 31);
-  if (n > kCandidates) return false;
-  int2* to = s_candidates + upto - __popc(in);
+  int upto = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i)
-    if (in >> i & 1u) *to++ = make_int2(key[i], e0 + i);
+    asm("{ .reg .pred p; setp.ge.s32 p, %1, %2; @p add.s32 %0, %0, 1; }" : "+r"(upto) : "r"(key[i]), "r"(bound));
+  const int count = upto;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1)
+    asm volatile("{ .reg .s32 r; .reg .pred p; shfl.sync.up.b32 r|p, %0, %1, 0, -1; @p add.s32 %0, %0, r; }" : "+r"(upto) : "r"(d));
+  const int n = __shfl_sync(kFull, upto, 31);
+  *fits = n <= kCandidates;
+  if (n > kCandidates) return 0.0f;
+  // `list`: s_list as a shared address; keys, then kCandidates words further their experts
+  unsigned to = list + 4 * (upto - count);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    asm volatile("{ .reg .pred p; setp.ge.s32 p, %1, %2; @p st.shared.s32 [%0], %1; @p st.shared.s32 [%0 + %4], %3; @p add.u32 %0, %0, 4; }"
+                 : "+r"(to)
+                 : "r"(key[i]), "r"(bound), "r"(e0 + i), "n"(4 * kCandidates)
+                 : "memory");
+  if (lane < 8 && n + lane < kCandidates) s_list[n + lane] = kTaken;
   __syncwarp();
-  int2 a = make_int2(kTaken, INT32_MAX), b = a;
-  if (lane < n) a = s_candidates[lane];
-  if (lane + 32 < n) b = s_candidates[lane + 32];
-  for (int j = 0; j < K; ++j) {
-    const int best = __reduce_max_sync(kFull, max(a.x, b.x));
-    // the lowest expert of those that hold it (the candidates are in no order of experts)
-    const int e = best == kTaken ? -1
-                                 : __reduce_min_sync(kFull, min(a.x == best ? a.y : INT32_MAX, b.x == best ? b.y : INT32_MAX));
-    if (lane == j) *slot_expert = e, *slot_key = best;
-    if (a.y == e) a.x = kTaken;
-    if (b.y == e) b.x = kTaken;
+  const int slots = min(K, n);
+  float part = 0.0f;
+  bool ties = false;
+  while (true) {
+    int taken = 0, takers = 0;
+    part = 0.0f;
+    for (int first = 0; first < n; first += 32) {
+      const int at = first + lane, own = at < n ? s_list[at] : kTaken;
+      const int rank = keys_above(s_list, n, own, at, ties);
+      const bool in = at < n && rank < K;
+      takers += __popc(__ballot_sync(kFull, in));
+      if (in) {
+        taken |= 1 << rank;
+        s_slot[rank] = s_list[kCandidates + at];
+        s_key[rank] = own;
+        part += exp_fast(key_value(own) - top);
+      }
+    }
+    if (ties || (takers == slots && __reduce_or_sync(kFull, taken) == (1 << slots) - 1)) break;
+    ties = true;
+    __syncwarp();
   }
-  return true;
+  if (lane >= n && lane < K) s_slot[lane] = -1, s_key[lane] = kTaken;  // fewer experts than slots
+  return part;
 }
 
 template <int F, int G, int V, int W>
@@ -350,8 +416,8 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
   const int E = a.place.shape.experts, K = a.place.shape.top_k, T = a.place.tokens;
   const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
   const int group = lane / G, gl = lane % G;
-  int2* s_candidates = reinterpret_cast<int2*>(smem) + warp * kCandidates;
-  int* s_count = reinterpret_cast<int*>(smem + (G == 32 ? 8 * kWarps * kCandidates : 0));
+  int* s_list = reinterpret_cast<int*>(smem) + warp * 2 * kCandidates;
+  int* s_count = reinterpret_cast<int*>(smem + (G == 32 ? 8 * kCandidates * kWarps : 0));
   float* s_prob = reinterpret_cast<float*>(s_count + kWarps * E);
   const int held = slots_held(kAtOnce, K);  // slots a warp keeps until it places them together
   int* s_slot = reinterpret_cast<int*>(s_prob + kWarps * E) + warp * (2 * held + 64);
@@ -362,11 +428,14 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
   for (int e = lane; e < E; e += 32) count[e] = 0;
   __syncwarp();
 
+  // this warp's tokens (the host keeps tokens * top_k in an int)
   const int per_warp = a.place.tokens_per_warp;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
-  const int64_t t0 = min(static_cast<int64_t>(T), unit * per_warp);
-  const int64_t t1 = min(static_cast<int64_t>(T), t0 + per_warp);
+  const int unit = static_cast<int>(blockIdx.x) * kWarps + warp;
+  const int t0 = static_cast<int>(min(static_cast<int64_t>(T), static_cast<int64_t>(unit) * per_warp));
+  const int t1 = T - t0 > per_warp ? t0 + per_warp : T;
   const int e0 = gl * V, have = max(0, min(V, E - e0));
+  const char* row = static_cast<const char*>(a.logits) + ((t0 + group) * a.ld + e0) * OutFormat<F>::kBytes;
+  const int64_t next_row = kAtOnce * a.ld * OutFormat<F>::kBytes;
   float prob[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) prob[i] = 0.0f;
@@ -376,14 +445,17 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
   const int turns = max(1, 32 / (kAtOnce * K));
   const int lane_token = lane / K;  // the held token of this lane's slot among the first 32
   int turn = 0;
-  int64_t th = t0;
-  for (int64_t tb = t0; tb < t1; tb += kAtOnce) {
-    const int64_t t = tb + group;
+  int th = t0;
+  for (int tb = t0; tb < t1; tb += kAtOnce, row += next_row) {
+    const int t = tb + group;
     const int slot0 = (turn * kAtOnce + group) * K;
-    const bool live = t < t1 && (a.mask == nullptr || a.mask[t] != 0);
     float v[V];
     int key[V];
-    load_row<F, V>(a.logits, t * a.ld + e0, live ? have : 0, a.vec != 0, -INFINITY, v);
+    load_row<F, V>(row, 0, t < t1 ? have : 0, a.vec != 0, -INFINITY, v);
+    if (a.mask != nullptr && t < t1 && a.mask[t] == 0) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = -INFINITY;
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) key[i] = order_key(v[i]);
     int mine = key[0];
@@ -392,16 +464,12 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
     const int largest = group_max<G>(mine);
     const bool valid = largest > kClosed;
     const float top = key_value(largest);
-    float chosen = 0.0f;
+    float chosen = 0.0f;  // the sum of exp(logit - top) over the chosen experts
     bool done = false;
     if constexpr (G == 32) {
       if (K >= 4 && K <= 8) {
-        int slot_expert = -1, slot_key = kTaken;
-        done = choose_of_candidates<V>(key, mine, e0, K, s_candidates, lane, &slot_expert, &slot_key);
-        if (done) {
-          if (lane < K) s_slot[slot0 + lane] = slot_expert, s_key[slot0 + lane] = slot_key;
-          chosen = group_sum<32>(slot_expert >= 0 ? exp_fast(key_value(slot_key) - top) : 0.0f);
-        }
+        chosen = choose_of_candidates<V>(key, mine, e0, K, s_list, static_cast<unsigned>(__cvta_generic_to_shared(s_list)), lane, s_slot + slot0, s_key + slot0, top, &done);
+        chosen = group_sum<32>(chosen);
       }
     }
     if (!done) {
@@ -427,11 +495,14 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
         best = group_max<G>(mine);
       }
     }
+    // exp(v - top) as 2^(v log2(e) - top log2(e)): the rounding of the second product is the same factor in all
+    // terms and in the sum. Without a valid logit all of them are -infinity, and give 0.
     float sum = 0.0f;
     float ex[V];
+    const float shift = valid ? -top * kLog2e : 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      ex[i] = i < have && valid ? exp_fast(v[i] - top) : 0.0f;
+      ex[i] = exp2_fast(fmaf(v[i], kLog2e, shift));
       sum += ex[i];
     }
     sum = group_sum<G>(sum);
@@ -449,7 +520,7 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
     __syncwarp();
     if (++turn < turns && tb + kAtOnce < t1) continue;
     // the slots of the held tokens, in order, 32 at a time
-    const int slots = static_cast<int>(min(t1, tb + kAtOnce) - th) * K;
+    const int slots = (min(t1, tb + kAtOnce) - th) * K;
     for (int s0 = 0; s0 < slots; s0 += 32) {
       const int s = s0 + lane;
       const int e = s < slots ? s_slot[s] : -1;
@@ -460,7 +531,7 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
       __syncwarp();
       if (s < slots) {
         const int h = s0 == 0 ? lane_token : s / K;
-        const int64_t at = th * K + s;
+        const int at = th * K + s;
         a.indices[at] = e;
         a.weights[at] = e >= 0 ? exp_fast(key_value(s_key[s]) - s_factor[32 + h]) * s_factor[h] : 0.0f;
         a.place.positions[at] = seen + __popc(same & ((1u << lane) - 1u));
@@ -505,7 +576,7 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
   }
   if (gridDim.x == 1) {
     __syncthreads();
-    place_block(a.place, 0, smem);
+    place_block(a.place, 0, true, true, smem);
   }
 }
 
@@ -514,7 +585,8 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
 __global__ void __launch_bounds__(1024) router_place_kernel(PlaceArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   cudaGridDependencySynchronize();
-  place_block(a, static_cast<int>(blockIdx.x), smem);
+  const int block = static_cast<int>(blockIdx.x);
+  place_block(a, block, block < a.blocks, block == a.blocks, smem);  // the last block, without slots, sums the losses
 }
 
 struct BackwardArgs {
@@ -764,7 +836,7 @@ int gg_router_run(gg_router* router, const gg_route* route, void* stream) {
         st = cudaGetLastError();
         if (st != cudaSuccess || blocks == 1) return;
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+        cfg.gridDim = dim3(static_cast<unsigned>(blocks + 1));
         cfg.blockDim = dim3(32 * warps);
         cfg.dynamicSmemBytes = place;
         cfg.stream = s;
