@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
@@ -21,6 +22,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB_NAME = "libgrouped_gemm_b200.so"
 LIB_PATH = os.path.join(PKG, LIB_NAME)
+CALLS_PATH = os.path.join(PKG, "_moe_native.so")  # the Python calls of the mixture-of-experts operators
 BUILD_DIR = os.path.join(PKG, "_build")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -66,7 +68,7 @@ def _deps():
 
 def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) -> str:
     deps = _deps()
-    if not force and not ptxas_info and _newer(LIB_PATH, deps + [__file__]):
+    if not force and not ptxas_info and _newer(LIB_PATH, deps + [__file__]) and _newer(CALLS_PATH, deps + [__file__]):
         return LIB_PATH
     os.makedirs(BUILD_DIR, exist_ok=True)
     cc = nvcc()
@@ -82,6 +84,12 @@ def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) 
     tmp = LIB_PATH + ".tmp"
     _run([cc, *ARCH, "-shared", "-o", tmp, *objs, "-lcudart_static", "-ldl", "-lrt", "-lpthread"], verbose)
     os.replace(tmp, LIB_PATH)
+    # a CPython module on top of the library, which it finds beside itself
+    tmp = CALLS_PATH + ".tmp"
+    cxx = shutil.which("g++") or "g++"
+    _run([cxx, "-std=c++17", "-O2", "-Wall", "-shared", "-fPIC", "-I" + INCLUDE, "-I" + sysconfig.get_paths()["include"],
+          os.path.join(CSRC, "moe_python.cpp"), "-o", tmp, "-L" + PKG, "-l:" + LIB_NAME, "-Wl,-rpath,$ORIGIN"], verbose)
+    os.replace(tmp, CALLS_PATH)
     return LIB_PATH
 
 

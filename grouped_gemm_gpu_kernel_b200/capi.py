@@ -192,9 +192,8 @@ def load() -> ctypes.CDLL:
         "gg_device_plan_prepared": ([vp, i32p, i32p, ctypes.c_int], ctypes.c_int),
         "gg_device_plan_destroy": ([vp], None),
         "gg_router_create": ([P(GGRouterConfig), P(vp)], ctypes.c_int),
-        # a pointer to the struct, or its bytes
-        "gg_router_run": ([vp, vp, vp], ctypes.c_int),
-        "gg_router_backward": ([vp, vp, vp], ctypes.c_int),
+        "gg_router_run": ([vp, P(GGRoute), vp], ctypes.c_int),
+        "gg_router_backward": ([vp, P(GGRouteGradient), vp], ctypes.c_int),
         "gg_router_destroy": ([vp], None),
         "gg_moe_dispatch": ([vp, ctypes.c_int, vp] + [ctypes.c_int] * 4 + [vp, ctypes.c_int, ctypes.c_int, vp],
                             ctypes.c_int),

@@ -23,7 +23,6 @@
 #include <cstdint>
 #include <new>
 #include <type_traits>
-#include <vector>
 
 #include "gg_epilogue_ops.cuh"
 #include "gg_internal.h"
@@ -649,7 +648,7 @@ int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** o
   gg_q4_plan* plan = new (std::nothrow) gg_q4_plan();
   if (!plan) return cudaErrorMemoryAllocation;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  std::vector<const void*> tables(3 * E);
+  const void* tables[3 * GG_Q4_MAX_EXPERTS];
   for (size_t e = 0; e < E; ++e) {
     tables[e] = q.q[e];
     tables[E + e] = q.scales[e];
@@ -676,7 +675,7 @@ int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** o
     return st;
   }
   unsigned char* base = static_cast<unsigned char*>(plan->block);
-  st = cudaMemcpyAsync(base + tables_at, tables.data(), tables.size() * sizeof(void*), cudaMemcpyHostToDevice, s);
+  st = cudaMemcpyAsync(base + tables_at, tables, 3 * E * sizeof(void*), cudaMemcpyHostToDevice, s);
   if (st == cudaSuccess && q.bias)
     st = cudaMemcpyAsync(base + bias_at, q.bias, E * sizeof(void*), cudaMemcpyHostToDevice, s);
   if (st == cudaSuccess) st = cudaMemsetAsync(base + status_at, 0, tables_at - status_at, s);

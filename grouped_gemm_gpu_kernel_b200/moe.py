@@ -15,38 +15,25 @@ constructors and tensor mismatches raise ValueError.
 from __future__ import annotations
 
 import ctypes
-import struct
+import importlib
 from typing import Optional, Sequence
 
 from . import capi
 
-_types = {}  # torch dtype -> GG_OUTPUT_*
-_f32 = _i32 = None
-_masks = ()
-
-# The checks below run before every launch, which a decoding step makes some ten of: each reads an attribute of a
-# tensor once (some 50 to 100 ns apiece), and the C structs are filled by one struct.pack.
-_ROUTE = struct.Struct("@10P2i")
-_ROUTE_GRADIENT = struct.Struct("@9P3i4x")
+_calls = None
 
 
-def _load_types():
-    global _f32, _i32, _masks
-    import torch
-
-    _types[torch.float32] = capi.GG_OUTPUT_F32
-    _types[torch.float16] = capi.GG_OUTPUT_F16
-    _types[torch.bfloat16] = capi.GG_OUTPUT_BF16
-    _f32, _i32, _masks = torch.float32, torch.int32, (torch.uint8, torch.bool)
-
-
-def _type_of(t, name: str) -> int:
-    if _f32 is None:
-        _load_types()
-    v = _types.get(t.dtype)
-    if v is None:
-        raise ValueError(f"{name}: float32, float16 or bfloat16 expected, got {t.dtype}")
-    return v
+def _native():
+    """The module that checks the tensors and makes the calls (csrc/moe_python.cpp; raises when it has not been built)."""
+    global _calls
+    if _calls is None:
+        capi.load()
+        try:
+            _calls = importlib.import_module("._moe_native", __package__)
+        except ImportError as e:
+            raise RuntimeError("the calls of the mixture-of-experts operators are missing; build them with "
+                               f"`python -m grouped_gemm_gpu_kernel_b200.build` ({e})") from e
+    return _calls
 
 
 def _stream(stream) -> Optional[int]:
@@ -55,31 +42,6 @@ def _stream(stream) -> Optional[int]:
     if isinstance(stream, int):
         return stream or None
     return getattr(stream, "cuda_stream", None) or None
-
-
-def _shape(t, name: str):
-    s = t.shape
-    if len(s) != 2:
-        raise ValueError(f"{name}: two dimensions expected, got {tuple(s)}")
-    return s
-
-
-def _pitch(t, rows: int, cols: int, name: str) -> int:
-    """The row pitch of a rows x cols device tensor with contiguous columns."""
-    if t.shape != (rows, cols):
-        raise ValueError(f"{name}: shape ({rows}, {cols}) expected, got {tuple(t.shape)}")
-    r, c = t.stride()
-    if (c != 1 and cols > 1) or (r < cols and rows > 1) or not t.is_cuda:
-        raise ValueError(f"{name}: a CUDA tensor with contiguous columns and rows that do not overlap expected")
-    return r if r >= cols and r > 0 else max(1, cols)
-
-
-def _packed(t, count: int, dtype, name: str) -> int:
-    """The address of a contiguous device tensor of `count` elements."""
-    if t.dtype is not dtype or t.numel() != count or not t.is_contiguous() or not t.is_cuda:
-        raise ValueError(f"{name}: a contiguous CUDA {dtype} tensor of {count} elements expected, got "
-                         f"{t.dtype} {tuple(t.shape)}")
-    return t.data_ptr()
 
 
 class MoeRouter:
@@ -93,7 +55,7 @@ class MoeRouter:
     def __init__(self, experts: int, top_k: int, capacity_tokens: int, logit_type: int = capi.GG_OUTPUT_F32,
                  normalize: bool = True):
         self._lib = capi.load()
-        self._h = None
+        self._h, self._p = None, 0
         cfg = capi.GGRouterConfig(int(experts), int(top_k), int(capacity_tokens), int(logit_type), 1 if normalize else 0)
         h = ctypes.c_void_p()
         st = self._lib.gg_router_create(ctypes.byref(cfg), ctypes.byref(h))
@@ -102,6 +64,8 @@ class MoeRouter:
         self._h = h
         self.experts, self.top_k, self.capacity_tokens = int(experts), int(top_k), int(capacity_tokens)
         self.logit_type = int(logit_type)
+        self._run, self._backward = _native().router_run, _native().router_backward
+        self._p = h.value
 
     def run(self, logits, indices, weights, positions, rows, losses, row_tokens=None, lse=None, prob_mean=None,
             token_mask=None, stream=None) -> int:
@@ -109,49 +73,20 @@ class MoeRouter:
         (tokens, top_k); rows (int32, experts); losses (float32, 3); optional row_tokens (int32,
         tokens * top_k), lse (float32, tokens), prob_mean (float32, experts). token_mask: uint8 or bool
         (tokens), zero where a token is not routed."""
-        if not self._h:
-            return capi.CUDA_ERROR_INVALID_DEVICE_POINTER
-        if _type_of(logits, "logits") != self.logit_type:
-            raise ValueError(f"logits: the router was made for another type than {logits.dtype}")
-        t, e = _shape(logits, "logits")[0], self.experts
-        slots = t * self.top_k
-        ld = _pitch(logits, t, e, "logits")
-        mask = 0
-        if token_mask is not None:
-            if token_mask.dtype not in _masks or token_mask.numel() != t or not token_mask.is_contiguous() or not token_mask.is_cuda:
-                raise ValueError("token_mask: one contiguous CUDA uint8 or bool per token expected")
-            mask = token_mask.data_ptr()
-        q = _ROUTE.pack(logits.data_ptr(), mask, _packed(indices, slots, _i32, "indices"),
-                        _packed(weights, slots, _f32, "weights"), _packed(positions, slots, _i32, "positions"),
-                        _packed(rows, e, _i32, "rows"), _packed(losses, 3, _f32, "losses"),
-                        0 if row_tokens is None else _packed(row_tokens, slots, _i32, "row_tokens"),
-                        0 if lse is None else _packed(lse, t, _f32, "lse"),
-                        0 if prob_mean is None else _packed(prob_mean, e, _f32, "prob_mean"), t, ld)
-        return self._lib.gg_router_run(self._h, q, _stream(stream))
+        return self._run(self._p, self.experts, self.top_k, self.logit_type, logits, indices, weights, positions, rows, losses,
+                         row_tokens, lse, prob_mean, token_mask, stream)
 
     def backward(self, logits, indices, weights, rows, losses, lse, grad_weights, grad_losses, grad_logits,
                  stream=None) -> int:
         """grad_logits from the run's inputs and outputs, the gradient of its weights (float32, tokens x
         top_k, or None) and of losses[0] and losses[1] (float32, 2, or None)."""
-        if not self._h:
-            return capi.CUDA_ERROR_INVALID_DEVICE_POINTER
-        if _type_of(logits, "logits") != self.logit_type or grad_logits.dtype is not logits.dtype:
-            raise ValueError("logits, grad_logits: the router's type expected")
-        t, e = _shape(logits, "logits")[0], self.experts
-        slots = t * self.top_k
-        ld, ldg = _pitch(logits, t, e, "logits"), _pitch(grad_logits, t, e, "grad_logits")
-        q = _ROUTE_GRADIENT.pack(logits.data_ptr(), _packed(indices, slots, _i32, "indices"),
-                                 _packed(weights, slots, _f32, "weights"), _packed(rows, e, _i32, "rows"),
-                                 _packed(losses, 3, _f32, "losses"), _packed(lse, t, _f32, "lse"),
-                                 0 if grad_weights is None else _packed(grad_weights, slots, _f32, "grad_weights"),
-                                 0 if grad_losses is None else _packed(grad_losses, 2, _f32, "grad_losses"),
-                                 grad_logits.data_ptr(), t, ld, ldg)
-        return self._lib.gg_router_backward(self._h, q, _stream(stream))
+        return self._backward(self._p, self.experts, self.top_k, self.logit_type, logits, indices, weights, rows, losses, lse,
+                              grad_weights, grad_losses, grad_logits, stream)
 
     def close(self):
         if self._h:
             self._lib.gg_router_destroy(self._h)
-            self._h = None
+            self._h, self._p = None, 0
 
     def __del__(self):
         try:
@@ -160,56 +95,22 @@ class MoeRouter:
             pass
 
 
-def _slots(positions, tokens: int) -> int:
-    t, k = _shape(positions, "positions")
-    if t != tokens:
-        raise ValueError(f"positions: ({tokens}, top_k) expected, got ({t}, {k})")
-    return k
-
-
 def moe_dispatch(x, positions, packed, stream=None) -> int:
     """packed[positions[t, j]] = x[t]: x (tokens, width), packed (rows, width), of one dtype of 1, 2 or 4
     bytes; positions (tokens, top_k) int32, entries outside packed's rows go nowhere."""
-    if _f32 is None:
-        _load_types()
-    t, w = _shape(x, "x")
-    k = _slots(positions, t)
-    if packed.dtype is not x.dtype:
-        raise ValueError("x, packed: one dtype expected")
-    r = _shape(packed, "packed")[0]
-    ldx, ldp = _pitch(x, t, w, "x"), _pitch(packed, r, w, "packed")
-    return capi.load().gg_moe_dispatch(x.data_ptr(), ldx, _packed(positions, t * k, _i32, "positions"), t, k, w,
-                                       x.element_size(), packed.data_ptr(), r, ldp, _stream(stream))
+    return (_calls or _native()).dispatch(x, positions, packed, stream)
 
 
 def moe_combine(packed, positions, out, weights=None, stream=None) -> int:
     """out[t] = sum over j of weights[t, j] * packed[positions[t, j]] (weights None: 1, the gradient of
     moe_dispatch); weights float32 (tokens, top_k)."""
-    pt, ot = _type_of(packed, "packed"), _type_of(out, "out")
-    t, w = _shape(out, "out")
-    k = _slots(positions, t)
-    r = _shape(packed, "packed")[0]
-    ldp, ldo = _pitch(packed, r, w, "packed"), _pitch(out, t, w, "out")
-    return capi.load().gg_moe_combine(packed.data_ptr(), pt, r, ldp, _packed(positions, t * k, _i32, "positions"),
-                                      None if weights is None else _packed(weights, t * k, _f32, "weights"), t, k, w,
-                                      out.data_ptr(), ot, ldo, _stream(stream))
+    return (_calls or _native()).combine(packed, positions, out, weights, stream)
 
 
 def moe_combine_backward(grad_out, packed, positions, weights, grad_packed, grad_weights, stream=None) -> int:
     """The gradients of moe_combine with weights: grad_packed (like packed) and grad_weights (float32,
     tokens x top_k)."""
-    ot, pt = _type_of(grad_out, "grad_out"), _type_of(packed, "packed")
-    t, w = _shape(grad_out, "grad_out")
-    k = _slots(positions, t)
-    r = _shape(packed, "packed")[0]
-    if grad_packed.dtype is not packed.dtype:
-        raise ValueError("packed, grad_packed: one dtype expected")
-    ldo, ldp, ldgp = (_pitch(grad_out, t, w, "grad_out"), _pitch(packed, r, w, "packed"),
-                      _pitch(grad_packed, r, w, "grad_packed"))
-    return capi.load().gg_moe_combine_backward(
-        grad_out.data_ptr(), ot, ldo, packed.data_ptr(), pt, r, ldp, _packed(positions, t * k, _i32, "positions"),
-        _packed(weights, t * k, _f32, "weights"), t, k, w, grad_packed.data_ptr(), ldgp,
-        _packed(grad_weights, t * k, _f32, "grad_weights"), _stream(stream))
+    return (_calls or _native()).combine_backward(grad_out, packed, positions, weights, grad_packed, grad_weights, stream)
 
 
 class Q4Plan:
@@ -227,7 +128,7 @@ class Q4Plan:
                  bias_ptrs: Optional[Sequence[Optional[int]]] = None, input_type: int = capi.GG_INPUT_F16,
                  output_type: int = capi.GG_OUTPUT_F32, activation: int = capi.GG_ACT_NONE, stream=None):
         self._lib = capi.load()
-        self._h = None
+        self._h, self._p = None, 0
         tables = []
         for name, ptrs in (("q", q_ptrs), ("scale", scale_ptrs), ("zero", zero_ptrs), ("bias", bias_ptrs)):
             if ptrs is None:
@@ -246,21 +147,13 @@ class Q4Plan:
         self._h = h
         self.experts, self.n, self.k = int(experts), int(n), int(k)
         self.input_type, self.output_type = int(input_type), int(output_type)
+        self._run = _native().q4_run
+        self._p = h.value
 
     def run(self, a, rows, d, row_tokens=None, stream=None) -> int:
         """a (a_rows, k); rows: int32 device tensor of `experts` counts (None with one expert: all rows of
         d); d (capacity rows, n). row_tokens: int32, one per row of d, the row of `a` that it reads."""
-        if not self._h:
-            return capi.CUDA_ERROR_INVALID_DEVICE_POINTER
-        if _type_of(a, "a") != (capi.GG_OUTPUT_F16 if self.input_type == capi.GG_INPUT_F16 else capi.GG_OUTPUT_BF16):
-            raise ValueError(f"a: the plan was made for another type than {a.dtype}")
-        if _type_of(d, "d") != self.output_type:
-            raise ValueError(f"d: the plan was made for another type than {d.dtype}")
-        ar, cap = _shape(a, "a")[0], _shape(d, "d")[0]
-        lda, ldd = _pitch(a, ar, self.k, "a"), _pitch(d, cap, self.n, "d")
-        return self._lib.gg_q4_plan_run(
-            self._h, a.data_ptr(), lda, ar, None if row_tokens is None else _packed(row_tokens, cap, _i32, "row_tokens"),
-            None if rows is None else _packed(rows, self.experts, _i32, "rows"), d.data_ptr(), ldd, cap, _stream(stream))
+        return self._run(self._p, self.experts, self.n, self.k, self.input_type, self.output_type, a, rows, d, row_tokens, stream)
 
     def status(self) -> int:
         """Synchronises; returns (then clears) the GG_STATUS_* bits of the plan's runs."""
@@ -273,7 +166,7 @@ class Q4Plan:
     def close(self):
         if self._h:
             self._lib.gg_q4_plan_destroy(self._h)
-            self._h = None
+            self._h, self._p = None, 0
 
     def __del__(self):
         try:
