@@ -111,6 +111,7 @@ __device__ __forceinline__ void load_row(const void* base, int64_t at, int have,
 
 // Warps of a forward block (one block an SM): as many as the registers of V experts a lane allow.
 __host__ __device__ constexpr int router_warps(int V) { return V <= 8 ? 32 : V <= 16 ? 16 : 8; }
+constexpr int kClusterMost = 8;   // blocks of a cluster that any launch may ask for
 constexpr int kFewWarps = 4;  // of a forward block that takes few tokens
 constexpr int kBackwardWarps = 8;
 constexpr int kBackwardBlocks = 4;  // of them an SM: the grid is one wave, and a warp walks its tokens
@@ -145,6 +146,7 @@ struct PlaceArgs {
   RouterShape shape;
   RouterWork work;
   int tokens, tokens_per_warp, blocks;
+  int cluster;  // blocks of the forward kernel's one cluster; 0: it has none, and a second kernel places the slots
   const int* indices;
   int* positions;
   int* rows;
@@ -561,10 +563,18 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
   for (int e = tid; e < E; e += 32 * kWarps) {
     int run = 0;
     float p = 0.0f;
-    for (int i = 0; i < kWarps; ++i) {
-      w.warp_before[(static_cast<int64_t>(blockIdx.x) * kWarps + i) * E + e] = run;
-      run += s_count[i * E + e];
-      p += s_prob[i * E + e];
+    static_assert(kWarps % 4 == 0, "four warps' numbers are read before the first is used");
+    for (int i0 = 0; i0 < kWarps; i0 += 4) {
+      int c[4];
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = s_count[(i0 + i) * E + e], f[i] = s_prob[(i0 + i) * E + e];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w.warp_before[(static_cast<int64_t>(blockIdx.x) * kWarps + i0 + i) * E + e] = run;
+        run += c[i];
+        p += f[i];
+      }
     }
     w.block_count[static_cast<int64_t>(blockIdx.x) * E + e] = run;
     w.block_prob[static_cast<int64_t>(blockIdx.x) * E + e] = p;
@@ -574,9 +584,10 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
     for (int i = 0; i < kWarps; ++i) sum += s_z[2 * i + tid];
     w.block_z[2 * blockIdx.x + tid] = sum;
   }
-  if (gridDim.x == 1) {
-    __syncthreads();
-    place_block(a.place, 0, true, true, smem);
+  if (a.place.cluster > 0) {  // the grid is one cluster: its blocks meet here, and place their own slots
+    if (a.place.cluster == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    place_block(a.place, static_cast<int>(blockIdx.x), true, blockIdx.x == 0, smem);
   }
 }
 
@@ -815,10 +826,16 @@ int gg_router_run(gg_router* router, const gg_route* route, void* stream) {
       constexpr int G = g(), V = v(), at_once = 32 / G;
       const auto launch = [&](auto warps_c) {
         constexpr int warps = warps_c();
-        // tokens a warp: whole turns, as few as fill the blocks
-        const int64_t share = (static_cast<int64_t>(q.tokens) + gg::kMaxBlocks * warps - 1) / (gg::kMaxBlocks * warps);
-        const int64_t per_warp = std::max<int64_t>(1, (share + at_once - 1) / at_once) * at_once;
-        const int blocks = static_cast<int>(std::max<int64_t>(1, (q.tokens + per_warp * warps - 1) / (per_warp * warps)));
+        // One cluster of blocks, where it has room for the tokens: they exchange their counts behind a barrier of the
+        // cluster, and the second launch falls away. Else as many blocks as there are SMs, tokens a warp in
+        // whole turns.
+        const int64_t turn = static_cast<int64_t>(warps) * at_once;
+        int cluster = 0;
+        if (warps == gg::kFewWarps && q.tokens <= gg::kClusterMost * turn)
+          for (cluster = 1; cluster * turn < q.tokens;) cluster *= 2;
+        const int64_t most = (cluster > 0 ? cluster : gg::kMaxBlocks) * turn;
+        const int64_t per_warp = std::max<int64_t>(1, (q.tokens + most - 1) / most) * at_once;
+        const int blocks = cluster > 0 ? cluster : static_cast<int>(std::max<int64_t>(1, (q.tokens + per_warp * warps - 1) / (per_warp * warps)));
         gg::ForwardArgs a{};
         a.logits = q.logits;
         a.mask = q.token_mask;
@@ -827,29 +844,34 @@ int gg_router_run(gg_router* router, const gg_route* route, void* stream) {
         a.lse = q.lse;
         a.ld = q.ld;
         a.vec = gg::rows_aligned(q.logits, q.ld, c.logit_type);
-        a.place = {{c.experts, c.top_k, c.normalize != 0}, router->work, q.tokens, static_cast<int>(per_warp), blocks,
+        a.place = {{c.experts, c.top_k, c.normalize != 0}, router->work, q.tokens, static_cast<int>(per_warp), blocks, cluster,
                    q.indices, q.positions, q.rows, q.row_tokens, q.prob_mean, q.losses};
         const size_t place = gg::place_smem(32 * warps, c.experts);
         const size_t forward = gg::forward_smem(G, warps, c.experts, c.top_k);
-        gg::router_forward_kernel<f(), G, V, warps>
-            <<<blocks, 32 * warps, blocks == 1 ? std::max(place, forward) : forward, s>>>(a);
-        st = cudaGetLastError();
-        if (st != cudaSuccess || blocks == 1) return;
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(static_cast<unsigned>(blocks + 1));
-        cfg.blockDim = dim3(32 * warps);
-        cfg.dynamicSmemBytes = place;
-        cfg.stream = s;
         cudaLaunchAttribute attr{};
+        cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+        cfg.blockDim = dim3(32 * warps);
+        cfg.dynamicSmemBytes = cluster > 0 ? std::max(place, forward) : forward;
+        cfg.stream = s;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim = {static_cast<unsigned>(std::max(1, cluster)), 1, 1};
+        cfg.attrs = &attr;
+        cfg.numAttrs = cluster > 1;
+        st = cudaLaunchKernelEx(&cfg, gg::router_forward_kernel<f(), G, V, warps>, a);
+        if (st != cudaSuccess || cluster > 0) return;
+        cfg.gridDim = dim3(static_cast<unsigned>(blocks + 1));
+        cfg.dynamicSmemBytes = place;
+        cfg.numAttrs = 1;
         attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr.val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
         st = cudaLaunchKernelEx(&cfg, gg::router_place_kernel, a.place);
       };
-      // A decoding step's few tokens: one block of a few warps, whose sums and scans are as much shorter
-      // (4 tokens of 64 experts, top 2: XX us against YY us with the full block).
-      if (V == 8 && q.tokens <= gg::kFewWarps * at_once) launch(std::integral_constant<int, V == 8 ? gg::kFewWarps : gg::router_warps(V)>());
+      // Few tokens: small blocks, so that all SMs work on them (a full block's warps share one SM's issue slots), as
+      // long as every warp has one turn (999 tokens of 37 experts, top 5: XX us against 13.1 in full blocks; 4 tokens
+      // of 64, top 2: 5.4 against 8.7).
+      constexpr int kFew = V == 8 ? gg::kFewWarps : gg::router_warps(V);
+      if (q.tokens <= static_cast<int64_t>(gg::kMaxBlocks) * kFew * at_once) launch(std::integral_constant<int, kFew>());
       else launch(std::integral_constant<int, gg::router_warps(V)>());
     });
   });

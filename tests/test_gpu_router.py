@@ -128,10 +128,11 @@ def test_more_slots_than_experts(cuda):
     assert (fw.indices[:, 3:] == -1).all() and (fw.weights[:, 3:] == 0).all()
 
 
-def test_no_tokens(cuda):
+@pytest.mark.parametrize("e", [16, 600])
+def test_no_tokens(cuda, e):
     import torch
-    fw = Forward(torch.empty(0, 16, device=cuda), 2)
-    assert fw.rows.tolist() == [0] * 16 and fw.losses.tolist() == [0.0] * 3 and fw.prob_mean.tolist() == [0.0] * 16
+    fw = Forward(torch.empty(0, e, device=cuda), 2)
+    assert fw.rows.tolist() == [0] * e and fw.losses.tolist() == [0.0] * 3 and fw.prob_mean.tolist() == [0.0] * e
 
 
 @pytest.mark.parametrize("t", [7, 2000])
