@@ -26,6 +26,7 @@
 
 #include "gg_epilogue_ops.cuh"
 #include "gg_internal.h"
+#include "gg_launch.cuh"
 #include "gg_ptx.cuh"
 #include "grouped_gemm_b200.h"
 
@@ -531,6 +532,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2) q4_kernel(const __grid_constant
     ptx::mbar_init(ptx::smem_addr(&s_bars[0][0] + tid), 1);
     ptx::fence_mbar_init();
   }
+  chained_begin();
   if (warp == 0) {
     const bool good = find_work(p, work, 8 * kNT, lane);
     if (lane == 0) {
@@ -745,11 +747,10 @@ int gg_q4_plan_run(gg_q4_plan* plan, const void* a, int lda, int a_rows, const i
     }
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(plan->grid[variant], most)));
     gg::with_q4(plan->bf16, plan->per_block, plan->zeros, [&](auto b, auto n, auto z) {
-      gg::q4_kernel<b(), n(), z(), nt(), vec_c()><<<grid, gg::kQ4Threads, plan->smem, s>>>(p);
+      st = gg::launch_chained(gg::q4_kernel<b(), n(), z(), nt(), vec_c()>, dim3(grid), gg::kQ4Threads, plan->smem, s, 1, p);
     });
   });
-  if (st != cudaSuccess) return st;
-  return cudaGetLastError();
+  return st;
 }
 
 int gg_q4_plan_status(gg_q4_plan* plan, int* status) {

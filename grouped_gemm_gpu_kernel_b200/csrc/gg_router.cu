@@ -18,6 +18,7 @@
 #include <new>
 
 #include "gg_epilogue_ops.cuh"
+#include "gg_launch.cuh"
 #include "grouped_gemm_b200.h"
 
 namespace gg {
@@ -431,6 +432,7 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
   __syncwarp();
 
   // this warp's tokens (the host keeps tokens * top_k in an int)
+  chained_begin();
   const int per_warp = a.place.tokens_per_warp;
   const int unit = static_cast<int>(blockIdx.x) * kWarps + warp;
   const int t0 = static_cast<int>(min(static_cast<int64_t>(T), static_cast<int64_t>(unit) * per_warp));
@@ -558,7 +560,6 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
       if (i < have) s_prob[warp * E + e0 + i] = prob[i];
   if (lane == 0) s_z[2 * warp] = z, s_z[2 * warp + 1] = n;
   __syncthreads();
-  cudaTriggerProgrammaticLaunchCompletion();
   const RouterWork& w = a.place.work;
   for (int e = tid; e < E; e += 32 * kWarps) {
     int run = 0;
@@ -591,11 +592,9 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
   }
 }
 
-// Launched so that its blocks may be set up while the forward kernel ends; nothing is read before the
-// forward kernel's writes are there.
 __global__ void __launch_bounds__(1024) router_place_kernel(PlaceArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
-  cudaGridDependencySynchronize();
+  chained_begin();
   const int block = static_cast<int>(blockIdx.x);
   place_block(a, block, block < a.blocks, block == a.blocks, smem);  // the last block, without slots, sums the losses
 }
@@ -631,6 +630,7 @@ __global__ void __launch_bounds__(32 * kBackwardWarps, V == 8 ? kBackwardBlocks 
   const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
   const int group = lane / G, gl = lane % G;
   const int e0 = gl * V, have = max(0, min(V, E - e0));
+  chained_begin();
   const float n = a.losses[2];
   const float inv_n = n > 0.0f ? 1.0f / n : 0.0f;
   const float g0 = a.grad_losses ? a.grad_losses[0] : 0.0f, g1 = a.grad_losses ? a.grad_losses[1] : 0.0f;
@@ -848,24 +848,10 @@ int gg_router_run(gg_router* router, const gg_route* route, void* stream) {
                    q.indices, q.positions, q.rows, q.row_tokens, q.prob_mean, q.losses};
         const size_t place = gg::place_smem(32 * warps, c.experts);
         const size_t forward = gg::forward_smem(G, warps, c.experts, c.top_k);
-        cudaLaunchConfig_t cfg{};
-        cudaLaunchAttribute attr{};
-        cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-        cfg.blockDim = dim3(32 * warps);
-        cfg.dynamicSmemBytes = cluster > 0 ? std::max(place, forward) : forward;
-        cfg.stream = s;
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim = {static_cast<unsigned>(std::max(1, cluster)), 1, 1};
-        cfg.attrs = &attr;
-        cfg.numAttrs = cluster > 1;
-        st = cudaLaunchKernelEx(&cfg, gg::router_forward_kernel<f(), G, V, warps>, a);
-        if (st != cudaSuccess || cluster > 0) return;
-        cfg.gridDim = dim3(static_cast<unsigned>(blocks + 1));
-        cfg.dynamicSmemBytes = place;
-        cfg.numAttrs = 1;
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
-        st = cudaLaunchKernelEx(&cfg, gg::router_place_kernel, a.place);
+        st = gg::launch_chained(gg::router_forward_kernel<f(), G, V, warps>, dim3(blocks), 32 * warps,
+                                cluster > 0 ? std::max(place, forward) : forward, s, cluster, a);
+        if (st == cudaSuccess && cluster == 0)
+          st = gg::launch_chained(gg::router_place_kernel, dim3(blocks + 1), 32 * warps, place, s, 1, a.place);
       };
       // Few tokens: small blocks, so that all SMs work on them (a full block's warps share one SM's issue slots), as
       // long as every warp has one turn (999 tokens of 37 experts, top 5: XX us against 13.1 in full blocks; 4 tokens
@@ -887,6 +873,7 @@ int gg_router_backward(const gg_router* router, const gg_route_gradient* gradien
   if (q.tokens == 0) return cudaSuccess;
   if (!q.logits || !q.indices || !q.weights || !q.rows || !q.losses || !q.lse || !q.grad_logits) return cudaErrorInvalidValue;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t st = cudaSuccess;
   gg::with_logits(c.logit_type, [&](auto f) {
     gg::with_layout(c.experts, [&](auto g, auto v) {
       constexpr int G = g(), V = v();
@@ -896,11 +883,12 @@ int gg_router_backward(const gg_router* router, const gg_route_gradient* gradien
                          gg::rows_aligned(q.logits, q.ld, c.logit_type),
                          gg::rows_aligned(q.grad_logits, q.ld_grad, c.logit_type)};
       const int64_t blocks = (static_cast<int64_t>(q.tokens) + warps * at_once - 1) / (warps * at_once);
-      gg::router_backward_kernel<f(), G, V>
-          <<<static_cast<int>(std::min<int64_t>(blocks, gg::kBackwardBlocks * gg::kMaxBlocks)), 32 * warps, 0, s>>>(a);
+      st = gg::launch_chained(gg::router_backward_kernel<f(), G, V>,
+                              dim3(static_cast<unsigned>(std::min<int64_t>(blocks, gg::kBackwardBlocks * gg::kMaxBlocks))), 32 * warps, 0,
+                              s, 1, a);
     });
   });
-  return cudaGetLastError();
+  return st;
 }
 
 void gg_router_destroy(gg_router* router) {

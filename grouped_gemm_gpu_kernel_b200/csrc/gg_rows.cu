@@ -11,6 +11,7 @@
 #include <type_traits>
 
 #include "gg_epilogue_ops.cuh"
+#include "gg_launch.cuh"
 #include "grouped_gemm_b200.h"
 
 namespace gg {
@@ -53,6 +54,7 @@ template <typename U, int UN>
 __global__ void __launch_bounds__(kRowsThreads) dispatch_kernel(RowsShape sh, const U* __restrict__ x, int64_t ldx,
                                                                 const int* __restrict__ positions,
                                                                 U* __restrict__ packed, int64_t ldp) {
+  chained_begin();
   const RowsPlace at = rows_place(sh.shift);
   if (at.t >= sh.tokens) return;
   const U* row = x + at.t * ldx;
@@ -155,6 +157,7 @@ __global__ void __launch_bounds__(kRowsThreads) combine_kernel(RowsShape sh, con
                                                                const float* __restrict__ weights, int width,
                                                                void* __restrict__ out, int64_t ldo) {
   constexpr int UN = units_per_turn(N, KS);
+  chained_begin();
   const RowsPlace at = rows_place(sh.shift);
   if (at.t >= sh.tokens) return;
   const int64_t slot0 = at.t * sh.top_k;
@@ -209,6 +212,7 @@ __global__ void __launch_bounds__(kRowsThreads) combine_backward_kernel(
     float* __restrict__ grad_weights) {
   constexpr int UN = units_per_turn(N, KS);
   __shared__ float s_part[kRowsThreads / 32][KS];
+  chained_begin();
   const RowsPlace at = rows_place(sh.shift);
   const int warp = static_cast<int>(threadIdx.x) / 32, lane = static_cast<int>(threadIdx.x) % 32;
   const bool live = at.t < sh.tokens;
@@ -342,6 +346,7 @@ int gg_moe_dispatch(const void* x, int ldx, const int* positions, int tokens, in
   const uint64_t row = static_cast<uint64_t>(width) * elem_bytes;
   const uint64_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(packed) | row |
                        static_cast<uint64_t>(ldx) * elem_bytes | static_cast<uint64_t>(ldp) * elem_bytes;
+  cudaError_t st = cudaSuccess;
   auto launch = [&](auto unit, auto per_turn) {
     using U = decltype(unit);
     constexpr int bytes = sizeof(U), UN = per_turn();
@@ -349,9 +354,9 @@ int gg_moe_dispatch(const void* x, int ldx, const int* positions, int tokens, in
     sh.shift = gg::group_shift(sh.units, UN);
     const int turn = UN << sh.shift;
     const dim3 grid(gg::token_blocks(tokens, sh.shift), static_cast<unsigned>(std::min(65535, (sh.units - 1) / turn + 1)));
-    gg::dispatch_kernel<U, UN><<<grid, gg::kRowsThreads, 0, s>>>(
-        sh, static_cast<const U*>(x), static_cast<int64_t>(ldx) * elem_bytes / bytes, positions, static_cast<U*>(packed),
-        static_cast<int64_t>(ldp) * elem_bytes / bytes);
+    st = gg::launch_chained(gg::dispatch_kernel<U, UN>, grid, gg::kRowsThreads, 0, s, 1, sh, static_cast<const U*>(x),
+                            static_cast<int64_t>(ldx) * elem_bytes / bytes, positions, static_cast<U*>(packed),
+                            static_cast<int64_t>(ldp) * elem_bytes / bytes);
   };
   using std::integral_constant;
   if (all % 16 == 0) launch(uint4(), integral_constant<int, 4>());
@@ -359,7 +364,7 @@ int gg_moe_dispatch(const void* x, int ldx, const int* positions, int tokens, in
   else if (all % 4 == 0) launch(uint32_t(), integral_constant<int, 8>());
   else if (all % 2 == 0) launch(uint16_t(), integral_constant<int, 8>());
   else launch(uint8_t(), integral_constant<int, 8>());
-  return cudaGetLastError();
+  return st;
 }
 
 int gg_moe_combine(const void* packed, int packed_type, int packed_rows, int ldp, const int* positions,
@@ -371,6 +376,7 @@ int gg_moe_combine(const void* packed, int packed_type, int packed_rows, int ldp
   if (tokens == 0 || width == 0) return cudaSuccess;
   if (!out || !positions || (!packed && packed_rows > 0)) return cudaErrorInvalidValue;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t st = cudaSuccess;
   gg::with_formats(packed_type, out_type, [&](auto pf, auto of) {
     gg::with_vector_and_slots(top_k, gg::vector_of(pf() == gg::kOutF32 ? 4 : 8, packed, ldp, gg::bytes_of(packed_type), out, ldo,
                                   gg::bytes_of(out_type)), [&](auto vec, auto slots) {
@@ -379,10 +385,11 @@ int gg_moe_combine(const void* packed, int packed_type, int packed_rows, int ldp
       sh.shift = gg::group_shift(sh.units, UN);
       const int turn = UN << sh.shift;
       const dim3 grid(gg::token_blocks(tokens, sh.shift), static_cast<unsigned>(std::min(65535, (sh.units - 1) / turn + 1)));
-      gg::combine_kernel<pf(), of(), N, KS><<<grid, gg::kRowsThreads, 0, s>>>(sh, packed, ldp, positions, weights, width, out, ldo);
+      st = gg::launch_chained(gg::combine_kernel<pf(), of(), N, KS>, grid, gg::kRowsThreads, 0, s, 1, sh, packed,
+                              static_cast<int64_t>(ldp), positions, weights, width, out, static_cast<int64_t>(ldo));
     });
   });
-  return cudaGetLastError();
+  return st;
 }
 
 int gg_moe_combine_backward(const void* grad_out, int out_type, int ldo, const void* packed, int packed_type,
@@ -397,17 +404,19 @@ int gg_moe_combine_backward(const void* grad_out, int out_type, int ldo, const v
       (packed_rows > 0 && width > 0 && (!packed || !grad_packed)))
     return cudaErrorInvalidValue;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t st = cudaSuccess;
   gg::with_formats(packed_type, out_type, [&](auto pf, auto of) {
     gg::with_vector_and_slots(top_k, gg::vector_of(pf() == gg::kOutF32 ? 4 : 8, packed, ldp, gg::bytes_of(packed_type), grad_out, ldo,
                                   gg::bytes_of(out_type), grad_packed, ldgp), [&](auto vec, auto slots) {
       constexpr int N = pf() == gg::kOutF32 && vec() == 8 ? 4 : vec(), KS = slots();
       gg::RowsShape sh{tokens, top_k, packed_rows, width > 0 ? (width - 1) / N + 1 : 0, 0};
       sh.shift = gg::group_shift(sh.units, 2 * gg::units_per_turn(N, KS));
-      gg::combine_backward_kernel<pf(), of(), N, KS><<<gg::token_blocks(tokens, sh.shift), gg::kRowsThreads, 0, s>>>(
-          sh, grad_out, ldo, packed, ldp, positions, weights, width, grad_packed, ldgp, grad_weights);
+      st = gg::launch_chained(gg::combine_backward_kernel<pf(), of(), N, KS>, dim3(gg::token_blocks(tokens, sh.shift)),
+                              gg::kRowsThreads, 0, s, 1, sh, grad_out, static_cast<int64_t>(ldo), packed, static_cast<int64_t>(ldp),
+                              positions, weights, width, grad_packed, static_cast<int64_t>(ldgp), grad_weights);
     });
   });
-  return cudaGetLastError();
+  return st;
 }
 
 }  // extern "C"
