@@ -80,17 +80,22 @@ __global__ void __launch_bounds__(kQ4Threads) q4_pack_kernel(Q4PackParams p) {
     const int kb = static_cast<int>(b % p.k_blocks), tile = static_cast<int>(b / p.k_blocks % p.n_tiles);
     const int e = static_cast<int>(b / p.k_blocks / p.n_tiles);
     const int o = kTileN * tile + 8 * h + lane / 4;
+    const unsigned char* row = o < p.n ? p.q[e] + o * p.ldq : nullptr;
+    const bool words = (reinterpret_cast<uintptr_t>(row) & 3u) == 0;
     unsigned w[4];
     for (int x = 0; x < 4; ++x) {
-      unsigned word = 0;
-      for (int v = 0; v < 8; ++v) {
-        const int k = kBlockK * kb + 32 * x + 8 * (lane % 4) + v;
-        unsigned q = 8;
-        if (o < p.n && k < p.k) q = (p.q[e][o * p.ldq + k / 2] >> (4 * (k % 2))) & 15u;
-        const int place = (v / 2) + 4 * (v % 2);
-        word |= q << (4 * place);
+      const int k = kBlockK * kb + 32 * x + 8 * (lane % 4);
+      unsigned in = 0x88888888u;  // eight values from k on; past k: 8
+      if (row && k + 8 <= p.k && words) {
+        in = *reinterpret_cast<const unsigned*>(row + k / 2);
+      } else if (row) {
+        for (int v = 0; v < 8 && k + v < p.k; ++v)
+          in = (in & ~(15u << (4 * v))) | ((row[(k + v) / 2] >> (4 * (v % 2))) & 15u) << (4 * v);
       }
-      w[x] = word;
+      // the even values to the low half, the odd ones to the high half
+      unsigned even = in & 0x0f0f0f0fu, odd = (in >> 4) & 0x0f0f0f0fu;
+      even = (even | even >> 4) & 0x00ff00ffu, odd = (odd | odd >> 4) & 0x00ff00ffu;
+      w[x] = ((even | even >> 8) & 0xffffu) | (odd | odd >> 8) << 16;
     }
     reinterpret_cast<uint4*>(p.out + b * p.record)[i % 64] = make_uint4(w[0], w[1], w[2], w[3]);
   }
