@@ -5,7 +5,9 @@
 Compiles every CUDA / C++ source under csrc/ with nvcc for ``arch=compute_100a,code=sm_100a``
 and links one shared library next to this file. The static CUDA runtime is linked in, so the
 library needs only the driver at run time; it is loaded with ctypes (Python) or linked directly
-(C/C++ callers of include/grouped_gemm_b200.h or include/grouped_gemm/grouped_gemm.cuh).
+(C/C++ callers of include/grouped_gemm_b200.h or include/grouped_gemm/grouped_gemm.cuh). On top of it
+csrc/moe_python.cpp becomes _moe_native.so, a CPython module that only the package's
+mixture-of-experts calls use (g++ and Python.h).
 """
 from __future__ import annotations
 

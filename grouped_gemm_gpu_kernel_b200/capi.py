@@ -35,6 +35,8 @@ GG_STATUS_BAD_PROBLEMS = 0x200
 GG_DEVICE_PLAN_MAX_PROBLEMS = 4096
 GG_ROUTER_MAX_EXPERTS = 1024
 GG_ROUTER_MAX_TOP_K = 32
+GG_ROUTER_MAX_SLOTS = 2147483647 - 65536
+GG_MOE_MAX_WIDTH = 1 << 30
 GG_Q4_MAX_EXPERTS = 1024
 GG_INPUT_F16 = 0
 GG_INPUT_BF16 = 1

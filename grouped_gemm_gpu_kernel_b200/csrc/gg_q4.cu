@@ -6,9 +6,18 @@
 // once, whole lines at a time. The weights stand as the A operand of mma.sync m16n8k16 (16 outputs
 // a tile, 8 rows of the activations as its columns): the differences q - zero are small integers,
 // exact in FP16 and BF16, so the tensor pipe's products are exact and its sums FP32, and the group's
-// scale multiplies the FP32 sum. tcgen05 would want 128 outputs and the unpacked operand in shared
-// or tensor memory, a detour that costs more than the matrix work of 8 columns; a fragment in
-// registers is fed from the unpacking directly.
+// scale multiplies the FP32 sum. tcgen05 would want 128 outputs a tile, which leaves most SMs without one
+// at these sizes, and the unpacked operand in shared or tensor memory; a fragment in registers is fed from
+// the unpacking directly.
+//
+// Measured (B200, FP16, group 128, inputs past L2): one row through 14336 x 4096, 12.7 us (2.3 TB/s of weights; 4.5 us
+// at the copy rate), of which some 5 are the start and the end of the kernel (4096 x 4096 takes 5.6); eight experts of
+// 4096 x 14336 with one row each, 51 us (4.6 TB/s), 64 rows in all 80. The copies alone, without the arithmetic, run at
+// 39 us there; the arithmetic alone, without the copies, at 47: about 165 instructions a block of 1 KB, of which
+// 98 are the unpacking and the products, at half of the issue slots (dependent steps of 16 warps an SM; 24 warps
+// at 80 registers take 20 % more instructions and no less time). Past 8 rows an expert the activations,
+// read once a tile from L1 or L2, are more bytes than the weights. Two tiles a task, which halves those reads,
+// gained 4 to 12 % above 16 rows and lost 8 to 10 % below and with group 64 and zeros: not kept.
 //
 // Weights are laid out once (gg_q4_plan_create), per expert as blocks of 16 outputs x 128 k, tile by tile
 // and along k in a tile. A block is what one step of a warp reads, in one piece:
@@ -505,8 +514,8 @@ __device__ __forceinline__ bool find_work(const Q4Params& p, Q4Work& w, int most
   w.tasks = bad ? 0 : chunks * p.n_tiles;
   // The split whose longest group is done first: its tasks times a share's blocks and what a task costs besides
   // (its sums and outputs, about kTaskCost blocks). One warp takes about as long for a block whether all or
-  // half of an SM's warps are busy, so few whole shares beat many with a short last round: 1792 tasks of 32
-  // blocks, XX us in one share against YY in four.
+  // half of an SM's warps are busy, so few whole shares beat many with a short last round: 896 tasks of 32
+  // blocks take 13.3 us in two shares, 14.7 in eight.
   const float warps = static_cast<float>(kQ4Warps * gridDim.x);
   float least = INFINITY;
   w.splits = 1;

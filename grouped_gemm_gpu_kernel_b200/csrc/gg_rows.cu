@@ -3,7 +3,11 @@
 //   combine           out[t, :] = sum_j w(t, j) packed[pos(t, j), :]
 //   combine backward  grad_packed[pos(t, j), :] = w(t, j) grad_out[t, :],
 //                     grad_weights(t, j) = <grad_out[t, :], packed[pos(t, j), :]>
-// All three move bytes and compute next to nothing: memory bandwidth bounds them.
+// All three move bytes and compute next to nothing: memory bandwidth bounds them. A token's row is
+// read once whatever top_k is (dispatch) or written once (combine), in 16-byte units where the rows allow.
+// Measured (B200, 8192 tokens of 4096 BF16, top 2, inputs past L2; share of the measured copy rate of 6.54 TB/s):
+// dispatch 32.3 us (0.95), combine 31.5 us (0.97), its gradient 57.8 us (0.89). Small calls are one launch:
+// 4 tokens of 4096, top 2, 1.7 and 1.9 us on the GPU, 3.4 us each on the host.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -147,8 +151,8 @@ __device__ __forceinline__ void store_vec(void* base, int64_t at, int have, cons
 
 // Slots of a token worked on together (KS): the smallest of 2, 4 and 8 that holds top_k where the vectors
 // are wide, and 4 where they are narrow. Units a thread loads per turn: as many as make 8 wide loads, or 16
-// narrow ones, in flight whatever top_k is. (16384 rows of 4096 BF16, top 2: 47 us, with 4 slots of 2 units, half of
-// the loads dead, 61 us.)
+// narrow ones, in flight whatever top_k is. (The combine of 16384 rows of 4096 BF16, top 2: 31.6 us; 61 with 4
+// slots of 2 units, half of the loads dead.)
 constexpr int units_per_turn(int N, int KS) { return N >= 4 ? 8 / KS : 4; }
 
 template <int PF, int OF, int N, int KS>
@@ -336,7 +340,7 @@ extern "C" {
 
 int gg_moe_dispatch(const void* x, int ldx, const int* positions, int tokens, int top_k, int width, int elem_bytes,
                     void* packed, int packed_rows, int ldp, void* stream) {
-  if (tokens < 0 || top_k < 1 || width < 0 || packed_rows < 0 || (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4) ||
+  if (tokens < 0 || top_k < 1 || width < 0 || width > GG_MOE_MAX_WIDTH || packed_rows < 0 || (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4) ||
       ldx < std::max(1, width) || ldp < std::max(1, width))
     return cudaErrorInvalidValue;
   if (tokens == 0 || width == 0 || packed_rows == 0) return cudaSuccess;
@@ -370,7 +374,7 @@ int gg_moe_dispatch(const void* x, int ldx, const int* positions, int tokens, in
 int gg_moe_combine(const void* packed, int packed_type, int packed_rows, int ldp, const int* positions,
                    const float* weights, int tokens, int top_k, int width, void* out, int out_type, int ldo,
                    void* stream) {
-  if (tokens < 0 || top_k < 1 || width < 0 || packed_rows < 0 || !gg::out_type_ok(packed_type) ||
+  if (tokens < 0 || top_k < 1 || width < 0 || width > GG_MOE_MAX_WIDTH || packed_rows < 0 || !gg::out_type_ok(packed_type) ||
       !gg::out_type_ok(out_type) || ldp < std::max(1, width) || ldo < std::max(1, width))
     return cudaErrorInvalidValue;
   if (tokens == 0 || width == 0) return cudaSuccess;
@@ -395,7 +399,7 @@ int gg_moe_combine(const void* packed, int packed_type, int packed_rows, int ldp
 int gg_moe_combine_backward(const void* grad_out, int out_type, int ldo, const void* packed, int packed_type,
                             int packed_rows, int ldp, const int* positions, const float* weights, int tokens,
                             int top_k, int width, void* grad_packed, int ldgp, float* grad_weights, void* stream) {
-  if (tokens < 0 || top_k < 1 || width < 0 || packed_rows < 0 || !gg::out_type_ok(packed_type) ||
+  if (tokens < 0 || top_k < 1 || width < 0 || width > GG_MOE_MAX_WIDTH || packed_rows < 0 || !gg::out_type_ok(packed_type) ||
       !gg::out_type_ok(out_type) || ldp < std::max(1, width) || ldo < std::max(1, width) ||
       ldgp < std::max(1, width))
     return cudaErrorInvalidValue;

@@ -18,7 +18,7 @@
  *                                     kernel ran out; D may be partly written
  *   other values are CUDA runtime errors passed through unchanged.
  * Asynchronous launches report such a timeout through a status word instead, read with
- * gg_executor_status, gg_baseline_status, gg_noalloc_status or gg_moe_plan_status.
+ * gg_executor_status, gg_baseline_status, gg_noalloc_status, gg_moe_plan_status or gg_q4_plan_status.
  * An empty problem set (or one with zero tiles) is a successful no-op that launches nothing.
  *
  * Each entry point replaces one function of the reference C++ API
@@ -400,10 +400,11 @@ void gg_moe_plan_destroy(gg_moe_plan* plan);
  * (GG_OUTPUT_F32 / F16 / BF16). */
 #define GG_ROUTER_MAX_EXPERTS 1024
 #define GG_ROUTER_MAX_TOP_K 32
+#define GG_ROUTER_MAX_SLOTS (2147483647 - 65536)
 typedef struct gg_router_config {
   int experts;         /* 1..GG_ROUTER_MAX_EXPERTS */
   int top_k;           /* 1..GG_ROUTER_MAX_TOP_K; may exceed experts (slots over hold -1) */
-  int capacity_tokens; /* most tokens of a run; capacity_tokens * top_k must fit an int */
+  int capacity_tokens; /* most tokens of a run; capacity_tokens * top_k at most GG_ROUTER_MAX_SLOTS */
   int logit_type;      /* GG_OUTPUT_F32, GG_OUTPUT_F16 or GG_OUTPUT_BF16: logits and their gradient */
   int normalize;       /* weights sum to 1 over the chosen experts */
 } gg_router_config;
@@ -457,7 +458,9 @@ void gg_router_destroy(gg_router* router);
 /* ---- rows into expert order and back ----------------------------------------------------------
  * No counterpart in the reference. The moves between a layer's tokens and the packed rows of the
  * grouped product, by the router's positions (tokens x top_k; an entry outside
- * [0, packed_rows) goes nowhere and reads nothing). Each is one launch on `stream`. */
+ * [0, packed_rows) goes nowhere and reads nothing; a packed row is named at most once, or else holds
+ * one of what was written to it). width: at most GG_MOE_MAX_WIDTH. Each is one launch on `stream`. */
+#define GG_MOE_MAX_WIDTH (1 << 30)
 
 /* packed[positions[t][j], :] = x[t, :]. Elements of elem_bytes (1, 2 or 4) bytes, copied as they are;
  * ldx and ldp in elements. Packed rows that no position names are not written. */
@@ -518,8 +521,8 @@ int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** o
  * rows: `experts` counts in device memory; NULL with experts == 1: all capacity_rows rows.
  * d: capacity_rows x n of the output type, pitch ldd (>= n); rows past the counts' sum are not written.
  * One launch on `stream`. Counts that are negative or sum to more than capacity_rows (or than
- * a_rows without row_tokens) compute nothing and raise GG_STATUS_BAD_ROWS. Runs of one plan may
- * overlap on several streams. */
+ * a_rows without row_tokens) compute nothing and raise GG_STATUS_BAD_ROWS; a bounded wait that ran out raises
+ * GG_STATUS_TIMEOUT_PRODUCER (D is then wrong in part). Runs of one plan may overlap on several streams. */
 int gg_q4_plan_run(gg_q4_plan* plan, const void* a, int lda, int a_rows, const int* row_tokens, const int* rows,
                    void* d, int ldd, int capacity_rows, void* stream);
 /* Synchronises; returns (then clears) the GG_STATUS_* bits of the plan's runs. */

@@ -11,7 +11,7 @@ GONE = capi.CUDA_ERROR_INVALID_DEVICE_POINTER
 PTR = 0x1000
 
 
-@pytest.mark.parametrize("cfg", [(0, 1, 8, 0), (1025, 1, 8, 0), (8, 0, 8, 0), (8, 33, 8, 0), (8, 2, -1, 0), (8, 2, 2 ** 30, 0),
+@pytest.mark.parametrize("cfg", [(0, 1, 8, 0), (1025, 1, 8, 0), (8, 0, 8, 0), (8, 33, 8, 0), (8, 2, -1, 0), (8, 2, 2 ** 30, 0), (8, 1, 2 ** 31 - 65536, 0),
                                  (8, 2, 8, 3), (8, 2, 8, -1)])
 def test_router_sizes_out_of_range_are_refused(cfg):
     with pytest.raises(ValueError):
@@ -59,7 +59,7 @@ def test_q4_tables_have_one_entry_per_expert():
         gg.Q4Plan(2, 16, 64, 32, [PTR, PTR], 32, [PTR, PTR], bias_ptrs=[None])
 
 
-@pytest.mark.parametrize("change", [dict(tokens=-1), dict(top_k=0), dict(width=-1), dict(rows=-1), dict(ld=7), dict(ldp=7),
+@pytest.mark.parametrize("change", [dict(tokens=-1), dict(top_k=0), dict(width=-1), dict(width=2 ** 30 + 1, ld=2 ** 30 + 1, ldp=2 ** 30 + 1), dict(rows=-1), dict(ld=7), dict(ldp=7),
                                     dict(x=None), dict(pos=None), dict(packed=None), dict(size=8), dict(size=0)])
 def test_row_moves_refuse_what_does_not_fit(change):
     lib = capi.load()
