@@ -17,6 +17,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
@@ -74,15 +75,17 @@ def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) 
         return LIB_PATH
     os.makedirs(BUILD_DIR, exist_ok=True)
     cc = nvcc()
-    objs = []
-    for src in SOURCES:
-        obj = os.path.join(BUILD_DIR, os.path.splitext(src)[0] + ".o")
+    objs = [os.path.join(BUILD_DIR, os.path.splitext(src)[0] + ".o") for src in SOURCES]
+
+    def compile_one(src, obj):
         extra = ["-Xptxas", "-v"] if (ptxas_info and src.endswith(".cu")) else []
         lang = ["-x", "cu"] if src.endswith(".cu") else []
-        res = _run([cc, *ARCH, *NVCC_FLAGS, *extra, *lang, "-c", os.path.join(CSRC, src), "-o", obj], verbose)
-        if ptxas_info:
-            sys.stdout.write(res.stderr)
-        objs.append(obj)
+        return _run([cc, *ARCH, *NVCC_FLAGS, *extra, *lang, "-c", os.path.join(CSRC, src), "-o", obj], verbose)
+
+    with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 1)) as pool:
+        for res in pool.map(compile_one, SOURCES, objs):
+            if ptxas_info:
+                sys.stdout.write(res.stderr)
     tmp = LIB_PATH + ".tmp"
     _run([cc, *ARCH, "-shared", "-o", tmp, *objs, "-lcudart_static", "-ldl", "-lrt", "-lpthread"], verbose)
     os.replace(tmp, LIB_PATH)

@@ -66,6 +66,7 @@ struct Q4Params {
   void* d;
   int64_t lda, ldd;
   int a_rows, capacity_rows;
+  int unit;                     // elements that the rows are made up of, aligned: 8, 4, 2 or 1
   const unsigned short* no_row; // k zeros, for a gathered row that does not exist
 };
 
@@ -211,12 +212,33 @@ __device__ __forceinline__ float q4_activate(float x, int act) {
   return x;
 }
 
-// Eight activations from `at` on, of which `have` exist (the others are zero), as four packed pairs.
-__device__ __forceinline__ uint4 load_pairs(const unsigned short* at, int have) {
-  unsigned v[8];
+// Eight activations from `at` on, of which `have` exist (the others are zero), as four packed pairs. The rows are
+// made up of units of 4 or 2 elements that are aligned to their size, or of single ones (the same for
+// a whole run, so the branch is).
+__device__ __forceinline__ uint4 load_units(const unsigned short* at, int have, int unit) {
+  uint4 x = make_uint4(0u, 0u, 0u, 0u);
+  if (unit == 4) {
+    if (have > 0) {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(at));
+      x.x = u.x, x.y = u.y;
+    }
+    if (have > 4) {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(at) + 1);
+      x.z = u.x, x.w = u.y;
+    }
+  } else if (unit == 2) {
+    const unsigned* u = reinterpret_cast<const unsigned*>(at);
+    if (have > 0) x.x = __ldg(u);
+    if (have > 2) x.y = __ldg(u + 1);
+    if (have > 4) x.z = __ldg(u + 2);
+    if (have > 6) x.w = __ldg(u + 3);
+  } else {
+    unsigned v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < have ? __ldg(at + i) : 0u;
-  return make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+    for (int i = 0; i < 8; ++i) v[i] = i < have ? __ldg(at + i) : 0u;
+    x = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+  }
+  return x;
 }
 
 // `bytes` (a multiple of 16) from global to shared memory, counted on the mbarrier.
@@ -433,7 +455,7 @@ struct Q4Warp {
     int k_left = p.k - kBlockK * kb0;  // activations of a row from the block on
     // Eight activations of 32-k word i from rows[j] on; past k (checked where a word may reach it) zeros.
     const auto load = [&](int i, int j, auto check) {
-      if constexpr (!kVec) return load_pairs(rows[j] + 32 * i, k_left - 32 * i - 8 * t4);
+      if constexpr (!kVec) return load_units(rows[j] + 32 * i, k_left - 32 * i - 8 * t4, p.unit);
       else if constexpr (check()) return __ldg(reinterpret_cast<const uint4*>(k_left > 32 * i + 8 * t4 ? rows[j] + 32 * i : p.no_row));
       else return __ldg(reinterpret_cast<const uint4*>(rows[j] + 32 * i));
     };
@@ -633,16 +655,16 @@ size_t q4_smem(int experts) {
          (5 * static_cast<size_t>(experts) + 2) * sizeof(int);
 }
 
-// The variants of a run: one for activations that are not read 16 bytes at a time, and two for those that
-// are: 8 rows at most, whose registers let the compiler order the block more freely, and 16 at a time (32 at a
+// The variants of a run, for activations that are read 16 bytes at a time or in smaller units: 8 rows at most, whose registers let the compiler order the block more freely, and 16 at a time (32 at a
 // time, in spilled registers, took 34 us where two chunks of 16, the second from L2, take 30).
-enum Q4Variant { kQ4Narrow, kQ4Rows8, kQ4Rows16, kQ4Variants };
+enum Q4Variant { kQ4Narrow8, kQ4Narrow16, kQ4Rows8, kQ4Rows16, kQ4Variants };
 
 template <typename F>
 void with_variant(int v, F f) {
   using std::bool_constant;
   using std::integral_constant;
-  if (v == kQ4Narrow) f(integral_constant<int, 1>(), bool_constant<false>());
+  if (v == kQ4Narrow8) f(integral_constant<int, 1>(), bool_constant<false>());
+  else if (v == kQ4Narrow16) f(integral_constant<int, 2>(), bool_constant<false>());
   else if (v == kQ4Rows8) f(integral_constant<int, 1>(), bool_constant<true>());
   else f(integral_constant<int, 2>(), bool_constant<true>());
 }
@@ -788,8 +810,11 @@ int gg_q4_plan_run(gg_q4_plan* plan, const void* a, int lda, int a_rows, const i
   p.d = d;
   p.ldd = ldd;
   p.capacity_rows = capacity_rows;
-  const bool vec = (reinterpret_cast<uintptr_t>(a) & 15u) == 0 && lda % 8 == 0 && p.k % 8 == 0;
-  const int variant = !vec ? gg::kQ4Narrow : capacity_rows <= 8 ? gg::kQ4Rows8 : gg::kQ4Rows16;
+  // the rows' bases, pitch and length in units; a last unit past k would read another row's values
+  p.unit = 8;
+  while (p.unit > 1 && (reinterpret_cast<uintptr_t>(a) % (2 * p.unit) != 0 || lda % p.unit != 0 || p.k % p.unit != 0)) p.unit /= 2;
+  const bool few = capacity_rows <= 8;
+  const int variant = p.unit == 8 ? (few ? gg::kQ4Rows8 : gg::kQ4Rows16) : few ? gg::kQ4Narrow8 : gg::kQ4Narrow16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t st = cudaSuccess;
   gg::with_variant(variant, [&](auto nt, auto vec_c) {

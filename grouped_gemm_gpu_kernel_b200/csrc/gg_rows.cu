@@ -149,11 +149,11 @@ __device__ __forceinline__ void store_vec(void* base, int64_t at, int have, cons
   }
 }
 
-// Slots of a token worked on together (KS): the smallest of 2, 4 and 8 that holds top_k where the vectors
-// are wide, and 4 where they are narrow. Units a thread loads per turn: as many as make 8 wide loads, or 16
-// narrow ones, in flight whatever top_k is. (The combine of 16384 rows of 4096 BF16, top 2: 31.6 us; 61 with 4
+// Slots of a token worked on together (KS): the smallest of 2, 4 and, where the vectors are wide, 8 that
+// holds top_k. Units a thread loads per turn: as many as make 8 wide loads, or 16 narrow ones, in flight
+// whatever top_k is. (The combine of 16384 rows of 4096 BF16, top 2: 31.6 us; 61 with 4
 // slots of 2 units, half of the loads dead.)
-constexpr int units_per_turn(int N, int KS) { return N >= 4 ? 8 / KS : 4; }
+constexpr int units_per_turn(int N, int KS) { return (N >= 4 ? 8 : 16) / KS; }
 
 template <int PF, int OF, int N, int KS>
 __global__ void __launch_bounds__(kRowsThreads) combine_kernel(RowsShape sh, const void* __restrict__ packed, int64_t ldp,
@@ -300,7 +300,9 @@ void with_formats(int packed_type, int out_type, F f) {
 template <typename F>
 void with_vector_and_slots(int top_k, int n, F f) {
   using std::integral_constant;
-  if (n == 2) f(integral_constant<int, 2>(), integral_constant<int, 4>());
+  if (n == 2 && top_k <= 2) f(integral_constant<int, 2>(), integral_constant<int, 2>());
+  else if (n == 2) f(integral_constant<int, 2>(), integral_constant<int, 4>());
+  else if (n == 1 && top_k <= 2) f(integral_constant<int, 1>(), integral_constant<int, 2>());
   else if (n == 1) f(integral_constant<int, 1>(), integral_constant<int, 4>());
   else if (top_k <= 2) f(integral_constant<int, 8>(), integral_constant<int, 2>());
   else if (top_k <= 4) f(integral_constant<int, 8>(), integral_constant<int, 4>());
