@@ -66,7 +66,6 @@ struct Q4Params {
   void* d;
   int64_t lda, ldd;
   int a_rows, capacity_rows;
-  int unit;                     // elements that the rows are made up of, aligned: 8, 4, 2 or 1
   const unsigned short* no_row; // k zeros, for a gathered row that does not exist
 };
 
@@ -212,33 +211,18 @@ __device__ __forceinline__ float q4_activate(float x, int act) {
   return x;
 }
 
-// Eight activations from `at` on, of which `have` exist (the others are zero), as four packed pairs. The rows are
-// made up of units of 4 or 2 elements that are aligned to their size, or of single ones (the same for
-// a whole run, so the branch is).
-__device__ __forceinline__ uint4 load_units(const unsigned short* at, int have, int unit) {
-  uint4 x = make_uint4(0u, 0u, 0u, 0u);
-  if (unit == 4) {
-    if (have > 0) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(at));
-      x.x = u.x, x.y = u.y;
-    }
-    if (have > 4) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(at) + 1);
-      x.z = u.x, x.w = u.y;
-    }
-  } else if (unit == 2) {
-    const unsigned* u = reinterpret_cast<const unsigned*>(at);
-    if (have > 0) x.x = __ldg(u);
-    if (have > 2) x.y = __ldg(u + 1);
-    if (have > 4) x.z = __ldg(u + 2);
-    if (have > 6) x.w = __ldg(u + 3);
-  } else {
-    unsigned v[8];
+// Eight activations from `at` on, of which `have` exist (the others are zero), as four packed pairs. kLoad: 2
+// where the rows are made up of aligned pairs, else 1.
+template <int kLoad>
+__device__ __forceinline__ uint4 load_units(const unsigned short* at, int have) {
+  unsigned v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < have ? __ldg(at + i) : 0u;
-    x = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+  for (int i = 0; i < 8; i += kLoad) {
+    if constexpr (kLoad == 2) v[i / 2] = i < have ? __ldg(reinterpret_cast<const unsigned*>(at) + i / 2) : 0u;
+    else v[i] = i < have ? __ldg(at + i) : 0u;
   }
-  return x;
+  if constexpr (kLoad == 2) return make_uint4(v[0], v[1], v[2], v[3]);
+  else return make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
 }
 
 // `bytes` (a multiple of 16) from global to shared memory, counted on the mbarrier.
@@ -336,7 +320,7 @@ __device__ __forceinline__ bool advance(const Q4Work& w, int n_tiles, Q4Place& c
   return true;
 }
 
-template <bool kBf16, int kPer, bool kZeros, int kNT, bool kVec>
+template <bool kBf16, int kPer, bool kZeros, int kNT, int kLoad>
 struct Q4Warp {
   static constexpr int kRecord = record_bytes(kPer, kZeros);
   static constexpr int kStageBytes = kStageBlocks * kRecord;
@@ -455,7 +439,7 @@ struct Q4Warp {
     int k_left = p.k - kBlockK * kb0;  // activations of a row from the block on
     // Eight activations of 32-k word i from rows[j] on; past k (checked where a word may reach it) zeros.
     const auto load = [&](int i, int j, auto check) {
-      if constexpr (!kVec) return load_units(rows[j] + 32 * i, k_left - 32 * i - 8 * t4, p.unit);
+      if constexpr (kLoad != 8) return load_units<kLoad>(rows[j] + 32 * i, k_left - 32 * i - 8 * t4);
       else if constexpr (check()) return __ldg(reinterpret_cast<const uint4*>(k_left > 32 * i + 8 * t4 ? rows[j] + 32 * i : p.no_row));
       else return __ldg(reinterpret_cast<const uint4*>(rows[j] + 32 * i));
     };
@@ -478,14 +462,14 @@ struct Q4Warp {
 #pragma unroll
       for (int j = 0; j < NT; ++j) rows[j] += kCount * kBlockK;
     };
-    constexpr int kTogether = kVec ? 2 : 1;
+    constexpr int kTogether = kLoad == 8 ? 2 : 1;
     for (int left = run; left > 0; left -= kStageBlocks) {
       wait_bounded(bars + 8 * stage, parity, p.timeout_ns, p.status);
       const unsigned char* at = ring + stage * kStageBytes;
       int blocks = min(kStageBlocks, left);
       // The words ahead are of these blocks and the next: within k for all lanes, or else looked at (past the
       // warp's last block they may be another share's: not used).
-      if constexpr (kVec) {
+      if constexpr (kLoad == 8) {
 #pragma unroll 1
         for (; blocks >= kTogether && k_left >= (kTogether + 1) * kBlockK; blocks -= kTogether, at += kTogether * kRecord)
           blocks_of(at, std::integral_constant<int, kTogether>(), std::false_type());
@@ -580,11 +564,11 @@ __device__ __forceinline__ bool find_work(const Q4Params& p, Q4Work& w, int lane
   return !bad;
 }
 
-// kPer: groups per 128-k block (1, 2 or 4). kNT: most rows of an expert worked on together, in eights. kVec:
-// the activations are read 16 bytes at a time (aligned rows, k a multiple of 8).
-template <bool kBf16, int kPer, bool kZeros, int kNT, bool kVec>
+// kPer: groups per 128-k block (1, 2 or 4). kNT: most rows of an expert worked on together, in eights. kLoad:
+// elements of the activations read at a time: 8 (aligned rows, k a multiple of 8), 2 or 1.
+template <bool kBf16, int kPer, bool kZeros, int kNT, int kLoad>
 __global__ void __launch_bounds__(kQ4Threads, 2) q4_kernel(const __grid_constant__ Q4Params p) {
-  using Warp = Q4Warp<kBf16, kPer, kZeros, kNT, kVec>;
+  using Warp = Q4Warp<kBf16, kPer, kZeros, kNT, kLoad>;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int s_plan[3];
   const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
@@ -655,18 +639,20 @@ size_t q4_smem(int experts) {
          (5 * static_cast<size_t>(experts) + 2) * sizeof(int);
 }
 
-// The variants of a run, for activations that are read 16 bytes at a time or in smaller units: 8 rows at most, whose registers let the compiler order the block more freely, and 16 at a time (32 at a
-// time, in spilled registers, took 34 us where two chunks of 16, the second from L2, take 30).
-enum Q4Variant { kQ4Narrow8, kQ4Narrow16, kQ4Rows8, kQ4Rows16, kQ4Variants };
+// The variants of a run, by the most rows any expert can have: 8, whose registers let the compiler order the block
+// more freely, or 16 at a time (32 at a time, in spilled registers, took 34 us where two chunks of 16, the second from
+// L2, take 30); and by the units in which the activations are read: 8, 2 or single elements, the last 8 rows at
+// a time only (the loads of 16 rows start a task too slowly: 19 rows of k 257 took 7.2 us, 5.2 so).
+enum Q4Variant { kQ4Single8, kQ4Pairs8, kQ4Pairs16, kQ4Rows8, kQ4Rows16, kQ4Variants };
 
 template <typename F>
 void with_variant(int v, F f) {
-  using std::bool_constant;
   using std::integral_constant;
-  if (v == kQ4Narrow8) f(integral_constant<int, 1>(), bool_constant<false>());
-  else if (v == kQ4Narrow16) f(integral_constant<int, 2>(), bool_constant<false>());
-  else if (v == kQ4Rows8) f(integral_constant<int, 1>(), bool_constant<true>());
-  else f(integral_constant<int, 2>(), bool_constant<true>());
+  if (v == kQ4Single8) f(integral_constant<int, 1>(), integral_constant<int, 1>());
+  else if (v == kQ4Pairs8) f(integral_constant<int, 1>(), integral_constant<int, 2>());
+  else if (v == kQ4Pairs16) f(integral_constant<int, 2>(), integral_constant<int, 2>());
+  else if (v == kQ4Rows8) f(integral_constant<int, 1>(), integral_constant<int, 8>());
+  else f(integral_constant<int, 2>(), integral_constant<int, 8>());
 }
 
 template <typename F>
@@ -741,8 +727,8 @@ int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** o
     gg::with_q4(q.input_type == GG_INPUT_BF16, per_block, q.zeros != nullptr, [&](auto b, auto n, auto z) {
       smem = gg::q4_smem<n(), z()>(q.experts);
       for (int v = 0; v < gg::kQ4Variants && st == cudaSuccess; ++v)
-        gg::with_variant(v, [&](auto nt, auto vec) {
-          const auto kernel = gg::q4_kernel<b(), n(), z(), nt(), vec()>;
+        gg::with_variant(v, [&](auto nt, auto load) {
+          const auto kernel = gg::q4_kernel<b(), n(), z(), nt(), load()>;
           st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     static_cast<int>(gg::q4_smem<n(), z()>(GG_Q4_MAX_EXPERTS)));
           if (st == cudaSuccess) st = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm[v], kernel, gg::kQ4Threads, smem);
@@ -810,14 +796,15 @@ int gg_q4_plan_run(gg_q4_plan* plan, const void* a, int lda, int a_rows, const i
   p.d = d;
   p.ldd = ldd;
   p.capacity_rows = capacity_rows;
-  // the rows' bases, pitch and length in units; a last unit past k would read another row's values
-  p.unit = 8;
-  while (p.unit > 1 && (reinterpret_cast<uintptr_t>(a) % (2 * p.unit) != 0 || lda % p.unit != 0 || p.k % p.unit != 0)) p.unit /= 2;
+  // units that the rows' starts and their length are multiples of (a last unit past k would read other values)
+  const auto made_of = [&](int unit) { return reinterpret_cast<uintptr_t>(a) % (2 * unit) == 0 && lda % unit == 0 && p.k % unit == 0; };
   const bool few = capacity_rows <= 8;
-  const int variant = p.unit == 8 ? (few ? gg::kQ4Rows8 : gg::kQ4Rows16) : few ? gg::kQ4Narrow8 : gg::kQ4Narrow16;
+  const int variant = made_of(8)   ? (few ? gg::kQ4Rows8 : gg::kQ4Rows16)
+                      : made_of(2) ? (few ? gg::kQ4Pairs8 : gg::kQ4Pairs16)
+                                   : gg::kQ4Single8;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t st = cudaSuccess;
-  gg::with_variant(variant, [&](auto nt, auto vec_c) {
+  gg::with_variant(variant, [&](auto nt, auto load) {
     // tasks and their weights are counted in an int: one task per tile of each chunk of rows, chunks at most this
     const int64_t chunks = std::min<int64_t>(capacity_rows, static_cast<int64_t>(capacity_rows) / (8 * nt()) + p.experts);
     const int64_t most = chunks * p.n_tiles;
@@ -827,7 +814,7 @@ int gg_q4_plan_run(gg_q4_plan* plan, const void* a, int lda, int a_rows, const i
     }
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(plan->grid[variant], most)));
     gg::with_q4(plan->bf16, plan->per_block, plan->zeros, [&](auto b, auto n, auto z) {
-      st = gg::launch_chained(gg::q4_kernel<b(), n(), z(), nt(), vec_c()>, dim3(grid), gg::kQ4Threads, plan->smem, s, 1, p);
+      st = gg::launch_chained(gg::q4_kernel<b(), n(), z(), nt(), load()>, dim3(grid), gg::kQ4Threads, plan->smem, s, 1, p);
     });
   });
   return st;
