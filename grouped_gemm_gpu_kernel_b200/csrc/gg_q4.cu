@@ -12,7 +12,7 @@
 //
 // Measured (B200, FP16, group 128, inputs past L2): one row through 14336 x 4096, 12.7 us (2.3 TB/s of weights; 4.5 us
 // at the copy rate), of which some 5 are the start and the end of the kernel (4096 x 4096 takes 5.6); eight experts of
-// 4096 x 14336 with one row each, 51 us (4.6 TB/s), 64 rows in all 80. The copies alone, without the arithmetic, run at
+// 4096 x 14336 with one row each, 51 us (4.6 TB/s), 64 rows in all 71. The copies alone, without the arithmetic, run at
 // 39 us there; the arithmetic alone, without the copies, at 47: about 165 instructions a block of 1 KB, of which
 // 98 are the unpacking and the products, at half of the issue slots (dependent steps of 16 warps an SM; 24 warps
 // at 80 registers take 20 % more instructions and no less time). Past 8 rows an expert the activations,
