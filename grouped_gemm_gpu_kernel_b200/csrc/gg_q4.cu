@@ -232,16 +232,31 @@ __device__ __forceinline__ void copy_bulk(uint32_t to, const void* from, uint32_
                : "memory");
 }
 
-// Waits for a phase, at most timeout_ns: a wait that runs out raises GG_STATUS_TIMEOUT_PRODUCER, and the
-// kernel goes on with what is in the stage, so that its barriers stay matched and it ends.
+// Whether a wait of the block's has run out. (At a constant address: one kept in a register, or a place ahead that a
+// wait may change, spills in the loop: 64 rows on eight experts of 4096 x 14336 then take 84 us, 76 so.)
+__shared__ int s_gave_up;
+
+__device__ __forceinline__ bool gave_up() {
+  int v;
+  asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v) : "r"(ptx::smem_addr(&s_gave_up)) : "memory");
+  return v != 0;
+}
+
+// Waits for the copy of a stage, at most timeout_ns; where that runs out raises GG_STATUS_TIMEOUT_PRODUCER and
+// waits as long again. If it has not come then, the block gives up: it starts no more copies (a copy is only ever
+// started into a stage whose last one was seen), and goes through its ranges with what is in the stages, so that
+// the barriers of its groups stay matched. Every copy under way still has its wait, a thousandth as long, before
+// the block ends; those for copies that were not started run out as well.
 __device__ __forceinline__ void wait_bounded(uint32_t bar, uint32_t parity, unsigned long long timeout_ns, int* status) {
   if (ptx::mbar_try_wait(bar, parity)) return;
-  const uint64_t start = ptx::global_timer_ns();
-  for (unsigned i = 0; !ptx::mbar_try_wait_sleep(bar, parity, 1000u); ++i)
-    if (ptx::global_timer_ns() - start > timeout_ns || i > 0x40000000u) {
-      atomicOr(status, GG_STATUS_TIMEOUT_PRODUCER);
-      return;
-    }
+  const unsigned long long limit = gave_up() ? timeout_ns / 1000 : timeout_ns;
+  for (int again = 0; again < 2; ++again) {
+    const uint64_t start = ptx::global_timer_ns();
+    for (unsigned i = 0; ptx::global_timer_ns() - start <= limit && i <= 0x40000000u; ++i)
+      if (ptx::mbar_try_wait_sleep(bar, parity, 1000u)) return;
+    atomicOr(status, GG_STATUS_TIMEOUT_PRODUCER);
+  }
+  asm volatile("st.shared.s32 [%0], %1;" ::"r"(ptx::smem_addr(&s_gave_up)), "r"(1) : "memory");
 }
 
 // The kernel's work is cut into tasks: a tile (16 outputs) of a busy expert against a chunk of up to 8 kNT of
@@ -346,7 +361,7 @@ struct Q4Warp {
   __device__ __forceinline__ void fetch(Ahead& c, int stage) const {
     if (c.left <= 0) return;
     const int blocks = min(kStageBlocks, c.left);
-    if (lane == 0) {
+    if (lane == 0 && !gave_up()) {
       ptx::mbar_arrive_expect_tx(bars + 8 * stage, blocks * kRecord);
       copy_bulk(ring_address + stage * kStageBytes, c.from, blocks * kRecord, bars + 8 * stage);
     }
@@ -584,6 +599,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2) q4_kernel(const __grid_constant
     ptx::mbar_init(ptx::smem_addr(&s_bars[0][0] + tid), 1);
     ptx::fence_mbar_init();
   }
+  if (tid == 0) s_gave_up = 0;
   chained_begin();
   if (warp == 0) {
     const bool good = find_work<kNT>(p, work, lane);
