@@ -10,9 +10,9 @@
 // at these sizes, and the unpacked operand in shared or tensor memory; a fragment in registers is fed from
 // the unpacking directly.
 //
-// Measured (B200, FP16, group 128, inputs past L2): one row through 14336 x 4096, 12.7 us (2.3 TB/s of weights; 4.5 us
-// at the copy rate), of which some 5 are the start and the end of the kernel (4096 x 4096 takes 5.6); eight experts of
-// 4096 x 14336 with one row each, 51 us (4.6 TB/s), 64 rows in all 71. The copies alone, without the arithmetic, run at
+// Measured (B200, FP16, group 128, inputs past L2): one row through 14336 x 4096, 12.8 us (2.3 TB/s of weights; 4.5 us
+// at the copy rate), of which some 5 are the start and the end of the kernel (4096 x 4096 takes 5.8); eight experts of
+// 4096 x 14336 with one row each, 52 us (4.5 TB/s), 64 rows in all 74. The copies alone, without the arithmetic, run at
 // 39 us there; the arithmetic alone, without the copies, at 47: about 165 instructions a block of 1 KB, of which
 // 98 are the unpacking and the products, at half of the issue slots (dependent steps of 16 warps an SM; 24 warps
 // at 80 registers take 20 % more instructions and no less time). Past 8 rows an expert the activations,
@@ -288,7 +288,7 @@ struct Q4Place {
 };
 
 // What a task weighs when the ranges are cut: a chunk of more than 8 rows against one of up to 8 (64 rows on eight
-// experts of 4096 x 14336, 3 to 14 each: 71 us with these, 78 with equal ones, 76 with 3 and 5).
+// experts of 4096 x 14336, 3 to 14 each: 71 us with these, 78 with equal ones, 76 with 3 and 5; 74 since copies wait for gave_up()).
 constexpr int kWeight8 = 3, kWeight16 = 4;
 
 // The weight of an expert's chunks: all but the last have 8 kNT rows.
