@@ -1149,6 +1149,9 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_gemm_sm100_kernel(const _
     ptx::tc_fence_after_sync();
     ptx::tmem_dealloc(tmem_base, L::kTmemCols);
   }
+  // As the second launch of an executor this grid overlaps the first and needs none of its results. The next kernel
+  // on the stream may be one that waits for this grid alone: this grid does not complete before the first has.
+  if (threadIdx.x == 0) ptx::wait_prerequisites();
 }
 
 // Runs the bounded wait on an mbarrier nothing completes; records the resulting status.

@@ -131,7 +131,8 @@ cudaError_t prepare_kernel(Variant v) {
 // Launch of a one-CTA variant that may start while the previous kernel on the stream (a CTA-pair
 // launch that triggers its dependents at start) still runs: the two work on disjoint outputs, so
 // this grid's CTAs take SMs as the previous grid's CTAs retire (programmatic stream serialisation;
-// the grid never waits on the previous one's results).
+// the grid uses none of the previous one's results and waits for it only before it ends, so that
+// what follows on the stream finds both done).
 template <int BM, int BN>
 cudaError_t launch_overlapping(const KernelParams& params, int grid, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};

@@ -1,6 +1,8 @@
 // gg_launch.cuh -- launches of the mixture-of-experts kernels, which follow one another in a layer: each may be set
 // up on the GPU while the kernel before it on the stream still runs (programmatic dependent launch), and
-// touches global memory only once that one is done. Any kernel may come before or after.
+// touches global memory only once that one is done. The wait covers the kernel just before and no other, so the end
+// of a kernel has to mean the end of all before it. An ordinary launch starts after them; a programmatic one, as
+// these and the second launch of an executor with tile classes, waits before it ends (griddepcontrol.wait).
 #pragma once
 
 #include <cuda_runtime.h>

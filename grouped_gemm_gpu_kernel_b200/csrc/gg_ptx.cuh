@@ -66,6 +66,9 @@ __device__ __forceinline__ bool mbar_try_wait_sleep(uint32_t bar, uint32_t parit
 // Lets the next kernel on the stream, if it was launched with programmatic stream serialisation,
 // start before this grid finishes (it then takes SMs as this grid's CTAs retire).
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Waits until the grids that this one was allowed to overlap have completed and their results are visible; returns
+// at once in a grid that was launched without programmatic stream serialisation.
+__device__ __forceinline__ void wait_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---- cp.async (16-byte copies global -> shared, completion tracked on an mbarrier) ------------
 // Copies `src_bytes` (0..16) bytes from global src to shared dst and zero-fills the rest of the 16;

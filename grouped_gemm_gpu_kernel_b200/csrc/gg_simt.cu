@@ -28,6 +28,7 @@
 
 #include "gg_epilogue_ops.cuh"
 #include "gg_internal.h"
+#include "gg_ptx.cuh"
 
 namespace gg {
 namespace {
@@ -209,7 +210,12 @@ __global__ void __launch_bounds__(kSimtThreads, 3) grouped_gemm_simt_kernel(cons
     __syncthreads();
     const int q = s_work[0], tile_m = s_work[1], tile_n = s_work[2];
     if (q < 0) {
-      if (tid == 0) finish_launch(p);  // warp 0 has made its last claim
+      if (tid == 0) {
+        finish_launch(p);  // warp 0 has made its last claim
+        // overlapping the tensor-core launch of an executor, this grid does not complete before that one: the
+        // next kernel on the stream may be one that waits for this grid alone
+        ptx::wait_prerequisites();
+      }
       break;
     }
     const int m = s_desc.m, n = s_desc.n, k = s_desc.k;
