@@ -504,14 +504,14 @@ __global__ void __launch_bounds__(32 * W) router_forward_kernel(ForwardArgs a) {
         best = group_max<G>(mine);
       }
     }
-    // exp(v - top) as 2^(v log2(e) - top log2(e)): the rounding of the second product is the same factor in all
-    // terms and in the sum. Without a valid logit all of them are -infinity, and give 0.
+    // The difference first, whose rounding is relative to it and not to top, and which no finite logits overflow
+    // (to -infinity at most). Without a valid logit all of them are -infinity, and give 0.
     float sum = 0.0f;
     float ex[V];
-    const float shift = valid ? -top * kLog2e : 0.0f;
+    const float from = valid ? top : 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      ex[i] = exp2_fast(fmaf(v[i], kLog2e, shift));
+      ex[i] = exp_fast(v[i] - from);
       sum += ex[i];
     }
     sum = group_sum<G>(sum);
