@@ -620,6 +620,11 @@ struct BackwardArgs {
   int vec, vec_grad;
 };
 
+// p = exp(l - lse) is off by lse's rounding to FP32, 2^-24 |lse| relative: up to here no more than by the exponential
+// itself (1e-6). A token past it has its p divided by their sum, which takes the common factor out (131072 tokens of
+// 256 FP32 logits: 51.6 us with no token past it, 54.4 with all of them, 50.0 without either).
+constexpr float kRoughLse = 16.0f;
+
 // dl = p (c_e - <c, p> + 2 g1 lse / n) + the weights' part, with c_e = g0 E f(e) / n. One pass: a
 // group of lanes reads its token's logits once and writes the gradient once; all loads of a turn are
 // issued before the first is used.
@@ -689,12 +694,21 @@ __global__ void __launch_bounds__(32 * kBackwardWarps, V == 8 ? kBackwardBlocks 
       if (e[i] >= 0 && e[i] < E) part[place(e[i])] = w[i] * (gw[i] - (a.shape.normalize ? dot_w : 0.0f));
       if (i * G + G >= K) break;
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = i < have && live ? exp_fast(v[i] - lse) : 0.0f;
+    const bool rough = live && fabsf(lse) > kRoughLse;
+    if (__any_sync(kFull, rough)) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum += v[i];
+      sum = group_sum<G>(sum);
+      const float inv = rough ? __fdividef(1.0f, sum) : 1.0f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] *= inv;
+    }
     float dot = 0.0f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      v[i] = i < have && live ? exp_fast(v[i] - lse) : 0.0f;
-      dot = fmaf(c[i], v[i], dot);
-    }
+    for (int i = 0; i < V; ++i) dot = fmaf(c[i], v[i], dot);
     dot = group_sum<G>(dot);
     const float common = 2.0f * g1 * inv_n * lse - dot - (a.shape.normalize ? 0.0f : dot_w);
     __syncwarp();
