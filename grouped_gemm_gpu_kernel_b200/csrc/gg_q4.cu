@@ -707,7 +707,7 @@ int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** o
   *out = nullptr;
   if (!problem) return cudaErrorInvalidValue;
   const gg_q4_problem& q = *problem;
-  if (q.experts < 1 || q.experts > GG_Q4_MAX_EXPERTS || q.n < 1 || q.k < 1 || q.ldq < (q.k + 1) / 2 || !q.q || !q.scales ||
+  if (q.experts < 1 || q.experts > GG_Q4_MAX_EXPERTS || q.n < 1 || q.k < 1 || q.ldq < q.k / 2 + q.k % 2 || !q.q || !q.scales ||
       (q.group != 32 && q.group != 64 && (q.group < 128 || q.group % 128 != 0)) ||
       (q.input_type != GG_INPUT_F16 && q.input_type != GG_INPUT_BF16) || q.output_type < GG_OUTPUT_F32 ||
       q.output_type > GG_OUTPUT_BF16 || q.activation < GG_ACT_NONE || q.activation > GG_ACT_GELU)

@@ -83,3 +83,13 @@ def test_empty_moves_need_no_device():
     assert lib.gg_moe_dispatch(None, 8, None, 0, 2, 8, 4, None, 4, 8, None) == 0
     assert lib.gg_moe_combine(None, 0, 0, 8, None, None, 0, 2, 8, None, 0, 8, None) == 0
     assert lib.gg_moe_combine_backward(None, 0, 8, None, 0, 0, 8, None, None, 0, 2, 8, None, 8, None, None) == 0
+
+
+def test_q4_rows_of_the_longest_k_need_their_bytes():
+    """k = 2^31 - 1 takes a pitch of 2^30 bytes like any other takes ceil(k / 2): a shorter one is refused."""
+    table = (ctypes.c_void_p * 1)(PTR)
+    cast = ctypes.cast(table, ctypes.POINTER(ctypes.c_void_p))
+    for k in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 3):
+        out = ctypes.c_void_p()
+        prob = capi.GGQ4Problem(cast, cast, None, None, 1, 16, k, 128, (k - 1) // 2, 0, 0, 0)
+        assert capi.load().gg_q4_plan_create(ctypes.byref(prob), None, ctypes.byref(out)) == BAD
