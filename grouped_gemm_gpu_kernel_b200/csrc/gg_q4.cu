@@ -205,8 +205,9 @@ __device__ __forceinline__ void mma16816(float (&c)[4], bool first, unsigned a0,
   }
 }
 
+// As in the grouped product's epilogue (a NaN's ReLU is 0), with GELU through the full-range exponential.
 __device__ __forceinline__ float q4_activate(float x, int act) {
-  if (act == GG_ACT_RELU) return x < 0.0f ? 0.0f : x;
+  if (act == GG_ACT_RELU) return fmaxf(x, 0.0f);
   if (act == GG_ACT_GELU) return x / (1.0f + expf(-1.5957691216057308f * fmaf(0.044715f * x, x * x, x)));
   return x;
 }

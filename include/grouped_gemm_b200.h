@@ -91,7 +91,7 @@ typedef struct gg_problem {
  * epilogue arithmetic stay FP32; D is rounded to nearest even once, at the store.
  * activation (no reference counterpart): applied to every element of D after the bias,
  *   D = act(alpha * A x B + beta * C + bias):
- *   GG_ACT_NONE (0), GG_ACT_RELU (max(x, 0)), GG_ACT_GELU (tanh form,
+ *   GG_ACT_NONE (0), GG_ACT_RELU (max(x, 0), which is 0 for a NaN), GG_ACT_GELU (tanh form,
  *   0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))), the approximation of Hendrycks and Gimpel).
  * a_layout / b_layout (no reference counterpart, whose operands are row-major): GG_LAYOUT_ROW_MAJOR
  *   (0: A is m x k with row pitch lda >= k, B is k x n with ldb >= n) or GG_LAYOUT_COL_MAJOR
@@ -507,7 +507,7 @@ typedef struct gg_q4_problem {
   int ldq;
   int input_type;                 /* GG_INPUT_F16 or GG_INPUT_BF16: type of A and the scales */
   int output_type;                /* GG_OUTPUT_*: type of D */
-  int activation;                 /* GG_ACT_* (GELU in its tanh form) */
+  int activation;                 /* GG_ACT_*, as in gg_config (ReLU of a NaN is 0, GELU in its tanh form) */
 } gg_q4_problem;
 #define GG_Q4_MAX_EXPERTS 1024
 typedef struct gg_q4_plan gg_q4_plan;

@@ -264,3 +264,21 @@ def test_tensors_that_do_not_fit_are_refused(cuda):
         plan.run(a, r, d, row_tokens=r)
     plan.close()
     assert plan.run(a, r, d) == capi.CUDA_ERROR_INVALID_DEVICE_POINTER
+
+
+@pytest.mark.parametrize("act", [gg.Activation.kReLU, gg.Activation.kGELU])
+def test_activation_of_nan_is_the_grouped_products(cuda, act):
+    """One name, one meaning: GG_ACT_RELU is max(x, 0), which is 0 for a NaN, and GELU of a NaN is a NaN, in the plan
+    of 4-bit experts as in the grouped product."""
+    import torch
+    wt = Weights(cuda, 1, 64, 128, 64, "f16", seed=8)
+    a = torch.randn(5, 128, device=cuda, generator=wt.g).half()
+    a[2, 7] = float("nan")
+    got, want = torch.full((5, 64), 5.0, device=cuda), torch.full((5, 64), 5.0, device=cuda)
+    assert wt.plan("f32", act).run(a, None, got) == 0
+    dense = wt.dense(0).t().half().contiguous()
+    cfg = gg.KernelConfig(128, 128, 64, activation=act)
+    problem = gg.ProblemDesc(5, 64, 128, a.data_ptr(), dense.data_ptr(), None, want.data_ptr(), 128, 64, 64, 64)
+    assert gg.run_grouped_gemm_once([problem], gg.SortMode.kNone, cfg) == 0
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert (got[2] == 0).all() if act == gg.Activation.kReLU else torch.isnan(got[2]).all()
