@@ -7,7 +7,8 @@ and links one shared library next to this file. The static CUDA runtime is linke
 library needs only the driver at run time; it is loaded with ctypes (Python) or linked directly
 (C/C++ callers of include/grouped_gemm_b200.h or include/grouped_gemm/grouped_gemm.cuh). On top of it
 csrc/moe_python.cpp becomes _moe_native.so, a CPython module that only the package's
-mixture-of-experts calls use (g++ and Python.h).
+mixture-of-experts calls use (g++ and Python.h); where those are missing the library is all that is
+made, and these calls raise.
 """
 from __future__ import annotations
 
@@ -17,6 +18,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -61,18 +63,27 @@ def _newer(target: str, deps) -> bool:
     return all(os.path.getmtime(d) <= t for d in deps)
 
 
+CALLS_SOURCE = os.path.join(CSRC, "moe_python.cpp")
+
+
 def _deps():
     out = []
     for root in (CSRC, INCLUDE):
         for dirpath, _, files in os.walk(root):
             out += [os.path.join(dirpath, f) for f in files if f.endswith((".cu", ".cuh", ".h", ".cpp"))]
+    out.remove(CALLS_SOURCE)
     return out
 
 
 def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) -> str:
-    deps = _deps()
-    if not force and not ptxas_info and _newer(LIB_PATH, deps + [__file__]) and _newer(CALLS_PATH, deps + [__file__]):
-        return LIB_PATH
+    if force or ptxas_info or not _newer(LIB_PATH, _deps() + [__file__]):
+        _build_library(verbose, ptxas_info)
+    if force or not _newer(CALLS_PATH, [CALLS_SOURCE, os.path.join(INCLUDE, "grouped_gemm_b200.h"), __file__]):
+        _build_calls(verbose)
+    return LIB_PATH
+
+
+def _build_library(verbose: bool, ptxas_info: bool) -> None:
     os.makedirs(BUILD_DIR, exist_ok=True)
     cc = nvcc()
     objs = [os.path.join(BUILD_DIR, os.path.splitext(src)[0] + ".o") for src in SOURCES]
@@ -89,13 +100,23 @@ def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) 
     tmp = LIB_PATH + ".tmp"
     _run([cc, *ARCH, "-shared", "-o", tmp, *objs, "-lcudart_static", "-ldl", "-lrt", "-lpthread"], verbose)
     os.replace(tmp, LIB_PATH)
-    # a CPython module on top of the library, which it finds beside itself
+
+
+def _build_calls(verbose: bool) -> None:
+    """The CPython module on top of the library, which it finds beside itself. The library's other callers do not need
+    it, so its absence is a warning."""
+    cxx, headers = shutil.which("g++"), sysconfig.get_paths()["include"]
+    if not cxx or not os.path.exists(os.path.join(headers, "Python.h")):
+        if os.path.exists(CALLS_PATH):
+            os.remove(CALLS_PATH)  # of other sources than the library's
+        warnings.warn(f"{os.path.basename(CALLS_PATH)} was not built: " +
+                      (f"no Python.h in {headers}" if cxx else "no g++") +
+                      "; the package's mixture-of-experts calls will raise")
+        return
     tmp = CALLS_PATH + ".tmp"
-    cxx = shutil.which("g++") or "g++"
-    _run([cxx, "-std=c++17", "-O2", "-Wall", "-shared", "-fPIC", "-I" + INCLUDE, "-I" + sysconfig.get_paths()["include"],
-          os.path.join(CSRC, "moe_python.cpp"), "-o", tmp, "-L" + PKG, "-l:" + LIB_NAME, "-Wl,-rpath,$ORIGIN"], verbose)
+    _run([cxx, "-std=c++17", "-O2", "-Wall", "-shared", "-fPIC", "-I" + INCLUDE, "-I" + headers, CALLS_SOURCE, "-o", tmp,
+          "-L" + PKG, "-l:" + LIB_NAME, "-Wl,-rpath,$ORIGIN"], verbose)
     os.replace(tmp, CALLS_PATH)
-    return LIB_PATH
 
 
 def main():
