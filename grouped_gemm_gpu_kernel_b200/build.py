@@ -6,7 +6,7 @@ Compiles every CUDA / C++ source under csrc/ with nvcc for ``arch=compute_100a,c
 and links one shared library next to this file. The static CUDA runtime is linked in, so the
 library needs only the driver at run time; it is loaded with ctypes (Python) or linked directly
 (C/C++ callers of include/grouped_gemm_b200.h or include/grouped_gemm/grouped_gemm.cuh). On top of it
-csrc/moe_python.cpp becomes _moe_native.so, a CPython module that only the package's
+csrc/moe_python.cpp becomes _moe_native.<ABI>.so, a CPython module that only the package's
 mixture-of-experts calls use (g++ and Python.h); where those are missing the library is all that is
 made, and these calls raise.
 """
@@ -27,7 +27,8 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB_NAME = "libgrouped_gemm_b200.so"
 LIB_PATH = os.path.join(PKG, LIB_NAME)
-CALLS_PATH = os.path.join(PKG, "_moe_native.so")  # the Python calls of the mixture-of-experts operators
+# the Python calls of the mixture-of-experts operators, named for the interpreter that they are compiled for
+CALLS_PATH = os.path.join(PKG, "_moe_native" + sysconfig.get_config_var("EXT_SUFFIX"))
 BUILD_DIR = os.path.join(PKG, "_build")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

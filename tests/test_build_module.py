@@ -80,3 +80,10 @@ def test_an_error_in_the_module_is_raised(monkeypatch, tmp_path):
     c.broken = True
     with pytest.raises(RuntimeError):
         gbuild.build()
+
+
+def test_the_module_carries_its_python():
+    """Named for the interpreter that it was made with, so that another one beside it makes its own and
+    never loads this."""
+    assert os.path.basename(gbuild.CALLS_PATH) == "_moe_native" + sysconfig.get_config_var("EXT_SUFFIX")
+    assert sysconfig.get_config_var("SOABI") in gbuild.CALLS_PATH
