@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(PKG, "libgrouped_gemm_b200.so")
 
 # Every declaration of include/grouped_gemm_b200.h; tests check the library exports each one.
 EXPORTED_SYMBOLS = (
-    "gg_abi_version", "gg_sort_mode_name", "gg_tile_count", "gg_prepare", "gg_query_occupancy",
+    "gg_abi_version", "gg_current_device", "gg_sort_mode_name", "gg_tile_count", "gg_prepare", "gg_query_occupancy",
     "gg_executor_create", "gg_executor_destroy", "gg_executor_build", "gg_executor_build_with_bias",
     "gg_executor_run",
     "gg_executor_problem_count", "gg_executor_total_tiles", "gg_executor_grid_ctas", "gg_executor_launches",
@@ -155,6 +155,7 @@ def load() -> ctypes.CDLL:
     vp = ctypes.c_void_p
     sig = {
         "gg_abi_version": ([], ctypes.c_int),
+        "gg_current_device": ([i32p], ctypes.c_int),
         "gg_sort_mode_name": ([ctypes.c_int], ctypes.c_char_p),
         "gg_tile_count": ([pp, pc], ctypes.c_int),
         "gg_prepare": ([pp, ctypes.c_int, pc, ctypes.c_int, pp, i32p, i32p, i32p], ctypes.c_int),

@@ -466,6 +466,8 @@ extern "C" {
 
 int gg_abi_version(void) { return GG_ABI_VERSION; }
 
+int gg_current_device(int* device) { return device ? cudaGetDevice(device) : cudaErrorInvalidValue; }
+
 const char* gg_sort_mode_name(int sort_mode) {
   switch (sort_mode) {
     case GG_SORT_NONE:

@@ -18,6 +18,13 @@ __device__ __forceinline__ void chained_begin() {
   cudaGridDependencySynchronize();
 }
 
+// cudaErrorInvalidDevice where another device is current than the one that a handle's memory is on.
+inline cudaError_t expect_device(int device) {
+  int now = 0;
+  const cudaError_t st = cudaGetDevice(&now);
+  return st != cudaSuccess ? st : now == device ? cudaSuccess : cudaErrorInvalidDevice;
+}
+
 // cluster > 1: blocks of the grid's clusters.
 template <typename... Params, typename... Args>
 cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, unsigned cluster,

@@ -696,7 +696,7 @@ struct gg_q4_plan {
   void* block = nullptr;  // blocks of weights | bias table | status | a row of zeros | the caller's pointers
   gg::Q4Params params{};
   bool bf16 = false, zeros = false;
-  int per_block = 1;
+  int per_block = 1, device = 0;
   int grid[gg::kQ4Variants] = {};  // resident blocks of each variant
   size_t smem = 0;
 };
@@ -792,6 +792,7 @@ int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** o
   plan->bf16 = q.input_type == GG_INPUT_BF16;
   plan->zeros = q.zeros != nullptr;
   plan->per_block = per_block;
+  plan->device = device;
   for (int v = 0; v < gg::kQ4Variants; ++v) plan->grid[v] = std::max(1, sms * per_sm[v]);
   plan->smem = smem;
   *out = plan;
@@ -820,7 +821,8 @@ int gg_q4_plan_run(gg_q4_plan* plan, const void* a, int lda, int a_rows, const i
                       : made_of(2) ? (few ? gg::kQ4Pairs8 : gg::kQ4Pairs16)
                                    : gg::kQ4Single8;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t st = cudaSuccess;
+  cudaError_t st = gg::expect_device(plan->device);
+  if (st != cudaSuccess) return st;
   gg::with_variant(variant, [&](auto nt, auto load) {
     // tasks and their weights are counted in an int: one task per tile of each chunk of rows, chunks at most this
     const int64_t chunks = std::min<int64_t>(capacity_rows, static_cast<int64_t>(capacity_rows) / (8 * nt()) + p.experts);
@@ -840,7 +842,8 @@ int gg_q4_plan_run(gg_q4_plan* plan, const void* a, int lda, int a_rows, const i
 int gg_q4_plan_status(gg_q4_plan* plan, int* status) {
   if (!plan || !plan->block) return cudaErrorInvalidDevicePointer;
   if (!status) return cudaErrorInvalidValue;
-  cudaError_t st = cudaDeviceSynchronize();
+  cudaError_t st = gg::expect_device(plan->device);
+  if (st == cudaSuccess) st = cudaDeviceSynchronize();
   if (st != cudaSuccess) return st;
   st = cudaMemcpy(status, plan->params.status, sizeof(int), cudaMemcpyDeviceToHost);
   if (st != cudaSuccess) return st;

@@ -783,6 +783,7 @@ struct gg_router {
   gg_router_config config{};
   void* block = nullptr;
   gg::RouterWork work{};
+  int device = 0;
 };
 
 extern "C" {
@@ -800,7 +801,11 @@ int gg_router_create(const gg_router_config* config, gg_router** out) {
   if (!r) return cudaErrorMemoryAllocation;
   r->config = c;
   size_t warps = 0;
-  cudaError_t st = cudaSuccess;
+  cudaError_t st = cudaGetDevice(&r->device);
+  if (st != cudaSuccess) {
+    delete r;
+    return st;
+  }
   gg::with_logits(c.logit_type, [&](auto f) {
     gg::with_layout(c.experts, [&](auto g, auto v) {
       constexpr int W = gg::router_warps(v());
@@ -839,7 +844,8 @@ int gg_router_run(gg_router* router, const gg_route* route, void* stream) {
   if (q.tokens < 0 || q.tokens > c.capacity_tokens || q.ld < c.experts || !q.rows || !q.losses) return cudaErrorInvalidValue;
   if (q.tokens > 0 && (!q.logits || !q.indices || !q.weights || !q.positions)) return cudaErrorInvalidValue;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t st = cudaSuccess;
+  cudaError_t st = gg::expect_device(router->device);
+  if (st != cudaSuccess) return st;
   gg::with_logits(c.logit_type, [&](auto f) {
     gg::with_layout(c.experts, [&](auto g, auto v) {
       constexpr int G = g(), V = v(), at_once = 32 / G;
@@ -892,7 +898,8 @@ int gg_router_backward(const gg_router* router, const gg_route_gradient* gradien
   if (q.tokens == 0) return cudaSuccess;
   if (!q.logits || !q.indices || !q.weights || !q.rows || !q.losses || !q.lse || !q.grad_logits) return cudaErrorInvalidValue;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t st = cudaSuccess;
+  cudaError_t st = gg::expect_device(router->device);
+  if (st != cudaSuccess) return st;
   gg::with_logits(c.logit_type, [&](auto f) {
     gg::with_layout(c.experts, [&](auto g, auto v) {
       constexpr int G = g(), V = v();

@@ -2,7 +2,7 @@
 // attributes and calls the C-ABI (include/grouped_gemm_b200.h). A decoding step makes some ten such calls, each of a
 // few microseconds on the GPU; with the checks in Python and the call through ctypes a call took 6.1 us on the
 // host, of which the launch is 2.9. The module knows a tensor only by its Python attributes (dtype, shape,
-// stride(), is_cuda, data_ptr()), so it is not tied to a version of torch.
+// stride(), get_device(), data_ptr()), so it is not tied to a version of torch.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -14,7 +14,7 @@
 namespace {
 
 // Interned attribute names, and torch's dtype objects (fetched on the first call).
-PyObject *n_dtype, *n_shape, *n_stride, *n_is_cuda, *n_data_ptr, *n_is_contiguous, *n_numel, *n_cuda_stream, *n_element_size;
+PyObject *n_dtype, *n_shape, *n_stride, *n_get_device, *n_data_ptr, *n_is_contiguous, *n_numel, *n_cuda_stream, *n_element_size;
 PyObject *t_f32, *t_f16, *t_bf16, *t_i32, *t_u8, *t_bool;
 
 bool load_types() {
@@ -44,6 +44,20 @@ bool call_int(PyObject* t, PyObject* name, int64_t* out) {
   *out = static_cast<int64_t>(PyLong_AsLongLong(v));
   Py_DECREF(v);
   return !(*out == -1 && PyErr_Occurred());
+}
+
+// Whether a tensor is on the current device, which the call's launch goes to (-1 of get_device(): on none). Each call
+// looks the device up once, and leaves it negative where there is none.
+bool on_device(PyObject* t, int device, bool* is) {
+  int64_t of = 0;
+  if (!call_int(t, n_get_device, &of)) return false;
+  *is = of >= 0 && of == device;
+  return true;
+}
+
+int current_device() {
+  int device = -1;
+  return gg_current_device(&device) == 0 ? device : -1;
 }
 
 bool pointer_of(PyObject* t, void** out) {
@@ -79,8 +93,8 @@ struct Matrix {
   int rows, cols, ld;
 };
 
-// A rows x cols device tensor with contiguous columns and rows that do not overlap; rows or cols < 0: any.
-bool matrix(PyObject* t, const char* what, int64_t rows, int64_t cols, Matrix* m) {
+// A rows x cols tensor of the device with contiguous columns and rows that do not overlap; rows or cols < 0: any.
+bool matrix(PyObject* t, const char* what, int device, int64_t rows, int64_t cols, Matrix* m) {
   int64_t r, c, sr, sc;
   if (!two_of(PyObject_GetAttr(t, n_shape), what, &r, &c)) return false;
   if ((rows >= 0 && r != rows) || (cols >= 0 && c != cols)) {
@@ -90,10 +104,11 @@ bool matrix(PyObject* t, const char* what, int64_t rows, int64_t cols, Matrix* m
     return false;
   }
   if (!two_of(PyObject_CallMethodNoArgs(t, n_stride), what, &sr, &sc)) return false;
-  PyObject* cuda = peek(t, n_is_cuda);
-  if (!cuda) return false;
-  if ((sc != 1 && c > 1) || (sr < c && r > 1) || cuda != Py_True) {
-    PyErr_Format(PyExc_ValueError, "%s: a CUDA tensor with contiguous columns and rows that do not overlap expected", what);
+  bool here;
+  if (!on_device(t, device, &here)) return false;
+  if ((sc != 1 && c > 1) || (sr < c && r > 1) || !here) {
+    PyErr_Format(PyExc_ValueError,
+                 "%s: a tensor on the current CUDA device (%d) with contiguous columns and rows that do not overlap expected", what, device);
     return false;
   }
   m->dtype = peek(t, n_dtype);
@@ -103,8 +118,8 @@ bool matrix(PyObject* t, const char* what, int64_t rows, int64_t cols, Matrix* m
   return m->dtype && pointer_of(t, &m->data);
 }
 
-// A contiguous device tensor of `count` elements of a dtype (or of `other`).
-bool flat(PyObject* t, const char* what, int64_t count, PyObject* dtype, void** data, PyObject* other = nullptr) {
+// A contiguous tensor of the device, of `count` elements of a dtype (or of `other`).
+bool flat(PyObject* t, const char* what, int device, int64_t count, PyObject* dtype, void** data, PyObject* other = nullptr) {
   PyObject* is = peek(t, n_dtype);
   if (!is) return false;
   int64_t have = 0;
@@ -112,10 +127,11 @@ bool flat(PyObject* t, const char* what, int64_t count, PyObject* dtype, void** 
   PyObject* cont = PyObject_CallMethodNoArgs(t, n_is_contiguous);
   if (!cont) return false;
   Py_DECREF(cont);
-  PyObject* cuda = peek(t, n_is_cuda);
-  if (!cuda) return false;
-  if ((is != dtype && is != other) || have != count || cont != Py_True || cuda != Py_True) {
-    PyErr_Format(PyExc_ValueError, "%s: a contiguous CUDA tensor of %lld elements of %R expected, got %lld of %R", what,
+  bool here;
+  if (!on_device(t, device, &here)) return false;
+  if ((is != dtype && is != other) || have != count || cont != Py_True || !here) {
+    PyErr_Format(PyExc_ValueError,
+                 "%s: a contiguous tensor on the current CUDA device (%d) of %lld elements of %R expected, got %lld of %R", what, device,
                  static_cast<long long>(count), dtype, static_cast<long long>(have), is);
     return false;
   }
@@ -124,16 +140,16 @@ bool flat(PyObject* t, const char* what, int64_t count, PyObject* dtype, void** 
 
 // The same, or NULL for None.
 template <typename T>
-bool flat_or_none(PyObject* t, const char* what, int64_t count, PyObject* dtype, T** data, PyObject* other = nullptr) {
+bool flat_or_none(PyObject* t, const char* what, int device, int64_t count, PyObject* dtype, T** data, PyObject* other = nullptr) {
   void* p = nullptr;
-  if (t != Py_None && !flat(t, what, count, dtype, &p, other)) return false;
+  if (t != Py_None && !flat(t, what, device, count, dtype, &p, other)) return false;
   *data = static_cast<T*>(p);
   return true;
 }
 template <typename T>
-bool flat_into(PyObject* t, const char* what, int64_t count, PyObject* dtype, T** data) {
+bool flat_into(PyObject* t, const char* what, int device, int64_t count, PyObject* dtype, T** data) {
   void* p = nullptr;
-  if (!flat(t, what, count, dtype, &p)) return false;
+  if (!flat(t, what, device, count, dtype, &p)) return false;
   *data = static_cast<T*>(p);
   return true;
 }
@@ -177,9 +193,9 @@ PyObject* status_of(F call) {  // the C-ABI throws nothing; a full launch queue 
   Py_END_ALLOW_THREADS return PyLong_FromLong(st);
 }
 
-bool router_logits(PyObject* t, PyObject* type, int experts, const char* what, Matrix* m) {
+bool router_logits(PyObject* t, PyObject* type, int experts, const char* what, int device, Matrix* m) {
   int is;
-  if (!matrix(t, what, -1, experts, m) || !output_type(m->dtype, what, &is)) return false;
+  if (!matrix(t, what, device, -1, experts, m) || !output_type(m->dtype, what, &is)) return false;
   if (is == PyLong_AsLong(type)) return true;
   PyErr_Format(PyExc_ValueError, "%s: the router was made for another type than %R", what, m->dtype);
   return false;
@@ -189,19 +205,20 @@ bool router_logits(PyObject* t, PyObject* type, int experts, const char* what, M
 //  token_mask, stream)
 PyObject* router_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arguments(n, 15)) return nullptr;
+  const int device = current_device();
   gg_router* router = static_cast<gg_router*>(PyLong_AsVoidPtr(a[0]));
   const int experts = static_cast<int>(PyLong_AsLong(a[1])), top_k = static_cast<int>(PyLong_AsLong(a[2]));
   Matrix l;
-  if (PyErr_Occurred() || !router_logits(a[4], a[3], experts, "logits", &l)) return nullptr;
+  if (PyErr_Occurred() || !router_logits(a[4], a[3], experts, "logits", device, &l)) return nullptr;
   const int64_t slots = static_cast<int64_t>(l.rows) * top_k;
   gg_route q{};
   void* mask = nullptr;
   void* stream;
-  if (!flat_into(a[5], "indices", slots, t_i32, &q.indices) || !flat_into(a[6], "weights", slots, t_f32, &q.weights) ||
-      !flat_into(a[7], "positions", slots, t_i32, &q.positions) || !flat_into(a[8], "rows", experts, t_i32, &q.rows) ||
-      !flat_into(a[9], "losses", 3, t_f32, &q.losses) || !flat_or_none(a[10], "row_tokens", slots, t_i32, &q.row_tokens) ||
-      !flat_or_none(a[11], "lse", l.rows, t_f32, &q.lse) || !flat_or_none(a[12], "prob_mean", experts, t_f32, &q.prob_mean) ||
-      !flat_or_none(a[13], "token_mask", l.rows, t_u8, &mask, t_bool) || !stream_of(a[14], &stream))
+  if (!flat_into(a[5], "indices", device, slots, t_i32, &q.indices) || !flat_into(a[6], "weights", device, slots, t_f32, &q.weights) ||
+      !flat_into(a[7], "positions", device, slots, t_i32, &q.positions) || !flat_into(a[8], "rows", device, experts, t_i32, &q.rows) ||
+      !flat_into(a[9], "losses", device, 3, t_f32, &q.losses) || !flat_or_none(a[10], "row_tokens", device, slots, t_i32, &q.row_tokens) ||
+      !flat_or_none(a[11], "lse", device, l.rows, t_f32, &q.lse) || !flat_or_none(a[12], "prob_mean", device, experts, t_f32, &q.prob_mean) ||
+      !flat_or_none(a[13], "token_mask", device, l.rows, t_u8, &mask, t_bool) || !stream_of(a[14], &stream))
     return nullptr;
   q.logits = l.data;
   q.token_mask = static_cast<const unsigned char*>(mask);
@@ -214,11 +231,12 @@ PyObject* router_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
 //  grad_logits, stream)
 PyObject* router_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arguments(n, 14)) return nullptr;
+  const int device = current_device();
   const gg_router* router = static_cast<const gg_router*>(PyLong_AsVoidPtr(a[0]));
   const int experts = static_cast<int>(PyLong_AsLong(a[1])), top_k = static_cast<int>(PyLong_AsLong(a[2]));
   Matrix l, g;
-  if (PyErr_Occurred() || !router_logits(a[4], a[3], experts, "logits", &l) ||
-      !router_logits(a[12], a[3], experts, "grad_logits", &g))
+  if (PyErr_Occurred() || !router_logits(a[4], a[3], experts, "logits", device, &l) ||
+      !router_logits(a[12], a[3], experts, "grad_logits", device, &g))
     return nullptr;
   if (g.rows != l.rows) {
     PyErr_SetString(PyExc_ValueError, "grad_logits: the shape of logits expected");
@@ -228,17 +246,17 @@ PyObject* router_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int *indices, *rows;
   float *weights, *losses, *lse, *grad_weights, *grad_losses;
   void* stream;
-  if (!flat_into(a[5], "indices", slots, t_i32, &indices) || !flat_into(a[6], "weights", slots, t_f32, &weights) ||
-      !flat_into(a[7], "rows", experts, t_i32, &rows) || !flat_into(a[8], "losses", 3, t_f32, &losses) ||
-      !flat_into(a[9], "lse", l.rows, t_f32, &lse) || !flat_or_none(a[10], "grad_weights", slots, t_f32, &grad_weights) ||
-      !flat_or_none(a[11], "grad_losses", 2, t_f32, &grad_losses) || !stream_of(a[13], &stream))
+  if (!flat_into(a[5], "indices", device, slots, t_i32, &indices) || !flat_into(a[6], "weights", device, slots, t_f32, &weights) ||
+      !flat_into(a[7], "rows", device, experts, t_i32, &rows) || !flat_into(a[8], "losses", device, 3, t_f32, &losses) ||
+      !flat_into(a[9], "lse", device, l.rows, t_f32, &lse) || !flat_or_none(a[10], "grad_weights", device, slots, t_f32, &grad_weights) ||
+      !flat_or_none(a[11], "grad_losses", device, 2, t_f32, &grad_losses) || !stream_of(a[13], &stream))
     return nullptr;
   const gg_route_gradient q{l.data, indices, weights, rows, losses, lse, grad_weights, grad_losses, g.data, l.rows, l.ld, g.ld};
   return status_of([&] { return gg_router_backward(router, &q, stream); });
 }
 
 // positions (tokens, top_k), contiguous.
-bool positions_of(PyObject* t, int tokens, int* top_k, int** data) {
+bool positions_of(PyObject* t, int device, int tokens, int* top_k, int** data) {
   int64_t r, c;
   if (!two_of(PyObject_GetAttr(t, n_shape), "positions", &r, &c)) return false;
   if (r != tokens) {
@@ -247,7 +265,7 @@ bool positions_of(PyObject* t, int tokens, int* top_k, int** data) {
     return false;
   }
   *top_k = static_cast<int>(c);
-  return flat_into(t, "positions", r * c, t_i32, data);
+  return flat_into(t, "positions", device, r * c, t_i32, data);
 }
 
 bool same_dtype(const Matrix& x, const Matrix& y, const char* what) {
@@ -258,12 +276,13 @@ bool same_dtype(const Matrix& x, const Matrix& y, const char* what) {
 
 // (x, positions, packed, stream)
 PyObject* dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  const int device = current_device();
   Matrix x, p;
   int k, *pos;
   int64_t bytes;
   void* stream;
-  if (!arguments(n, 4) || !matrix(a[0], "x", -1, -1, &x) || !matrix(a[2], "packed", -1, x.cols, &p) ||
-      !same_dtype(x, p, "x, packed") || !positions_of(a[1], x.rows, &k, &pos) || !call_int(a[0], n_element_size, &bytes) ||
+  if (!arguments(n, 4) || !matrix(a[0], "x", device, -1, -1, &x) || !matrix(a[2], "packed", device, -1, x.cols, &p) ||
+      !same_dtype(x, p, "x, packed") || !positions_of(a[1], device, x.rows, &k, &pos) || !call_int(a[0], n_element_size, &bytes) ||
       !stream_of(a[3], &stream))
     return nullptr;
   return status_of([&] {
@@ -273,13 +292,14 @@ PyObject* dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // (packed, positions, out, weights, stream)
 PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  const int device = current_device();
   Matrix p, o;
   int k, *pos, pt, ot;
   float* weights;
   void* stream;
-  if (!arguments(n, 5) || !matrix(a[2], "out", -1, -1, &o) || !matrix(a[0], "packed", -1, o.cols, &p) ||
-      !output_type(p.dtype, "packed", &pt) || !output_type(o.dtype, "out", &ot) || !positions_of(a[1], o.rows, &k, &pos) ||
-      !flat_or_none(a[3], "weights", static_cast<int64_t>(o.rows) * k, t_f32, &weights) || !stream_of(a[4], &stream))
+  if (!arguments(n, 5) || !matrix(a[2], "out", device, -1, -1, &o) || !matrix(a[0], "packed", device, -1, o.cols, &p) ||
+      !output_type(p.dtype, "packed", &pt) || !output_type(o.dtype, "out", &ot) || !positions_of(a[1], device, o.rows, &k, &pos) ||
+      !flat_or_none(a[3], "weights", device, static_cast<int64_t>(o.rows) * k, t_f32, &weights) || !stream_of(a[4], &stream))
     return nullptr;
   return status_of([&] {
     return gg_moe_combine(p.data, pt, p.rows, p.ld, pos, weights, o.rows, k, o.cols, o.data, ot, o.ld, stream);
@@ -288,16 +308,17 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // (grad_out, packed, positions, weights, grad_packed, grad_weights, stream)
 PyObject* combine_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  const int device = current_device();
   Matrix g, p, gp;
   int k, *pos, pt, ot;
   float *weights, *grad_weights;
   void* stream;
-  if (!arguments(n, 7) || !matrix(a[0], "grad_out", -1, -1, &g) || !matrix(a[1], "packed", -1, g.cols, &p) ||
-      !matrix(a[4], "grad_packed", p.rows, g.cols, &gp) || !same_dtype(p, gp, "packed, grad_packed") ||
-      !output_type(g.dtype, "grad_out", &ot) || !output_type(p.dtype, "packed", &pt) || !positions_of(a[2], g.rows, &k, &pos))
+  if (!arguments(n, 7) || !matrix(a[0], "grad_out", device, -1, -1, &g) || !matrix(a[1], "packed", device, -1, g.cols, &p) ||
+      !matrix(a[4], "grad_packed", device, p.rows, g.cols, &gp) || !same_dtype(p, gp, "packed, grad_packed") ||
+      !output_type(g.dtype, "grad_out", &ot) || !output_type(p.dtype, "packed", &pt) || !positions_of(a[2], device, g.rows, &k, &pos))
     return nullptr;
   const int64_t slots = static_cast<int64_t>(g.rows) * k;
-  if (!flat_into(a[3], "weights", slots, t_f32, &weights) || !flat_into(a[5], "grad_weights", slots, t_f32, &grad_weights) ||
+  if (!flat_into(a[3], "weights", device, slots, t_f32, &weights) || !flat_into(a[5], "grad_weights", device, slots, t_f32, &grad_weights) ||
       !stream_of(a[6], &stream))
     return nullptr;
   return status_of([&] {
@@ -309,19 +330,20 @@ PyObject* combine_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // (handle, experts, n, k, input_type, output_type, a, rows, d, row_tokens, stream)
 PyObject* q4_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arguments(n, 11)) return nullptr;
+  const int device = current_device();
   gg_q4_plan* plan = static_cast<gg_q4_plan*>(PyLong_AsVoidPtr(a[0]));
   const long experts = PyLong_AsLong(a[1]), cols = PyLong_AsLong(a[2]), k = PyLong_AsLong(a[3]), in = PyLong_AsLong(a[4]),
              out = PyLong_AsLong(a[5]);
   Matrix x, d;
   int dt, *rows, *row_tokens;
   void* stream;
-  if (PyErr_Occurred() || !matrix(a[6], "a", -1, k, &x) || !matrix(a[8], "d", -1, cols, &d) || !output_type(d.dtype, "d", &dt))
+  if (PyErr_Occurred() || !matrix(a[6], "a", device, -1, k, &x) || !matrix(a[8], "d", device, -1, cols, &d) || !output_type(d.dtype, "d", &dt))
     return nullptr;
   if (x.dtype != (in == GG_INPUT_F16 ? t_f16 : t_bf16) || dt != out) {
     PyErr_Format(PyExc_ValueError, "a, d: the plan was made for other types than %R, %R", x.dtype, d.dtype);
     return nullptr;
   }
-  if (!flat_or_none(a[7], "rows", experts, t_i32, &rows) || !flat_or_none(a[9], "row_tokens", d.rows, t_i32, &row_tokens) ||
+  if (!flat_or_none(a[7], "rows", device, experts, t_i32, &rows) || !flat_or_none(a[9], "row_tokens", device, d.rows, t_i32, &row_tokens) ||
       !stream_of(a[10], &stream))
     return nullptr;
   return status_of([&] { return gg_q4_plan_run(plan, x.data, x.ld, x.rows, row_tokens, rows, d.data, d.ld, d.rows, stream); });
@@ -338,7 +360,7 @@ PyMODINIT_FUNC PyInit__moe_native() {
   struct {
     PyObject** to;
     const char* name;
-  } names[] = {{&n_dtype, "dtype"}, {&n_shape, "shape"}, {&n_stride, "stride"}, {&n_is_cuda, "is_cuda"}, {&n_data_ptr, "data_ptr"},
+  } names[] = {{&n_dtype, "dtype"}, {&n_shape, "shape"}, {&n_stride, "stride"}, {&n_get_device, "get_device"}, {&n_data_ptr, "data_ptr"},
                {&n_is_contiguous, "is_contiguous"}, {&n_numel, "numel"}, {&n_cuda_stream, "cuda_stream"},
                {&n_element_size, "element_size"}};
   for (auto& n : names)

@@ -4,7 +4,8 @@ gradient, the moves of rows into expert order and back, and the experts in 4-bit
 Every call goes through the C-ABI (include/grouped_gemm_b200.h, which states the definitions) and
 follows the package's manner: buffers are the caller's, calls enqueue on the given stream (None: the
 legacy default stream) without synchronising, functions return the cudaError_t value as an int, and
-constructors and tensor mismatches raise ValueError.
+constructors and tensor mismatches raise ValueError. All tensors are on the current CUDA device, and routers and
+plans run on the one that was current when they were made.
 
     router = gg.MoeRouter(experts=64, top_k=2, capacity_tokens=8192)
     router.run(logits, indices, weights, positions, rows, losses, lse=lse)

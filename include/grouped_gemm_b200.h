@@ -193,6 +193,8 @@ typedef struct gg_shard_piece {
 typedef struct gg_executor gg_executor;
 
 int gg_abi_version(void);
+/* The device that this thread's launches go to (cudaGetDevice), for a binding to compare its buffers' with. */
+int gg_current_device(int* device);
 
 /* reference src/grouped_gemm.cu:952-965 (sort_mode_name): "none", "sort_by_k", "sort_by_tiles",
  * "sort_by_tiles_then_k", or "unknown". */
@@ -445,8 +447,9 @@ typedef struct gg_route_gradient {
 } gg_route_gradient;
 
 typedef struct gg_router gg_router;
-/* Allocates the router's workspace (per-block counts and sums). Sizes out of range or an unknown
- * logit_type -> cudaErrorInvalidValue before any device work. */
+/* Allocates the router's workspace (per-block counts and sums) on the current device. Sizes out of range or an
+ * unknown logit_type -> cudaErrorInvalidValue before any device work. A run or backward pass while another device
+ * is current -> cudaErrorInvalidDevice. */
 int gg_router_create(const gg_router_config* config, gg_router** out);
 /* Enqueues on `stream`, without host synchronisation. tokens == 0 writes zero rows and losses.
  * Runs of one router on two streams at once race on its workspace: one router per concurrent stream. */
@@ -511,8 +514,8 @@ typedef struct gg_q4_problem {
 } gg_q4_problem;
 #define GG_Q4_MAX_EXPERTS 1024
 typedef struct gg_q4_plan gg_q4_plan;
-/* Allocates the plan's copy of the weights, fills it in order on `stream` and synchronises that
- * stream. Errors: sizes or types out of range, null pointers -> cudaErrorInvalidValue before any
+/* Allocates the plan's copy of the weights on the current device, fills it in order on `stream` and synchronises
+ * that stream. A run or status call while another device is current -> cudaErrorInvalidDevice. Errors: sizes or types out of range, null pointers -> cudaErrorInvalidValue before any
  * device work; CUDA errors passed through. */
 int gg_q4_plan_create(const gg_q4_problem* problem, void* stream, gg_q4_plan** out);
 /* a: rows of the input type, pitch lda (>= k); packed row r reads row r of a, or row row_tokens[r]

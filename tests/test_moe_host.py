@@ -93,3 +93,7 @@ def test_q4_rows_of_the_longest_k_need_their_bytes():
         out = ctypes.c_void_p()
         prob = capi.GGQ4Problem(cast, cast, None, None, 1, 16, k, 128, (k - 1) // 2, 0, 0, 0)
         assert capi.load().gg_q4_plan_create(ctypes.byref(prob), None, ctypes.byref(out)) == BAD
+
+
+def test_current_device_needs_a_place():
+    assert capi.load().gg_current_device(None) == BAD
