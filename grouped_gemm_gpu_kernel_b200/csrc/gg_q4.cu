@@ -6,17 +6,20 @@
 // once, whole lines at a time. The weights stand as the A operand of mma.sync m16n8k16 (16 outputs
 // a tile, 8 rows of the activations as its columns): the differences q - zero are small integers,
 // exact in FP16 and BF16, so the tensor pipe's products are exact and its sums FP32, and the group's
-// scale multiplies the FP32 sum. tcgen05 would want 128 outputs a tile, which leaves most SMs without one
-// at these sizes, and the unpacked operand in shared or tensor memory; a fragment in registers is fed from
-// the unpacking directly.
+// scale multiplies the FP32 sum. tcgen05 takes 128 outputs a tile, and the unpacked operand from shared or tensor
+// memory: through one matrix of 4096 or 14336 outputs that is 32 or 112 tiles for 148 SMs without a split of k over
+// blocks; a fragment in registers is fed from the unpacking directly. With experts enough for the tiles and rows enough
+// to pay for the way through shared memory, tcgen05 would unpack a tile once, where this kernel does for every 16 rows:
+// that form is not here.
 //
-// Measured (B200, FP16, group 128, inputs past L2): one row through 14336 x 4096, 12.8 us (2.3 TB/s of weights; 4.5 us
-// at the copy rate), of which some 5 are the start and the end of the kernel (4096 x 4096 takes 5.8); eight experts of
-// 4096 x 14336 with one row each, 52 us (4.5 TB/s), 64 rows in all 74. The copies alone, without the arithmetic, run at
-// 39 us there; the arithmetic alone, without the copies, at 47: about 165 instructions a block of 1 KB, of which
-// 98 are the unpacking and the products, at half of the issue slots (dependent steps of 16 warps an SM; 24 warps
-// at 80 registers take 20 % more instructions and no less time). Past 8 rows an expert the activations,
-// read once a tile from L1 or L2, are more bytes than the weights. Two tiles a task, which halves those reads,
+// Measured (B200, FP16, group 128, inputs past L2): one row through 14336 x 4096, 12.1 us (2.4 TB/s of weights; 4.5 us
+// at the copy rate), of which some 5 are the start and the end of the kernel (4096 x 4096 takes 6.6); eight experts of
+// 4096 x 14336 with one row each, 52 us (4.5 TB/s), 8 each 62, 64 rows as 3 to 14 each 70. The copies alone, without the
+// arithmetic, run at 39 us there; the arithmetic alone, without the copies, at 47: about 165 instructions a block of
+// 1 KB, of which 98 are the unpacking and the products, at half of the issue slots (dependent steps of 16 warps an SM;
+// 24 warps at 80 registers take 20 % more instructions and no less time). Past 8 rows an expert the activations,
+// read once a tile from L1 or L2, are more bytes than the weights, and past 16 the unpacking is done again: 256
+// rows 151 us, 1024 673, 8192 6.2 ms. Two tiles a task, which halves those reads,
 // gained 4 to 12 % above 16 rows and lost 8 to 10 % below and with group 64 and zeros: not kept.
 //
 // Weights are laid out once (gg_q4_plan_create), per expert as blocks of 16 outputs x 128 k, tile by tile
@@ -153,7 +156,8 @@ struct Q4Zero {
 };
 
 // The eight nibbles of a word as four pairs q - zero, exact (whole numbers below 2048, below 256 in
-// BF16). FP16's ten mantissa bits leave room to take two of the four pairs without a shift.
+// BF16), by a widely published method: a nibble put into the low mantissa bits of a fixed power of two makes the
+// number power + q, without a conversion. FP16's ten mantissa bits leave room to take two of the four pairs without a shift.
 __device__ __forceinline__ unsigned and_or(unsigned x, unsigned mask, unsigned add) {  // (x & mask) | add
   unsigned d;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(mask), "r"(add));
@@ -289,7 +293,7 @@ struct Q4Place {
 };
 
 // What a task weighs when the ranges are cut: a chunk of more than 8 rows against one of up to 8 (64 rows on eight
-// experts of 4096 x 14336, 3 to 14 each: 71 us with these, 78 with equal ones, 76 with 3 and 5; 74 since copies wait for gave_up()).
+// experts of 4096 x 14336, 3 to 14 each: 71 us with these, 78 with equal ones, 76 with 3 and 5).
 constexpr int kWeight8 = 3, kWeight16 = 4;
 
 // The weight of an expert's chunks: all but the last have 8 kNT rows.

@@ -11,10 +11,12 @@
 // kernel adds them (for few tokens the blocks of one cluster do both in one launch). No atomics: ranks and
 // sums have a fixed order, and the same inputs give the same bits.
 //
-// What bounds it (B200): up to some ten thousand tokens the launches (4 tokens of 64 experts 5.5 us, 999 of 37 8.4 us,
-// 16384 of 64 11.9 us, where the logits' bytes would take 0.6); then the instructions of choosing (131072 tokens of 256
-// FP32 logits, top 8: 84.7 us, 82 % of the forward kernel's issue slots, some 480 a token; the bytes would take
-// 24 us). The gradient reads the logits and writes their gradient once: 49.6 us there, 0.83 of the copy rate.
+// What bounds it (B200): up to some ten thousand tokens the launches (4 tokens of 64 experts 5.5 us, 999 of 37 8.5 us,
+// 16384 of 64 11.8 us, where the logits' bytes would take 0.6); then the instructions of choosing (131072 tokens of 256
+// FP32 logits, top 8: 85 us, 80 % of the forward kernel's issue slots, some 484 a token; the bytes would take
+// 24 us), all the more where the choice goes by rounds of maxima: 233 us there with top 16, 432 with top 32. 32768 tokens
+// of 512 experts, top 8, take 54 us, of 1024, 32 experts a lane in 8 warps an SM, 169. The gradient reads the logits and
+// writes their gradient once: 51 us for 131072 of 256, 0.81 of the copy rate.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -67,9 +69,10 @@ __device__ __forceinline__ int group_max(int v) {
   }
 }
 
-// exp(x) for x <= 0: 2^-22 + |x| 2^-24 relative (the exponential unit, and the scaled argument's
-// rounding), and 0 below 2^-126. expf() costs four times the instructions for 2^-23, which a softmax
-// over logits rounded to 16 or 24 bits has no use for.
+// exp(x) for x <= 0: 2^-22 + |x| 2^-23 relative (the exponential unit, and the roundings of log2(e) and of the scaled
+// argument), and 0 below 2^-126. expf() costs four times the instructions for 2^-23. What that would gain is lost on a
+// probability before: the terms that make up a sum have |x| of a few units, so its error is a few 2^-22, and a term of
+// larger |x| is off by more of itself, but is that much smaller (1e-5 of e^-64 at x = -64).
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -337,15 +340,6 @@ struct ForwardArgs {
   PlaceArgs place;
 };
 
-// The top_k largest keys of a token that a whole warp holds, V consecutive experts a lane, when
-// top_k <= 8: the smallest of the maxima of eight groups of four lanes bounds the 8th largest key from below,
-// so only keys from it on are candidates. On random logits that leaves about 22 (the draws until
-// every group was hit). They are gathered in shared memory in the order of experts, one a lane (two where they are
-// more than 32), and each lane counts the keys above its own: that is its slot. The counts depend on no
-// other lane's, unlike rounds that take one maximum after the other (131072 tokens of 256 experts, top 8: this kernel
-// 77 us, 91 with such rounds on the candidates, 114 with rounds on all keys). Equal keys give a slot twice, and leave one empty unless it is the last; then, and
-// only then, the keys before a lane's own are counted from its own on. Writes the slots and returns the
-// lane's part of the sum of exp(key - top); fits: false where there are more than kCandidates, and nothing is written.
 // The keys in list[0, n) (a multiple of 8 is read; those past n are kTaken) above `own`, which is at `at`; with
 // `ties` the equal ones before it as well.
 __device__ __forceinline__ int keys_above(const int* list, int n, int own, int at, bool ties) {
@@ -364,6 +358,19 @@ __device__ __forceinline__ int keys_above(const int* list, int n, int own, int a
   return rank;
 }
 
+// The top_k largest keys of a token that a whole warp holds, V consecutive experts a lane, when
+// top_k <= 8: the smallest of the maxima of eight groups of four lanes bounds the 8th largest key from below,
+// so only keys from it on are candidates. On random logits that leaves about 22 (the draws until
+// every group was hit), where every group has an open expert: with 225 to 256 experts, 449 to 512 or 897 to 1024.
+// With fewer a group holds none, all open experts are candidates, too many, and the bound and the scan are spent for
+// nothing (131072 tokens of 160 experts, top 8: 147 us forward, 84 of 256; 32768 of 384: 77, of 512: 54). Candidates
+// are gathered in shared memory in the order of experts, one a lane (two where they are
+// more than 32), and each lane counts the keys above its own: that is its slot. The counts depend on no
+// other lane's, unlike rounds that take one maximum after the other (131072 tokens of 256 experts, top 8: this kernel
+// 77 us, 91 with such rounds on the candidates, 114 with rounds on all keys). Equal keys give a slot twice, and leave
+// one empty unless it is the last; then, and only then, the keys before a lane's own are counted from its own on (BF16
+// logits near 100, most of whose tokens tie: 132 us forward, 98 near 0). Writes the slots and returns the
+// lane's part of the sum of exp(key - top); fits: false where there are more than kCandidates, and nothing is written.
 template <int V>
 __device__ __forceinline__ float choose_of_candidates(const int (&key)[V], int mine, int e0, int K, int* s_list, unsigned list, int lane,
                                                       int* s_slot, int* s_key, float top, bool* fits) {
@@ -622,7 +629,7 @@ struct BackwardArgs {
 
 // p = exp(l - lse) is off by lse's rounding to FP32, 2^-24 |lse| relative: up to here no more than by the exponential
 // itself (1e-6). A token past it has its p divided by their sum, which takes the common factor out (131072 tokens of
-// 256 FP32 logits: 51.6 us with no token past it, 54.4 with all of them, 50.0 without either).
+// 256 FP32 logits: 51.6 us with no token past it, 54.4 with all of them, 50.0 without the check).
 constexpr float kRoughLse = 16.0f;
 
 // dl = p (c_e - <c, p> + 2 g1 lse / n) + the weights' part, with c_e = g0 E f(e) / n. One pass: a
@@ -879,8 +886,8 @@ int gg_router_run(gg_router* router, const gg_route* route, void* stream) {
           st = gg::launch_chained(gg::router_place_kernel, dim3(blocks + 1), 32 * warps, place, s, 1, a.place);
       };
       // Few tokens: small blocks, so that all SMs work on them (a full block's warps share one SM's issue slots), as
-      // long as every warp has one turn (999 tokens of 37 experts, top 5: 8.8 us against 13.1 in full blocks; 4 tokens
-      // of 64, top 2: 5.4 against 8.7).
+      // long as every warp has one turn (999 tokens of 37 experts, top 5: 8.5 us against 13.1 in full blocks; 4 tokens
+      // of 64, top 2: 5.5 against 8.7).
       constexpr int kFew = V == 8 ? gg::kFewWarps : gg::router_warps(V);
       if (q.tokens <= static_cast<int64_t>(gg::kMaxBlocks) * kFew * at_once) launch(std::integral_constant<int, kFew>());
       else launch(std::integral_constant<int, gg::router_warps(V)>());
