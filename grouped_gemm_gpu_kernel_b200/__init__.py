@@ -20,6 +20,7 @@ from dataclasses import dataclass, field
 from typing import List, Optional, Sequence
 
 from . import capi
+from .ffn import F8Plan, GatedPlan, RmsNorm
 from .moe import MoeRouter, Q4Plan, moe_combine, moe_combine_backward, moe_dispatch
 
 __all__ = [
@@ -29,7 +30,7 @@ __all__ = [
     "NATIVE_CONFIGS", "REFERENCE_CONFIGS", "PAIR_CONFIGS", "selftest_wait_timeout", "capi", "MoePlan",
     "selftest_wait_timeout_word", "baseline_status", "noalloc_status", "DevicePlan",
     "InputType", "OutputType", "Activation", "Layout", "TileClasses",
-    "MoeRouter", "moe_dispatch", "moe_combine", "moe_combine_backward", "Q4Plan",
+    "MoeRouter", "moe_dispatch", "moe_combine", "moe_combine_backward", "Q4Plan", "RmsNorm", "F8Plan", "GatedPlan",
 ]
 
 
@@ -49,10 +50,13 @@ class InputType(enum.IntEnum):
 
 
 class OutputType(enum.IntEnum):
-    """Element type of every C and D (GG_OUTPUT_*); the reference's is FP32."""
+    """Element type of every C and D (GG_OUTPUT_*); the reference's is FP32. RmsNorm and the gated F8Plan also write
+    8-bit floats with a scale for each row and 128 columns."""
     kF32 = capi.GG_OUTPUT_F32
     kF16 = capi.GG_OUTPUT_F16
     kBF16 = capi.GG_OUTPUT_BF16
+    kE4M3 = capi.GG_OUTPUT_E4M3
+    kE5M2 = capi.GG_OUTPUT_E5M2
 
 
 class Layout(enum.IntEnum):
@@ -75,10 +79,11 @@ class TileClasses(enum.IntEnum):
 
 
 class Activation(enum.IntEnum):
-    """Applied to D after the bias (GG_ACT_*); GELU is the tanh form."""
+    """Applied to D after the bias (GG_ACT_*); GELU is the tanh form. SiLU: F8Plan and GatedPlan only."""
     kNone = capi.GG_ACT_NONE
     kReLU = capi.GG_ACT_RELU
     kGELU = capi.GG_ACT_GELU
+    kSiLU = capi.GG_ACT_SILU
 
 
 @dataclass

@@ -35,7 +35,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
               "--expt-relaxed-constexpr", "-I" + INCLUDE, "-I" + CSRC]
 SOURCES = ["gg_kernels.cu", "gg_host.cu", "gg_copy.cu", "gg_simt.cu", "gg_ipc.cu", "gg_router.cu",
-           "gg_rows.cu", "gg_q4.cu", "grouped_gemm_api.cpp"]
+           "gg_rows.cu", "gg_q4.cu", "gg_norm.cu", "gg_f8.cu", "gg_gated.cu", "grouped_gemm_api.cpp"]
 
 
 def nvcc() -> str:

@@ -29,6 +29,9 @@ EXPORTED_SYMBOLS = (
     "gg_router_create", "gg_router_run", "gg_router_backward", "gg_router_destroy",
     "gg_moe_dispatch", "gg_moe_combine", "gg_moe_combine_backward",
     "gg_q4_plan_create", "gg_q4_plan_run", "gg_q4_plan_status", "gg_q4_plan_destroy",
+    "gg_norm_create", "gg_norm_run", "gg_norm_backward", "gg_norm_destroy",
+    "gg_f8_plan_create", "gg_f8_plan_run", "gg_f8_plan_status", "gg_f8_plan_destroy",
+    "gg_gated_plan_create", "gg_gated_plan_run", "gg_gated_plan_backward", "gg_gated_plan_status", "gg_gated_plan_destroy",
 )
 GG_STATUS_BAD_ROWS = 0x100
 GG_STATUS_BAD_PROBLEMS = 0x200
@@ -38,6 +41,10 @@ GG_ROUTER_MAX_TOP_K = 32
 GG_ROUTER_MAX_SLOTS = 2147483647 - 65536
 GG_MOE_MAX_WIDTH = 1 << 30
 GG_Q4_MAX_EXPERTS = 1024
+GG_NORM_MAX_WIDTH = 32768
+GG_F8_MAX_EXPERTS = 1024
+GG_GATED_MAX_EXPERTS = 1024
+GG_SCALE_BLOCK = 128
 GG_INPUT_F16 = 0
 GG_INPUT_BF16 = 1
 GG_INPUT_E4M3 = 2
@@ -45,9 +52,12 @@ GG_INPUT_E5M2 = 3
 GG_OUTPUT_F32 = 0
 GG_OUTPUT_F16 = 1
 GG_OUTPUT_BF16 = 2
+GG_OUTPUT_E4M3 = 3
+GG_OUTPUT_E5M2 = 4
 GG_ACT_NONE = 0
 GG_ACT_RELU = 1
 GG_ACT_GELU = 2
+GG_ACT_SILU = 3
 GG_LAYOUT_ROW_MAJOR = 0
 GG_LAYOUT_COL_MAJOR = 1
 GG_TILE_CLASSES_NONE = 0
@@ -139,6 +149,42 @@ class GGQ4Problem(ctypes.Structure):
         (name, ctypes.c_int) for name in ("experts", "n", "k", "group", "ldq", "input_type", "output_type", "activation")]
 
 
+class GGNormConfig(ctypes.Structure):
+    _fields_ = [("width", ctypes.c_int), ("type", ctypes.c_int), ("weight_type", ctypes.c_int), ("eps", ctypes.c_float)]
+
+
+class GGNorm(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "residual", "residual_out", "weight", "y", "q", "scales", "rstd")] + [
+        (name, ctypes.c_int) for name in ("q_type", "rows", "ldx", "ldr", "ldro", "ldy", "ldq", "lds")]
+
+
+class GGNormGradient(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("h", "weight", "rstd", "grad_y", "grad_h", "grad_x", "grad_weight")] + [
+        (name, ctypes.c_int) for name in ("rows", "ldh", "ldgy", "ldgh", "ldgx")]
+
+
+class GGF8Problem(ctypes.Structure):
+    _fields_ = [(name, ctypes.POINTER(ctypes.c_void_p)) for name in ("b", "b_scales", "up", "up_scales", "bias")] + [
+        (name, ctypes.c_int) for name in ("experts", "n", "k", "ldb", "input_type", "output_type", "activation")]
+
+
+class GGGatedProblem(ctypes.Structure):
+    _fields_ = [(name, ctypes.POINTER(ctypes.c_void_p)) for name in ("gate", "up")] + [
+        (name, ctypes.c_int) for name in ("experts", "n", "k", "ldw", "type", "activation")]
+
+
+class GGGated(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "rows", "h", "gate", "up")] + [
+        (name, ctypes.c_int) for name in ("ldx", "ldh", "ldg", "capacity_rows")]
+
+
+class GGGatedGradient(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "x", "gate", "up", "grad_h", "rows", "grad_gate", "grad_up", "grad_x", "grad_wg", "grad_wu")] + [
+        ("expert_stride", ctypes.c_longlong)] + [(name, ctypes.c_int) for name in (
+            "weight_grad_type", "ldx", "ldg", "ldgh", "ldgg", "ldgx", "ldgw", "capacity_rows")]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -208,6 +254,19 @@ def load() -> ctypes.CDLL:
         "gg_q4_plan_run": ([vp, vp, ctypes.c_int, ctypes.c_int, vp, vp, vp, ctypes.c_int, ctypes.c_int, vp], ctypes.c_int),
         "gg_q4_plan_status": ([vp, i32p], ctypes.c_int),
         "gg_q4_plan_destroy": ([vp], None),
+        "gg_norm_create": ([P(GGNormConfig), P(vp)], ctypes.c_int),
+        "gg_norm_run": ([vp, P(GGNorm), vp], ctypes.c_int),
+        "gg_norm_backward": ([vp, P(GGNormGradient), vp], ctypes.c_int),
+        "gg_norm_destroy": ([vp], None),
+        "gg_f8_plan_create": ([P(GGF8Problem), P(vp)], ctypes.c_int),
+        "gg_f8_plan_run": ([vp, vp, ctypes.c_int, vp, ctypes.c_int, vp, vp, ctypes.c_int, vp, ctypes.c_int, ctypes.c_int, vp], ctypes.c_int),
+        "gg_f8_plan_status": ([vp, i32p], ctypes.c_int),
+        "gg_f8_plan_destroy": ([vp], None),
+        "gg_gated_plan_create": ([P(GGGatedProblem), P(vp)], ctypes.c_int),
+        "gg_gated_plan_run": ([vp, P(GGGated), vp], ctypes.c_int),
+        "gg_gated_plan_backward": ([vp, P(GGGatedGradient), vp], ctypes.c_int),
+        "gg_gated_plan_status": ([vp, i32p], ctypes.c_int),
+        "gg_gated_plan_destroy": ([vp], None),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

@@ -1,0 +1,447 @@
+// gg_f8.cu -- rows in 8 bits against expert weights in 8 bits, with a scale for each row and 128 values of k on the one
+// side and for each block of 128 outputs x 128 values of k on the other:
+//   G(r, o) = sum over b of sa(r, b) * sb(o / 128, b) * P_b(r, o),   P_b(r, o) = sum over k in block b of A(r, k) * B(o, k)
+//   D = act(G + bias), or act(G) * U with a second matrix of weights.
+//
+// tcgen05 (kind::f8f6f4) computes P_b of a 128 x BN tile into tensor memory, a new accumulator for each b: one stage of
+// shared memory is one b (128 bytes a row), four products of K = 32. The scales are FP32 numbers, so they cannot be left to
+// the scaled form of the instruction, whose scales are powers of two: eight warps read each P_b back and add it, times its scale, to
+// sums in their registers, BN / 2 a thread, two at a time (fma.rn.f32x2). Meanwhile the tensor cores work on the next b.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <new>
+#include <vector>
+
+#include "gg_expert_tiles.cuh"
+#include "gg_internal.h"
+#include "gg_launch.cuh"
+#include "gg_scale8.cuh"
+#include "grouped_gemm_b200.h"
+
+namespace gg {
+namespace {
+
+using namespace tiles;
+
+struct F8Params {
+  CUtensorMap a_map;            // boxes of kBoxRows rows x 128 bytes
+  const CUtensorMap* maps;      // [experts][2]: the weights', boxes of a tile's outputs x 128 bytes
+  const float* const* b_scales; // [experts]
+  const float* const* up_scales;
+  const float* const* bias;     // NULL: none
+  const float* a_scales;
+  const int* rows;
+  char* d;
+  float* d_scales;
+  int64_t d_pitch, ldas, ldds;  // d_pitch in bytes
+  int experts, n, k_blocks, tiles_n, capacity, input_format, output_type, activation;
+  bool aligned;
+  int* status;
+  unsigned long long timeout_ns;
+};
+
+template <int BN>
+struct F8Shape {
+  static constexpr int kStageBytes = kABytes + BN * kRowBytes;
+  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : BN == 64 ? 8 : 9;
+  static constexpr int kAccumulators = BN == 256 ? 2 : 4;
+  static constexpr int kTmemColumns = kAccumulators * BN;
+  static constexpr int kBars = 2 * kStages + 2 * kAccumulators + 4 + 1;
+  static_assert(kTmemColumns >= 32 && kTmemColumns <= 512);
+  static_assert(layout(kStages * kStageBytes, kMaxExperts, kBars).bytes + 1024 <= 232448, "shared memory of a block");
+};
+
+// acc += p * s for two values.
+__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t p0, uint32_t p1, uint64_t s) {
+  asm("{\n\t.reg .b64 p;\n\tmov.b64 p, {%1, %2};\n\tfma.rn.f32x2 %0, p, %3, %0;\n\t}" : "+l"(acc) : "r"(p0), "r"(p1), "l"(s));
+}
+__device__ __forceinline__ uint64_t twice(float s) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(v) : "r"(__float_as_uint(s)));
+  return v;
+}
+__device__ __forceinline__ float half_of(uint64_t v, int i) { return __uint_as_float(static_cast<uint32_t>(v >> (32 * i))); }
+
+template <int BN, bool kGated>
+__global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_constant__ F8Params p) {
+  using S = F8Shape<BN>;
+  constexpr int kStages = S::kStages, kAcc = S::kAccumulators;
+  constexpr int kWidth = kGated ? BN / 2 : BN;  // outputs of a tile
+  constexpr int kMine = kWidth / 2;             // outputs of an epilogue warp
+
+  extern __shared__ uint8_t smem_dyn[];
+  uint8_t* smem = smem_dyn + ((1024u - (ptx::smem_addr(smem_dyn) & 1023u)) & 1023u);
+  const uint32_t sbase = ptx::smem_addr(smem);
+  const Layout l = layout(kStages * S::kStageBytes, p.experts, S::kBars);
+  int* first_row = reinterpret_cast<int*>(smem + l.table);
+  int* first_tile = first_row + p.experts + 1;
+  const uint32_t bar0 = sbase + l.bars;
+  const auto full = [&](int s) { return bar0 + 8u * s; };
+  const auto empty = [&](int s) { return bar0 + 8u * (kStages + s); };
+  const auto ready = [&](int b) { return bar0 + 8u * (2 * kStages + b); };
+  const auto taken = [&](int b) { return bar0 + 8u * (2 * kStages + kAcc + b); };
+  const auto pair = [&](int q) { return bar0 + 8u * (2 * kStages + 2 * kAcc + q); };
+  const uint32_t drained = bar0 + 8u * (2 * kStages + 2 * kAcc + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + l.words);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + l.words + 4);
+  __shared__ float top[2][2][kTileRows];  // largest magnitudes of the 8-bit output: [tile parity][half][row]
+
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(full(s), 1), ptx::mbar_init(empty(s), 1);
+    for (int b = 0; b < kAcc; ++b) ptx::mbar_init(ready(b), 1), ptx::mbar_init(taken(b), kEpilogueWarps);
+    for (int q = 0; q < 4; ++q) ptx::mbar_init(pair(q), 2);
+    ptx::mbar_init(drained, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == kProductWarp) {
+    ptx::tmem_alloc(ptx::smem_addr(tmem_slot), S::kTmemColumns);
+    ptx::tmem_relinquish();
+  }
+  chained_begin();
+  if (warp == 0) expert_table(p.rows, p.experts, p.capacity, p.tiles_n, first_row, first_tile, p.status, lane);
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  const int total = first_tile[p.experts], grid = static_cast<int>(gridDim.x);
+
+  // What every role knows of tile t: its expert, first packed row, rows there, and place along the outputs.
+  struct Tile {
+    int e, row, rows, n;
+  };
+  const auto tile_at = [&](int t) {
+    Tile x;
+    x.e = expert_of(first_tile, p.experts, t);
+    const int count = first_row[x.e + 1] - first_row[x.e];
+    int m;
+    place(t - first_tile[x.e], (count + kTileRows - 1) / kTileRows, p.tiles_n, m, x.n);
+    x.row = first_row[x.e] + m * kTileRows;
+    x.rows = min(kTileRows, count - m * kTileRows);
+    return x;
+  };
+
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
+        const Tile x = tile_at(t);
+        const int boxes = (x.rows + kBoxRows - 1) / kBoxRows;
+        const CUtensorMap* maps = p.maps + 2 * x.e;
+        for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+          const int st = static_cast<int>(it % kStages);
+          ok = wait_phase(empty(st), ((it / kStages) & 1u) ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER);
+          if (!ok) break;
+          const uint32_t a = sbase + static_cast<uint32_t>(st * S::kStageBytes), b = a + kABytes;
+          ptx::mbar_arrive_expect_tx(full(st), static_cast<uint32_t>(boxes * kBoxRows + BN) * kRowBytes);
+          for (int i = 0; i < boxes; ++i)
+            ptx::tma_load_2d(a + i * kBoxRows * kRowBytes, &p.a_map, full(st), kb * kRowBytes, x.row + i * kBoxRows);
+          ptx::tma_load_2d(b, maps, full(st), kb * kRowBytes, x.n * kWidth);
+          if constexpr (kGated) ptx::tma_load_2d(b + kWidth * kRowBytes, maps + 1, full(st), kb * kRowBytes, x.n * kWidth);
+        }
+      }
+      if (!ok || *abort_flag) drain_loads<kStages>(it, full);
+    }
+  } else if (warp == kProductWarp) {
+    if (lane == 0) {
+      const uint32_t idesc = ptx::idesc_f32acc(kTileRows, BN, static_cast<uint32_t>(p.input_format - GG_INPUT_E4M3), false, false);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
+        for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+          const int st = static_cast<int>(it % kStages), buf = static_cast<int>(it % kAcc);
+          ok = wait_phase(taken(buf), ((it / kAcc) & 1u) ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA) &&
+               wait_phase(full(st), (it / kStages) & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          const uint32_t a = sbase + static_cast<uint32_t>(st * S::kStageBytes), b = a + kABytes;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            ptx::tc_mma_f8(tmem + static_cast<uint32_t>(buf * BN), ptx::smem_desc_sw128(a + kk * 32u, 16u, 1024u),
+                           ptx::smem_desc_sw128(b + kk * 32u, 16u, 1024u), idesc, kk != 0);
+          ptx::tc_commit(empty(st));
+          ptx::tc_commit(ready(buf));
+        }
+      }
+      ptx::tc_commit(drained);  // before tensor memory is freed
+      wait_drain(drained, 0u, 100000000ull);
+    }
+    __syncwarp();
+  } else if (warp < kEpilogueWarps) {
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    unsigned char* stage = smem + l.staging + warp * kStagingBytes;
+    const int scale_rows = (p.n - 1) / GG_SCALE_BLOCK;  // the last one
+    uint32_t it = 0, done = 0;
+    bool ok = true;
+    for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid, ++done) {
+      const Tile x = tile_at(t);
+      const bool mine = quarter * 32 < x.rows;  // some of the warp's rows are there
+      const int row = quarter * 32 + lane, column = x.n * kWidth + half * kMine;
+      const float* sa = p.a_scales + static_cast<int64_t>(x.row + min(row, x.rows - 1)) * p.ldas;
+      const int64_t at = static_cast<int64_t>(min(column / GG_SCALE_BLOCK, scale_rows)) * p.k_blocks;
+      const float* sb = p.b_scales[x.e] + at;
+      const float* su = kGated ? p.up_scales[x.e] + at : nullptr;
+      uint64_t acc[BN / 4];  // this row's sums: kMine outputs, and as many of U
+#pragma unroll
+      for (int j = 0; j < BN / 4; ++j) acc[j] = 0;
+      float a_next = mine ? __ldg(sa) : 0.0f, b_next = __ldg(sb), u_next = kGated ? __ldg(su) : 0.0f;
+      for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+        const uint64_t s0 = twice(a_next * b_next), s1 = kGated ? twice(a_next * u_next) : 0;
+        if (kb + 1 < p.k_blocks && mine) {
+          a_next = __ldg(sa + kb + 1), b_next = __ldg(sb + kb + 1);
+          if constexpr (kGated) u_next = __ldg(su + kb + 1);
+        }
+        const int buf = static_cast<int>(it % kAcc);
+        ok = __all_sync(0xffffffffu, wait_phase(ready(buf), (it / kAcc) & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_EPILOGUE));
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        if (mine) {
+          constexpr int kPiece = kMine < 32 ? kMine : 32;
+          const uint32_t from = lanes + static_cast<uint32_t>(buf * BN + half * kMine);
+#pragma unroll
+          for (int c = 0; c < (kGated ? 2 : 1) * kMine; c += kPiece) {
+            uint32_t r[kPiece];
+            tmem_read(from + static_cast<uint32_t>(kGated && c >= kMine ? kWidth + c - kMine : c), r);
+#pragma unroll
+            for (int j = 0; j < kPiece / 2; ++j) fma2(acc[c / 2 + j], r[2 * j], r[2 * j + 1], kGated && c >= kMine ? s1 : s0);
+          }
+        }
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(taken(buf));
+      }
+      if (!ok) break;
+      const Out o{p.d + static_cast<int64_t>(x.row + quarter * 32) * p.d_pitch, p.d_pitch, min(32, x.rows - quarter * 32), p.n, p.aligned};
+      const auto value = [&](int c) {  // output c of the warp's, before its rounding
+        const float g = half_of(acc[c / 2], c % 2);
+        if constexpr (kGated) return activate_more(g, p.activation) * half_of(acc[(kMine + c) / 2], c % 2);
+        else return g;
+      };
+      if (BN == 256 && kGated && p.output_type > GG_OUTPUT_BF16) {
+        if constexpr (BN == 256 && kGated) {
+          // a tile's 128 outputs are one block of the result: its largest magnitude is of this warp's 64 and its partner's
+          float v[kMine];
+          uint32_t most = 0;
+#pragma unroll
+          for (int c = 0; c < kMine; ++c) {
+            v[c] = value(c);
+            most = max(most, magnitude(v[c]));
+          }
+          float* mine_top = top[done & 1u][half];
+          mine_top[row] = __uint_as_float(most);
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(pair(quarter));
+          ok = __all_sync(0xffffffffu, wait_phase(pair(quarter), done & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_EPILOGUE));
+          if (!ok) break;
+          most = max(most, __float_as_uint(top[done & 1u][half ^ 1][row]));
+          if (mine) {
+            const bool e5m2 = p.output_type == GG_OUTPUT_E5M2;
+            const Scale8 s(most, e5m2 ? 57344.0f : 448.0f);
+            if (half == 0 && row < x.rows) p.d_scales[static_cast<int64_t>(x.row + row) * p.ldds + x.n] = s.scale;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              *staging_unit(stage, lane, u) =
+                  make_uint4(s.four(v[16 * u], v[16 * u + 1], v[16 * u + 2], v[16 * u + 3], e5m2),
+                             s.four(v[16 * u + 4], v[16 * u + 5], v[16 * u + 6], v[16 * u + 7], e5m2),
+                             s.four(v[16 * u + 8], v[16 * u + 9], v[16 * u + 10], v[16 * u + 11], e5m2),
+                             s.four(v[16 * u + 12], v[16 * u + 13], v[16 * u + 14], v[16 * u + 15], e5m2));
+            write_out<1, 4>(stage, lane, o, column);
+          }
+        }
+      } else if (mine) {
+        constexpr int kPiece = kMine < 32 ? kMine : 32;
+        const float* bias = !kGated && p.bias ? p.bias[x.e] : nullptr;
+#pragma unroll
+        for (int c = 0; c < kMine; c += kPiece) {
+          float v[kPiece];
+#pragma unroll
+          for (int j = 0; j < kPiece; ++j) v[j] = value(c + j);
+          if constexpr (!kGated) {
+            if (bias) {
+#pragma unroll
+              for (int j = 0; j < kPiece; ++j)
+                if (column + c + j < p.n) v[j] += __ldg(bias + column + c + j);
+            }
+            if (p.activation != GG_ACT_NONE) {
+#pragma unroll
+              for (int j = 0; j < kPiece; ++j) v[j] = activate_more(v[j], p.activation);
+            }
+          }
+          store_columns(stage, lane, v, p.output_type, o, column + c);
+        }
+      }
+    }
+  }
+
+  __syncthreads();
+  if (warp == kProductWarp) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc(tmem, S::kTmemColumns);
+  }
+}
+
+template <typename Do>
+void with_shape(int bn, bool gated, Do go) {
+  using std::integral_constant;
+  if (gated) {
+    if (bn == 256) go(integral_constant<int, 256>(), std::true_type());
+    else if (bn == 128) go(integral_constant<int, 128>(), std::true_type());
+    else go(integral_constant<int, 64>(), std::true_type());
+  } else {
+    if (bn == 256) go(integral_constant<int, 256>(), std::false_type());
+    else if (bn == 128) go(integral_constant<int, 128>(), std::false_type());
+    else if (bn == 64) go(integral_constant<int, 64>(), std::false_type());
+    else go(integral_constant<int, 32>(), std::false_type());
+  }
+}
+
+constexpr int kShapes = 4;  // 256, 128, 64, 32
+int width_of(int shape) { return 256 >> shape; }
+
+}  // namespace
+}  // namespace gg
+
+struct gg_f8_plan {
+  gg_f8_problem problem{};
+  unsigned char* block = nullptr;  // maps of every shape | tables of scales and biases | status
+  const CUtensorMap* maps[gg::kShapes] = {};
+  gg::F8Params params{};
+  int device = 0, sms = 0;
+};
+
+extern "C" {
+
+int gg_f8_plan_create(const gg_f8_problem* problem, gg_f8_plan** out) {
+  if (!out) return cudaErrorInvalidValue;
+  *out = nullptr;
+  if (!problem) return cudaErrorInvalidValue;
+  const gg_f8_problem& q = *problem;
+  const bool gated = q.up != nullptr, eight = q.output_type > GG_OUTPUT_BF16;
+  const auto off16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 != 0; };
+  if (q.experts < 1 || q.experts > GG_F8_MAX_EXPERTS || q.n < 1 || q.k < 1 || q.ldb < q.k || q.ldb % 16 != 0 || !q.b || !q.b_scales ||
+      (gated != (q.up_scales != nullptr)) || (gated && q.bias) || (q.input_type != GG_INPUT_E4M3 && q.input_type != GG_INPUT_E5M2) ||
+      q.output_type < GG_OUTPUT_F32 || q.output_type > GG_OUTPUT_E5M2 || (eight && !gated) || q.activation < GG_ACT_NONE ||
+      q.activation > GG_ACT_SILU)
+    return cudaErrorInvalidValue;
+  for (int e = 0; e < q.experts; ++e)
+    if (!q.b[e] || !q.b_scales[e] || off16(q.b[e]) || (gated && (!q.up[e] || !q.up_scales[e] || off16(q.up[e])))) return cudaErrorInvalidValue;
+
+  gg_f8_plan* plan = new (std::nothrow) gg_f8_plan();
+  if (!plan) return cudaErrorMemoryAllocation;
+  const size_t E = static_cast<size_t>(q.experts);
+  const size_t map_bytes = 2 * E * sizeof(CUtensorMap), tables_at = gg::kShapes * map_bytes, status_at = tables_at + 3 * E * sizeof(void*);
+  std::vector<unsigned char> host(status_at + sizeof(int), 0);
+  const auto maps = [&](int shape) { return reinterpret_cast<CUtensorMap*>(host.data() + shape * map_bytes); };
+  const float** tables = reinterpret_cast<const float**>(host.data() + tables_at);
+  cudaError_t st = cudaGetDevice(&plan->device);
+  if (st == cudaSuccess) st = cudaDeviceGetAttribute(&plan->sms, cudaDevAttrMultiProcessorCount, plan->device);
+  for (int e = 0; e < q.experts && st == cudaSuccess; ++e) {
+    tables[e] = q.b_scales[e];
+    tables[E + e] = gated ? q.up_scales[e] : nullptr;
+    tables[2 * E + e] = q.bias ? q.bias[e] : nullptr;
+    for (int s = 0; s < gg::kShapes && st == cudaSuccess; ++s) {
+      const int box = gg::width_of(s) / (gated ? 2 : 1);
+      if (!gg::encode_rows(&maps(s)[2 * e], 1, q.b[e], q.k, q.n, q.ldb, 128, box) ||
+          (gated && !gg::encode_rows(&maps(s)[2 * e + 1], 1, q.up[e], q.k, q.n, q.ldb, 128, box)))
+        st = cudaErrorInvalidValue;
+    }
+  }
+  for (int s = 0; s < gg::kShapes && st == cudaSuccess; ++s)
+    gg::with_shape(gg::width_of(s), gated, [&](auto bn, auto g) {
+      using S = gg::F8Shape<bn()>;
+      st = cudaFuncSetAttribute(gg::f8_kernel<bn(), g()>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                gg::tiles::layout(S::kStages * S::kStageBytes, gg::tiles::kMaxExperts, S::kBars).bytes);
+    });
+  if (st == cudaSuccess) st = cudaMalloc(reinterpret_cast<void**>(&plan->block), host.size());
+  if (st == cudaSuccess) st = cudaMemcpy(plan->block, host.data(), host.size(), cudaMemcpyHostToDevice);
+  if (st == cudaSuccess) st = cudaDeviceSynchronize();
+  if (st != cudaSuccess) {
+    if (plan->block) cudaFree(plan->block);
+    delete plan;
+    return st;
+  }
+  plan->problem = q;
+  for (int s = 0; s < gg::kShapes; ++s) plan->maps[s] = reinterpret_cast<const CUtensorMap*>(plan->block + s * map_bytes);
+  const float* const* on = reinterpret_cast<const float* const*>(plan->block + tables_at);
+  gg::F8Params& p = plan->params;
+  p.b_scales = on;
+  p.up_scales = on + E;
+  p.bias = q.bias ? on + 2 * E : nullptr;
+  p.experts = q.experts;
+  p.n = q.n;
+  p.k_blocks = (q.k - 1) / 128 + 1;
+  p.input_format = q.input_type;
+  p.output_type = q.output_type;
+  p.activation = q.activation;
+  p.status = reinterpret_cast<int*>(plan->block + status_at);
+  p.timeout_ns = gg::wait_limit_ns();
+  *out = plan;
+  return cudaSuccess;
+}
+
+int gg_f8_plan_run(gg_f8_plan* plan, const void* a, int lda, const float* a_scales, int ldas, const int* rows, void* d, int ldd,
+                   float* d_scales, int ldds, int capacity_rows, void* stream) {
+  if (!plan || !plan->block) return cudaErrorInvalidDevicePointer;
+  const gg_f8_problem& q = plan->problem;
+  gg::F8Params p = plan->params;
+  const bool gated = q.up != nullptr, eight = q.output_type > GG_OUTPUT_BF16;
+  if (capacity_rows < 0 || (!rows && q.experts != 1)) return cudaErrorInvalidValue;
+  if (capacity_rows == 0 && !rows) return cudaSuccess;
+  if (capacity_rows > 0 && (!a || !a_scales || !d || lda < q.k || lda % 16 != 0 || reinterpret_cast<uintptr_t>(a) % 16 != 0 || ldas < p.k_blocks ||
+                            ldd < q.n || (eight && (!d_scales || ldds < (q.n - 1) / GG_SCALE_BLOCK + 1))))
+    return cudaErrorInvalidValue;
+  cudaError_t st = gg::expect_device(plan->device);
+  if (st != cudaSuccess) return st;
+  const int bytes = q.output_type == GG_OUTPUT_F32 ? 4 : eight ? 1 : 2;
+  p.a_scales = a_scales;
+  p.ldas = ldas;
+  p.rows = rows;
+  p.d = static_cast<char*>(d);
+  p.d_pitch = static_cast<int64_t>(ldd) * bytes;
+  p.d_scales = d_scales;
+  p.ldds = ldds;
+  p.capacity = capacity_rows;
+  p.aligned = reinterpret_cast<uintptr_t>(d) % 16 == 0 && p.d_pitch % 16 == 0;
+  if (capacity_rows > 0 && !gg::encode_rows(&p.a_map, 1, a, q.k, capacity_rows, lda, 128, gg::tiles::kBoxRows)) return cudaErrorInvalidValue;
+  // 128-row tiles at most, if every expert's rows end in a part of one
+  const int64_t stretches = std::min<int64_t>(capacity_rows, static_cast<int64_t>(capacity_rows) / gg::tiles::kTileRows + q.experts);
+  int shape = 0;
+  const auto tiles_n = [&](int s) { return (static_cast<int64_t>(q.n) * (gated ? 2 : 1) - 1) / gg::width_of(s) + 1; };
+  while (!eight && shape < (gated ? 2 : 3) && stretches * tiles_n(shape) < plan->sms) ++shape;
+  const int64_t most = stretches * tiles_n(shape);
+  if (most > INT32_MAX) return cudaErrorInvalidValue;
+  p.tiles_n = static_cast<int>(tiles_n(shape));
+  p.maps = plan->maps[shape];
+  const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(plan->sms, most)));
+  gg::with_shape(gg::width_of(shape), gated, [&](auto bn, auto g) {
+    using S = gg::F8Shape<bn()>;
+    st = gg::launch_chained(gg::f8_kernel<bn(), g()>, dim3(grid), gg::tiles::kTileThreads,
+                            static_cast<size_t>(gg::tiles::layout(S::kStages * S::kStageBytes, q.experts, S::kBars).bytes),
+                            static_cast<cudaStream_t>(stream), 1, p);
+  });
+  return st;
+}
+
+int gg_f8_plan_status(gg_f8_plan* plan, int* status) {
+  if (!plan || !plan->block) return cudaErrorInvalidDevicePointer;
+  if (!status) return cudaErrorInvalidValue;
+  cudaError_t st = gg::expect_device(plan->device);
+  if (st == cudaSuccess) st = cudaDeviceSynchronize();
+  if (st == cudaSuccess) st = cudaMemcpy(status, plan->params.status, sizeof(int), cudaMemcpyDeviceToHost);
+  if (st != cudaSuccess) return st;
+  return cudaMemset(plan->params.status, 0, sizeof(int));
+}
+
+void gg_f8_plan_destroy(gg_f8_plan* plan) {
+  if (!plan) return;
+  if (plan->block) cudaFree(plan->block);
+  delete plan;
+}
+
+}  // extern "C"

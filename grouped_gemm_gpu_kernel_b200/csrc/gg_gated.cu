@@ -1,0 +1,582 @@
+// gg_gated.cu -- the gated feed-forward of experts, h = act(x Wg) * (x Wu), and its gradient, on packed rows whose counts are in
+// device memory.
+//
+// Three products of one shape, a 128 x 256 tile from stages of 64 deep (kind::f16, FP32 sums in tensor memory, two
+// accumulators so that one tile is taken out while the next is computed):
+//   forward   columns 0-127 of a tile are x Wg and 128-255 x Wu for the same 128 inner columns, so h is made from
+//             two columns of one lane and gate and up need not leave the SM;
+//   rows      grad_x = grad_gate Wg^T + grad_up Wu^T is one sum along both matrices' inner size;
+//   weights   grad_Wg and grad_Wu = x^T [grad_gate | grad_up], the forward's tile with the expert's rows as the inner
+//             size. The last stage of an expert can hold rows of the next one: the warp that issues the
+//             products clears them in shared memory first (at most 15 rows: it stops at the next multiple of 16, the depth
+//             of a product).
+// Before the two gradients one pass over gate, up and grad_h makes grad_gate and grad_up.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <new>
+#include <vector>
+
+#include "gg_expert_tiles.cuh"
+#include "gg_internal.h"
+#include "gg_launch.cuh"
+#include "grouped_gemm_b200.h"
+
+namespace gg {
+namespace {
+
+using namespace tiles;
+
+constexpr int kForward = 0, kRowGradient = 1, kWeightGradient = 2;
+constexpr int kBN = 256;       // columns of an accumulator
+constexpr int kDepth = 64;     // values of k of a stage
+constexpr int kStages = 4;
+constexpr int kAcc = 2;
+constexpr int kStageBytes = kABytes + kBN * kRowBytes;
+constexpr int kBars = 2 * kStages + 2 * kAcc + 1;
+constexpr int kChunkBytes = kDepth * kRowBytes;  // 64 columns x 64 values of k, a row of shared memory for each k
+static_assert(layout(kStages * kStageBytes, kMaxExperts, kBars).bytes <= 232448, "shared memory of a block");
+
+struct GatedParams {
+  CUtensorMap in[3];        // forward: x; rows: grad_gate, grad_up; weights: x, grad_gate, grad_up
+  const CUtensorMap* maps;  // [experts][2]: Wg's and Wu's
+  const int* rows;
+  char* out[3];             // forward: h, gate, up (the last two may be NULL); rows: grad_x; weights: grad_Wg, grad_Wu
+  int64_t pitch[3];         // bytes
+  int64_t expert_bytes;     // weights: from one expert's gradient to the next
+  int experts, inner, tiles_m, tiles_n, columns, out_rows, capacity, type, out_type, activation;
+  // inner: forward k, rows n; tiles_m, out_rows: weights (k); columns: of the outputs
+  bool aligned[3];
+  int* status;
+  unsigned long long timeout_ns;
+};
+
+template <int kMode>
+__global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_constant__ GatedParams p) {
+  constexpr int kWidth = kMode == kRowGradient ? kBN : kBN / 2;  // output columns of a tile
+  extern __shared__ uint8_t smem_dyn[];
+  uint8_t* smem = smem_dyn + ((1024u - (ptx::smem_addr(smem_dyn) & 1023u)) & 1023u);
+  const uint32_t sbase = ptx::smem_addr(smem);
+  const Layout l = layout(kStages * kStageBytes, p.experts, kBars);
+  int* first_row = reinterpret_cast<int*>(smem + l.table);
+  int* first_tile = first_row + p.experts + 1;
+  const uint32_t bar0 = sbase + l.bars;
+  const auto full = [&](int s) { return bar0 + 8u * s; };
+  const auto empty = [&](int s) { return bar0 + 8u * (kStages + s); };
+  const auto ready = [&](int b) { return bar0 + 8u * (2 * kStages + b); };
+  const auto taken = [&](int b) { return bar0 + 8u * (2 * kStages + kAcc + b); };
+  const uint32_t drained = bar0 + 8u * (2 * kStages + 2 * kAcc);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + l.words);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + l.words + 4);
+
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(full(s), 1), ptx::mbar_init(empty(s), 1);
+    for (int b = 0; b < kAcc; ++b) ptx::mbar_init(ready(b), 1), ptx::mbar_init(taken(b), kEpilogueWarps);
+    ptx::mbar_init(drained, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == kProductWarp) {
+    ptx::tmem_alloc(ptx::smem_addr(tmem_slot), kAcc * kBN);
+    ptx::tmem_relinquish();
+  }
+  chained_begin();
+  if (warp == 0) expert_table(p.rows, p.experts, p.capacity, p.tiles_n, first_row, first_tile, p.status, lane);
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  const int grid = static_cast<int>(gridDim.x);
+  const int per_expert = p.tiles_m * p.tiles_n;  // weights
+  const bool bad = first_tile[p.experts] < 0;
+  const int total = bad ? 0 : kMode == kWeightGradient ? p.experts * per_expert : first_tile[p.experts];
+
+  struct Tile {
+    int e, row, rows, m, n, depth;  // first packed row and rows of the tile (weights: of the expert); k blocks
+  };
+  const auto tile_at = [&](int t) {
+    Tile x;
+    if constexpr (kMode == kWeightGradient) {
+      x.e = t / per_expert;
+      place(t - x.e * per_expert, p.tiles_m, p.tiles_n, x.m, x.n);
+      x.row = first_row[x.e];
+      x.rows = first_row[x.e + 1] - x.row;
+      x.depth = (x.rows + kDepth - 1) / kDepth;
+    } else {
+      x.e = expert_of(first_tile, p.experts, t);
+      const int count = first_row[x.e + 1] - first_row[x.e];
+      place(t - first_tile[x.e], (count + kTileRows - 1) / kTileRows, p.tiles_n, x.m, x.n);
+      x.row = first_row[x.e] + x.m * kTileRows;
+      x.rows = min(kTileRows, count - x.m * kTileRows);
+      x.depth = (kMode == kRowGradient ? 2 : 1) * ((p.inner + kDepth - 1) / kDepth);
+    }
+    return x;
+  };
+
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
+        const Tile x = tile_at(t);
+        const CUtensorMap* maps = p.maps + 2 * x.e;
+        const int boxes = (x.rows + kBoxRows - 1) / kBoxRows;
+        const uint32_t bytes = static_cast<uint32_t>((kMode == kWeightGradient ? kTileRows : boxes * kBoxRows) + kBN) * kRowBytes;
+        for (int kb = 0; kb < x.depth; ++kb, ++it) {
+          const int st = static_cast<int>(it % kStages);
+          ok = wait_phase(empty(st), ((it / kStages) & 1u) ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER);
+          if (!ok) break;
+          const uint32_t a = sbase + static_cast<uint32_t>(st * kStageBytes), b = a + kABytes;
+          ptx::mbar_arrive_expect_tx(full(st), bytes);
+          if constexpr (kMode == kForward) {
+            for (int i = 0; i < boxes; ++i)
+              ptx::tma_load_2d(a + i * kBoxRows * kRowBytes, &p.in[0], full(st), kb * kDepth, x.row + i * kBoxRows);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              ptx::tma_load_2d(b + i * kChunkBytes, maps + i / 2, full(st), x.n * kWidth + i % 2 * kDepth, kb * kDepth);
+          } else if constexpr (kMode == kRowGradient) {
+            const int second = kb >= x.depth / 2, at = (second ? kb - x.depth / 2 : kb) * kDepth;
+            for (int i = 0; i < boxes; ++i)
+              ptx::tma_load_2d(a + i * kBoxRows * kRowBytes, &p.in[second], full(st), at, x.row + i * kBoxRows);
+            ptx::tma_load_2d(b, maps + second, full(st), at, x.n * kWidth);
+          } else {
+            const int at = x.row + kb * kDepth;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) ptx::tma_load_2d(a + i * kChunkBytes, &p.in[0], full(st), x.m * kTileRows + i * kDepth, at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              ptx::tma_load_2d(b + i * kChunkBytes, &p.in[1 + i / 2], full(st), x.n * kWidth + i % 2 * kDepth, at);
+          }
+        }
+      }
+      if (!ok || *abort_flag) drain_loads<kStages>(it, full);
+    }
+  } else if (warp == kProductWarp) {
+    // the forward's weights and all of the weights' gradient have k as their rows in shared memory
+    constexpr bool kAWide = kMode == kWeightGradient, kBWide = kMode != kRowGradient;
+    const uint32_t idesc = ptx::idesc_f32acc(kTileRows, kBN, static_cast<uint32_t>(p.type), kAWide, kBWide);
+    uint32_t it = 0, done = 0;
+    bool ok = true;
+    for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid, ++done) {
+      const Tile x = tile_at(t);
+      const int buf = static_cast<int>(done % kAcc);
+      ok = __all_sync(0xffffffffu, wait_phase(taken(buf), ((done / kAcc) & 1u) ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
+      if (!ok) break;
+      ptx::tc_fence_after_sync();
+      const uint32_t d = tmem + static_cast<uint32_t>(buf * kBN);
+      for (int kb = 0; kb < x.depth; ++kb, ++it) {
+        const int st = static_cast<int>(it % kStages);
+        ok = __all_sync(0xffffffffu, wait_phase(full(st), (it / kStages) & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
+        if (!ok) break;
+        const uint32_t a = sbase + static_cast<uint32_t>(st * kStageBytes), b = a + kABytes;
+        int steps = kDepth / 16;
+        if constexpr (kMode == kWeightGradient) {
+          const int left = x.rows - kb * kDepth;
+          if (left < kDepth) {
+            steps = (left + 15) / 16;
+            const int clear = steps * 16 - left;  // rows of the next expert, or of none
+            // 2 pieces of A and 4 of B, one after the other, hold a 128-byte row of 64 columns for each k
+            for (int i = lane; i < clear * 6 * 8; i += 32)
+              *reinterpret_cast<uint4*>(smem + st * kStageBytes + i / (clear * 8) * kChunkBytes + (left + i / 8 % clear) * kRowBytes + i % 8 * 16) =
+                  make_uint4(0u, 0u, 0u, 0u);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        ptx::tc_fence_after_sync();
+        if (lane == 0) {
+          for (int kk = 0; kk < steps; ++kk)
+            ptx::tc_mma_f16(d, kAWide ? ptx::smem_desc_sw128(a + kk * 2048u, kChunkBytes, 1024u) : ptx::smem_desc_sw128(a + kk * 32u, 16u, 1024u),
+                            kBWide ? ptx::smem_desc_sw128(b + kk * 2048u, kChunkBytes, 1024u) : ptx::smem_desc_sw128(b + kk * 32u, 16u, 1024u),
+                            idesc, kb != 0 || kk != 0);
+          ptx::tc_commit(empty(st));
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+      if (lane == 0) {
+        if (x.depth > 0) ptx::tc_commit(ready(buf));
+        else ptx::mbar_arrive(ready(buf));  // an expert without rows: zeros
+      }
+      __syncwarp();
+    }
+    if (lane == 0) {
+      ptx::tc_commit(drained);  // before tensor memory is freed
+      wait_drain(drained, 0u, 100000000ull);
+    }
+    __syncwarp();
+  } else if (warp < kEpilogueWarps) {
+    const int quarter = warp & 3, half = warp >> 2;
+    unsigned char* stage = smem + l.staging + warp * kStagingBytes;
+    uint32_t done = 0;
+    for (int t = static_cast<int>(blockIdx.x); t < total; t += grid, ++done) {
+      const Tile x = tile_at(t);
+      const int buf = static_cast<int>(done % kAcc);
+      if (!__all_sync(0xffffffffu, wait_phase(ready(buf), (done / kAcc) & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_EPILOGUE)))
+        break;
+      ptx::tc_fence_after_sync();
+      const uint32_t from = tmem + static_cast<uint32_t>(buf * kBN) + (static_cast<uint32_t>(quarter * 32) << 16);
+      const int rows = (kMode == kWeightGradient ? p.out_rows - x.m * kTileRows : x.rows) - quarter * 32;  // from this warp's first on
+      const int64_t row0 = (kMode == kWeightGradient ? x.m * kTileRows : x.row) + quarter * 32;
+      const auto out = [&](int i) {
+        return Out{p.out[i] + row0 * p.pitch[i] + (kMode == kWeightGradient ? x.e * p.expert_bytes : 0), p.pitch[i], min(32, rows), p.columns,
+                   p.aligned[i]};
+      };
+      if (rows > 0) {
+        if constexpr (kMode == kForward) {
+#pragma unroll
+          for (int c = half * 64; c < half * 64 + 64; c += 32) {
+            uint32_t g[32], u[32];
+            tmem_read(from + c, g);
+            tmem_read(from + 128 + c, u);
+            const int column = x.n * kWidth + c;
+            float v[32];
+            if (p.out[1]) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(g[j]);
+              store_columns(stage, lane, v, p.out_type, out(1), column);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(u[j]);
+              store_columns(stage, lane, v, p.out_type, out(2), column);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = activate_more(__uint_as_float(g[j]), p.activation) * __uint_as_float(u[j]);
+            store_columns(stage, lane, v, p.out_type, out(0), column);
+          }
+        } else {
+          // half a tile: 128 columns of grad_x, or grad_Wg's (half 0) or grad_Wu's (half 1)
+          const Out o = out(kMode == kWeightGradient ? half : 0);
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 32) {
+            uint32_t r[32];
+            float v[32];
+            if (kMode == kWeightGradient && x.depth == 0) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+            } else {
+              tmem_read(from + half * 128 + c, r);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+            }
+            store_columns(stage, lane, v, p.out_type, o, x.n * kWidth + (kMode == kWeightGradient ? 0 : half * 128) + c);
+          }
+        }
+      }
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(taken(buf));
+    }
+  }
+
+  __syncthreads();
+  if (warp == kProductWarp) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc(tmem, kAcc * kBN);
+  }
+}
+
+// act'(x) and act(x), in full precision: the pass is bound by memory.
+__device__ __forceinline__ void slope_of(float x, int act, float& slope, float& value) {
+  if (act == GG_ACT_SILU) {
+    const float s = __fdividef(1.0f, 1.0f + __expf(fminf(-x, 80.0f)));
+    value = x * s;
+    slope = s * fmaf(x, 1.0f - s, 1.0f);
+  } else if (act == GG_ACT_GELU) {
+    // 0.5 (1 + tanh(u)) = s with s = 1 / (1 + exp(-2u)), u = c (x + 0.044715 x^3); its derivative is 2 s (1 - s) u'
+    const float c = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+    const float s = __fdividef(1.0f, 1.0f + __expf(fminf(-c * fmaf(0.044715f * x, x * x, x), 80.0f)));
+    value = x * s;
+    slope = fmaf(x * s * (1.0f - s), c * fmaf(3.0f * 0.044715f * x, x, 1.0f), s);
+  } else if (act == GG_ACT_RELU) {
+    value = fmaxf(x, 0.0f);
+    slope = x > 0.0f ? 1.0f : 0.0f;
+  } else {
+    value = x;
+    slope = 1.0f;
+  }
+}
+
+struct GateGradientParams {
+  const void* gate;
+  const void* up;
+  const void* grad_h;
+  void* grad_gate;
+  void* grad_up;
+  const int* rows;
+  int64_t ldg, ldgh, ldgg;
+  int experts, n, capacity, activation;
+};
+
+constexpr int kGateThreads = 256;
+
+// grad_gate and grad_up of the rows that are there: eight columns a thread and step.
+template <int F, bool kVec>
+__global__ void __launch_bounds__(kGateThreads) gate_gradient_kernel(const GateGradientParams p) {
+  __shared__ long long s_rows;
+  __shared__ int s_bad;
+  if (threadIdx.x == 0) s_rows = p.rows ? 0 : p.capacity, s_bad = 0;
+  chained_begin();
+  __syncthreads();
+  if (p.rows) {  // their sum; bad counts are reported by the products that follow
+    long long sum = 0;
+    bool bad = false;
+    for (int e = threadIdx.x; e < p.experts; e += kGateThreads) {
+      const int r = p.rows[e];
+      bad = bad || r < 0;
+      sum += r;
+    }
+    atomicAdd(reinterpret_cast<unsigned long long*>(&s_rows), static_cast<unsigned long long>(sum));
+    if (bad) s_bad = 1;
+  }
+  __syncthreads();
+  if (s_bad || s_rows > p.capacity) return;
+  const int per_row = (p.n + 7) / 8;
+  const int64_t pieces = s_rows * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kGateThreads + threadIdx.x; i < pieces; i += static_cast<int64_t>(gridDim.x) * kGateThreads) {
+    const int64_t r = i / per_row;
+    const int c = static_cast<int>(i % per_row) * 8;
+    const unsigned short* gate = static_cast<const unsigned short*>(p.gate) + r * p.ldg + c;
+    const unsigned short* up = static_cast<const unsigned short*>(p.up) + r * p.ldg + c;
+    const unsigned short* gh = static_cast<const unsigned short*>(p.grad_h) + r * p.ldgh + c;
+    unsigned short* gg = static_cast<unsigned short*>(p.grad_gate) + r * p.ldgg + c;
+    unsigned short* gu = static_cast<unsigned short*>(p.grad_up) + r * p.ldgg + c;
+    if (kVec && c + 8 <= p.n) {
+      const uint4 a = *reinterpret_cast<const uint4*>(gate), b = *reinterpret_cast<const uint4*>(up), d = *reinterpret_cast<const uint4*>(gh);
+      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w}, dw[4] = {d.x, d.y, d.z, d.w};
+      uint32_t gw[4], uw[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = unpack2<F>(aw[j]), u = unpack2<F>(bw[j]), g = unpack2<F>(dw[j]);
+        float s0, v0, s1, v1;
+        slope_of(x.x, p.activation, s0, v0);
+        slope_of(x.y, p.activation, s1, v1);
+        gw[j] = pack2<F>(g.x * u.x * s0, g.y * u.y * s1);
+        uw[j] = pack2<F>(g.x * v0, g.y * v1);
+      }
+      *reinterpret_cast<uint4*>(gg) = make_uint4(gw[0], gw[1], gw[2], gw[3]);
+      *reinterpret_cast<uint4*>(gu) = make_uint4(uw[0], uw[1], uw[2], uw[3]);
+    } else {
+      for (int j = 0; j < 8 && c + j < p.n; ++j) {
+        const float x = widen16<F>(gate[j]), u = widen16<F>(up[j]), g = widen16<F>(gh[j]);
+        float s, v;
+        slope_of(x, p.activation, s, v);
+        store_out<F>(gg, j, g * u * s);
+        store_out<F>(gu, j, g * v);
+      }
+    }
+  }
+}
+
+bool on16(const void* p, int64_t pitch_bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && pitch_bytes % 16 == 0; }
+
+}  // namespace
+}  // namespace gg
+
+struct gg_gated_plan {
+  gg_gated_problem problem{};
+  unsigned char* block = nullptr;        // maps forward | maps rows | status
+  const CUtensorMap* maps[2] = {};
+  int* status = nullptr;
+  int device = 0, sms = 0;
+};
+
+namespace {
+
+gg::GatedParams common(const gg_gated_plan* plan, const int* rows, int capacity) {
+  gg::GatedParams p{};
+  p.rows = rows;
+  p.experts = plan->problem.experts;
+  p.capacity = capacity;
+  p.type = plan->problem.type;
+  p.out_type = plan->problem.type == GG_INPUT_F16 ? GG_OUTPUT_F16 : GG_OUTPUT_BF16;
+  p.activation = plan->problem.activation;
+  p.status = plan->status;
+  p.timeout_ns = gg::wait_limit_ns();
+  return p;
+}
+
+void set_out(gg::GatedParams& p, int i, void* out, int ld, int bytes) {
+  p.out[i] = static_cast<char*>(out);
+  p.pitch[i] = static_cast<int64_t>(ld) * bytes;
+  p.aligned[i] = gg::on16(out, p.pitch[i]);
+}
+
+template <int kMode>
+cudaError_t launch(const gg_gated_plan* plan, const gg::GatedParams& p, int64_t most, cudaStream_t stream) {
+  if (most > INT32_MAX) return cudaErrorInvalidValue;
+  const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(plan->sms, most)));
+  return gg::launch_chained(gg::gated_kernel<kMode>, dim3(grid), gg::tiles::kTileThreads,
+                            static_cast<size_t>(gg::tiles::layout(gg::kStages * gg::kStageBytes, p.experts, gg::kBars).bytes), stream, 1, p);
+}
+
+// 128-row stretches of all experts at most.
+int64_t stretches(const gg_gated_plan* plan, int capacity) {
+  return std::min<int64_t>(capacity, static_cast<int64_t>(capacity) / gg::tiles::kTileRows + plan->problem.experts);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gg_gated_plan_create(const gg_gated_problem* problem, gg_gated_plan** out) {
+  if (!out) return cudaErrorInvalidValue;
+  *out = nullptr;
+  if (!problem) return cudaErrorInvalidValue;
+  const gg_gated_problem& q = *problem;
+  const auto off16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 != 0; };
+  if (q.experts < 1 || q.experts > GG_GATED_MAX_EXPERTS || q.n < 1 || q.k < 1 || q.ldw < q.n || q.ldw % 8 != 0 || !q.gate || !q.up ||
+      (q.type != GG_INPUT_F16 && q.type != GG_INPUT_BF16) || q.activation < GG_ACT_NONE || q.activation > GG_ACT_SILU)
+    return cudaErrorInvalidValue;
+  for (int e = 0; e < q.experts; ++e)
+    if (!q.gate[e] || !q.up[e] || off16(q.gate[e]) || off16(q.up[e])) return cudaErrorInvalidValue;
+
+  gg_gated_plan* plan = new (std::nothrow) gg_gated_plan();
+  if (!plan) return cudaErrorMemoryAllocation;
+  const size_t E = static_cast<size_t>(q.experts), map_bytes = 2 * E * sizeof(CUtensorMap), status_at = 2 * map_bytes;
+  std::vector<unsigned char> host(status_at + sizeof(int), 0);
+  CUtensorMap* forward = reinterpret_cast<CUtensorMap*>(host.data());
+  CUtensorMap* rows = forward + 2 * E;
+  const int kind = q.type == GG_INPUT_F16 ? 2 : 3;
+  const int64_t pitch = static_cast<int64_t>(q.ldw) * 2;
+  cudaError_t st = cudaGetDevice(&plan->device);
+  if (st == cudaSuccess) st = cudaDeviceGetAttribute(&plan->sms, cudaDevAttrMultiProcessorCount, plan->device);
+  for (int e = 0; e < q.experts && st == cudaSuccess; ++e)
+    for (int i = 0; i < 2 && st == cudaSuccess; ++i) {
+      const void* w = i == 0 ? q.gate[e] : q.up[e];
+      if (!gg::encode_rows(&forward[2 * e + i], kind, w, q.n, q.k, pitch, 64, gg::kDepth) ||
+          !gg::encode_rows(&rows[2 * e + i], kind, w, q.n, q.k, pitch, gg::kDepth, gg::kBN))
+        st = cudaErrorInvalidValue;
+    }
+  const int smem = gg::tiles::layout(gg::kStages * gg::kStageBytes, gg::tiles::kMaxExperts, gg::kBars).bytes;
+  if (st == cudaSuccess) st = cudaFuncSetAttribute(gg::gated_kernel<gg::kForward>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (st == cudaSuccess) st = cudaFuncSetAttribute(gg::gated_kernel<gg::kRowGradient>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (st == cudaSuccess) st = cudaFuncSetAttribute(gg::gated_kernel<gg::kWeightGradient>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (st == cudaSuccess) st = cudaMalloc(reinterpret_cast<void**>(&plan->block), host.size());
+  if (st == cudaSuccess) st = cudaMemcpy(plan->block, host.data(), host.size(), cudaMemcpyHostToDevice);
+  if (st == cudaSuccess) st = cudaDeviceSynchronize();
+  if (st != cudaSuccess) {
+    if (plan->block) cudaFree(plan->block);
+    delete plan;
+    return st;
+  }
+  plan->problem = q;
+  plan->maps[0] = reinterpret_cast<const CUtensorMap*>(plan->block);
+  plan->maps[1] = plan->maps[0] + 2 * E;
+  plan->status = reinterpret_cast<int*>(plan->block + status_at);
+  *out = plan;
+  return cudaSuccess;
+}
+
+int gg_gated_plan_run(gg_gated_plan* plan, const gg_gated* call, void* stream) {
+  if (!plan || !plan->block) return cudaErrorInvalidDevicePointer;
+  const gg_gated_problem& q = plan->problem;
+  if (!call || call->capacity_rows < 0 || (!call->rows && q.experts != 1)) return cudaErrorInvalidValue;
+  const gg_gated& c = *call;
+  if (c.capacity_rows == 0 && !c.rows) return cudaSuccess;
+  if (c.capacity_rows > 0 && (!c.x || !c.h || c.ldx < q.k || !gg::on16(c.x, static_cast<int64_t>(c.ldx) * 2) || c.ldh < q.n ||
+                              (!c.gate != !c.up) || (c.gate && c.ldg < q.n)))
+    return cudaErrorInvalidValue;
+  cudaError_t st = gg::expect_device(plan->device);
+  if (st != cudaSuccess) return st;
+  gg::GatedParams p = common(plan, c.rows, c.capacity_rows);
+  p.maps = plan->maps[0];
+  p.inner = q.k;
+  p.columns = q.n;
+  p.tiles_n = (q.n - 1) / 128 + 1;
+  set_out(p, 0, c.h, c.ldh, 2);
+  set_out(p, 1, c.gate, c.ldg, 2);
+  set_out(p, 2, c.up, c.ldg, 2);
+  if (c.capacity_rows > 0 && !gg::encode_rows(&p.in[0], q.type == GG_INPUT_F16 ? 2 : 3, c.x, q.k, c.capacity_rows,
+                                              static_cast<int64_t>(c.ldx) * 2, gg::kDepth, gg::tiles::kBoxRows))
+    return cudaErrorInvalidValue;
+  return launch<gg::kForward>(plan, p, stretches(plan, c.capacity_rows) * p.tiles_n, static_cast<cudaStream_t>(stream));
+}
+
+int gg_gated_plan_backward(gg_gated_plan* plan, const gg_gated_gradient* gradient, void* stream) {
+  if (!plan || !plan->block) return cudaErrorInvalidDevicePointer;
+  const gg_gated_problem& q = plan->problem;
+  if (!gradient || gradient->capacity_rows < 0 || (!gradient->rows && q.experts != 1)) return cudaErrorInvalidValue;
+  const gg_gated_gradient& c = *gradient;
+  const int type16 = q.type == GG_INPUT_F16 ? GG_OUTPUT_F16 : GG_OUTPUT_BF16;
+  if ((!c.grad_wg != !c.grad_wu) || (c.grad_wg && ((c.weight_grad_type != GG_OUTPUT_F32 && c.weight_grad_type != type16) || c.ldgw < q.n ||
+                                                   (q.experts > 1 && c.expert_stride < static_cast<int64_t>(q.k - 1) * c.ldgw + q.n))))
+    return cudaErrorInvalidValue;
+  if (c.capacity_rows > 0 &&
+      (!c.gate || !c.up || !c.grad_h || !c.grad_gate || !c.grad_up || c.ldg < q.n || c.ldgh < q.n || c.ldgg < q.n ||
+       !gg::on16(c.grad_gate, static_cast<int64_t>(c.ldgg) * 2) || !gg::on16(c.grad_up, static_cast<int64_t>(c.ldgg) * 2) ||
+       (c.grad_x && c.ldgx < q.k) || (c.grad_wg && (!c.x || c.ldx < q.k || !gg::on16(c.x, static_cast<int64_t>(c.ldx) * 2)))))
+    return cudaErrorInvalidValue;
+  cudaError_t st = gg::expect_device(plan->device);
+  if (st != cudaSuccess) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int kind = q.type == GG_INPUT_F16 ? 2 : 3;
+  const int64_t pitch_g = static_cast<int64_t>(c.ldgg) * 2;
+  // nothing is launched before every check has passed
+  gg::GatedParams px = common(plan, c.rows, c.capacity_rows), pw = px;
+  if (c.capacity_rows > 0 && c.grad_x) {
+    px.maps = plan->maps[1];
+    px.inner = q.n;
+    px.columns = q.k;
+    px.tiles_n = (q.k - 1) / gg::kBN + 1;
+    set_out(px, 0, c.grad_x, c.ldgx, 2);
+    if (!gg::encode_rows(&px.in[0], kind, c.grad_gate, q.n, c.capacity_rows, pitch_g, gg::kDepth, gg::tiles::kBoxRows) ||
+        !gg::encode_rows(&px.in[1], kind, c.grad_up, q.n, c.capacity_rows, pitch_g, gg::kDepth, gg::tiles::kBoxRows))
+      return cudaErrorInvalidValue;
+  }
+  if (c.grad_wg) {
+    const int bytes = c.weight_grad_type == GG_OUTPUT_F32 ? 4 : 2;
+    pw.maps = plan->maps[0];
+    pw.columns = q.n;
+    pw.out_rows = q.k;
+    pw.tiles_m = (q.k - 1) / gg::tiles::kTileRows + 1;
+    pw.tiles_n = (q.n - 1) / 128 + 1;
+    pw.out_type = c.weight_grad_type;
+    set_out(pw, 0, c.grad_wg, c.ldgw, bytes);
+    set_out(pw, 1, c.grad_wu, c.ldgw, bytes);
+    pw.expert_bytes = c.expert_stride * bytes;
+    for (int i = 0; i < 2; ++i) pw.aligned[i] = pw.aligned[i] && (q.experts == 1 || pw.expert_bytes % 16 == 0);
+    if (c.capacity_rows > 0 &&
+        (!gg::encode_rows(&pw.in[0], kind, c.x, q.k, c.capacity_rows, static_cast<int64_t>(c.ldx) * 2, 64, gg::kDepth) ||
+         !gg::encode_rows(&pw.in[1], kind, c.grad_gate, q.n, c.capacity_rows, pitch_g, 64, gg::kDepth) ||
+         !gg::encode_rows(&pw.in[2], kind, c.grad_up, q.n, c.capacity_rows, pitch_g, 64, gg::kDepth)))
+      return cudaErrorInvalidValue;
+  }
+  const int64_t most_x = px.maps ? stretches(plan, c.capacity_rows) * px.tiles_n : 0;
+  const int64_t most_w = pw.maps ? static_cast<int64_t>(q.experts) * pw.tiles_m * pw.tiles_n : 0;
+  if (most_x > INT32_MAX || most_w > INT32_MAX) return cudaErrorInvalidValue;
+
+  if (c.capacity_rows > 0) {
+    gg::GateGradientParams g{c.gate, c.up, c.grad_h, c.grad_gate, c.grad_up, c.rows, c.ldg, c.ldgh, c.ldgg, q.experts, q.n, c.capacity_rows, q.activation};
+    const bool vec = gg::on16(c.gate, static_cast<int64_t>(c.ldg) * 2) && gg::on16(c.up, static_cast<int64_t>(c.ldg) * 2) &&
+                     gg::on16(c.grad_h, static_cast<int64_t>(c.ldgh) * 2);
+    const int64_t want = (static_cast<int64_t>(c.capacity_rows) * ((q.n + 7) / 8) + gg::kGateThreads - 1) / gg::kGateThreads;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(want, static_cast<int64_t>(plan->sms) * 8)));
+    const auto go = [&](auto kernel) { st = gg::launch_chained(kernel, grid, gg::kGateThreads, 0, s, 1, g); };
+    if (kind == 2) vec ? go(gg::gate_gradient_kernel<gg::kOutF16, true>) : go(gg::gate_gradient_kernel<gg::kOutF16, false>);
+    else vec ? go(gg::gate_gradient_kernel<gg::kOutBF16, true>) : go(gg::gate_gradient_kernel<gg::kOutBF16, false>);
+  }
+  if (st == cudaSuccess && px.maps) st = launch<gg::kRowGradient>(plan, px, most_x, s);
+  if (st == cudaSuccess && pw.maps) st = launch<gg::kWeightGradient>(plan, pw, most_w, s);
+  return st;
+}
+
+int gg_gated_plan_status(gg_gated_plan* plan, int* status) {
+  if (!plan || !plan->block) return cudaErrorInvalidDevicePointer;
+  if (!status) return cudaErrorInvalidValue;
+  cudaError_t st = gg::expect_device(plan->device);
+  if (st == cudaSuccess) st = cudaDeviceSynchronize();
+  if (st == cudaSuccess) st = cudaMemcpy(status, plan->status, sizeof(int), cudaMemcpyDeviceToHost);
+  if (st != cudaSuccess) return st;
+  return cudaMemset(plan->status, 0, sizeof(int));
+}
+
+void gg_gated_plan_destroy(gg_gated_plan* plan) {
+  if (!plan) return;
+  if (plan->block) cudaFree(plan->block);
+  delete plan;
+}
+
+}  // extern "C"

@@ -379,6 +379,13 @@ cudaError_t take_status(int* word, int* bits) {
 
 unsigned long long wait_limit_ns() { return wait_timeout_ns(); }
 
+bool encode_rows(CUtensorMap* map, int kind, const void* base, int inner, int outer, long long pitch, int box_inner, int box_outer) {
+  const CUtensorMapDataType type = kind == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : kind == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode_2d(map, type, base, inner, outer, pitch, box_inner, box_outer);
+}
+
 }  // namespace gg
 
 // ---- the executor ------------------------------------------------------------------------------

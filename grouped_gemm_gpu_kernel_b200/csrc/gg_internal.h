@@ -44,6 +44,11 @@ cudaError_t kernel_occupancy(Variant v, int* active_blocks_per_sm, cudaFuncAttri
 cudaError_t kernel_resident_ctas(Variant v, int* ctas);
 cudaError_t launch_wait_selftest(int* status, unsigned long long timeout_ns, cudaStream_t stream);
 
+// The tensor map of a row-major matrix on this GPU (`outer` rows of `inner` elements, pitch in bytes) for boxes of
+// box_outer rows x box_inner elements (128 bytes, 128-byte swizzle); elements of 8 bits or of 16 (kind 1, 2: FP16, 3: BF16).
+// False where the base or the pitch is off a 16-byte boundary.
+bool encode_rows(CUtensorMap* map, int kind, const void* base, int inner, int outer, long long pitch, int box_inner, int box_outer);
+
 // The limit of every wait inside a kernel (GG_WAIT_TIMEOUT_MS, 2 s by default).
 unsigned long long wait_limit_ns();
 

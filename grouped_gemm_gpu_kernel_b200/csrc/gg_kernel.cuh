@@ -42,40 +42,10 @@
 #include "gg_epilogue_ops.cuh"
 #include "gg_params.cuh"
 #include "gg_ptx.cuh"
+#include "gg_wait.cuh"
 #include "grouped_gemm_b200.h"
 
 namespace gg {
-
-// ---- bounded waits ---------------------------------------------------------------------------
-__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
-                                       unsigned long long timeout_ns, int code) {
-  const uint64_t t0 = ptx::global_timer_ns();
-  for (uint32_t i = 0;; ++i) {
-    if (ptx::mbar_try_wait(bar, parity)) return true;
-    if ((i & 31u) == 31u) {
-      if (*abort_flag) return false;
-      if (ptx::global_timer_ns() - t0 > timeout_ns || i > 0x40000000u) {
-        *abort_flag = 1;
-        atomicOr(status, code);
-        return false;
-      }
-    }
-  }
-}
-
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
-                                           unsigned long long timeout_ns, int code) {
-  if (ptx::mbar_try_wait(bar, parity)) return true;
-  return wait_slow(bar, parity, abort_flag, status, timeout_ns, code);
-}
-
-// Drain wait used after an abort: ignores the abort flag, gives up after `limit_ns`.
-__device__ __noinline__ void wait_drain(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
-  const uint64_t t0 = ptx::global_timer_ns();
-  while (!ptx::mbar_try_wait(bar, parity)) {
-    if (ptx::global_timer_ns() - t0 > limit_ns) return;
-  }
-}
 
 // ---- scheduler helpers -----------------------------------------------------------------------
 // Index q with offs[q] <= tile < offs[q+1] (empty problems are skipped because their two offsets

@@ -15,7 +15,7 @@ namespace {
 
 // Interned attribute names, and torch's dtype objects (fetched on the first call).
 PyObject *n_dtype, *n_shape, *n_stride, *n_get_device, *n_data_ptr, *n_is_contiguous, *n_numel, *n_cuda_stream, *n_element_size;
-PyObject *t_f32, *t_f16, *t_bf16, *t_i32, *t_u8, *t_bool;
+PyObject *t_f32, *t_f16, *t_bf16, *t_i32, *t_u8, *t_e4m3, *t_e5m2, *t_bool;
 
 bool load_types() {
   if (t_bool) return true;
@@ -26,7 +26,9 @@ bool load_types() {
   t_bf16 = PyObject_GetAttrString(torch, "bfloat16");
   t_i32 = PyObject_GetAttrString(torch, "int32");
   t_u8 = PyObject_GetAttrString(torch, "uint8");
-  t_bool = t_f32 && t_f16 && t_bf16 && t_i32 && t_u8 ? PyObject_GetAttrString(torch, "bool") : nullptr;
+  t_e4m3 = PyObject_GetAttrString(torch, "float8_e4m3fn");
+  t_e5m2 = PyObject_GetAttrString(torch, "float8_e5m2");
+  t_bool = t_f32 && t_f16 && t_bf16 && t_i32 && t_u8 && t_e4m3 && t_e5m2 ? PyObject_GetAttrString(torch, "bool") : nullptr;
   Py_DECREF(torch);
   return t_bool != nullptr;
 }
@@ -163,6 +165,26 @@ bool output_type(PyObject* dtype, const char* what, int* type) {
     return false;
   }
   return true;
+}
+
+// The dtype of an output type (GG_OUTPUT_*), and of an input type.
+PyObject* dtype_of_output(long type) {
+  PyObject* const of[] = {t_f32, t_f16, t_bf16, t_e4m3, t_e5m2};
+  return type >= 0 && type < 5 ? of[type] : nullptr;
+}
+PyObject* dtype_of_input(long type) {
+  PyObject* const of[] = {t_f16, t_bf16, t_e4m3, t_e5m2};
+  return type >= 0 && type < 4 ? of[type] : nullptr;
+}
+
+// A matrix of one dtype, or with `optional` None (data NULL).
+bool typed(PyObject* t, const char* what, int device, int64_t rows, int64_t cols, PyObject* dtype, Matrix* m, bool optional = false) {
+  *m = Matrix{};
+  if (optional && t == Py_None) return true;
+  if (!matrix(t, what, device, rows, cols, m)) return false;
+  if (m->dtype == dtype) return true;
+  PyErr_Format(PyExc_ValueError, "%s: %R expected, got %R", what, dtype, m->dtype);
+  return false;
 }
 
 // None (the legacy default stream), a handle, or an object with cuda_stream.
@@ -349,9 +371,185 @@ PyObject* q4_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return status_of([&] { return gg_q4_plan_run(plan, x.data, x.ld, x.rows, row_tokens, rows, d.data, d.ld, d.rows, stream); });
 }
 
+// (handle, width, type, weight_type, x, weight, y, residual, residual_out, q, scales, rstd, stream)
+PyObject* norm_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments(n, 13)) return nullptr;
+  const int device = current_device();
+  const gg_norm_plan* plan = static_cast<const gg_norm_plan*>(PyLong_AsVoidPtr(a[0]));
+  const long width = PyLong_AsLong(a[1]);
+  PyObject *type = dtype_of_output(PyLong_AsLong(a[2])), *wtype = dtype_of_output(PyLong_AsLong(a[3]));
+  if (PyErr_Occurred()) return nullptr;
+  Matrix x, y, r, ro, q{}, s{};
+  gg_norm c{};
+  void *weight, *stream;
+  if (!typed(a[4], "x", device, -1, width, type, &x) || !flat_or_none(a[5], "weight", device, width, wtype, &weight) ||
+      !typed(a[6], "y", device, x.rows, width, type, &y, true) || !typed(a[7], "residual", device, x.rows, width, type, &r, true) ||
+      !typed(a[8], "residual_out", device, x.rows, width, type, &ro, true) || !flat_or_none(a[11], "rstd", device, x.rows, t_f32, &c.rstd) ||
+      !stream_of(a[12], &stream))
+    return nullptr;
+  if ((a[9] == Py_None) != (a[10] == Py_None)) {
+    PyErr_SetString(PyExc_ValueError, "q, scales: one is missing");
+    return nullptr;
+  }
+  if (a[9] != Py_None) {
+    if (!matrix(a[9], "q", device, x.rows, width, &q) || !typed(a[10], "scales", device, x.rows, (width + GG_SCALE_BLOCK - 1) / GG_SCALE_BLOCK, t_f32, &s))
+      return nullptr;
+    if (q.dtype != t_e4m3 && q.dtype != t_e5m2) {
+      PyErr_Format(PyExc_ValueError, "q: float8_e4m3fn or float8_e5m2 expected, got %R", q.dtype);
+      return nullptr;
+    }
+    c.q_type = q.dtype == t_e4m3 ? GG_OUTPUT_E4M3 : GG_OUTPUT_E5M2;
+  }
+  c.x = x.data, c.residual = r.data, c.residual_out = ro.data, c.weight = weight, c.y = y.data, c.q = q.data;
+  c.scales = static_cast<float*>(s.data);
+  c.rows = x.rows, c.ldx = x.ld, c.ldr = r.ld, c.ldro = ro.ld, c.ldy = y.ld, c.ldq = q.ld, c.lds = s.ld;
+  return status_of([&] { return gg_norm_run(plan, &c, stream); });
+}
+
+// (handle, width, type, weight_type, h, weight, rstd, grad_y, grad_x, grad_weight, grad_h, stream)
+PyObject* norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments(n, 12)) return nullptr;
+  const int device = current_device();
+  gg_norm_plan* plan = static_cast<gg_norm_plan*>(PyLong_AsVoidPtr(a[0]));
+  const long width = PyLong_AsLong(a[1]);
+  PyObject *type = dtype_of_output(PyLong_AsLong(a[2])), *wtype = dtype_of_output(PyLong_AsLong(a[3]));
+  if (PyErr_Occurred()) return nullptr;
+  Matrix h, gy, gx, gh;
+  gg_norm_gradient c{};
+  void *weight, *rstd, *stream;
+  if (!typed(a[4], "h", device, -1, width, type, &h) || !flat_or_none(a[5], "weight", device, width, wtype, &weight) ||
+      !flat(a[6], "rstd", device, h.rows, t_f32, &rstd) || !typed(a[7], "grad_y", device, h.rows, width, type, &gy) ||
+      !typed(a[8], "grad_x", device, h.rows, width, type, &gx) || !flat_or_none(a[9], "grad_weight", device, width, t_f32, &c.grad_weight) ||
+      !typed(a[10], "grad_h", device, h.rows, width, type, &gh, true) || !stream_of(a[11], &stream))
+    return nullptr;
+  c.h = h.data, c.weight = weight, c.rstd = static_cast<const float*>(rstd), c.grad_y = gy.data, c.grad_h = gh.data, c.grad_x = gx.data;
+  c.rows = h.rows, c.ldh = h.ld, c.ldgy = gy.ld, c.ldgh = gh.ld, c.ldgx = gx.ld;
+  return status_of([&] { return gg_norm_backward(plan, &c, stream); });
+}
+
+// (handle, experts, n, k, input_type, output_type, a, a_scales, rows, d, d_scales, stream)
+PyObject* f8_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments(n, 12)) return nullptr;
+  const int device = current_device();
+  gg_f8_plan* plan = static_cast<gg_f8_plan*>(PyLong_AsVoidPtr(a[0]));
+  const long experts = PyLong_AsLong(a[1]), cols = PyLong_AsLong(a[2]), k = PyLong_AsLong(a[3]), out = PyLong_AsLong(a[5]);
+  PyObject* in = dtype_of_input(PyLong_AsLong(a[4]));
+  if (PyErr_Occurred()) return nullptr;
+  const auto blocks = [](long v) { return (v + GG_SCALE_BLOCK - 1) / GG_SCALE_BLOCK; };
+  const bool eight = out == GG_OUTPUT_E4M3 || out == GG_OUTPUT_E5M2;
+  Matrix x, sx, d, sd;
+  int* rows;
+  void* stream;
+  if (!typed(a[9], "d", device, -1, cols, dtype_of_output(out), &d) || !typed(a[6], "a", device, d.rows, k, in, &x) ||
+      !typed(a[7], "a_scales", device, d.rows, blocks(k), t_f32, &sx) || !flat_or_none(a[8], "rows", device, experts, t_i32, &rows) ||
+      !typed(a[10], "d_scales", device, d.rows, blocks(cols), t_f32, &sd, true) || !stream_of(a[11], &stream))
+    return nullptr;
+  if (eight != (a[10] != Py_None)) {
+    PyErr_SetString(PyExc_ValueError, "d_scales: expected with a d of 8 bits, and with no other");
+    return nullptr;
+  }
+  return status_of([&] {
+    return gg_f8_plan_run(plan, x.data, x.ld, static_cast<const float*>(sx.data), sx.ld, rows, d.data, d.ld, static_cast<float*>(sd.data),
+                          sd.ld, d.rows, stream);
+  });
+}
+
+// (handle, experts, n, k, type, x, rows, h, gate, up, stream)
+PyObject* gated_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments(n, 11)) return nullptr;
+  const int device = current_device();
+  gg_gated_plan* plan = static_cast<gg_gated_plan*>(PyLong_AsVoidPtr(a[0]));
+  const long experts = PyLong_AsLong(a[1]), inner = PyLong_AsLong(a[2]), k = PyLong_AsLong(a[3]);
+  PyObject* type = dtype_of_input(PyLong_AsLong(a[4]));
+  if (PyErr_Occurred()) return nullptr;
+  Matrix x, h, g, u;
+  int* rows;
+  void* stream;
+  if (!typed(a[5], "x", device, -1, k, type, &x) || !flat_or_none(a[6], "rows", device, experts, t_i32, &rows) ||
+      !typed(a[7], "h", device, x.rows, inner, type, &h) || !typed(a[8], "gate", device, x.rows, inner, type, &g, true) ||
+      !typed(a[9], "up", device, x.rows, inner, type, &u, true) || !stream_of(a[10], &stream))
+    return nullptr;
+  if ((a[8] == Py_None) != (a[9] == Py_None) || g.ld != u.ld) {
+    PyErr_SetString(PyExc_ValueError, "gate, up: both or none expected, with one pitch");
+    return nullptr;
+  }
+  const gg_gated c{x.data, rows, h.data, g.data, u.data, x.ld, h.ld, g.ld, x.rows};
+  return status_of([&] { return gg_gated_plan_run(plan, &c, stream); });
+}
+
+// The gradient of an expert's weights: (experts, k, n), contiguous columns.
+bool weight_gradient(PyObject* t, const char* what, int device, long experts, long k, long cols, Matrix* m, long long* stride) {
+  *m = Matrix{};
+  *stride = 0;
+  if (t == Py_None) return true;
+  PyObject* shape = PyObject_GetAttr(t, n_shape);
+  PyObject* strides = shape ? PyObject_CallMethodNoArgs(t, n_stride) : nullptr;
+  long long v[6] = {};
+  bool ok = strides && PyTuple_Check(shape) && PyTuple_Check(strides) && PyTuple_GET_SIZE(shape) == 3 && PyTuple_GET_SIZE(strides) == 3;
+  for (int i = 0; ok && i < 3; ++i) {
+    v[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
+    v[3 + i] = PyLong_AsLongLong(PyTuple_GET_ITEM(strides, i));
+  }
+  Py_XDECREF(shape);
+  Py_XDECREF(strides);
+  if (PyErr_Occurred()) return false;
+  bool here = false;
+  if (!on_device(t, device, &here)) return false;
+  const long long ld = k > 1 ? v[4] : v[4] >= cols ? v[4] : cols, each = experts > 1 ? v[3] : (k - 1) * ld + cols;
+  if (!ok || !here || v[0] != experts || v[1] != k || v[2] != cols || (v[5] != 1 && cols > 1) || ld < cols || ld > INT_MAX ||
+      each < (k - 1) * ld + cols) {
+    PyErr_Format(PyExc_ValueError,
+                 "%s: a tensor on the current CUDA device (%d) of shape (%ld, %ld, %ld) with contiguous columns and no overlap expected", what,
+                 device, experts, k, cols);
+    return false;
+  }
+  m->dtype = peek(t, n_dtype);
+  m->ld = static_cast<int>(ld);
+  *stride = each;
+  return m->dtype && pointer_of(t, &m->data);
+}
+
+// (handle, experts, n, k, type, x, gate, up, grad_h, rows, grad_gate, grad_up, grad_x, grad_gate_w, grad_up_w, stream)
+PyObject* gated_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments(n, 16)) return nullptr;
+  const int device = current_device();
+  gg_gated_plan* plan = static_cast<gg_gated_plan*>(PyLong_AsVoidPtr(a[0]));
+  const long experts = PyLong_AsLong(a[1]), inner = PyLong_AsLong(a[2]), k = PyLong_AsLong(a[3]);
+  PyObject* type = dtype_of_input(PyLong_AsLong(a[4]));
+  if (PyErr_Occurred()) return nullptr;
+  Matrix x, g, u, gh, gg, gu, gx, wg, wu;
+  long long sg, su;
+  gg_gated_gradient c{};
+  int* rows;
+  void* stream;
+  if (!typed(a[5], "x", device, -1, k, type, &x) || !typed(a[6], "gate", device, x.rows, inner, type, &g) ||
+      !typed(a[7], "up", device, x.rows, inner, type, &u) || !typed(a[8], "grad_h", device, x.rows, inner, type, &gh) ||
+      !flat_or_none(a[9], "rows", device, experts, t_i32, &rows) || !typed(a[10], "grad_gate", device, x.rows, inner, type, &gg) ||
+      !typed(a[11], "grad_up", device, x.rows, inner, type, &gu) || !typed(a[12], "grad_x", device, x.rows, k, type, &gx, true) ||
+      !weight_gradient(a[13], "grad_gate_w", device, experts, k, inner, &wg, &sg) ||
+      !weight_gradient(a[14], "grad_up_w", device, experts, k, inner, &wu, &su) || !stream_of(a[15], &stream))
+    return nullptr;
+  if (g.ld != u.ld || gg.ld != gu.ld) {
+    PyErr_SetString(PyExc_ValueError, "gate, up and grad_gate, grad_up: one pitch expected");
+    return nullptr;
+  }
+  if ((a[13] == Py_None) != (a[14] == Py_None) || wg.dtype != wu.dtype || wg.ld != wu.ld || sg != su ||
+      (wg.dtype && wg.dtype != t_f32 && wg.dtype != type)) {
+    PyErr_SetString(PyExc_ValueError, "grad_gate_w, grad_up_w: both or none expected, float32 or of the plan's type, with the same strides");
+    return nullptr;
+  }
+  c.x = x.data, c.gate = g.data, c.up = u.data, c.grad_h = gh.data, c.rows = rows, c.grad_gate = gg.data, c.grad_up = gu.data;
+  c.grad_x = gx.data, c.grad_wg = wg.data, c.grad_wu = wu.data, c.expert_stride = sg;
+  c.weight_grad_type = wg.dtype == t_f32 ? GG_OUTPUT_F32 : wg.dtype == t_f16 ? GG_OUTPUT_F16 : GG_OUTPUT_BF16;
+  c.ldx = x.ld, c.ldg = g.ld, c.ldgh = gh.ld, c.ldgg = gg.ld, c.ldgx = gx.ld, c.ldgw = wg.ld;
+  c.capacity_rows = x.rows;
+  return status_of([&] { return gg_gated_plan_backward(plan, &c, stream); });
+}
+
 #define GG_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {GG_METHOD(router_run), GG_METHOD(router_backward),  GG_METHOD(dispatch), GG_METHOD(combine),
-                         GG_METHOD(combine_backward), GG_METHOD(q4_run), {nullptr, nullptr, 0, nullptr}};
+                         GG_METHOD(combine_backward), GG_METHOD(q4_run), GG_METHOD(norm_run), GG_METHOD(norm_backward),
+                         GG_METHOD(f8_run), GG_METHOD(gated_run), GG_METHOD(gated_backward), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_moe_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

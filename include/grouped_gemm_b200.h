@@ -132,9 +132,16 @@ typedef struct gg_problem {
 #define GG_OUTPUT_F32 0
 #define GG_OUTPUT_F16 1
 #define GG_OUTPUT_BF16 2
+/* 8-bit floats (GG_INPUT_E4M3, GG_INPUT_E5M2) with an FP32 scale for each row and GG_SCALE_BLOCK columns. Only
+ * gg_norm_run and the gated form of gg_f8_plan_create write them. */
+#define GG_OUTPUT_E4M3 3
+#define GG_OUTPUT_E5M2 4
+#define GG_SCALE_BLOCK 128
 #define GG_ACT_NONE 0
 #define GG_ACT_RELU 1
 #define GG_ACT_GELU 2
+/* x / (1 + exp(-x)). Only gg_f8_plan_create and gg_gated_plan_create take it. */
+#define GG_ACT_SILU 3
 #define GG_LAYOUT_ROW_MAJOR 0
 #define GG_LAYOUT_COL_MAJOR 1
 #define GG_TILE_CLASSES_NONE 0
@@ -531,6 +538,175 @@ int gg_q4_plan_run(gg_q4_plan* plan, const void* a, int lda, int a_rows, const i
 /* Synchronises; returns (then clears) the GG_STATUS_* bits of the plan's runs. */
 int gg_q4_plan_status(gg_q4_plan* plan, int* status);
 void gg_q4_plan_destroy(gg_q4_plan* plan);
+
+/* ---- root-mean-square norm ---------------------------------------------------------------------
+ * No counterpart in the reference. The norm before a layer's router and experts, with the addition of the
+ * residual before it, and with the rows in 8 bits for gg_f8_plan_run:
+ *   h = x + residual, rounded to the rows' type (h = x without a residual)
+ *   rstd(r) = 1 / sqrt(mean over c of h(r, c)^2 + eps)
+ *   y(r, c) = h(r, c) * rstd(r) * weight(c)
+ *   8 bits: scale(r, b) = the largest |y| of columns 128 b to 128 b + 127, over the largest finite number of the
+ *   type (448 or 57344); q = y / scale(r, b), rounded to nearest even; y is not rounded in between. A block whose largest |y|
+ *   is below 2^-100 has scale 0 and q 0; one that holds an infinity or a NaN has a scale that is not finite.
+ * Everything but what is stored is FP32. The sums are taken in a fixed order: the same call gives the same bits. */
+#define GG_NORM_MAX_WIDTH 32768
+typedef struct gg_norm_config {
+  int width;       /* 1..GG_NORM_MAX_WIDTH */
+  int type;        /* GG_OUTPUT_F32, GG_OUTPUT_F16 or GG_OUTPUT_BF16: x, residual, h, y and their gradients */
+  int weight_type; /* the same type, or GG_OUTPUT_F32 */
+  float eps;       /* >= 0 */
+} gg_norm_config;
+
+/* One forward pass. All pointers are device memory; pitches in elements. Any alignment works; rows that start on
+ * 16-byte boundaries are fastest. residual_out and y may each be x or residual (every element is read before it is
+ * written, by the same thread). */
+typedef struct gg_norm {
+  const void* x;
+  const void* residual;   /* optional */
+  void* residual_out;     /* optional: h */
+  const void* weight;     /* optional: width values of weight_type; NULL: ones */
+  void* y;                /* optional */
+  void* q;                /* optional: 8 bits */
+  float* scales;          /* with q: rows x ceil(width / 128) */
+  float* rstd;            /* optional (needed by the backward pass): rows */
+  int q_type;             /* with q: GG_OUTPUT_E4M3 or GG_OUTPUT_E5M2 */
+  int rows;
+  int ldx, ldr, ldro, ldy, ldq, lds; /* of x, residual, residual_out, y, q and scales; those of absent ones are not read */
+} gg_norm;
+
+/* The gradient: with xhat = h * rstd and g = grad_y * weight,
+ *   grad_x(r, c) = rstd(r) * (g - xhat * mean over the row of g * xhat) + grad_h(r, c)   (of x and of the residual alike)
+ *   grad_weight(c) = sum over r of grad_y * xhat                                         (FP32)
+ * grad_x may be grad_y or grad_h. */
+typedef struct gg_norm_gradient {
+  const void* h;          /* the forward pass's h (x without a residual) */
+  const void* weight;     /* as in the forward pass */
+  const float* rstd;
+  const void* grad_y;
+  const void* grad_h;     /* optional: what reaches h past the norm */
+  void* grad_x;
+  float* grad_weight;     /* optional: width values */
+  int rows;
+  int ldh, ldgy, ldgh, ldgx;
+} gg_norm_gradient;
+
+typedef struct gg_norm_plan gg_norm_plan;
+/* Allocates the workspace of grad_weight on the current device. Sizes or types out of range, or eps negative or not
+ * finite -> cudaErrorInvalidValue before any device work. A run or backward pass while another device is current
+ * -> cudaErrorInvalidDevice. */
+int gg_norm_create(const gg_norm_config* config, gg_norm_plan** out);
+/* One launch on `stream`; uses no workspace. rows == 0 launches nothing. */
+int gg_norm_run(const gg_norm_plan* plan, const gg_norm* call, void* stream);
+/* One launch on `stream`, and a second one with grad_weight (rows == 0: zeros). Passes with grad_weight of one plan on
+ * two streams at once race on its workspace: one plan per concurrent stream. */
+int gg_norm_backward(gg_norm_plan* plan, const gg_norm_gradient* gradient, void* stream);
+void gg_norm_destroy(gg_norm_plan* plan);
+
+/* ---- experts with 8-bit weights and a scale for each block of 128 ------------------------------
+ * No counterpart in the reference. The rows of every expert, in 8 bits with a scale for each row and 128 values of
+ * k, against its weights, in 8 bits with a scale for each block of 128 outputs x 128 values of k:
+ *   G(r, o) = sum over blocks b of k:  sa(r, b) * sb(o / 128, b) * sum over k in b of A(r, k) * B(o, k)
+ *   D(r, o) = act(G(r, o) + bias(o)),     or gated     D(r, o) = act(G(r, o)) * U(r, o)
+ * with U the same product with a second matrix of weights. Rows are packed as in gg_moe_plan_run (expert 0's rows
+ * first) with the counts in device memory. The products are exact, their sums and the scales' products FP32; D is rounded
+ * once, in the gated form also to 8 bits with a scale for each row and 128 outputs, by the rule of gg_norm_run: the
+ * rows of the next product. With experts = 1 and no counts it is a plain matrix product. */
+typedef struct gg_f8_problem {
+  const void* const* b;             /* host array of `experts` device pointers: n rows of k bytes, pitch ldb, 16-byte aligned */
+  const float* const* b_scales;     /* host array of device pointers: ceil(n / 128) x ceil(k / 128), packed */
+  const void* const* up;            /* optional (gated): U's weights, like b */
+  const float* const* up_scales;    /* with up: like b_scales */
+  const float* const* bias;         /* optional, not with up: host array of device pointers (NULL entries: none): n FP32 values */
+  int experts;                      /* 1..GG_F8_MAX_EXPERTS */
+  int n;                            /* outputs, >= 1 */
+  int k;                            /* inputs, >= 1 */
+  int ldb;                          /* a multiple of 16, >= k */
+  int input_type;                   /* GG_INPUT_E4M3 or GG_INPUT_E5M2: A and the weights */
+  int output_type;                  /* GG_OUTPUT_F32, F16 or BF16; with up also GG_OUTPUT_E4M3 or E5M2 */
+  int activation;                   /* GG_ACT_* (ReLU of a NaN is 0, GELU in its tanh form) */
+} gg_f8_problem;
+#define GG_F8_MAX_EXPERTS 1024
+typedef struct gg_f8_plan gg_f8_plan;
+/* The plan refers to the weights where they are (they and the scales are read by every run) and synchronises the
+ * device once, to write its tables. Errors: sizes or types out of range, null pointers, weights or a pitch off a 16-byte
+ * boundary -> cudaErrorInvalidValue before any device work; CUDA errors passed through. */
+int gg_f8_plan_create(const gg_f8_problem* problem, gg_f8_plan** out);
+/* a: capacity_rows x k, pitch lda (a multiple of 16, >= k), 16-byte aligned; a_scales: capacity_rows x ceil(k / 128),
+ * pitch ldas. rows: `experts` counts in device memory; NULL with experts == 1: all capacity_rows rows.
+ * d: capacity_rows x n of the output type, pitch ldd (>= n), any alignment; d_scales (8-bit D): capacity_rows x
+ * ceil(n / 128), pitch ldds. Rows past the counts' sum are not written. One launch on `stream`. Counts that are negative or
+ * sum to more than capacity_rows compute nothing and raise GG_STATUS_BAD_ROWS; a bounded wait that ran out raises
+ * GG_STATUS_TIMEOUT_* (D is then wrong in part). Runs of one plan may overlap on several streams. While another device
+ * is current -> cudaErrorInvalidDevice. */
+int gg_f8_plan_run(gg_f8_plan* plan, const void* a, int lda, const float* a_scales, int ldas, const int* rows, void* d, int ldd,
+                   float* d_scales, int ldds, int capacity_rows, void* stream);
+/* Synchronises; returns (then clears) the GG_STATUS_* bits of the plan's runs. */
+int gg_f8_plan_status(gg_f8_plan* plan, int* status);
+void gg_f8_plan_destroy(gg_f8_plan* plan);
+
+/* ---- gated feed-forward of experts -------------------------------------------------------------
+ * No counterpart in the reference. For the rows of every expert, packed with the counts in device memory,
+ *   gate = x Wg,  up = x Wu,  h = act(gate) * up
+ * in one kernel, and its gradient from grad_h:
+ *   grad_gate = grad_h * up * act'(gate)        grad_up = grad_h * act(gate)
+ *   grad_x = grad_gate Wg^T + grad_up Wu^T      grad_Wg = x^T grad_gate,  grad_Wu = x^T grad_up
+ * with the row counts on the device throughout. 16-bit values, FP32 sums; h is computed from gate and up before
+ * they are rounded, the gradients from what is stored. (The way down, h Wd and grad_h = grad_y Wd^T, is a gg_moe_plan.)
+ * Matrices have rows that start on 16-byte boundaries (base and pitch); sizes are free. */
+typedef struct gg_gated_problem {
+  const void* const* gate;  /* host array of `experts` device pointers: Wg, k x n, row pitch ldw */
+  const void* const* up;    /* the same for Wu */
+  int experts;              /* 1..GG_GATED_MAX_EXPERTS */
+  int n;                    /* inner size, >= 1 */
+  int k;                    /* outer size, >= 1 */
+  int ldw;                  /* a multiple of 8, >= n */
+  int type;                 /* GG_INPUT_F16 or GG_INPUT_BF16: all 16-bit matrices */
+  int activation;           /* GG_ACT_* (ReLU of a NaN is 0 and its gradient at 0 is 0, GELU in its tanh form) */
+} gg_gated_problem;
+#define GG_GATED_MAX_EXPERTS 1024
+
+/* One forward pass; capacity_rows rows are allocated. */
+typedef struct gg_gated {
+  const void* x;       /* rows x k, pitch ldx (a multiple of 8) */
+  const int* rows;     /* `experts` counts in device memory; NULL with experts == 1: all capacity_rows rows */
+  void* h;             /* rows x n, pitch ldh */
+  void* gate;          /* optional, with up: rows x n, pitch ldg: for the backward pass */
+  void* up;
+  int ldx, ldh, ldg;
+  int capacity_rows;
+} gg_gated;
+
+/* One backward pass. grad_gate and grad_up may each be gate, up or grad_h, with that one's pitch (every element is read
+ * before it is written, by the same thread). */
+typedef struct gg_gated_gradient {
+  const void* x;
+  const void* gate;
+  const void* up;
+  const void* grad_h;  /* pitch ldgh */
+  const int* rows;
+  void* grad_gate;     /* rows x n, pitch ldgg (a multiple of 8) */
+  void* grad_up;
+  void* grad_x;        /* optional: rows x k, pitch ldgx */
+  void* grad_wg;       /* optional, with grad_wu: expert e's at e * expert_stride elements, k x n, pitch ldgw */
+  void* grad_wu;
+  long long expert_stride;
+  int weight_grad_type; /* GG_OUTPUT_F32, or the 16-bit type of the plan; an expert without rows gets zeros */
+  int ldx, ldg, ldgh, ldgg, ldgx, ldgw;
+  int capacity_rows;
+} gg_gated_gradient;
+
+typedef struct gg_gated_plan gg_gated_plan;
+/* The plan refers to the weights where they are and synchronises the device once, to write its tables. Errors as for
+ * gg_f8_plan_create. */
+int gg_gated_plan_create(const gg_gated_problem* problem, gg_gated_plan** out);
+/* One launch on `stream`. Rows past the counts' sum are not written. Bad counts and waits as for gg_f8_plan_run. Runs of
+ * one plan may overlap on several streams. While another device is current -> cudaErrorInvalidDevice. */
+int gg_gated_plan_run(gg_gated_plan* plan, const gg_gated* call, void* stream);
+/* One to three launches on `stream`: grad_gate and grad_up, grad_x, grad_wg with grad_wu. */
+int gg_gated_plan_backward(gg_gated_plan* plan, const gg_gated_gradient* gradient, void* stream);
+/* Synchronises; returns (then clears) the GG_STATUS_* bits of the plan's runs. */
+int gg_gated_plan_status(gg_gated_plan* plan, int* status);
+void gg_gated_plan_destroy(gg_gated_plan* plan);
 
 /* ---- grouped GEMM prepared on the device ----------------------------------------------------
  * No counterpart in the reference, whose problem set is prepared on the host
