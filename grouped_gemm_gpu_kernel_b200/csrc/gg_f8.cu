@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "gg_expert_tiles.cuh"
@@ -26,8 +27,16 @@ namespace {
 
 using namespace tiles;
 
+// Scales in shared memory, brought there by a warp of its own (a row's lie in a line of their own, which can be as far as L2 or
+// DRAM: read by the warps that use them, a kblock waits for them): kScaleSlots slots of kScaleBlocks blocks of k, each the tile's
+// 128 rows' and two of the weights', kScaleSlots + 2 slots ahead.
+constexpr int kScaleWarp = 9;
+constexpr int kScaleBlocks = 4;
+constexpr int kScaleSlots = 3;
+constexpr int kScaleBytes = kScaleBlocks * (kTileRows + 2) * 4 + 16;  // and which tile they are of
+
 struct F8Params {
-  CUtensorMap a_map;            // boxes of kBoxRows rows x 128 bytes
+  CUtensorMap a_map, a_box;     // 128 rows, and kBoxRows, x 128 bytes
   const CUtensorMap* maps;      // [experts][2]: the weights', boxes of a tile's outputs x 128 bytes
   const float* const* b_scales; // [experts]
   const float* const* up_scales;
@@ -38,7 +47,8 @@ struct F8Params {
   float* d_scales;
   int64_t d_pitch, ldas, ldds;  // d_pitch in bytes
   int experts, n, k_blocks, tiles_n, capacity, input_format, output_type, activation;
-  bool aligned;
+  bool aligned, wide;   // D's rows start on 16- and on 32-byte boundaries
+  bool scales_aligned;  // A's scales' rows start on 16-byte boundaries
   int* status;
   unsigned long long timeout_ns;
 };
@@ -46,24 +56,24 @@ struct F8Params {
 template <int BN>
 struct F8Shape {
   static constexpr int kStageBytes = kABytes + BN * kRowBytes;
-  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : BN == 64 ? 8 : 9;
+  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;  // even: each loading warp has its own
   static constexpr int kAccumulators = BN == 256 ? 2 : 4;
   static constexpr int kTmemColumns = kAccumulators * BN;
-  static constexpr int kBars = 2 * kStages + 2 * kAccumulators + 4 + 1;
-  static_assert(kTmemColumns >= 32 && kTmemColumns <= 512);
-  static_assert(layout(kStages * kStageBytes, kMaxExperts, kBars).bytes + 1024 <= 232448, "shared memory of a block");
+  static constexpr int kBars = 2 * kStages + 2 * kAccumulators + 4 + 2 * kScaleSlots + 1;
+  static_assert(kStages % 2 == 0 && kTmemColumns >= 32 && kTmemColumns <= 512);
+  static_assert(layout(kStages * kStageBytes, kMaxExperts, kBars, kScaleSlots * kScaleBytes).bytes + 2048 <= 232448, "shared memory of a block");
 };
 
 // acc += p * s for two values.
 __device__ __forceinline__ void fma2(uint64_t& acc, uint32_t p0, uint32_t p1, uint64_t s) {
   asm("{\n\t.reg .b64 p;\n\tmov.b64 p, {%1, %2};\n\tfma.rn.f32x2 %0, p, %3, %0;\n\t}" : "+l"(acc) : "r"(p0), "r"(p1), "l"(s));
 }
+__device__ __forceinline__ float half_of(uint64_t v, int i) { return __uint_as_float(static_cast<uint32_t>(v >> (32 * i))); }
 __device__ __forceinline__ uint64_t twice(float s) {
   uint64_t v;
   asm("mov.b64 %0, {%1, %1};" : "=l"(v) : "r"(__float_as_uint(s)));
   return v;
 }
-__device__ __forceinline__ float half_of(uint64_t v, int i) { return __uint_as_float(static_cast<uint32_t>(v >> (32 * i))); }
 
 template <int BN, bool kGated>
 __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_constant__ F8Params p) {
@@ -75,7 +85,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
   extern __shared__ uint8_t smem_dyn[];
   uint8_t* smem = smem_dyn + ((1024u - (ptx::smem_addr(smem_dyn) & 1023u)) & 1023u);
   const uint32_t sbase = ptx::smem_addr(smem);
-  const Layout l = layout(kStages * S::kStageBytes, p.experts, S::kBars);
+  const Layout l = layout(kStages * S::kStageBytes, p.experts, S::kBars, kScaleSlots * kScaleBytes);
   int* first_row = reinterpret_cast<int*>(smem + l.table);
   int* first_tile = first_row + p.experts + 1;
   const uint32_t bar0 = sbase + l.bars;
@@ -84,7 +94,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
   const auto ready = [&](int b) { return bar0 + 8u * (2 * kStages + b); };
   const auto taken = [&](int b) { return bar0 + 8u * (2 * kStages + kAcc + b); };
   const auto pair = [&](int q) { return bar0 + 8u * (2 * kStages + 2 * kAcc + q); };
-  const uint32_t drained = bar0 + 8u * (2 * kStages + 2 * kAcc + 4);
+  const auto scales_in = [&](uint32_t i) { return bar0 + 8u * (2 * kStages + 2 * kAcc + 4 + i); };
+  const auto scales_used = [&](uint32_t i) { return bar0 + 8u * (2 * kStages + 2 * kAcc + 4 + kScaleSlots + i); };
+  const uint32_t drained = bar0 + 8u * (2 * kStages + 2 * kAcc + 4 + 2 * kScaleSlots);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + l.words);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + l.words + 4);
   __shared__ float top[2][2][kTileRows];  // largest magnitudes of the 8-bit output: [tile parity][half][row]
@@ -94,6 +106,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
     for (int s = 0; s < kStages; ++s) ptx::mbar_init(full(s), 1), ptx::mbar_init(empty(s), 1);
     for (int b = 0; b < kAcc; ++b) ptx::mbar_init(ready(b), 1), ptx::mbar_init(taken(b), kEpilogueWarps);
     for (int q = 0; q < 4; ++q) ptx::mbar_init(pair(q), 2);
+    for (uint32_t i = 0; i < kScaleSlots; ++i) ptx::mbar_init(scales_in(i), 1), ptx::mbar_init(scales_used(i), kEpilogueWarps);
     ptx::mbar_init(drained, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
@@ -102,6 +115,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
     ptx::tmem_alloc(ptx::smem_addr(tmem_slot), S::kTmemColumns);
     ptx::tmem_relinquish();
   }
+  clear_rows<kStages, S::kStageBytes>(smem);
   chained_begin();
   if (warp == 0) expert_table(p.rows, p.experts, p.capacity, p.tiles_n, first_row, first_tile, p.status, lane);
   ptx::tc_fence_before_sync();
@@ -111,7 +125,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
   const int total = first_tile[p.experts], grid = static_cast<int>(gridDim.x);
 
   // What every role knows of tile t: its expert, first packed row, rows there, and place along the outputs.
-  struct Tile {
+  struct alignas(16) Tile {
     int e, row, rows, n;
   };
   const auto tile_at = [&](int t) {
@@ -125,158 +139,250 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
     return x;
   };
 
-  if (warp == kLoadWarp) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
-        const Tile x = tile_at(t);
-        const int boxes = (x.rows + kBoxRows - 1) / kBoxRows;
-        const CUtensorMap* maps = p.maps + 2 * x.e;
-        for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-          const int st = static_cast<int>(it % kStages);
-          ok = wait_phase(empty(st), ((it / kStages) & 1u) ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER);
-          if (!ok) break;
-          const uint32_t a = sbase + static_cast<uint32_t>(st * S::kStageBytes), b = a + kABytes;
-          ptx::mbar_arrive_expect_tx(full(st), static_cast<uint32_t>(boxes * kBoxRows + BN) * kRowBytes);
-          for (int i = 0; i < boxes; ++i)
-            ptx::tma_load_2d(a + i * kBoxRows * kRowBytes, &p.a_map, full(st), kb * kRowBytes, x.row + i * kBoxRows);
-          ptx::tma_load_2d(b, maps, full(st), kb * kRowBytes, x.n * kWidth);
-          if constexpr (kGated) ptx::tma_load_2d(b + kWidth * kRowBytes, maps + 1, full(st), kb * kRowBytes, x.n * kWidth);
-        }
-      }
-      if (!ok || *abort_flag) drain_loads<kStages>(it, full);
-    }
-  } else if (warp == kProductWarp) {
-    if (lane == 0) {
-      const uint32_t idesc = ptx::idesc_f32acc(kTileRows, BN, static_cast<uint32_t>(p.input_format - GG_INPUT_E4M3), false, false);
-      uint32_t it = 0;
-      bool ok = true;
-      for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
-        for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-          const int st = static_cast<int>(it % kStages), buf = static_cast<int>(it % kAcc);
-          ok = wait_phase(taken(buf), ((it / kAcc) & 1u) ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA) &&
-               wait_phase(full(st), (it / kStages) & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA);
-          if (!ok) break;
-          ptx::tc_fence_after_sync();
-          const uint32_t a = sbase + static_cast<uint32_t>(st * S::kStageBytes), b = a + kABytes;
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            ptx::tc_mma_f8(tmem + static_cast<uint32_t>(buf * BN), ptx::smem_desc_sw128(a + kk * 32u, 16u, 1024u),
-                           ptx::smem_desc_sw128(b + kk * 32u, 16u, 1024u), idesc, kk != 0);
-          ptx::tc_commit(empty(st));
-          ptx::tc_commit(ready(buf));
-        }
-      }
-      ptx::tc_commit(drained);  // before tensor memory is freed
-      wait_drain(drained, 0u, 100000000ull);
-    }
-    __syncwarp();
-  } else if (warp < kEpilogueWarps) {
+  if (warp < kEpilogueWarps) {
+    epilogue_registers();
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     unsigned char* stage = smem + l.staging + warp * kStagingBytes;
-    const int scale_rows = (p.n - 1) / GG_SCALE_BLOCK;  // the last one
-    uint32_t it = 0, done = 0;
+    uint32_t it = 0, done = 0, slot = 0;
     bool ok = true;
-    for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid, ++done) {
-      const Tile x = tile_at(t);
+    for (int t = static_cast<int>(blockIdx.x); t < total; t += grid, ++done) {
+      // the tile comes with its first scales: finding it takes the warp that brings them 1000 cycles
+      const auto slot_at = [&](uint32_t i) { return smem + l.own + i % kScaleSlots * kScaleBytes; };
+      ok = __all_sync(0xffffffffu, wait_phase_inline(scales_in(slot % kScaleSlots), (slot / kScaleSlots) & 1u, abort_flag, p.status, p.timeout_ns,
+                                                     GG_STATUS_TIMEOUT_EPILOGUE));
+      if (!ok) break;
+      const Tile x = *reinterpret_cast<const Tile*>(slot_at(slot) + kScaleBytes - 16);
       const bool mine = quarter * 32 < x.rows;  // some of the warp's rows are there
       const int row = quarter * 32 + lane, column = x.n * kWidth + half * kMine;
-      const float* sa = p.a_scales + static_cast<int64_t>(x.row + min(row, x.rows - 1)) * p.ldas;
-      const int64_t at = static_cast<int64_t>(min(column / GG_SCALE_BLOCK, scale_rows)) * p.k_blocks;
-      const float* sb = p.b_scales[x.e] + at;
-      const float* su = kGated ? p.up_scales[x.e] + at : nullptr;
       uint64_t acc[BN / 4];  // this row's sums: kMine outputs, and as many of U
 #pragma unroll
       for (int j = 0; j < BN / 4; ++j) acc[j] = 0;
-      float a_next = mine ? __ldg(sa) : 0.0f, b_next = __ldg(sb), u_next = kGated ? __ldg(su) : 0.0f;
-      for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-        const uint64_t s0 = twice(a_next * b_next), s1 = kGated ? twice(a_next * u_next) : 0;
-        if (kb + 1 < p.k_blocks && mine) {
-          a_next = __ldg(sa + kb + 1), b_next = __ldg(sb + kb + 1);
-          if constexpr (kGated) u_next = __ldg(su + kb + 1);
-        }
-        const int buf = static_cast<int>(it % kAcc);
-        ok = __all_sync(0xffffffffu, wait_phase(ready(buf), (it / kAcc) & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_EPILOGUE));
+      for (int kb0 = 0; ok && kb0 < p.k_blocks; kb0 += kScaleBlocks, ++slot) {
+        const float* scales = reinterpret_cast<const float*>(slot_at(slot));
+        ok = kb0 == 0 || __all_sync(0xffffffffu, wait_phase_inline(scales_in(slot % kScaleSlots), (slot / kScaleSlots) & 1u, abort_flag, p.status, p.timeout_ns,
+                                                       GG_STATUS_TIMEOUT_EPILOGUE));
         if (!ok) break;
-        ptx::tc_fence_after_sync();
-        if (mine) {
-          constexpr int kPiece = kMine < 32 ? kMine : 32;
-          const uint32_t from = lanes + static_cast<uint32_t>(buf * BN + half * kMine);
 #pragma unroll
-          for (int c = 0; c < (kGated ? 2 : 1) * kMine; c += kPiece) {
-            uint32_t r[kPiece];
-            tmem_read(from + static_cast<uint32_t>(kGated && c >= kMine ? kWidth + c - kMine : c), r);
+        for (int i = 0; i < kScaleBlocks; ++i) {
+          if (kb0 + i >= p.k_blocks) break;
+          const float a = scales[i * kTileRows + row];
+          const float2 b = *reinterpret_cast<const float2*>(scales + kScaleBlocks * kTileRows + 2 * i);
+          const uint64_t s0 = twice(a * (kGated || half == 0 ? b.x : b.y)), s1 = kGated ? twice(a * b.y) : 0;
+          const uint32_t buf = it % kAcc;
+          ok = __all_sync(0xffffffffu, wait_phase_inline(ready(static_cast<int>(buf)), (it / kAcc) & 1u, abort_flag, p.status, p.timeout_ns,
+                                                         GG_STATUS_TIMEOUT_EPILOGUE));
+          if (!ok) break;
+          ++it;
+          ptx::tc_fence_after_sync();
+          // a piece is read while the one before it is added up
+          constexpr int kPiece = kMine < 32 || BN == 256 ? 16 : 32, kPieces = (kGated ? 2 : 1) * kMine / kPiece;
+          const uint32_t from = lanes + buf * BN + static_cast<uint32_t>(half * kMine);
+          const auto at_piece = [&](int c) { return from + static_cast<uint32_t>(kGated && c * kPiece >= kMine ? kWidth + c * kPiece - kMine : c * kPiece); };
+          uint32_t r[2][kPiece];
+          if (mine) tmem_start(at_piece(0), r[0]);
 #pragma unroll
-            for (int j = 0; j < kPiece / 2; ++j) fma2(acc[c / 2 + j], r[2 * j], r[2 * j + 1], kGated && c >= kMine ? s1 : s0);
+          for (int c = 0; c < kPieces; ++c) {
+            if (mine) {
+              tmem_wait(r[c % 2]);
+              if (c + 1 < kPieces) tmem_start(at_piece(c + 1), r[(c + 1) % 2]);
+            }
+            if (c + 1 == kPieces) {  // all of it is read
+              ptx::tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) ptx::mbar_arrive(taken(static_cast<int>(buf)));
+            }
+            if (mine) {
+#pragma unroll
+              for (int j = 0; j < kPiece / 2; ++j)
+                fma2(acc[c * kPiece / 2 + j], r[c % 2][2 * j], r[c % 2][2 * j + 1], kGated && c * kPiece >= kMine ? s1 : s0);
+            }
           }
         }
-        ptx::tc_fence_before_sync();
+        if (!ok) break;
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(taken(buf));
+        if (lane == 0) ptx::mbar_arrive(scales_used(slot % kScaleSlots));
       }
       if (!ok) break;
-      const Out o{p.d + static_cast<int64_t>(x.row + quarter * 32) * p.d_pitch, p.d_pitch, min(32, x.rows - quarter * 32), p.n, p.aligned};
-      const auto value = [&](int c) {  // output c of the warp's, before its rounding
-        const float g = half_of(acc[c / 2], c % 2);
-        if constexpr (kGated) return activate_more(g, p.activation) * half_of(acc[(kMine + c) / 2], c % 2);
-        else return g;
+      const Out o{p.d + static_cast<int64_t>(x.row + quarter * 32) * p.d_pitch, p.d_pitch, min(32, x.rows - quarter * 32), p.n, p.aligned, p.wide};
+      const float* bias = !kGated && p.bias ? p.bias[x.e] : nullptr;
+      // N of the warp's outputs from c on, before their rounding
+      const auto values = [&](auto& v, int c) {
+        constexpr int N = sizeof(v) / sizeof(float);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = half_of(acc[(c + j) / 2], j % 2);
+        if (!kGated && bias) {
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            if (column + c + j < p.n) v[j] += __ldg(bias + column + c + j);
+        }
+        activate_all(v, p.activation);
+        if constexpr (kGated) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) v[j] *= half_of(acc[(kMine + c + j) / 2], j % 2);
+        }
       };
-      if (BN == 256 && kGated && p.output_type > GG_OUTPUT_BF16) {
-        if constexpr (BN == 256 && kGated) {
-          // a tile's 128 outputs are one block of the result: its largest magnitude is of this warp's 64 and its partner's
-          float v[kMine];
-          uint32_t most = 0;
+      bool eight = false;
+      if constexpr (BN == 256 && kGated) eight = p.output_type > GG_OUTPUT_BF16;
+      if (!eight) {
+        if (mine) {
+          constexpr int kPiece = kMine < 32 ? kMine : 32;
 #pragma unroll
-          for (int c = 0; c < kMine; ++c) {
-            v[c] = value(c);
-            most = max(most, magnitude(v[c]));
-          }
-          float* mine_top = top[done & 1u][half];
-          mine_top[row] = __uint_as_float(most);
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(pair(quarter));
-          ok = __all_sync(0xffffffffu, wait_phase(pair(quarter), done & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_EPILOGUE));
-          if (!ok) break;
-          most = max(most, __float_as_uint(top[done & 1u][half ^ 1][row]));
-          if (mine) {
-            const bool e5m2 = p.output_type == GG_OUTPUT_E5M2;
-            const Scale8 s(most, e5m2 ? 57344.0f : 448.0f);
-            if (half == 0 && row < x.rows) p.d_scales[static_cast<int64_t>(x.row + row) * p.ldds + x.n] = s.scale;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              *staging_unit(stage, lane, u) =
-                  make_uint4(s.four(v[16 * u], v[16 * u + 1], v[16 * u + 2], v[16 * u + 3], e5m2),
-                             s.four(v[16 * u + 4], v[16 * u + 5], v[16 * u + 6], v[16 * u + 7], e5m2),
-                             s.four(v[16 * u + 8], v[16 * u + 9], v[16 * u + 10], v[16 * u + 11], e5m2),
-                             s.four(v[16 * u + 12], v[16 * u + 13], v[16 * u + 14], v[16 * u + 15], e5m2));
-            write_out<1, 4>(stage, lane, o, column);
+          for (int c = 0; c < kMine; c += kPiece) {
+            float v[kPiece];
+            values(v, c);
+            store_columns(stage, lane, v, p.output_type, o, column + c);
           }
         }
-      } else if (mine) {
-        constexpr int kPiece = kMine < 32 ? kMine : 32;
-        const float* bias = !kGated && p.bias ? p.bias[x.e] : nullptr;
+      } else if constexpr (BN == 256 && kGated) {
+        // a tile's 128 outputs are one block of the result: its largest magnitude is of this warp's 64 and its partner's
+        float v[kMine];
+        values(v, 0);
+        uint32_t most = 0;
 #pragma unroll
-        for (int c = 0; c < kMine; c += kPiece) {
-          float v[kPiece];
+        for (int c = 0; c < kMine; ++c) most = max(most, magnitude(v[c]));
+        top[done & 1u][half][row] = __uint_as_float(most);
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(pair(quarter));
+        ok = __all_sync(0xffffffffu, wait_phase_inline(pair(quarter), done & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_EPILOGUE));
+        if (!ok) break;
+        most = max(most, __float_as_uint(top[done & 1u][half ^ 1][row]));
+        if (mine) {
+          const bool e5m2 = p.output_type == GG_OUTPUT_E5M2;
+          const Scale8 s(most, e5m2 ? 57344.0f : 448.0f);
+          if (half == 0 && row < x.rows) p.d_scales[static_cast<int64_t>(x.row + row) * p.ldds + x.n] = s.scale;
+          const auto put = [&](auto kind) {
+            uint32_t w[kMine / 4];
 #pragma unroll
-          for (int j = 0; j < kPiece; ++j) v[j] = value(c + j);
-          if constexpr (!kGated) {
-            if (bias) {
-#pragma unroll
-              for (int j = 0; j < kPiece; ++j)
-                if (column + c + j < p.n) v[j] += __ldg(bias + column + c + j);
-            }
-            if (p.activation != GG_ACT_NONE) {
-#pragma unroll
-              for (int j = 0; j < kPiece; ++j) v[j] = activate_more(v[j], p.activation);
-            }
-          }
-          store_columns(stage, lane, v, p.output_type, o, column + c);
+            for (int i = 0; i < kMine / 4; ++i) w[i] = s.four(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], kind());
+            store_bytes(stage, lane, w, o, column);
+          };
+          if (e5m2) put(std::true_type());
+          else put(std::false_type());
         }
       }
     }
+    __syncthreads();
+    return;
+  }
+  other_registers();
+  if (warp >= kLoadWarp) {
+    const bool leader = ptx::elect_one();
+    RowLoads<kStages> rows;
+    Ring<kStages, 2> stage;
+    stage.at = warp - kLoadWarp;
+    int skip = stage.at;  // blocks of k until this warp's next
+    bool ok = true;
+    for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
+      const Tile x = tile_at(t);
+      const CUtensorMap* maps = p.maps + 2 * x.e;
+      int kb = skip;
+      for (; kb < p.k_blocks; kb += 2) {
+        ok = __all_sync(0xffffffffu, wait_phase_inline(empty(stage.at), stage.phase ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER));
+        if (!ok) break;
+        const uint32_t a = sbase + static_cast<uint32_t>(stage.at * S::kStageBytes), b = a + kABytes, bar = full(stage.at);
+        const uint32_t bytes = rows.bytes(stage.at / 2, x.rows) + BN * kRowBytes;
+        if (leader) {
+          ptx::mbar_arrive_expect_tx(bar, bytes);
+          rows.load(&p.a_map, &p.a_box, a, bar, kb * kRowBytes, x.row, p.capacity);
+          ptx::tma_load_2d(b, maps, bar, kb * kRowBytes, x.n * kWidth);
+          if constexpr (kGated) ptx::tma_load_2d(b + kWidth * kRowBytes, maps + 1, bar, kb * kRowBytes, x.n * kWidth);
+        }
+        __syncwarp();
+        stage.next();
+      }
+      skip = kb - p.k_blocks;
+    }
+    if (!ok || *abort_flag) drain_loads<kStages>(stage, full);
+  } else if (warp == kScaleWarp) {
+    const int last = (p.n - 1) / GG_SCALE_BLOCK;
+    uint32_t slot = 0;
+    bool ok = true;
+    for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
+      const Tile x = tile_at(t);
+      // of the weights: lane 2 i + w takes block i of k, w: the tile's first or second half of outputs, or gated B or U
+      const int64_t column = x.n * kWidth + (kGated ? 0 : lane % 2 * (kWidth / 2));
+      const float* const* table = kGated && lane % 2 ? p.up_scales : p.b_scales;
+      const float* sb = table[x.e] + min(column / GG_SCALE_BLOCK, static_cast<int64_t>(last)) * p.k_blocks;
+      const float* sa[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sa[j] = p.a_scales + static_cast<int64_t>(x.row + min(j * 32 + lane, x.rows - 1)) * p.ldas;
+      // A slot's scales are asked for two slots before they are written: their way from L2 takes longer than a slot lasts.
+      struct Group {
+        float a[4][kScaleBlocks], b;
+      };
+      const auto fetch = [&](Group& g, int kb0) {
+        g.b = lane < 2 * kScaleBlocks && kb0 + lane / 2 < p.k_blocks ? __ldg(sb + kb0 + lane / 2) : 0.0f;
+        const bool four = p.scales_aligned && kb0 + kScaleBlocks <= p.k_blocks;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j * 32 < x.rows && four) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(sa[j] + kb0));
+            g.a[j][0] = v.x, g.a[j][1] = v.y, g.a[j][2] = v.z, g.a[j][3] = v.w;
+          } else {
+#pragma unroll
+            for (int i = 0; i < kScaleBlocks; ++i) g.a[j][i] = j * 32 < x.rows && kb0 + i < p.k_blocks ? __ldg(sa[j] + kb0 + i) : 0.0f;
+          }
+        }
+      };
+      const auto hand_over = [&](const Group& g) {
+        ok = __all_sync(0xffffffffu, wait_phase_inline(scales_used(slot % kScaleSlots), ((slot / kScaleSlots) & 1u) ^ 1u, abort_flag, p.status,
+                                                       p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER));
+        if (!ok) return;
+        float* to = reinterpret_cast<float*>(smem + l.own + slot % kScaleSlots * kScaleBytes);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < kScaleBlocks; ++i) to[i * kTileRows + j * 32 + lane] = g.a[j][i];
+        if (lane < 2 * kScaleBlocks) to[kScaleBlocks * kTileRows + lane] = g.b;
+        if (lane == 0) *reinterpret_cast<Tile*>(reinterpret_cast<unsigned char*>(to) + kScaleBytes - 16) = x;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(scales_in(slot % kScaleSlots));
+        ++slot;
+      };
+      Group even, odd;
+      fetch(even, 0);
+      fetch(odd, kScaleBlocks);
+      for (int kb0 = 0; ok && kb0 < p.k_blocks; kb0 += 2 * kScaleBlocks) {
+        hand_over(even);
+        fetch(even, kb0 + 2 * kScaleBlocks);
+        if (!ok || kb0 + kScaleBlocks >= p.k_blocks) break;
+        hand_over(odd);
+        fetch(odd, kb0 + 3 * kScaleBlocks);
+      }
+    }
+  } else if (warp == kProductWarp) {
+    const bool leader = ptx::elect_one();
+    const uint32_t idesc = ptx::idesc_f32acc(kTileRows, BN, static_cast<uint32_t>(p.input_format - GG_INPUT_E4M3), false, false);
+    // descriptors of a stage's operands: an address in units of 16 bytes in their low bits, so a stage and a step of K are additions
+    const uint64_t a0 = ptx::smem_desc_sw128(sbase, 16u, 1024u), b0 = ptx::smem_desc_sw128(sbase + kABytes, 16u, 1024u);
+    Ring<kStages> stage;
+    Ring<kAcc> acc;
+    bool ok = true;
+    for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
+      for (int kb = 0; kb < p.k_blocks; ++kb) {
+        ok = __all_sync(0xffffffffu, wait_phase_inline(full(stage.at), stage.phase, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA) &&
+                                         wait_phase_inline(taken(acc.at), acc.phase ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        const uint64_t a = a0 + static_cast<uint32_t>(stage.at * (S::kStageBytes / 16)), b = b0 + static_cast<uint32_t>(stage.at * (S::kStageBytes / 16));
+        const uint32_t d = tmem + static_cast<uint32_t>(acc.at * BN);
+        if (leader) {
+#pragma unroll
+          for (uint32_t kk = 0; kk < 4; ++kk) ptx::tc_mma_f8(d, a + 2 * kk, b + 2 * kk, idesc, kk != 0);
+          ptx::tc_commit(empty(stage.at));
+          ptx::tc_commit(ready(acc.at));
+        }
+        __syncwarp();
+        stage.next();
+        acc.next();
+      }
+    }
+    if (leader) {
+      ptx::tc_commit(drained);  // before tensor memory is freed
+      wait_drain_inline(drained, 0u, 100000000ull);
+    }
+    __syncwarp();
   }
 
   __syncthreads();
@@ -355,8 +461,12 @@ int gg_f8_plan_create(const gg_f8_problem* problem, gg_f8_plan** out) {
   for (int s = 0; s < gg::kShapes && st == cudaSuccess; ++s)
     gg::with_shape(gg::width_of(s), gated, [&](auto bn, auto g) {
       using S = gg::F8Shape<bn()>;
-      st = cudaFuncSetAttribute(gg::f8_kernel<bn(), g()>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                gg::tiles::layout(S::kStages * S::kStageBytes, gg::tiles::kMaxExperts, S::kBars).bytes);
+      cudaFuncAttributes attributes{};
+      st = cudaFuncGetAttributes(&attributes, gg::f8_kernel<bn(), g()>);
+      // what the warpgroups take and give up has to be what the block is launched with
+      if (st == cudaSuccess && attributes.numRegs != gg::tiles::kLaunchRegisters) st = cudaErrorInvalidConfiguration;
+      if (st == cudaSuccess) st = cudaFuncSetAttribute(gg::f8_kernel<bn(), g()>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                gg::tiles::layout(S::kStages * S::kStageBytes, gg::tiles::kMaxExperts, S::kBars, gg::kScaleSlots * gg::kScaleBytes).bytes);
     });
   if (st == cudaSuccess) st = cudaMalloc(reinterpret_cast<void**>(&plan->block), host.size());
   if (st == cudaSuccess) st = cudaMemcpy(plan->block, host.data(), host.size(), cudaMemcpyHostToDevice);
@@ -401,6 +511,7 @@ int gg_f8_plan_run(gg_f8_plan* plan, const void* a, int lda, const float* a_scal
   const int bytes = q.output_type == GG_OUTPUT_F32 ? 4 : eight ? 1 : 2;
   p.a_scales = a_scales;
   p.ldas = ldas;
+  p.scales_aligned = reinterpret_cast<uintptr_t>(a_scales) % 16 == 0 && ldas % 4 == 0;
   p.rows = rows;
   p.d = static_cast<char*>(d);
   p.d_pitch = static_cast<int64_t>(ldd) * bytes;
@@ -408,7 +519,10 @@ int gg_f8_plan_run(gg_f8_plan* plan, const void* a, int lda, const float* a_scal
   p.ldds = ldds;
   p.capacity = capacity_rows;
   p.aligned = reinterpret_cast<uintptr_t>(d) % 16 == 0 && p.d_pitch % 16 == 0;
-  if (capacity_rows > 0 && !gg::encode_rows(&p.a_map, 1, a, q.k, capacity_rows, lda, 128, gg::tiles::kBoxRows)) return cudaErrorInvalidValue;
+  p.wide = reinterpret_cast<uintptr_t>(d) % 32 == 0 && p.d_pitch % 32 == 0;
+  if (capacity_rows > 0 && (!gg::encode_rows(&p.a_map, 1, a, q.k, capacity_rows, lda, 128, gg::tiles::kTileRows) ||
+                            !gg::encode_rows(&p.a_box, 1, a, q.k, capacity_rows, lda, 128, gg::tiles::kBoxRows)))
+    return cudaErrorInvalidValue;
   // 128-row tiles at most, if every expert's rows end in a part of one
   const int64_t stretches = std::min<int64_t>(capacity_rows, static_cast<int64_t>(capacity_rows) / gg::tiles::kTileRows + q.experts);
   int shape = 0;
@@ -422,7 +536,7 @@ int gg_f8_plan_run(gg_f8_plan* plan, const void* a, int lda, const float* a_scal
   gg::with_shape(gg::width_of(shape), gated, [&](auto bn, auto g) {
     using S = gg::F8Shape<bn()>;
     st = gg::launch_chained(gg::f8_kernel<bn(), g()>, dim3(grid), gg::tiles::kTileThreads,
-                            static_cast<size_t>(gg::tiles::layout(S::kStages * S::kStageBytes, q.experts, S::kBars).bytes),
+                            static_cast<size_t>(gg::tiles::layout(S::kStages * S::kStageBytes, q.experts, S::kBars, gg::kScaleSlots * gg::kScaleBytes).bytes),
                             static_cast<cudaStream_t>(stream), 1, p);
   });
   return st;

@@ -40,7 +40,7 @@ constexpr int kChunkBytes = kDepth * kRowBytes;  // 64 columns x 64 values of k,
 static_assert(layout(kStages * kStageBytes, kMaxExperts, kBars).bytes <= 232448, "shared memory of a block");
 
 struct GatedParams {
-  CUtensorMap in[3];        // forward: x; rows: grad_gate, grad_up; weights: x, grad_gate, grad_up
+  CUtensorMap in[4];        // forward: x; rows: grad_gate, grad_up (each 128 rows, then boxes); weights: x, grad_gate, grad_up
   const CUtensorMap* maps;  // [experts][2]: Wg's and Wu's
   const int* rows;
   char* out[3];             // forward: h, gate, up (the last two may be NULL); rows: grad_x; weights: grad_Wg, grad_Wu
@@ -48,7 +48,7 @@ struct GatedParams {
   int64_t expert_bytes;     // weights: from one expert's gradient to the next
   int experts, inner, tiles_m, tiles_n, columns, out_rows, capacity, type, out_type, activation;
   // inner: forward k, rows n; tiles_m, out_rows: weights (k); columns: of the outputs
-  bool aligned[3];
+  bool aligned[3], wide[3];  // rows start on 16- and on 32-byte boundaries
   int* status;
   unsigned long long timeout_ns;
 };
@@ -83,6 +83,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
     ptx::tmem_alloc(ptx::smem_addr(tmem_slot), kAcc * kBN);
     ptx::tmem_relinquish();
   }
+  if constexpr (kMode != kWeightGradient) clear_rows<kStages, kStageBytes>(smem);
   chained_begin();
   if (warp == 0) expert_table(p.rows, p.experts, p.capacity, p.tiles_n, first_row, first_tile, p.status, lane);
   ptx::tc_fence_before_sync();
@@ -116,62 +117,69 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
     return x;
   };
 
-  if (warp == kLoadWarp) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
-        const Tile x = tile_at(t);
-        const CUtensorMap* maps = p.maps + 2 * x.e;
-        const int boxes = (x.rows + kBoxRows - 1) / kBoxRows;
-        const uint32_t bytes = static_cast<uint32_t>((kMode == kWeightGradient ? kTileRows : boxes * kBoxRows) + kBN) * kRowBytes;
-        for (int kb = 0; kb < x.depth; ++kb, ++it) {
-          const int st = static_cast<int>(it % kStages);
-          ok = wait_phase(empty(st), ((it / kStages) & 1u) ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER);
-          if (!ok) break;
-          const uint32_t a = sbase + static_cast<uint32_t>(st * kStageBytes), b = a + kABytes;
-          ptx::mbar_arrive_expect_tx(full(st), bytes);
+  if (warp >= kLoadWarp) {
+    const bool leader = ptx::elect_one();
+    RowLoads<kStages> rows;
+    Ring<kStages, 2> stage;
+    stage.at = warp - kLoadWarp;
+    int skip = stage.at;  // stages of 64 until this warp's next
+    bool ok = true;
+    for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
+      const Tile x = tile_at(t);
+      const CUtensorMap* maps = p.maps + 2 * x.e;
+      int kb = skip;
+      for (; kb < x.depth; kb += 2) {
+        ok = __all_sync(0xffffffffu, wait_phase_inline(empty(stage.at), stage.phase ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER));
+        if (!ok) break;
+        const uint32_t a = sbase + static_cast<uint32_t>(stage.at * kStageBytes), b = a + kABytes, bar = full(stage.at);
+        const uint32_t bytes = (kMode == kWeightGradient ? kABytes : rows.bytes(stage.at / 2, x.rows)) + kBN * kRowBytes;
+        if (leader) {
+          ptx::mbar_arrive_expect_tx(bar, bytes);
           if constexpr (kMode == kForward) {
-            for (int i = 0; i < boxes; ++i)
-              ptx::tma_load_2d(a + i * kBoxRows * kRowBytes, &p.in[0], full(st), kb * kDepth, x.row + i * kBoxRows);
+            rows.load(&p.in[0], &p.in[1], a, bar, kb * kDepth, x.row, p.capacity);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              ptx::tma_load_2d(b + i * kChunkBytes, maps + i / 2, full(st), x.n * kWidth + i % 2 * kDepth, kb * kDepth);
+              ptx::tma_load_2d(b + i * kChunkBytes, maps + i / 2, bar, x.n * kWidth + i % 2 * kDepth, kb * kDepth);
           } else if constexpr (kMode == kRowGradient) {
             const int second = kb >= x.depth / 2, at = (second ? kb - x.depth / 2 : kb) * kDepth;
-            for (int i = 0; i < boxes; ++i)
-              ptx::tma_load_2d(a + i * kBoxRows * kRowBytes, &p.in[second], full(st), at, x.row + i * kBoxRows);
-            ptx::tma_load_2d(b, maps + second, full(st), at, x.n * kWidth);
+            rows.load(&p.in[2 * second], &p.in[2 * second + 1], a, bar, at, x.row, p.capacity);
+            ptx::tma_load_2d(b, maps + second, bar, at, x.n * kWidth);
           } else {
             const int at = x.row + kb * kDepth;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) ptx::tma_load_2d(a + i * kChunkBytes, &p.in[0], full(st), x.m * kTileRows + i * kDepth, at);
+            for (int i = 0; i < 2; ++i) ptx::tma_load_2d(a + i * kChunkBytes, &p.in[0], bar, x.m * kTileRows + i * kDepth, at);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              ptx::tma_load_2d(b + i * kChunkBytes, &p.in[1 + i / 2], full(st), x.n * kWidth + i % 2 * kDepth, at);
+              ptx::tma_load_2d(b + i * kChunkBytes, &p.in[1 + i / 2], bar, x.n * kWidth + i % 2 * kDepth, at);
           }
         }
+        __syncwarp();
+        stage.next();
       }
-      if (!ok || *abort_flag) drain_loads<kStages>(it, full);
+      skip = kb - x.depth;
     }
+    if (!ok || *abort_flag) drain_loads<kStages>(stage, full);
   } else if (warp == kProductWarp) {
     // the forward's weights and all of the weights' gradient have k as their rows in shared memory
     constexpr bool kAWide = kMode == kWeightGradient, kBWide = kMode != kRowGradient;
+    const bool leader = ptx::elect_one();
     const uint32_t idesc = ptx::idesc_f32acc(kTileRows, kBN, static_cast<uint32_t>(p.type), kAWide, kBWide);
-    uint32_t it = 0, done = 0;
+    // descriptors of a stage's operands: an address in units of 16 bytes in their low bits, so a stage and a step of K are additions
+    constexpr uint32_t kStepA = (kAWide ? 2048 : 32) / 16, kStepB = (kBWide ? 2048 : 32) / 16;
+    const uint64_t a0 = ptx::smem_desc_sw128(sbase, kAWide ? kChunkBytes : 16u, 1024u);
+    const uint64_t b0 = ptx::smem_desc_sw128(sbase + kABytes, kBWide ? kChunkBytes : 16u, 1024u);
+    Ring<kStages> stage;
+    Ring<kAcc> acc;
     bool ok = true;
-    for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid, ++done) {
+    for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
       const Tile x = tile_at(t);
-      const int buf = static_cast<int>(done % kAcc);
-      ok = __all_sync(0xffffffffu, wait_phase(taken(buf), ((done / kAcc) & 1u) ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
+      ok = __all_sync(0xffffffffu, wait_phase_inline(taken(acc.at), acc.phase ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
       if (!ok) break;
       ptx::tc_fence_after_sync();
-      const uint32_t d = tmem + static_cast<uint32_t>(buf * kBN);
-      for (int kb = 0; kb < x.depth; ++kb, ++it) {
-        const int st = static_cast<int>(it % kStages);
-        ok = __all_sync(0xffffffffu, wait_phase(full(st), (it / kStages) & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
+      const uint32_t d = tmem + static_cast<uint32_t>(acc.at * kBN);
+      for (int kb = 0; kb < x.depth; ++kb) {
+        ok = __all_sync(0xffffffffu, wait_phase_inline(full(stage.at), stage.phase, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
         if (!ok) break;
-        const uint32_t a = sbase + static_cast<uint32_t>(st * kStageBytes), b = a + kABytes;
         int steps = kDepth / 16;
         if constexpr (kMode == kWeightGradient) {
           const int left = x.rows - kb * kDepth;
@@ -180,32 +188,34 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
             const int clear = steps * 16 - left;  // rows of the next expert, or of none
             // 2 pieces of A and 4 of B, one after the other, hold a 128-byte row of 64 columns for each k
             for (int i = lane; i < clear * 6 * 8; i += 32)
-              *reinterpret_cast<uint4*>(smem + st * kStageBytes + i / (clear * 8) * kChunkBytes + (left + i / 8 % clear) * kRowBytes + i % 8 * 16) =
+              *reinterpret_cast<uint4*>(smem + stage.at * kStageBytes + i / (clear * 8) * kChunkBytes + (left + i / 8 % clear) * kRowBytes + i % 8 * 16) =
                   make_uint4(0u, 0u, 0u, 0u);
             ptx::fence_proxy_async_smem();
             __syncwarp();
           }
         }
         ptx::tc_fence_after_sync();
-        if (lane == 0) {
-          for (int kk = 0; kk < steps; ++kk)
-            ptx::tc_mma_f16(d, kAWide ? ptx::smem_desc_sw128(a + kk * 2048u, kChunkBytes, 1024u) : ptx::smem_desc_sw128(a + kk * 32u, 16u, 1024u),
-                            kBWide ? ptx::smem_desc_sw128(b + kk * 2048u, kChunkBytes, 1024u) : ptx::smem_desc_sw128(b + kk * 32u, 16u, 1024u),
-                            idesc, kb != 0 || kk != 0);
-          ptx::tc_commit(empty(st));
+        const uint64_t a = a0 + static_cast<uint32_t>(stage.at * (kStageBytes / 16)), b = b0 + static_cast<uint32_t>(stage.at * (kStageBytes / 16));
+        if (leader) {
+#pragma unroll
+          for (uint32_t kk = 0; kk < kDepth / 16; ++kk)
+            if (kMode != kWeightGradient || static_cast<int>(kk) < steps) ptx::tc_mma_f16(d, a + kStepA * kk, b + kStepB * kk, idesc, kb != 0 || kk != 0);
+          ptx::tc_commit(empty(stage.at));
         }
         __syncwarp();
+        stage.next();
       }
       if (!ok) break;
-      if (lane == 0) {
-        if (x.depth > 0) ptx::tc_commit(ready(buf));
-        else ptx::mbar_arrive(ready(buf));  // an expert without rows: zeros
+      if (leader) {
+        if (x.depth > 0) ptx::tc_commit(ready(acc.at));
+        else ptx::mbar_arrive(ready(acc.at));  // an expert without rows: zeros
       }
       __syncwarp();
+      acc.next();
     }
-    if (lane == 0) {
+    if (leader) {
       ptx::tc_commit(drained);  // before tensor memory is freed
-      wait_drain(drained, 0u, 100000000ull);
+      wait_drain_inline(drained, 0u, 100000000ull);
     }
     __syncwarp();
   } else if (warp < kEpilogueWarps) {
@@ -215,7 +225,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
     for (int t = static_cast<int>(blockIdx.x); t < total; t += grid, ++done) {
       const Tile x = tile_at(t);
       const int buf = static_cast<int>(done % kAcc);
-      if (!__all_sync(0xffffffffu, wait_phase(ready(buf), (done / kAcc) & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_EPILOGUE)))
+      if (!__all_sync(0xffffffffu, wait_phase_inline(ready(buf), (done / kAcc) & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_EPILOGUE)))
         break;
       ptx::tc_fence_after_sync();
       const uint32_t from = tmem + static_cast<uint32_t>(buf * kBN) + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -223,11 +233,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
       const int64_t row0 = (kMode == kWeightGradient ? x.m * kTileRows : x.row) + quarter * 32;
       const auto out = [&](int i) {
         return Out{p.out[i] + row0 * p.pitch[i] + (kMode == kWeightGradient ? x.e * p.expert_bytes : 0), p.pitch[i], min(32, rows), p.columns,
-                   p.aligned[i]};
+                   p.aligned[i], p.wide[i]};
       };
       if (rows > 0) {
         if constexpr (kMode == kForward) {
-#pragma unroll
+#pragma unroll 1
           for (int c = half * 64; c < half * 64 + 64; c += 32) {
             uint32_t g[32], u[32];
             tmem_read(from + c, g);
@@ -243,7 +253,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
               store_columns(stage, lane, v, p.out_type, out(2), column);
             }
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = activate_more(__uint_as_float(g[j]), p.activation) * __uint_as_float(u[j]);
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(g[j]);
+            activate_all(v, p.activation);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] *= __uint_as_float(u[j]);
             store_columns(stage, lane, v, p.out_type, out(0), column);
           }
         } else {
@@ -370,7 +383,8 @@ __global__ void __launch_bounds__(kGateThreads) gate_gradient_kernel(const GateG
   }
 }
 
-bool on16(const void* p, int64_t pitch_bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && pitch_bytes % 16 == 0; }
+bool on(int bytes, const void* p, int64_t pitch) { return reinterpret_cast<uintptr_t>(p) % bytes == 0 && pitch % bytes == 0; }
+bool on16(const void* p, int64_t pitch) { return on(16, p, pitch); }
 
 }  // namespace
 }  // namespace gg
@@ -401,7 +415,8 @@ gg::GatedParams common(const gg_gated_plan* plan, const int* rows, int capacity)
 void set_out(gg::GatedParams& p, int i, void* out, int ld, int bytes) {
   p.out[i] = static_cast<char*>(out);
   p.pitch[i] = static_cast<int64_t>(ld) * bytes;
-  p.aligned[i] = gg::on16(out, p.pitch[i]);
+  p.aligned[i] = gg::on(16, out, p.pitch[i]);
+  p.wide[i] = gg::on(32, out, p.pitch[i]);
 }
 
 template <int kMode>
@@ -410,6 +425,13 @@ cudaError_t launch(const gg_gated_plan* plan, const gg::GatedParams& p, int64_t 
   const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(plan->sms, most)));
   return gg::launch_chained(gg::gated_kernel<kMode>, dim3(grid), gg::tiles::kTileThreads,
                             static_cast<size_t>(gg::tiles::layout(gg::kStages * gg::kStageBytes, p.experts, gg::kBars).bytes), stream, 1, p);
+}
+
+// The maps of packed rows for RowLoads: whole tiles and boxes.
+bool encode_both(CUtensorMap* maps, int type, const void* rows, int columns, int count, int ld) {
+  const int kind = type == GG_INPUT_F16 ? 2 : 3;
+  return gg::encode_rows(&maps[0], kind, rows, columns, count, static_cast<int64_t>(ld) * 2, gg::kDepth, gg::tiles::kTileRows) &&
+         gg::encode_rows(&maps[1], kind, rows, columns, count, static_cast<int64_t>(ld) * 2, gg::kDepth, gg::tiles::kBoxRows);
 }
 
 // 128-row stretches of all experts at most.
@@ -489,9 +511,7 @@ int gg_gated_plan_run(gg_gated_plan* plan, const gg_gated* call, void* stream) {
   set_out(p, 0, c.h, c.ldh, 2);
   set_out(p, 1, c.gate, c.ldg, 2);
   set_out(p, 2, c.up, c.ldg, 2);
-  if (c.capacity_rows > 0 && !gg::encode_rows(&p.in[0], q.type == GG_INPUT_F16 ? 2 : 3, c.x, q.k, c.capacity_rows,
-                                              static_cast<int64_t>(c.ldx) * 2, gg::kDepth, gg::tiles::kBoxRows))
-    return cudaErrorInvalidValue;
+  if (c.capacity_rows > 0 && !encode_both(&p.in[0], q.type, c.x, q.k, c.capacity_rows, c.ldx)) return cudaErrorInvalidValue;
   return launch<gg::kForward>(plan, p, stretches(plan, c.capacity_rows) * p.tiles_n, static_cast<cudaStream_t>(stream));
 }
 
@@ -522,8 +542,8 @@ int gg_gated_plan_backward(gg_gated_plan* plan, const gg_gated_gradient* gradien
     px.columns = q.k;
     px.tiles_n = (q.k - 1) / gg::kBN + 1;
     set_out(px, 0, c.grad_x, c.ldgx, 2);
-    if (!gg::encode_rows(&px.in[0], kind, c.grad_gate, q.n, c.capacity_rows, pitch_g, gg::kDepth, gg::tiles::kBoxRows) ||
-        !gg::encode_rows(&px.in[1], kind, c.grad_up, q.n, c.capacity_rows, pitch_g, gg::kDepth, gg::tiles::kBoxRows))
+    if (!encode_both(&px.in[0], q.type, c.grad_gate, q.n, c.capacity_rows, c.ldgg) ||
+        !encode_both(&px.in[2], q.type, c.grad_up, q.n, c.capacity_rows, c.ldgg))
       return cudaErrorInvalidValue;
   }
   if (c.grad_wg) {
@@ -537,7 +557,10 @@ int gg_gated_plan_backward(gg_gated_plan* plan, const gg_gated_gradient* gradien
     set_out(pw, 0, c.grad_wg, c.ldgw, bytes);
     set_out(pw, 1, c.grad_wu, c.ldgw, bytes);
     pw.expert_bytes = c.expert_stride * bytes;
-    for (int i = 0; i < 2; ++i) pw.aligned[i] = pw.aligned[i] && (q.experts == 1 || pw.expert_bytes % 16 == 0);
+    for (int i = 0; i < 2; ++i) {
+      pw.aligned[i] = pw.aligned[i] && (q.experts == 1 || pw.expert_bytes % 16 == 0);
+      pw.wide[i] = pw.wide[i] && (q.experts == 1 || pw.expert_bytes % 32 == 0);
+    }
     if (c.capacity_rows > 0 &&
         (!gg::encode_rows(&pw.in[0], kind, c.x, q.k, c.capacity_rows, static_cast<int64_t>(c.ldx) * 2, 64, gg::kDepth) ||
          !gg::encode_rows(&pw.in[1], kind, c.grad_gate, q.n, c.capacity_rows, pitch_g, 64, gg::kDepth) ||

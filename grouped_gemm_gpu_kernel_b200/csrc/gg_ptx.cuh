@@ -88,6 +88,14 @@ __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 
+// True in one lane of a converged warp. A loop that the whole warp goes through, with single-thread instructions behind this, keeps
+// addresses and descriptors in uniform registers; in a branch of one lane each has to be moved there.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 // ---- proxy fences -------------------------------------------------------------------------
 // Orders this thread's generic-proxy shared-memory writes before later async-proxy accesses
 // (TMA store reads, tcgen05.mma operand reads).
