@@ -63,8 +63,9 @@ __device__ __forceinline__ void activate_all(float (&v)[N], int act) {
   }
 }
 
-// first_row[e], first_tile[e] for e = 0..experts (totals at the end), by one warp. `per_row_tile`: tiles of one 128-row
-// stretch of an expert. Counts that are negative or sum to more than `capacity` leave no rows, and -1 as the total of tiles.
+// first_row[e], first_tile[e] for e = 0..experts (totals at the end), by one warp. `per_row_tile`: tiles of one stretch of kStretch
+// rows of an expert. Counts that are negative or sum to more than `capacity` leave no rows, and -1 as the total of tiles.
+template <int kStretch = kTileRows>
 __device__ __forceinline__ void expert_table(const int* rows, int experts, int capacity, int per_row_tile, int* first_row, int* first_tile,
                                              int* status, int lane) {
   int row = 0, tile = 0;
@@ -73,7 +74,7 @@ __device__ __forceinline__ void expert_table(const int* rows, int experts, int c
     if (lane == 0) {
       first_row[0] = first_tile[0] = 0;
       first_row[1] = capacity;
-      first_tile[1] = (capacity + kTileRows - 1) / kTileRows * per_row_tile;
+      first_tile[1] = (capacity + kStretch - 1) / kStretch * per_row_tile;
     }
     return;
   }
@@ -86,7 +87,7 @@ __device__ __forceinline__ void expert_table(const int* rows, int experts, int c
     bad = bad || __any_sync(0xffffffffu, r < 0 || r > capacity);
     if (bad) break;
     long long sum = r;
-    int t = (r + kTileRows - 1) / kTileRows * per_row_tile;
+    int t = (r + kStretch - 1) / kStretch * per_row_tile;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long s = __shfl_up_sync(0xffffffffu, sum, o);

@@ -10,6 +10,10 @@
 //             size. The last stage of an expert can hold rows of the next one: the warp that issues the
 //             products clears them in shared memory first (at most 15 rows: it stops at the next multiple of 16, the depth
 //             of a product).
+// Each comes in two forms. On one CTA a tile takes 48 KB of operands for a stage of 64, which its shared memory both takes in and
+// feeds to the tensor cores: 96 KB in 512 cycles of products at their full rate, and 128 bytes a cycle is what it has. On a
+// pair (cta_group::2, 256 x 256) each CTA has 128 rows of the one operand and half of the other: 32 KB, six stages in
+// place of four, and a third less from L2. Tiles of 256 rows leave more of an expert's last tile empty.
 // Before the two gradients one pass over gate, up and grad_h makes grad_gate and grad_up.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -32,12 +36,17 @@ using namespace tiles;
 constexpr int kForward = 0, kRowGradient = 1, kWeightGradient = 2;
 constexpr int kBN = 256;       // columns of an accumulator
 constexpr int kDepth = 64;     // values of k of a stage
-constexpr int kStages = 4;
 constexpr int kAcc = 2;
-constexpr int kStageBytes = kABytes + kBN * kRowBytes;
-constexpr int kBars = 2 * kStages + 2 * kAcc + 1;
+template <bool kPair>
+struct GatedShape {
+  static constexpr int kStages = kPair ? 6 : 4;
+  static constexpr int kStageBytes = kABytes + kBN / (kPair ? 2 : 1) * kRowBytes;
+  static constexpr int kBars = 2 * kStages + 2 * kAcc + 1 + 2;
+  static constexpr int kStretch = kPair ? 2 * kTileRows : kTileRows;  // rows of a tile
+  static constexpr int smem(int experts) { return layout(kStages * kStageBytes, experts, kBars).bytes; }
+  static_assert(layout(kStages * kStageBytes, kMaxExperts, kBars).bytes <= 232448, "shared memory of a block");
+};
 constexpr int kChunkBytes = kDepth * kRowBytes;  // 64 columns x 64 values of k, a row of shared memory for each k
-static_assert(layout(kStages * kStageBytes, kMaxExperts, kBars).bytes <= 232448, "shared memory of a block");
 
 struct GatedParams {
   CUtensorMap in[4];        // forward: x; rows: grad_gate, grad_up (each 128 rows, then boxes); weights: x, grad_gate, grad_up
@@ -53,13 +62,24 @@ struct GatedParams {
   unsigned long long timeout_ns;
 };
 
-template <int kMode>
+// Zeros in the rows `left` and on, up to the next multiple of 16, of kChunks pieces of shared memory that hold a 128-byte row of 64
+// columns for each k: rows of the next expert, or of none. By one warp, between the loads' barrier and a proxy fence.
+template <int kChunks>
+__device__ __forceinline__ void clear_after(uint8_t* stage, int left, int lane) {
+  const int first = left % kDepth, rows = 16 - first % 16;
+  for (int i = lane; i < rows * kChunks * 8; i += 32)
+    *reinterpret_cast<uint4*>(stage + i / (rows * 8) * kChunkBytes + (first + i / 8 % rows) * kRowBytes + i % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+}
+
+template <int kMode, bool kPair>
 __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_constant__ GatedParams p) {
+  using S = GatedShape<kPair>;
+  constexpr int kStages = S::kStages, kStageBytes = S::kStageBytes;
   constexpr int kWidth = kMode == kRowGradient ? kBN : kBN / 2;  // output columns of a tile
   extern __shared__ uint8_t smem_dyn[];
   uint8_t* smem = smem_dyn + ((1024u - (ptx::smem_addr(smem_dyn) & 1023u)) & 1023u);
   const uint32_t sbase = ptx::smem_addr(smem);
-  const Layout l = layout(kStages * kStageBytes, p.experts, kBars);
+  const Layout l = layout(kStages * kStageBytes, p.experts, S::kBars);
   int* first_row = reinterpret_cast<int*>(smem + l.table);
   int* first_tile = first_row + p.experts + 1;
   const uint32_t bar0 = sbase + l.bars;
@@ -68,35 +88,45 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
   const auto ready = [&](int b) { return bar0 + 8u * (2 * kStages + b); };
   const auto taken = [&](int b) { return bar0 + 8u * (2 * kStages + kAcc + b); };
   const uint32_t drained = bar0 + 8u * (2 * kStages + 2 * kAcc);
+  const auto cut = [&](int w) { return bar0 + 8u * (2 * kStages + 2 * kAcc + 1 + w); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + l.words);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + l.words + 4);
 
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
+  const int rank = kPair ? static_cast<int>(ptx::cluster_ctarank()) : 0;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) ptx::mbar_init(full(s), 1), ptx::mbar_init(empty(s), 1);
-    for (int b = 0; b < kAcc; ++b) ptx::mbar_init(ready(b), 1), ptx::mbar_init(taken(b), kEpilogueWarps);
+    // a pair's stages and accumulators are counted on the barriers of its first CTA
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(full(s), kPair ? 2 : 1), ptx::mbar_init(empty(s), 1);
+    for (int b = 0; b < kAcc; ++b) ptx::mbar_init(ready(b), 1), ptx::mbar_init(taken(b), (kPair ? 2 : 1) * kEpilogueWarps);
     ptx::mbar_init(drained, 1);
+    for (int w = 0; w < 2; ++w) ptx::mbar_init(cut(w), 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
+  if constexpr (kPair) ptx::cluster_sync();  // the barriers are there before the other CTA uses them
   if (warp == kProductWarp) {
-    ptx::tmem_alloc(ptx::smem_addr(tmem_slot), kAcc * kBN);
-    ptx::tmem_relinquish();
+    if constexpr (kPair) {
+      ptx::tmem_alloc_pair(ptx::smem_addr(tmem_slot), kAcc * kBN);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(ptx::smem_addr(tmem_slot), kAcc * kBN);
+      ptx::tmem_relinquish();
+    }
   }
-  if constexpr (kMode != kWeightGradient) clear_rows<kStages, kStageBytes>(smem);
+  if constexpr (kMode != kWeightGradient && !kPair) clear_rows<kStages, kStageBytes>(smem);
   chained_begin();
-  if (warp == 0) expert_table(p.rows, p.experts, p.capacity, p.tiles_n, first_row, first_tile, p.status, lane);
+  if (warp == 0) expert_table<S::kStretch>(p.rows, p.experts, p.capacity, p.tiles_n, first_row, first_tile, p.status, lane);
   ptx::tc_fence_before_sync();
   __syncthreads();
   ptx::tc_fence_after_sync();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  const int grid = static_cast<int>(gridDim.x);
+  const int grid = static_cast<int>(gridDim.x) / (kPair ? 2 : 1), block = static_cast<int>(blockIdx.x) / (kPair ? 2 : 1);
   const int per_expert = p.tiles_m * p.tiles_n;  // weights
   const bool bad = first_tile[p.experts] < 0;
   const int total = bad ? 0 : kMode == kWeightGradient ? p.experts * per_expert : first_tile[p.experts];
 
   struct Tile {
-    int e, row, rows, m, n, depth;  // first packed row and rows of the tile (weights: of the expert); k blocks
+    int e, row, rows, m, n, depth;  // this CTA's first packed row and rows of the tile (weights: of the expert); stages of 64
   };
   const auto tile_at = [&](int t) {
     Tile x;
@@ -109,13 +139,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
     } else {
       x.e = expert_of(first_tile, p.experts, t);
       const int count = first_row[x.e + 1] - first_row[x.e];
-      place(t - first_tile[x.e], (count + kTileRows - 1) / kTileRows, p.tiles_n, x.m, x.n);
-      x.row = first_row[x.e] + x.m * kTileRows;
-      x.rows = min(kTileRows, count - x.m * kTileRows);
+      place(t - first_tile[x.e], (count + S::kStretch - 1) / S::kStretch, p.tiles_n, x.m, x.n);
+      x.row = first_row[x.e] + x.m * S::kStretch + rank * kTileRows;
+      x.rows = min(kTileRows, count - x.m * S::kStretch - rank * kTileRows);  // none for the second CTA of a pair: not positive
       x.depth = (kMode == kRowGradient ? 2 : 1) * ((p.inner + kDepth - 1) / kDepth);
     }
     return x;
   };
+  // the first of this CTA's 128 columns of A of the weights' gradient
+  const auto first_k = [&](const Tile& x) { return x.m * S::kStretch + rank * kTileRows; };
 
   if (warp >= kLoadWarp) {
     const bool leader = ptx::elect_one();
@@ -123,114 +155,160 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
     Ring<kStages, 2> stage;
     stage.at = warp - kLoadWarp;
     int skip = stage.at;  // stages of 64 until this warp's next
+    uint32_t cuts = 0;
     bool ok = true;
-    for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
+    for (int t = block; ok && t < total; t += grid) {
       const Tile x = tile_at(t);
       const CUtensorMap* maps = p.maps + 2 * x.e;
       int kb = skip;
       for (; kb < x.depth; kb += 2) {
         ok = __all_sync(0xffffffffu, wait_phase_inline(empty(stage.at), stage.phase ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER));
         if (!ok) break;
-        const uint32_t a = sbase + static_cast<uint32_t>(stage.at * kStageBytes), b = a + kABytes, bar = full(stage.at);
-        const uint32_t bytes = (kMode == kWeightGradient ? kABytes : rows.bytes(stage.at / 2, x.rows)) + kBN * kRowBytes;
+        const uint32_t a = sbase + static_cast<uint32_t>(stage.at * kStageBytes), b = a + kABytes;
+        const uint32_t counted = kPair ? ptx::mapa_shared(full(stage.at), 0) : full(stage.at);
+        // the last stage of an expert with rows of the next one in it, on a pair: loaded, cleared, then handed over
+        const int left = x.rows - kb * kDepth;
+        const bool clear = kPair && kMode == kWeightGradient && left < kDepth && left % 16 != 0;
+        const uint32_t bar = clear ? cut(warp - kLoadWarp) : counted;
+        const auto load = [&](uint32_t to, const CUtensorMap* map, int at, int row) {
+          if (kPair && !clear) ptx::tma_load_2d_pair(to, map, bar, at, row);
+          else ptx::tma_load_2d(to, map, bar, at, row);
+        };
+        const uint32_t bytes = kPair || kMode == kWeightGradient ? kStageBytes : rows.bytes(stage.at / 2, x.rows) + kBN * kRowBytes;
         if (leader) {
-          ptx::mbar_arrive_expect_tx(bar, bytes);
+          if (clear || !kPair) ptx::mbar_arrive_expect_tx(bar, bytes);
+          else if (rank == 0) ptx::mbar_arrive_expect_tx(full(stage.at), 2 * kStageBytes);
           if constexpr (kMode == kForward) {
-            rows.load(&p.in[0], &p.in[1], a, bar, kb * kDepth, x.row, p.capacity);
+            if constexpr (kPair) {
+              load(a, &p.in[0], kb * kDepth, x.row);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              ptx::tma_load_2d(b + i * kChunkBytes, maps + i / 2, bar, x.n * kWidth + i % 2 * kDepth, kb * kDepth);
+              for (int i = 0; i < 2; ++i) load(b + i * kChunkBytes, maps + rank, x.n * kWidth + i * kDepth, kb * kDepth);
+            } else {
+              rows.load(&p.in[0], &p.in[1], a, bar, kb * kDepth, x.row, p.capacity);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) load(b + i * kChunkBytes, maps + i / 2, x.n * kWidth + i % 2 * kDepth, kb * kDepth);
+            }
           } else if constexpr (kMode == kRowGradient) {
             const int second = kb >= x.depth / 2, at = (second ? kb - x.depth / 2 : kb) * kDepth;
-            rows.load(&p.in[2 * second], &p.in[2 * second + 1], a, bar, at, x.row, p.capacity);
-            ptx::tma_load_2d(b, maps + second, bar, at, x.n * kWidth);
+            if constexpr (kPair) {
+              load(a, &p.in[2 * second], at, x.row);
+              load(b, maps + second, at, x.n * kWidth + rank * kTileRows);
+            } else {
+              rows.load(&p.in[2 * second], &p.in[2 * second + 1], a, bar, at, x.row, p.capacity);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) load(b + i * kTileRows * kRowBytes, maps + second, at, x.n * kWidth + i * kTileRows);
+            }
           } else {
             const int at = x.row + kb * kDepth;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) ptx::tma_load_2d(a + i * kChunkBytes, &p.in[0], bar, x.m * kTileRows + i * kDepth, at);
+            for (int i = 0; i < 2; ++i) load(a + i * kChunkBytes, &p.in[0], first_k(x) + i * kDepth, at);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              ptx::tma_load_2d(b + i * kChunkBytes, &p.in[1 + i / 2], bar, x.n * kWidth + i % 2 * kDepth, at);
+            for (int i = 0; i < (kPair ? 2 : 4); ++i)
+              load(b + i * kChunkBytes, &p.in[1 + (kPair ? rank : i / 2)], x.n * kWidth + i % 2 * kDepth, at);
           }
+          if (kPair && !clear && rank != 0) ptx::mbar_arrive_cluster_relaxed(counted);  // counts; the bytes are tracked by themselves
         }
         __syncwarp();
+        if (clear) {
+          ok = __all_sync(0xffffffffu, wait_phase_inline(bar, cuts & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER));
+          if (!ok) break;
+          ++cuts;
+          clear_after<kStageBytes / kChunkBytes>(smem + stage.at * kStageBytes, left, lane);
+          ptx::fence_proxy_async_all();  // the other CTA's tensor cores read it too
+          __syncwarp();
+          if (lane == 0) {
+            if (rank == 0) ptx::mbar_arrive(full(stage.at));
+            else ptx::mbar_arrive_cluster(counted);
+          }
+        }
         stage.next();
       }
       skip = kb - x.depth;
     }
-    if (!ok || *abort_flag) drain_loads<kStages>(stage, full);
+    if ((!ok || *abort_flag) && rank == 0) drain_loads<kStages>(stage, full);
   } else if (warp == kProductWarp) {
-    // the forward's weights and all of the weights' gradient have k as their rows in shared memory
-    constexpr bool kAWide = kMode == kWeightGradient, kBWide = kMode != kRowGradient;
-    const bool leader = ptx::elect_one();
-    const uint32_t idesc = ptx::idesc_f32acc(kTileRows, kBN, static_cast<uint32_t>(p.type), kAWide, kBWide);
-    // descriptors of a stage's operands: an address in units of 16 bytes in their low bits, so a stage and a step of K are additions
-    constexpr uint32_t kStepA = (kAWide ? 2048 : 32) / 16, kStepB = (kBWide ? 2048 : 32) / 16;
-    const uint64_t a0 = ptx::smem_desc_sw128(sbase, kAWide ? kChunkBytes : 16u, 1024u);
-    const uint64_t b0 = ptx::smem_desc_sw128(sbase + kABytes, kBWide ? kChunkBytes : 16u, 1024u);
-    Ring<kStages> stage;
-    Ring<kAcc> acc;
-    bool ok = true;
-    for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
-      const Tile x = tile_at(t);
-      ok = __all_sync(0xffffffffu, wait_phase_inline(taken(acc.at), acc.phase ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
-      if (!ok) break;
-      ptx::tc_fence_after_sync();
-      const uint32_t d = tmem + static_cast<uint32_t>(acc.at * kBN);
-      for (int kb = 0; kb < x.depth; ++kb) {
-        ok = __all_sync(0xffffffffu, wait_phase_inline(full(stage.at), stage.phase, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
+    if (rank == 0) {
+      // the forward's weights and all of the weights' gradient have k as their rows in shared memory
+      constexpr bool kAWide = kMode == kWeightGradient, kBWide = kMode != kRowGradient;
+      const bool leader = ptx::elect_one();
+      const uint32_t idesc = ptx::idesc_f32acc(S::kStretch, kBN, static_cast<uint32_t>(p.type), kAWide, kBWide);
+      // descriptors of a stage's operands: an address in units of 16 bytes in their low bits, so a stage and a step of K are additions
+      constexpr uint32_t kStepA = (kAWide ? 2048 : 32) / 16, kStepB = (kBWide ? 2048 : 32) / 16;
+      const uint64_t a0 = ptx::smem_desc_sw128(sbase, kAWide ? kChunkBytes : 16u, 1024u);
+      const uint64_t b0 = ptx::smem_desc_sw128(sbase + kABytes, kBWide ? kChunkBytes : 16u, 1024u);
+      Ring<kStages> stage;
+      Ring<kAcc> acc;
+      bool ok = true;
+      for (int t = block; ok && t < total; t += grid) {
+        const Tile x = tile_at(t);
+        ok = __all_sync(0xffffffffu, wait_phase_inline<kPair>(taken(acc.at), acc.phase ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
         if (!ok) break;
-        int steps = kDepth / 16;
-        if constexpr (kMode == kWeightGradient) {
-          const int left = x.rows - kb * kDepth;
-          if (left < kDepth) {
-            steps = (left + 15) / 16;
-            const int clear = steps * 16 - left;  // rows of the next expert, or of none
-            // 2 pieces of A and 4 of B, one after the other, hold a 128-byte row of 64 columns for each k
-            for (int i = lane; i < clear * 6 * 8; i += 32)
-              *reinterpret_cast<uint4*>(smem + stage.at * kStageBytes + i / (clear * 8) * kChunkBytes + (left + i / 8 % clear) * kRowBytes + i % 8 * 16) =
-                  make_uint4(0u, 0u, 0u, 0u);
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
+        ptx::tc_fence_after_sync();
+        const uint32_t d = tmem + static_cast<uint32_t>(acc.at * kBN);
+        for (int kb = 0; kb < x.depth; ++kb) {
+          ok = __all_sync(0xffffffffu, wait_phase_inline<kPair>(full(stage.at), stage.phase, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
+          if (!ok) break;
+          int steps = kDepth / 16;
+          if constexpr (kMode == kWeightGradient) {
+            const int left = x.rows - kb * kDepth;
+            if (left < kDepth) {
+              steps = (left + 15) / 16;
+              if (!kPair && left % 16 != 0) {
+                clear_after<kStageBytes / kChunkBytes>(smem + stage.at * kStageBytes, left, lane);
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+              }
+            }
+          }
+          ptx::tc_fence_after_sync();
+          const uint64_t a = a0 + static_cast<uint32_t>(stage.at * (kStageBytes / 16)), b = b0 + static_cast<uint32_t>(stage.at * (kStageBytes / 16));
+          if (leader) {
+#pragma unroll
+            for (uint32_t kk = 0; kk < kDepth / 16; ++kk)
+              if (kMode != kWeightGradient || static_cast<int>(kk) < steps) {
+                if constexpr (kPair) ptx::tc_mma_f16_pair(d, a + kStepA * kk, b + kStepB * kk, idesc, kb != 0 || kk != 0);
+                else ptx::tc_mma_f16(d, a + kStepA * kk, b + kStepB * kk, idesc, kb != 0 || kk != 0);
+              }
+            if constexpr (kPair) ptx::tc_commit_pair_mc(empty(stage.at), 0x3);
+            else ptx::tc_commit(empty(stage.at));
+          }
+          __syncwarp();
+          stage.next();
+        }
+        if (!ok) break;
+        if (leader) {
+          if (x.depth > 0) {
+            if constexpr (kPair) ptx::tc_commit_pair_mc(ready(acc.at), 0x3);
+            else ptx::tc_commit(ready(acc.at));
+          } else {  // an expert without rows: zeros
+            ptx::mbar_arrive(ready(acc.at));
+            if constexpr (kPair) ptx::mbar_arrive_cluster(ptx::mapa_shared(ready(acc.at), 1));
           }
         }
-        ptx::tc_fence_after_sync();
-        const uint64_t a = a0 + static_cast<uint32_t>(stage.at * (kStageBytes / 16)), b = b0 + static_cast<uint32_t>(stage.at * (kStageBytes / 16));
-        if (leader) {
-#pragma unroll
-          for (uint32_t kk = 0; kk < kDepth / 16; ++kk)
-            if (kMode != kWeightGradient || static_cast<int>(kk) < steps) ptx::tc_mma_f16(d, a + kStepA * kk, b + kStepB * kk, idesc, kb != 0 || kk != 0);
-          ptx::tc_commit(empty(stage.at));
-        }
         __syncwarp();
-        stage.next();
+        acc.next();
       }
-      if (!ok) break;
       if (leader) {
-        if (x.depth > 0) ptx::tc_commit(ready(acc.at));
-        else ptx::mbar_arrive(ready(acc.at));  // an expert without rows: zeros
+        // before tensor memory is freed
+        if constexpr (kPair) ptx::tc_commit_pair(drained);
+        else ptx::tc_commit(drained);
+        wait_drain_inline(drained, 0u, 100000000ull);
       }
       __syncwarp();
-      acc.next();
     }
-    if (leader) {
-      ptx::tc_commit(drained);  // before tensor memory is freed
-      wait_drain_inline(drained, 0u, 100000000ull);
-    }
-    __syncwarp();
   } else if (warp < kEpilogueWarps) {
     const int quarter = warp & 3, half = warp >> 2;
     unsigned char* stage = smem + l.staging + warp * kStagingBytes;
     uint32_t done = 0;
-    for (int t = static_cast<int>(blockIdx.x); t < total; t += grid, ++done) {
+    for (int t = block; t < total; t += grid, ++done) {
       const Tile x = tile_at(t);
       const int buf = static_cast<int>(done % kAcc);
       if (!__all_sync(0xffffffffu, wait_phase_inline(ready(buf), (done / kAcc) & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_EPILOGUE)))
         break;
       ptx::tc_fence_after_sync();
       const uint32_t from = tmem + static_cast<uint32_t>(buf * kBN) + (static_cast<uint32_t>(quarter * 32) << 16);
-      const int rows = (kMode == kWeightGradient ? p.out_rows - x.m * kTileRows : x.rows) - quarter * 32;  // from this warp's first on
-      const int64_t row0 = (kMode == kWeightGradient ? x.m * kTileRows : x.row) + quarter * 32;
+      const int rows = (kMode == kWeightGradient ? p.out_rows - first_k(x) : x.rows) - quarter * 32;  // from this warp's first on
+      const int64_t row0 = (kMode == kWeightGradient ? first_k(x) : x.row) + quarter * 32;
       const auto out = [&](int i) {
         return Out{p.out[i] + row0 * p.pitch[i] + (kMode == kWeightGradient ? x.e * p.expert_bytes : 0), p.pitch[i], min(32, rows), p.columns,
                    p.aligned[i], p.wide[i]};
@@ -280,14 +358,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
       }
       ptx::tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(taken(buf));
+      if (lane == 0) {
+        if (rank == 0) ptx::mbar_arrive(taken(buf));
+        else ptx::mbar_arrive_cluster(ptx::mapa_shared(taken(buf), 0));
+      }
     }
   }
 
-  __syncthreads();
+  if constexpr (kPair) {
+    __syncwarp();
+    ptx::cluster_sync();  // neither CTA ends while the other may still use its shared memory
+    if (*abort_flag) {    // after an abort, loads may still be landing
+      const uint64_t t0 = ptx::global_timer_ns();
+      while (ptx::global_timer_ns() - t0 < 200000ull) {
+      }
+    }
+  } else {
+    __syncthreads();
+  }
   if (warp == kProductWarp) {
     ptx::tc_fence_after_sync();
-    ptx::tmem_dealloc(tmem, kAcc * kBN);
+    if constexpr (kPair) ptx::tmem_dealloc_pair(tmem, kAcc * kBN);
+    else ptx::tmem_dealloc(tmem, kAcc * kBN);
   }
 }
 
@@ -395,9 +487,13 @@ struct gg_gated_plan {
   const CUtensorMap* maps[2] = {};
   int* status = nullptr;
   int device = 0, sms = 0;
+  int pairs = 0;  // that the GPU holds at a time
 };
 
 namespace {
+
+constexpr int kPairRows = 512;     // rows of an expert, in the mean, from which on its tiles are of 256
+constexpr int kPairColumns = 256;  // k from which on the weights' gradients' are
 
 gg::GatedParams common(const gg_gated_plan* plan, const int* rows, int capacity) {
   gg::GatedParams p{};
@@ -419,12 +515,32 @@ void set_out(gg::GatedParams& p, int i, void* out, int ld, int bytes) {
   p.wide[i] = gg::on(32, out, p.pitch[i]);
 }
 
-template <int kMode>
+// The kernel of one form: `most` tiles at most.
+template <int kMode, bool kPair>
 cudaError_t launch(const gg_gated_plan* plan, const gg::GatedParams& p, int64_t most, cudaStream_t stream) {
-  if (most > INT32_MAX) return cudaErrorInvalidValue;
-  const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(plan->sms, most)));
-  return gg::launch_chained(gg::gated_kernel<kMode>, dim3(grid), gg::tiles::kTileThreads,
-                            static_cast<size_t>(gg::tiles::layout(gg::kStages * gg::kStageBytes, p.experts, gg::kBars).bytes), stream, 1, p);
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(kPair ? plan->pairs : plan->sms, most)) * (kPair ? 2 : 1);
+  return gg::launch_chained(gg::gated_kernel<kMode, kPair>, dim3(static_cast<unsigned>(grid)), gg::tiles::kTileThreads,
+                            static_cast<size_t>(gg::GatedShape<kPair>::smem(p.experts)), stream, kPair ? 2 : 1, p);
+}
+
+template <int kMode, bool kPair>
+cudaError_t prepare(gg_gated_plan* plan) {
+  const int smem = gg::GatedShape<kPair>::smem(gg::tiles::kMaxExperts);
+  cudaError_t st = cudaFuncSetAttribute(gg::gated_kernel<kMode, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (!kPair || st != cudaSuccess) return st;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {2, 1, 1};
+  cfg.gridDim = dim3(2);
+  cfg.blockDim = dim3(gg::tiles::kTileThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int pairs = 0;
+  st = cudaOccupancyMaxActiveClusters(&pairs, gg::gated_kernel<kMode, kPair>, &cfg);
+  plan->pairs = std::max(1, pairs);
+  return st;
 }
 
 // The maps of packed rows for RowLoads: whole tiles and boxes.
@@ -434,10 +550,13 @@ bool encode_both(CUtensorMap* maps, int type, const void* rows, int columns, int
          gg::encode_rows(&maps[1], kind, rows, columns, count, static_cast<int64_t>(ld) * 2, gg::kDepth, gg::tiles::kBoxRows);
 }
 
-// 128-row stretches of all experts at most.
-int64_t stretches(const gg_gated_plan* plan, int capacity) {
-  return std::min<int64_t>(capacity, static_cast<int64_t>(capacity) / gg::tiles::kTileRows + plan->problem.experts);
+// Tile rows (128 or 256 of an expert) of all experts at most.
+int64_t stretches(const gg_gated_plan* plan, int capacity, bool pair) {
+  return std::min<int64_t>(capacity, static_cast<int64_t>(capacity) / (pair ? 256 : 128) + plan->problem.experts);
 }
+
+// Whether tiles of 256 rows on pairs of CTAs take the rows, or of 128.
+bool rows_in_pairs(const gg_gated_plan* plan, int capacity) { return capacity / plan->problem.experts >= kPairRows; }
 
 }  // namespace
 
@@ -469,13 +588,15 @@ int gg_gated_plan_create(const gg_gated_problem* problem, gg_gated_plan** out) {
     for (int i = 0; i < 2 && st == cudaSuccess; ++i) {
       const void* w = i == 0 ? q.gate[e] : q.up[e];
       if (!gg::encode_rows(&forward[2 * e + i], kind, w, q.n, q.k, pitch, 64, gg::kDepth) ||
-          !gg::encode_rows(&rows[2 * e + i], kind, w, q.n, q.k, pitch, gg::kDepth, gg::kBN))
+          !gg::encode_rows(&rows[2 * e + i], kind, w, q.n, q.k, pitch, gg::kDepth, gg::tiles::kTileRows))
         st = cudaErrorInvalidValue;
     }
-  const int smem = gg::tiles::layout(gg::kStages * gg::kStageBytes, gg::tiles::kMaxExperts, gg::kBars).bytes;
-  if (st == cudaSuccess) st = cudaFuncSetAttribute(gg::gated_kernel<gg::kForward>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (st == cudaSuccess) st = cudaFuncSetAttribute(gg::gated_kernel<gg::kRowGradient>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (st == cudaSuccess) st = cudaFuncSetAttribute(gg::gated_kernel<gg::kWeightGradient>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (st == cudaSuccess) st = prepare<gg::kForward, false>(plan);
+  if (st == cudaSuccess) st = prepare<gg::kRowGradient, false>(plan);
+  if (st == cudaSuccess) st = prepare<gg::kWeightGradient, false>(plan);
+  if (st == cudaSuccess) st = prepare<gg::kForward, true>(plan);
+  if (st == cudaSuccess) st = prepare<gg::kRowGradient, true>(plan);
+  if (st == cudaSuccess) st = prepare<gg::kWeightGradient, true>(plan);
   if (st == cudaSuccess) st = cudaMalloc(reinterpret_cast<void**>(&plan->block), host.size());
   if (st == cudaSuccess) st = cudaMemcpy(plan->block, host.data(), host.size(), cudaMemcpyHostToDevice);
   if (st == cudaSuccess) st = cudaDeviceSynchronize();
@@ -512,7 +633,11 @@ int gg_gated_plan_run(gg_gated_plan* plan, const gg_gated* call, void* stream) {
   set_out(p, 1, c.gate, c.ldg, 2);
   set_out(p, 2, c.up, c.ldg, 2);
   if (c.capacity_rows > 0 && !encode_both(&p.in[0], q.type, c.x, q.k, c.capacity_rows, c.ldx)) return cudaErrorInvalidValue;
-  return launch<gg::kForward>(plan, p, stretches(plan, c.capacity_rows) * p.tiles_n, static_cast<cudaStream_t>(stream));
+  const bool pair = rows_in_pairs(plan, c.capacity_rows);
+  const int64_t most = stretches(plan, c.capacity_rows, pair) * p.tiles_n;
+  if (most > INT32_MAX) return cudaErrorInvalidValue;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return pair ? launch<gg::kForward, true>(plan, p, most, s) : launch<gg::kForward, false>(plan, p, most, s);
 }
 
 int gg_gated_plan_backward(gg_gated_plan* plan, const gg_gated_gradient* gradient, void* stream) {
@@ -534,6 +659,7 @@ int gg_gated_plan_backward(gg_gated_plan* plan, const gg_gated_gradient* gradien
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int kind = q.type == GG_INPUT_F16 ? 2 : 3;
   const int64_t pitch_g = static_cast<int64_t>(c.ldgg) * 2;
+  const bool pair_x = rows_in_pairs(plan, c.capacity_rows), pair_w = q.k >= kPairColumns;
   // nothing is launched before every check has passed
   gg::GatedParams px = common(plan, c.rows, c.capacity_rows), pw = px;
   if (c.capacity_rows > 0 && c.grad_x) {
@@ -551,7 +677,7 @@ int gg_gated_plan_backward(gg_gated_plan* plan, const gg_gated_gradient* gradien
     pw.maps = plan->maps[0];
     pw.columns = q.n;
     pw.out_rows = q.k;
-    pw.tiles_m = (q.k - 1) / gg::tiles::kTileRows + 1;
+    pw.tiles_m = (q.k - 1) / (pair_w ? 256 : 128) + 1;
     pw.tiles_n = (q.n - 1) / 128 + 1;
     pw.out_type = c.weight_grad_type;
     set_out(pw, 0, c.grad_wg, c.ldgw, bytes);
@@ -567,7 +693,7 @@ int gg_gated_plan_backward(gg_gated_plan* plan, const gg_gated_gradient* gradien
          !gg::encode_rows(&pw.in[2], kind, c.grad_up, q.n, c.capacity_rows, pitch_g, 64, gg::kDepth)))
       return cudaErrorInvalidValue;
   }
-  const int64_t most_x = px.maps ? stretches(plan, c.capacity_rows) * px.tiles_n : 0;
+  const int64_t most_x = px.maps ? stretches(plan, c.capacity_rows, pair_x) * px.tiles_n : 0;
   const int64_t most_w = pw.maps ? static_cast<int64_t>(q.experts) * pw.tiles_m * pw.tiles_n : 0;
   if (most_x > INT32_MAX || most_w > INT32_MAX) return cudaErrorInvalidValue;
 
@@ -581,8 +707,10 @@ int gg_gated_plan_backward(gg_gated_plan* plan, const gg_gated_gradient* gradien
     if (kind == 2) vec ? go(gg::gate_gradient_kernel<gg::kOutF16, true>) : go(gg::gate_gradient_kernel<gg::kOutF16, false>);
     else vec ? go(gg::gate_gradient_kernel<gg::kOutBF16, true>) : go(gg::gate_gradient_kernel<gg::kOutBF16, false>);
   }
-  if (st == cudaSuccess && px.maps) st = launch<gg::kRowGradient>(plan, px, most_x, s);
-  if (st == cudaSuccess && pw.maps) st = launch<gg::kWeightGradient>(plan, pw, most_w, s);
+  if (st == cudaSuccess && px.maps)
+    st = pair_x ? launch<gg::kRowGradient, true>(plan, px, most_x, s) : launch<gg::kRowGradient, false>(plan, px, most_x, s);
+  if (st == cudaSuccess && pw.maps)
+    st = pair_w ? launch<gg::kWeightGradient, true>(plan, pw, most_w, s) : launch<gg::kWeightGradient, false>(plan, pw, most_w, s);
   return st;
 }
 

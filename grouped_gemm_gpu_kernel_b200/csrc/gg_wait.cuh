@@ -32,11 +32,13 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volati
 
 // The same without a call, for code that holds more in registers than a call lets it keep, and for waits that are mostly short:
 // the clock is first read after 32 tries (a read takes some 300 cycles, more than what is waited for).
+// kCluster: what another CTA of the cluster wrote before it arrived is visible then.
+template <bool kCluster = false>
 __device__ __forceinline__ bool wait_phase_inline(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
                                                   unsigned long long timeout_ns, int code) {
   uint64_t t0 = 0;
   for (uint32_t i = 0;; ++i) {
-    if (ptx::mbar_try_wait(bar, parity)) return true;
+    if (kCluster ? ptx::mbar_try_wait_cluster(bar, parity) : ptx::mbar_try_wait(bar, parity)) return true;
     if ((i & 31u) == 31u) {
       if (*abort_flag) return false;
       const uint64_t now = ptx::global_timer_ns();

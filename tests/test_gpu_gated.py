@@ -166,6 +166,17 @@ def test_activations(cuda, act, kind):
     c.check_backward()
 
 
+@pytest.mark.parametrize("counts", [[512], [513, 700], [1000, 24], [0, 1537, 600], [256 * 3 + 1, 256 * 3 - 1, 640]])
+@pytest.mark.parametrize("n,k", [(128, 64), (300, 520), (72, 256), (131, 130)])
+def test_rows_in_tiles_of_256(cuda, counts, n, k):
+    """Rows and k enough for tiles on pairs of CTAs, with last tiles of which one CTA has no part."""
+    c = Case(counts, n, k)
+    assert c.forward() == 0
+    c.check_forward()
+    assert c.backward() == 0
+    c.check_backward()
+
+
 def test_many_tiles(cuda):
     """More tiles than SMs, several stretches of rows of one expert, and experts enough for a full table."""
     c = Case([1000, 300, 0, 2500], 1100, 400)
