@@ -6,10 +6,12 @@
 //   grad_weight = sum over rows of grad_y * xhat
 //
 // Memory bounds it: a row is read once, stays in registers through the sum over it, and is written once. A row
-// belongs to a team of 32 to 1024 threads of a block. A team goes through it in spans of 256 values for a
-// warp, 8 for a thread: 8 in a piece where rows are aligned (16 bytes of 16-bit values), so that 16 lanes hold a block of 128
-// columns, and else every 32nd of 256, so that a warp's loads of single values are whole lines, and 4 of a lane's 8 are of
-// one block. h is rounded to its type first and the norm is of what is stored, as the gradient finds it.
+// belongs to a team of 1 to 16 warps (more than one: a whole block), each of which holds a span of 256 of its values, 8 a thread, or
+// with wider rows than the block has warps for 2 to 8 spans. In a span a thread has 8 values in a piece where rows are
+// aligned (16 bytes of 16-bit values), so that 16 lanes hold a block of 128 columns, and else every 32nd of 256, so that a
+// warp's loads of single values are whole lines, and 4 of a lane's 8 are of one block. The teams that fit the GPU go through the rows,
+// and a team asks for its next row before it adds this one up. h is rounded to its type first and the norm is of
+// what is stored, as the gradient finds it.
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
@@ -28,10 +30,10 @@ namespace gg {
 namespace {
 
 constexpr int kSpan = 256;  // values that a warp takes in one piece
-constexpr int kManyRows = 2048;
 
-// Warps of a row at most, where each holds so many spans: by registers (8 values a span, three times that in the gradient).
-__host__ __device__ constexpr int most_warps(int spans, bool gradient) { return gradient && spans > 1 ? 16 : 32; }
+constexpr int kMostWarps = 16;  // of a row, which leaves a thread 128 registers
+// Whether the next row's values fit beside this one's.
+__host__ __device__ constexpr bool asks_ahead(int spans) { return spans <= 2; }
 
 struct NormParams {
   const void* x;
@@ -66,36 +68,38 @@ __device__ __forceinline__ int column(int span, int lane, int j) {
   return span * kSpan + (kVec ? lane * 8 + j : j * 32 + lane);
 }
 
-// This lane's 8 values of a span of a row of `width` (zeros past it).
+// This lane's 8 values of a span of a row of `width` (zeros past it), as they are stored.
 template <int F, bool kVec>
-__device__ __forceinline__ void load8(const void* base, int64_t at, int span, int lane, int width, float (&v)[8]) {
-  const int c0 = column<kVec>(span, lane, 0);
-  if (kVec && c0 + 8 <= width) {
-    const char* p = static_cast<const char*>(base) + (at + c0) * OutFormat<F>::kBytes;
-    if constexpr (F == kOutF32) {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 16);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct Eight {
+  static constexpr int kWords = F == kOutF32 ? 8 : 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const void* base, int64_t at, int span, int lane, int width) {
+    const int c0 = column<kVec>(span, lane, 0);
+    if (kVec && c0 + 8 <= width) {
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(base) + (at + c0) * OutFormat<F>::kBytes);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack2<F>(w[i]);
-        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 u = p[i];
+        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = column<kVec>(span, lane, j);
+      if (c < width) {
+        if constexpr (F == kOutF32) w[j] = static_cast<const uint32_t*>(base)[at + c];
+        else w[j / 2] |= static_cast<uint32_t>(static_cast<const unsigned short*>(base)[at + c]) << (16 * (j % 2));
       }
     }
-    return;
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int c = column<kVec>(span, lane, j);
-    v[j] = 0.0f;
-    if (c < width) {
-      if constexpr (F == kOutF32) v[j] = static_cast<const float*>(base)[at + c];
-      else v[j] = widen16<F>(static_cast<const unsigned short*>(base)[at + c]);
-    }
+  __device__ __forceinline__ float value(int j) const {
+    if constexpr (F == kOutF32) return __uint_as_float(w[j]);
+    else return widen16<F>(static_cast<unsigned short>(w[j / 2] >> (16 * (j % 2))));
   }
-}
+};
 
 template <int F, bool kVec>
 __device__ __forceinline__ void store8(void* base, int64_t at, int span, int lane, int width, const float (&v)[8]) {
@@ -130,170 +134,213 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// The sum over a team of `warps` warps (a whole block where it is more than one), the same in every thread. `sums`: 32
-// floats of shared memory, used by one sum at a time.
-__device__ __forceinline__ float team_sum(float v, int warps, float* sums) {
+// The sum over a team of `warps` warps (a whole block where it is more than one), the same in every thread. `sums`: two times 32
+// floats of shared memory, taken in turn (`turn`).
+__device__ __forceinline__ float team_sum(float v, int warps, float* sums, int turn) {
   v = warp_sum(v);
   if (warps == 1) return v;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  float* at = sums + 32 * (turn & 1);
+  if (lane == 0) at[warp] = v;
   __syncthreads();
-  if (lane == 0) sums[warp] = v;
-  __syncthreads();
-  return warp_sum(lane < warps ? sums[lane] : 0.0f);
+  return warp_sum(lane < warps ? at[lane] : 0.0f);
+}
+
+// Which row a thread's team starts with, how far it is to its next one, and which of the team's warps this is.
+struct Place {
+  int64_t row, step;
+  int member;
+  __device__ __forceinline__ Place(int warps) {
+    const int warp = threadIdx.x / 32, teams = warps == 1 ? blockDim.x / 32 : 1;
+    row = static_cast<int64_t>(blockIdx.x) * teams + (warps == 1 ? warp : 0);
+    step = static_cast<int64_t>(gridDim.x) * teams;
+    member = warps == 1 ? 0 : warp;
+  }
+};
+
+// y in 8 bits: a span's part of this lane.
+template <bool kVec>
+__device__ __forceinline__ void store_8bit(const NormParams& p, int64_t row, int span, int lane, const float (&y)[8]) {
+  if constexpr (kVec) {
+    const int c0 = column<kVec>(span, lane, 0);
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, magnitude(y[j]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const Scale8 s(top, p.largest);
+    if (lane % 16 == 0 && c0 < p.width) p.scales[row * p.lds + c0 / GG_SCALE_BLOCK] = s.scale;
+    const uint2 b = make_uint2(s.four(y[0], y[1], y[2], y[3], p.e5m2), s.four(y[4], y[5], y[6], y[7], p.e5m2));
+    unsigned char* q = p.q + row * p.ldq + c0;
+    if (c0 + 8 <= p.width) {
+      *reinterpret_cast<uint2*>(q) = b;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c0 + j < p.width) q[j] = static_cast<unsigned char>((j < 4 ? b.x : b.y) >> (8 * (j % 4)));
+    }
+  } else {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, magnitude(y[4 * half + j]));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const Scale8 s(top, p.largest);
+      const int b0 = span * kSpan + half * GG_SCALE_BLOCK;
+      if (lane == 0 && b0 < p.width) p.scales[row * p.lds + b0 / GG_SCALE_BLOCK] = s.scale;
+      const uint32_t b = s.four(y[4 * half], y[4 * half + 1], y[4 * half + 2], y[4 * half + 3], p.e5m2);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = b0 + j * 32 + lane;
+        if (c < p.width) p.q[row * p.ldq + c] = static_cast<unsigned char>(b >> (8 * j));
+      }
+    }
+  }
 }
 
 // F: type of the rows; W: of the weight; kSpans: spans that a warp holds; kVec: rows aligned.
 template <int F, int W, int kSpans, bool kVec>
-__global__ void __launch_bounds__(32 * most_warps(kSpans, false)) norm_kernel(const NormParams p, int warps) {
-  __shared__ float sums[32];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, member = warps == 1 ? 0 : warp;
-  const int64_t row = warps == 1 ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + warp : blockIdx.x;
+__global__ void __launch_bounds__(32 * kMostWarps) norm_kernel(const NormParams p, int warps) {
+  __shared__ float sums[64];
+  const int lane = threadIdx.x % 32;
+  const Place at(warps);
   chained_begin();
-  if (row >= p.rows) return;  // whole teams
-  float h[kSpans][8];
-  float sum = 0.0f;
+  Eight<F, kVec> x[kSpans], r[kSpans];
+  const auto ask = [&](int64_t row) {
+    if (row >= p.rows) return;
 #pragma unroll
-  for (int i = 0; i < kSpans; ++i) load8<F, kVec>(p.x, row * p.ldx, member + i * warps, lane, p.width, h[i]);
-  if (p.residual) {
+    for (int i = 0; i < kSpans; ++i) x[i].load(p.x, row * p.ldx, at.member + i * warps, lane, p.width);
+    if (p.residual) {
+#pragma unroll
+      for (int i = 0; i < kSpans; ++i) r[i].load(p.residual, row * p.ldr, at.member + i * warps, lane, p.width);
+    }
+  };
+  if constexpr (asks_ahead(kSpans)) ask(at.row);
+  int turn = 0;
+  for (int64_t row = at.row; row < p.rows; row += at.step, ++turn) {  // whole teams
+    if constexpr (!asks_ahead(kSpans)) ask(row);
+    float h[kSpans][8];
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSpans; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[i][j] = p.residual ? rounded<F>(x[i].value(j) + r[i].value(j)) : x[i].value(j);
 #pragma unroll
     for (int i = 0; i < kSpans; ++i) {
-      float r[8];
-      load8<F, kVec>(p.residual, row * p.ldr, member + i * warps, lane, p.width, r);
+      if (p.residual_out) store8<F, kVec>(p.residual_out, row * p.ldro, at.member + i * warps, lane, p.width, h[i]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] = rounded<F>(h[i][j] + r[j]);
+      for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
     }
-  }
+    if constexpr (asks_ahead(kSpans)) ask(row + at.step);
+    sum = team_sum(sum, warps, sums, turn);
+    // both steps are correctly rounded
+    const float rstd = __frcp_rn(__fsqrt_rn(sum / static_cast<float>(p.width) + p.eps));
+    if (p.rstd && at.member == 0 && lane == 0) p.rstd[row] = rstd;
+    if (!p.y && !p.q) continue;
 #pragma unroll
-  for (int i = 0; i < kSpans; ++i) {
-    if (p.residual_out) store8<F, kVec>(p.residual_out, row * p.ldro, member + i * warps, lane, p.width, h[i]);
+    for (int i = 0; i < kSpans; ++i) {
+      const int span = at.member + i * warps;
+      if (span * kSpan >= p.width) break;
+      float y[8];
+      if (p.weight) {
+        Eight<W, kVec> w;
+        w.load(p.weight, 0, span, lane, p.width);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
-  }
-  sum = team_sum(sum, warps, sums);
-  // no reciprocal square root of its own: both steps are correctly rounded
-  const float rstd = __frcp_rn(__fsqrt_rn(sum / static_cast<float>(p.width) + p.eps));
-  if (p.rstd && member == 0 && lane == 0) p.rstd[row] = rstd;
-#pragma unroll
-  for (int i = 0; i < kSpans; ++i) {
-    const int span = member + i * warps;
-    if (span * kSpan >= p.width) break;
-    float w[8];
-    if (p.weight) {
-      load8<W, kVec>(p.weight, 0, span, lane, p.width, w);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = 1.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] *= h[i][j] * rstd;
-    if (p.y) store8<F, kVec>(p.y, row * p.ldy, span, lane, p.width, w);
-    if (!p.q) continue;
-    const int c0 = column<kVec>(span, lane, 0);
-    if constexpr (kVec) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, magnitude(w[j]));
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const Scale8 s(top, p.largest);
-      if (lane % 16 == 0 && c0 < p.width) p.scales[row * p.lds + c0 / GG_SCALE_BLOCK] = s.scale;
-      const uint2 b = make_uint2(s.four(w[0], w[1], w[2], w[3], p.e5m2), s.four(w[4], w[5], w[6], w[7], p.e5m2));
-      unsigned char* q = p.q + row * p.ldq + c0;
-      if (c0 + 8 <= p.width) {
-        *reinterpret_cast<uint2*>(q) = b;
+        for (int j = 0; j < 8; ++j) y[j] = h[i][j] * rstd * w.value(j);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c0 + j < p.width) q[j] = static_cast<unsigned char>((j < 4 ? b.x : b.y) >> (8 * (j % 4)));
+        for (int j = 0; j < 8; ++j) y[j] = h[i][j] * rstd;
       }
-    } else {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) top = max(top, magnitude(w[4 * half + j]));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const Scale8 s(top, p.largest);
-        const int b0 = span * kSpan + half * GG_SCALE_BLOCK;
-        if (lane == 0 && b0 < p.width) p.scales[row * p.lds + b0 / GG_SCALE_BLOCK] = s.scale;
-        const uint32_t b = s.four(w[4 * half], w[4 * half + 1], w[4 * half + 2], w[4 * half + 3], p.e5m2);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = b0 + j * 32 + lane;
-          if (c < p.width) p.q[row * p.ldq + c] = static_cast<unsigned char>(b >> (8 * j));
-        }
-      }
+      if (p.y) store8<F, kVec>(p.y, row * p.ldy, span, lane, p.width, y);
+      if (p.q) store_8bit<kVec>(p, row, span, lane, y);
     }
   }
 }
 
-// The grid's teams go through the rows; each thread adds up its columns' part of grad_weight on the way.
+// Each thread adds up its columns' part of grad_weight on its team's way through the rows.
 template <int F, int W, int kSpans, bool kVec>
-__global__ void __launch_bounds__(32 * most_warps(kSpans, true)) norm_gradient_kernel(const NormGradientParams p, int warps) {
-  __shared__ float sums[32];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, member = warps == 1 ? 0 : warp;
-  const int teams = warps == 1 ? blockDim.x / 32 : 1;
-  const int64_t team = static_cast<int64_t>(blockIdx.x) * teams + (warps == 1 ? warp : 0);
+__global__ void __launch_bounds__(32 * kMostWarps) norm_gradient_kernel(const NormGradientParams p, int warps) {
+  __shared__ float sums[64];
+  const int lane = threadIdx.x % 32;
+  const Place at(warps);
   chained_begin();
   float gw[kSpans][8];
 #pragma unroll
   for (int i = 0; i < kSpans; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) gw[i][j] = 0.0f;
-  for (int64_t row = team; row < p.rows; row += static_cast<int64_t>(gridDim.x) * teams) {
-    float h[kSpans][8], g[kSpans][8];
+  Eight<F, kVec> rh[kSpans], rg[kSpans], rp[kSpans];
+  float rstd_next = 0.0f;
+  const auto ask = [&](int64_t row) {
+    if (row >= p.rows) return;
 #pragma unroll
     for (int i = 0; i < kSpans; ++i) {
-      load8<F, kVec>(p.h, row * p.ldh, member + i * warps, lane, p.width, h[i]);
-      load8<F, kVec>(p.grad_y, row * p.ldgy, member + i * warps, lane, p.width, g[i]);
+      rh[i].load(p.h, row * p.ldh, at.member + i * warps, lane, p.width);
+      rg[i].load(p.grad_y, row * p.ldgy, at.member + i * warps, lane, p.width);
+      if (asks_ahead(kSpans) && p.grad_h) rp[i].load(p.grad_h, row * p.ldgh, at.member + i * warps, lane, p.width);
     }
-    const float rstd = p.rstd[row];
+    rstd_next = p.rstd[row];
+  };
+  if constexpr (asks_ahead(kSpans)) ask(at.row);
+  int turn = 0;
+  for (int64_t row = at.row; row < p.rows; row += at.step, ++turn) {
+    if constexpr (!asks_ahead(kSpans)) ask(row);
+    const float rstd = rstd_next;
+    float h[kSpans][8], g[kSpans][8];
+    Eight<F, kVec> past[kSpans];
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kSpans; ++i) {
-      float w[8];
-      if (p.weight) {
-        load8<W, kVec>(p.weight, 0, member + i * warps, lane, p.width, w);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = 1.0f;
-      }
+      Eight<W, kVec> w;
+      if (p.weight) w.load(p.weight, 0, at.member + i * warps, lane, p.width);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        h[i][j] *= rstd;
-        gw[i][j] = fmaf(g[i][j], h[i][j], gw[i][j]);
-        g[i][j] *= w[j];
+        h[i][j] = rh[i].value(j) * rstd;
+        gw[i][j] = fmaf(rg[i].value(j), h[i][j], gw[i][j]);
+        g[i][j] = p.weight ? rg[i].value(j) * w.value(j) : rg[i].value(j);
         sum = fmaf(g[i][j], h[i][j], sum);
       }
+      if constexpr (asks_ahead(kSpans)) past[i] = rp[i];
     }
-    const float mean = team_sum(sum, warps, sums) / static_cast<float>(p.width);
+    if constexpr (asks_ahead(kSpans)) ask(row + at.step);
+    const float mean = team_sum(sum, warps, sums, turn) / static_cast<float>(p.width);
 #pragma unroll
     for (int i = 0; i < kSpans; ++i) {
-      const int span = member + i * warps;
-      float past[8];
-      if (p.grad_h) {
-        load8<F, kVec>(p.grad_h, row * p.ldgh, span, lane, p.width, past);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) past[j] = 0.0f;
+      const int span = at.member + i * warps;
+      if constexpr (!asks_ahead(kSpans)) {
+        if (p.grad_h) past[i].load(p.grad_h, row * p.ldgh, span, lane, p.width);
       }
+      float gx[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) past[j] = fmaf(rstd, fmaf(-h[i][j], mean, g[i][j]), past[j]);
-      store8<F, kVec>(p.grad_x, row * p.ldgx, span, lane, p.width, past);
+      for (int j = 0; j < 8; ++j) gx[j] = fmaf(rstd, fmaf(-h[i][j], mean, g[i][j]), p.grad_h ? past[i].value(j) : 0.0f);
+      store8<F, kVec>(p.grad_x, row * p.ldgx, span, lane, p.width, gx);
     }
   }
   if (!p.partial) return;
+  if (warps == 1) {  // a block of several teams: their sum, in order
+    __shared__ float part[kMostWarps][kSpan];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[threadIdx.x / 32][column<kVec>(0, lane, j)] = gw[0][j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
+      float v = 0.0f;
+      for (unsigned t = 0; t < blockDim.x / 32; ++t) v += part[t][c];
+      p.partial[static_cast<int64_t>(blockIdx.x) * p.width + c] = v;
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < kSpans; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int c = column<kVec>(member + i * warps, lane, j);
-      if (c < p.width) p.partial[team * p.width + c] = gw[i][j];
+      const int c = column<kVec>(at.member + i * warps, lane, j);
+      if (c < p.width) p.partial[static_cast<int64_t>(blockIdx.x) * p.width + c] = gw[i][j];
     }
 }
 
-// grad_weight[c] = the sum of the teams' parts, a warp's every 32nd part first, then the warps'.
+// grad_weight[c] = the sum of the blocks' parts, a warp's every 32nd part first, then the warps'.
 constexpr int kSumWarps = 32;
 __global__ void __launch_bounds__(32 * kSumWarps) norm_weight_sum_kernel(const float* partial, int parts, int width, float* out) {
   __shared__ float sums[kSumWarps][33];
@@ -310,18 +357,17 @@ __global__ void __launch_bounds__(32 * kSumWarps) norm_weight_sum_kernel(const f
   if (lane == 0 && blockIdx.x * 32 + warp < width) out[blockIdx.x * 32 + warp] = s;
 }
 
-// The warps that hold a row, and the spans that each of them does.
+// The warps that hold a row, the spans that each of them does (as few as the warps allow: 16384 rows of 4096 in BF16 take 101,
+// 111 and 118 us with 1, 2 and 4, and the gradient 142, 218 and 249), and the threads of a block.
 struct Team {
-  int warps, spans;
+  int warps, spans, threads;
 };
-Team team_of(int width, int64_t rows, bool gradient) {
-  const int spans = (width - 1) / kSpan + 1, most = gradient ? 8 : 4;
-  // with rows enough to fill the GPU a few warps that hold more each (fewer sums across warps), else all the warps there are
-  for (int each = 1;; each *= 2) {
-    const int warps = (spans + each - 1) / each;
-    if (warps <= (rows >= kManyRows ? 4 : most_warps(each, gradient))) return {warps, each};
-    if (each == most || (warps <= most_warps(each, gradient) && each >= 4)) return {warps, each};
-  }
+Team team_of(int width, bool gradient) {
+  const int spans = (width - 1) / kSpan + 1;
+  int each = 1;
+  while ((spans + each - 1) / each > kMostWarps) each *= 2;
+  const int warps = (spans + each - 1) / each;
+  return {warps, each, 32 * (warps > 1 ? warps : gradient ? 16 : 4)};
 }
 
 template <typename Do>
@@ -334,14 +380,14 @@ void with_types(int type, int weight_type, Do go) {
   else go(integral_constant<int, kOutBF16>(), integral_constant<int, kOutF32>());
 }
 
-template <bool kGradient, typename Do>
+template <typename Do>
 void with_spans(int spans, bool vec, Do go) {
   using std::integral_constant;
   const auto one = [&](auto v) {
     if (spans == 1) go(integral_constant<int, 1>(), v);
     else if (spans == 2) go(integral_constant<int, 2>(), v);
-    else if (spans == 4 || !kGradient) go(integral_constant<int, 4>(), v);
-    else go(integral_constant<int, kGradient ? 8 : 4>(), v);
+    else if (spans == 4) go(integral_constant<int, 4>(), v);
+    else go(integral_constant<int, 8>(), v);
   };
   if (vec) one(std::true_type());
   else one(std::false_type());
@@ -360,15 +406,10 @@ bool rows_on(const void* p, int64_t ld, int bytes, int to) {
 struct gg_norm_plan {
   gg_norm_config config{};
   float* partial = nullptr;
-  int device = 0, sms = 0;
+  gg::Team team{}, gradient_team{};
+  int blocks[2] = {}, gradient_blocks[2] = {};  // that the GPU holds at a time; [aligned rows]
+  int device = 0;
 };
-
-namespace {
-// Teams that go through the rows of a gradient: enough threads to keep memory busy, and no more parts of
-// grad_weight than that.
-constexpr int kGradientThreads = 1024;
-int gradient_teams(const gg_norm_plan* plan, const gg::Team& t) { return plan->sms * std::max(1, kGradientThreads / (32 * t.warps)); }
-}  // namespace
 
 extern "C" {
 
@@ -383,12 +424,28 @@ int gg_norm_create(const gg_norm_config* config, gg_norm_plan** out) {
   if (!plan) return cudaErrorMemoryAllocation;
   plan->config = *config;
   cudaError_t st = cudaGetDevice(&plan->device);
-  if (st == cudaSuccess) st = cudaDeviceGetAttribute(&plan->sms, cudaDevAttrMultiProcessorCount, plan->device);
-  if (st == cudaSuccess) {
-    const size_t teams = static_cast<size_t>(std::max(gradient_teams(plan, gg::team_of(config->width, INT32_MAX, true)),
-                                                      gradient_teams(plan, gg::team_of(config->width, 1, true))));
-    st = cudaMalloc(reinterpret_cast<void**>(&plan->partial), teams * config->width * sizeof(float));
-  }
+  int sms = 0;
+  if (st == cudaSuccess) st = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, plan->device);
+  plan->team = gg::team_of(config->width, false);
+  plan->gradient_team = gg::team_of(config->width, true);
+  gg::with_types(config->type, config->weight_type, [&](auto f, auto wt) {
+    for (int vec = 0; vec < 2; ++vec) {
+      const auto count = [&](auto kernel, int threads, int* blocks) {
+        int per_sm = 0;
+        if (st == cudaSuccess) st = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0);
+        *blocks = sms * std::max(1, per_sm);
+      };
+      gg::with_spans(plan->team.spans, vec != 0, [&](auto n, auto v) {
+        count(gg::norm_kernel<f(), wt(), n(), v()>, plan->team.threads, &plan->blocks[vec]);
+      });
+      gg::with_spans(plan->gradient_team.spans, vec != 0, [&](auto n, auto v) {
+        count(gg::norm_gradient_kernel<f(), wt(), n(), v()>, plan->gradient_team.threads, &plan->gradient_blocks[vec]);
+      });
+    }
+  });
+  if (st == cudaSuccess)
+    st = cudaMalloc(reinterpret_cast<void**>(&plan->partial),
+                    static_cast<size_t>(std::max(plan->gradient_blocks[0], plan->gradient_blocks[1])) * config->width * sizeof(float));
   if (st != cudaSuccess) {
     delete plan;
     return st;
@@ -417,12 +474,12 @@ int gg_norm_run(const gg_norm_plan* plan, const gg_norm* call, void* stream) {
   p.largest = p.e5m2 ? 57344.0f : 448.0f;
   const bool vec = gg::rows_on(q.x, q.ldx, b, 16) && gg::rows_on(q.residual, q.ldr, b, 16) && gg::rows_on(q.residual_out, q.ldro, b, 16) &&
                    gg::rows_on(q.y, q.ldy, b, 16) && gg::rows_on(q.q, q.ldq, 1, 8) && gg::rows_on(q.weight, 0, 1, 16);
-  const gg::Team t = gg::team_of(w, q.rows, false);
-  const int teams = t.warps == 1 ? 4 : 1;
-  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(q.rows) + teams - 1) / teams);
+  const gg::Team& t = plan->team;
+  const int teams = t.threads / (32 * t.warps);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(plan->blocks[vec], (static_cast<int64_t>(q.rows) + teams - 1) / teams));
   gg::with_types(plan->config.type, plan->config.weight_type, [&](auto f, auto wt) {
-    gg::with_spans<false>(t.spans, vec, [&](auto n, auto v) {
-      st = gg::launch_chained(gg::norm_kernel<f(), wt(), n(), v()>, dim3(grid), static_cast<unsigned>(32 * t.warps * teams), 0,
+    gg::with_spans(t.spans, vec, [&](auto n, auto v) {
+      st = gg::launch_chained(gg::norm_kernel<f(), wt(), n(), v()>, dim3(grid), static_cast<unsigned>(t.threads), 0,
                               static_cast<cudaStream_t>(stream), 1, p, t.warps);
     });
   });
@@ -446,20 +503,19 @@ int gg_norm_backward(gg_norm_plan* plan, const gg_norm_gradient* gradient, void*
   p.rows = q.rows, p.width = w;
   const bool vec = gg::rows_on(q.h, q.ldh, b, 16) && gg::rows_on(q.grad_y, q.ldgy, b, 16) && gg::rows_on(q.grad_h, q.ldgh, b, 16) &&
                    gg::rows_on(q.grad_x, q.ldgx, b, 16) && gg::rows_on(q.weight, 0, 1, 16);
-  const gg::Team t = gg::team_of(w, q.rows, true);
-  const int per = t.warps == 1 ? 4 : 1;
-  const int most = gradient_teams(plan, t);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(std::max(1, most / per), (static_cast<int64_t>(q.rows) + per - 1) / per));
+  const gg::Team& t = plan->gradient_team;
+  const int teams = t.threads / (32 * t.warps);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(plan->gradient_blocks[vec], (static_cast<int64_t>(q.rows) + teams - 1) / teams));
   if (q.rows > 0)
     gg::with_types(plan->config.type, plan->config.weight_type, [&](auto f, auto wt) {
-      gg::with_spans<true>(t.spans, vec, [&](auto n, auto v) {
-        st = gg::launch_chained(gg::norm_gradient_kernel<f(), wt(), n(), v()>, dim3(grid), static_cast<unsigned>(32 * t.warps * per), 0, s,
+      gg::with_spans(t.spans, vec, [&](auto n, auto v) {
+        st = gg::launch_chained(gg::norm_gradient_kernel<f(), wt(), n(), v()>, dim3(grid), static_cast<unsigned>(t.threads), 0, s,
                                 1, p, t.warps);
       });
     });
   if (st == cudaSuccess && q.grad_weight)
     st = gg::launch_chained(gg::norm_weight_sum_kernel, dim3(static_cast<unsigned>((w + 31) / 32)), 32 * gg::kSumWarps, 0, s, 1,
-                            static_cast<const float*>(plan->partial), static_cast<int>(grid) * per, w, q.grad_weight);
+                            static_cast<const float*>(plan->partial), static_cast<int>(grid), w, q.grad_weight);
   return st;
 }
 
