@@ -410,6 +410,20 @@ void with_shape(int bn, bool gated, Do go) {
 constexpr int kShapes = 4;  // 256, 128, 64, 32
 int width_of(int shape) { return 256 >> shape; }
 
+// What a run with tiles of one width takes: its tiles go over the SMs in rounds, in each of which a block of k takes an SM so
+// long (0.50, 0.345, 0.30 and 0.28 us, measured with one round of 148 tiles), or memory so long as the round's weights
+// take it, and a tile some 4 us more (2.3 with the narrowest). 64 rows on 8 experts of 4096 x 14336 are 128 tiles of 256, one round, or
+// 256 of 128, two: 82 us against 87; of 4736 x 14336, 152 and 296 tiles, two rounds each: 146 us against 79.
+double expected_us(int shape, int64_t stretches, int64_t tiles_n, int k_blocks, int experts, int sms) {
+  constexpr double kBlock[kShapes] = {0.50, 0.345, 0.30, 0.28}, kTile[kShapes] = {4.2, 2.9, 2.4, 2.3};
+  constexpr double kBytesPerUs = 6.5e6;
+  const int64_t tiles = stretches * tiles_n;
+  // an expert's weights come from memory once, from L2 for its further rows
+  const double bytes = width_of(shape) * 128.0 * std::min(1.0, static_cast<double>(experts) / std::max<int64_t>(1, stretches));
+  const auto round = [&](int64_t n) { return k_blocks * std::max(kBlock[shape], n * bytes / kBytesPerUs) + kTile[shape]; };
+  return static_cast<double>(tiles / sms) * round(sms) + (tiles % sms ? round(tiles % sms) : 0.0);
+}
+
 }  // namespace
 }  // namespace gg
 
@@ -525,9 +539,12 @@ int gg_f8_plan_run(gg_f8_plan* plan, const void* a, int lda, const float* a_scal
     return cudaErrorInvalidValue;
   // 128-row tiles at most, if every expert's rows end in a part of one
   const int64_t stretches = std::min<int64_t>(capacity_rows, static_cast<int64_t>(capacity_rows) / gg::tiles::kTileRows + q.experts);
-  int shape = 0;
   const auto tiles_n = [&](int s) { return (static_cast<int64_t>(q.n) * (gated ? 2 : 1) - 1) / gg::width_of(s) + 1; };
-  while (!eight && shape < (gated ? 2 : 3) && stretches * tiles_n(shape) < plan->sms) ++shape;
+  int shape = 0;
+  for (int s = 1; !eight && s < (gated ? 3 : gg::kShapes); ++s)
+    if (gg::expected_us(s, stretches, tiles_n(s), p.k_blocks, q.experts, plan->sms) <
+        gg::expected_us(shape, stretches, tiles_n(shape), p.k_blocks, q.experts, plan->sms))
+      shape = s;
   const int64_t most = stretches * tiles_n(shape);
   if (most > INT32_MAX) return cudaErrorInvalidValue;
   p.tiles_n = static_cast<int>(tiles_n(shape));

@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_kernel(const NormParams 
 
 // Each thread adds up its columns' part of grad_weight on its team's way through the rows.
 template <int F, int W, int kSpans, bool kVec>
-__global__ void __launch_bounds__(32 * kMostWarps) norm_gradient_kernel(const NormGradientParams p, int warps) {
+__global__ void __launch_bounds__(32 * kMostWarps, kSpans == 1 && F != kOutF32 ? 2 : 1) norm_gradient_kernel(const NormGradientParams p, int warps) {
   __shared__ float sums[64];
   const int lane = threadIdx.x % 32;
   const Place at(warps);
