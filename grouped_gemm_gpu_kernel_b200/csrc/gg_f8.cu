@@ -175,17 +175,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
           if (!ok) break;
           ++it;
           ptx::tc_fence_after_sync();
-          // a piece is read while the one before it is added up
-          constexpr int kPiece = kMine < 32 || BN == 256 ? 16 : 32, kPieces = (kGated ? 2 : 1) * kMine / kPiece;
+          constexpr int kPiece = kMine < 32 ? 16 : 32, kPieces = (kGated ? 2 : 1) * kMine / kPiece;
           const uint32_t from = lanes + buf * BN + static_cast<uint32_t>(half * kMine);
           const auto at_piece = [&](int c) { return from + static_cast<uint32_t>(kGated && c * kPiece >= kMine ? kWidth + c * kPiece - kMine : c * kPiece); };
-          uint32_t r[2][kPiece];
-          if (mine) tmem_start(at_piece(0), r[0]);
+          // One piece at a time: two, each read while the one before it is added up, leave too few registers (16384 rows on 64
+          // experts of 14336 x 4096: pieces of 32, 1345 us, of 16, 1395; two of 16 in turn 1430, two of 32 1860).
+          uint32_t r[kPiece];
+          if (mine) tmem_start(at_piece(0), r);
 #pragma unroll
           for (int c = 0; c < kPieces; ++c) {
             if (mine) {
-              tmem_wait(r[c % 2]);
-              if (c + 1 < kPieces) tmem_start(at_piece(c + 1), r[(c + 1) % 2]);
+              if (c) tmem_start(at_piece(c), r);
+              tmem_wait(r);
             }
             if (c + 1 == kPieces) {  // all of it is read
               ptx::tc_fence_before_sync();
@@ -195,7 +196,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
             if (mine) {
 #pragma unroll
               for (int j = 0; j < kPiece / 2; ++j)
-                fma2(acc[c * kPiece / 2 + j], r[c % 2][2 * j], r[c % 2][2 * j + 1], kGated && c * kPiece >= kMine ? s1 : s0);
+                fma2(acc[c * kPiece / 2 + j], r[2 * j], r[2 * j + 1], kGated && c * kPiece >= kMine ? s1 : s0);
             }
           }
         }
@@ -358,24 +359,27 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
     const uint64_t a0 = ptx::smem_desc_sw128(sbase, 16u, 1024u), b0 = ptx::smem_desc_sw128(sbase + kABytes, 16u, 1024u);
     Ring<kStages> stage;
     Ring<kAcc> acc;
-    bool ok = true;
+    bool ok = true, have = false;  // have: the next block of k has been seen to be there, with room for its products
     for (int t = static_cast<int>(blockIdx.x); ok && t < total; t += grid) {
       for (int kb = 0; kb < p.k_blocks; ++kb) {
-        ok = __all_sync(0xffffffffu, wait_phase_inline(full(stage.at), stage.phase, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA) &&
-                                         wait_phase_inline(taken(acc.at), acc.phase ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
+        if (!have)
+          ok = __all_sync(0xffffffffu, wait_phase_inline(full(stage.at), stage.phase, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA) &&
+                                           wait_phase_inline(taken(acc.at), acc.phase ^ 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_MMA));
         if (!ok) break;
         ptx::tc_fence_after_sync();
         const uint64_t a = a0 + static_cast<uint32_t>(stage.at * (S::kStageBytes / 16)), b = b0 + static_cast<uint32_t>(stage.at * (S::kStageBytes / 16));
-        const uint32_t d = tmem + static_cast<uint32_t>(acc.at * BN);
+        const uint32_t d = tmem + static_cast<uint32_t>(acc.at * BN), done_stage = empty(stage.at), done_acc = ready(acc.at);
+        stage.next();
+        acc.next();
+        // asked before this block's products are issued, so that the answer is on its way meanwhile
+        const bool next_full = ptx::mbar_test_wait(full(stage.at), stage.phase), next_taken = ptx::mbar_test_wait(taken(acc.at), acc.phase ^ 1u);
         if (leader) {
 #pragma unroll
           for (uint32_t kk = 0; kk < 4; ++kk) ptx::tc_mma_f8(d, a + 2 * kk, b + 2 * kk, idesc, kk != 0);
-          ptx::tc_commit(empty(stage.at));
-          ptx::tc_commit(ready(acc.at));
+          ptx::tc_commit(done_stage);
+          ptx::tc_commit(done_acc);
         }
-        __syncwarp();
-        stage.next();
-        acc.next();
+        have = __all_sync(0xffffffffu, next_full && next_taken);
       }
     }
     if (leader) {
@@ -540,10 +544,11 @@ int gg_f8_plan_run(gg_f8_plan* plan, const void* a, int lda, const float* a_scal
   // 128-row tiles at most, if every expert's rows end in a part of one
   const int64_t stretches = std::min<int64_t>(capacity_rows, static_cast<int64_t>(capacity_rows) / gg::tiles::kTileRows + q.experts);
   const auto tiles_n = [&](int s) { return (static_cast<int64_t>(q.n) * (gated ? 2 : 1) - 1) / gg::width_of(s) + 1; };
+  // and as many as there are likely to be: one for each expert, or half of an expert's last one empty
+  const int64_t likely = std::max<int64_t>(std::min(capacity_rows, q.experts), (capacity_rows / gg::tiles::kTileRows) + q.experts / 2);
   int shape = 0;
   for (int s = 1; !eight && s < (gated ? 3 : gg::kShapes); ++s)
-    if (gg::expected_us(s, stretches, tiles_n(s), p.k_blocks, q.experts, plan->sms) <
-        gg::expected_us(shape, stretches, tiles_n(shape), p.k_blocks, q.experts, plan->sms))
+    if (gg::expected_us(s, likely, tiles_n(s), p.k_blocks, q.experts, plan->sms) < gg::expected_us(shape, likely, tiles_n(shape), p.k_blocks, q.experts, plan->sms))
       shape = s;
   const int64_t most = stretches * tiles_n(shape);
   if (most > INT32_MAX) return cudaErrorInvalidValue;
