@@ -7,9 +7,9 @@
 //             two columns of one lane and gate and up need not leave the SM;
 //   rows      grad_x = grad_gate Wg^T + grad_up Wu^T is one sum along both matrices' inner size;
 //   weights   grad_Wg and grad_Wu = x^T [grad_gate | grad_up], the forward's tile with the expert's rows as the inner
-//             size. The last stage of an expert can hold rows of the next one: the warp that issues the
-//             products clears them in shared memory first (at most 15 rows: it stops at the next multiple of 16, the depth
-//             of a product).
+//             size. The last stage of an expert can hold rows of the next one: a warp of its own clears them in
+//             shared memory (at most 15 rows: up to the next multiple of 16, the depth of a product) before that
+//             stage is handed over.
 // Each comes in two forms. On one CTA a tile takes 48 KB of operands for a stage of 64, which its shared memory both takes in and
 // feeds to the tensor cores: 96 KB in 512 cycles of products at their full rate, and 128 bytes a cycle is what it has. On a
 // pair (cta_group::2, 256 x 256) each CTA has 128 rows of the one operand and half of the other: 32 KB, six stages in
@@ -34,6 +34,7 @@ namespace {
 using namespace tiles;
 
 constexpr int kForward = 0, kRowGradient = 1, kWeightGradient = 2;
+constexpr int kClearWarp = 9;
 constexpr int kBN = 256;       // columns of an accumulator
 constexpr int kDepth = 64;     // values of k of a stage
 constexpr int kAcc = 2;
@@ -41,7 +42,7 @@ template <bool kPair>
 struct GatedShape {
   static constexpr int kStages = kPair ? 6 : 4;
   static constexpr int kStageBytes = kABytes + kBN / (kPair ? 2 : 1) * kRowBytes;
-  static constexpr int kBars = 2 * kStages + 2 * kAcc + 1 + 2;
+  static constexpr int kBars = 3 * kStages + 2 * kAcc + 1;
   static constexpr int kStretch = kPair ? 2 * kTileRows : kTileRows;  // rows of a tile
   static constexpr int smem(int experts) { return layout(kStages * kStageBytes, experts, kBars).bytes; }
   static_assert(layout(kStages * kStageBytes, kMaxExperts, kBars).bytes <= 232448, "shared memory of a block");
@@ -63,7 +64,7 @@ struct GatedParams {
 };
 
 // Zeros in the rows `left` and on, up to the next multiple of 16, of kChunks pieces of shared memory that hold a 128-byte row of 64
-// columns for each k: rows of the next expert, or of none. By one warp, between the loads' barrier and a proxy fence.
+// columns for each k. By one warp, between the loads' barrier and a proxy fence.
 template <int kChunks>
 __device__ __forceinline__ void clear_after(uint8_t* stage, int left, int lane) {
   const int first = left % kDepth, rows = 16 - first % 16;
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
   const auto ready = [&](int b) { return bar0 + 8u * (2 * kStages + b); };
   const auto taken = [&](int b) { return bar0 + 8u * (2 * kStages + kAcc + b); };
   const uint32_t drained = bar0 + 8u * (2 * kStages + 2 * kAcc);
-  const auto cut = [&](int w) { return bar0 + 8u * (2 * kStages + 2 * kAcc + 1 + w); };
+  const auto cut = [&](int s) { return bar0 + 8u * (2 * kStages + 2 * kAcc + 1 + s); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + l.words);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + l.words + 4);
 
@@ -96,10 +97,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
   const int rank = kPair ? static_cast<int>(ptx::cluster_ctarank()) : 0;
   if (threadIdx.x == 0) {
     // a pair's stages and accumulators are counted on the barriers of its first CTA
-    for (int s = 0; s < kStages; ++s) ptx::mbar_init(full(s), kPair ? 2 : 1), ptx::mbar_init(empty(s), 1);
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(full(s), kPair ? 2 : 1), ptx::mbar_init(empty(s), 1), ptx::mbar_init(cut(s), 1);
     for (int b = 0; b < kAcc; ++b) ptx::mbar_init(ready(b), 1), ptx::mbar_init(taken(b), (kPair ? 2 : 1) * kEpilogueWarps);
     ptx::mbar_init(drained, 1);
-    for (int w = 0; w < 2; ++w) ptx::mbar_init(cut(w), 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
@@ -146,6 +146,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
     }
     return x;
   };
+  // Whether stage kb of a tile ends within 16 rows of k: what follows there is another expert's, or no row.
+  const auto is_cut = [&](const Tile& x, int kb) { return kMode == kWeightGradient && kb + 1 == x.depth && x.rows % 16 != 0; };
   // the first of this CTA's 128 columns of A of the weights' gradient
   const auto first_k = [&](const Tile& x) { return x.m * S::kStretch + rank * kTileRows; };
 
@@ -155,7 +157,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
     Ring<kStages, 2> stage;
     stage.at = warp - kLoadWarp;
     int skip = stage.at;  // stages of 64 until this warp's next
-    uint32_t cuts = 0;
     bool ok = true;
     for (int t = block; ok && t < total; t += grid) {
       const Tile x = tile_at(t);
@@ -166,10 +167,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
         if (!ok) break;
         const uint32_t a = sbase + static_cast<uint32_t>(stage.at * kStageBytes), b = a + kABytes;
         const uint32_t counted = kPair ? ptx::mapa_shared(full(stage.at), 0) : full(stage.at);
-        // the last stage of an expert with rows of the next one in it, on a pair: loaded, cleared, then handed over
-        const int left = x.rows - kb * kDepth;
-        const bool clear = kPair && kMode == kWeightGradient && left < kDepth && left % 16 != 0;
-        const uint32_t bar = clear ? cut(warp - kLoadWarp) : counted;
+        const bool clear = is_cut(x, kb);  // handed over by the warp that clears it
+        const uint32_t bar = clear ? cut(stage.at) : counted;
         const auto load = [&](uint32_t to, const CUtensorMap* map, int at, int row) {
           if (kPair && !clear) ptx::tma_load_2d_pair(to, map, bar, at, row);
           else ptx::tma_load_2d(to, map, bar, at, row);
@@ -209,23 +208,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
           if (kPair && !clear && rank != 0) ptx::mbar_arrive_cluster_relaxed(counted);  // counts; the bytes are tracked by themselves
         }
         __syncwarp();
-        if (clear) {
-          ok = __all_sync(0xffffffffu, wait_phase_inline(bar, cuts & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER));
-          if (!ok) break;
-          ++cuts;
-          clear_after<kStageBytes / kChunkBytes>(smem + stage.at * kStageBytes, left, lane);
-          ptx::fence_proxy_async_all();  // the other CTA's tensor cores read it too
-          __syncwarp();
-          if (lane == 0) {
-            if (rank == 0) ptx::mbar_arrive(full(stage.at));
-            else ptx::mbar_arrive_cluster(counted);
-          }
-        }
         stage.next();
       }
       skip = kb - x.depth;
     }
     if ((!ok || *abort_flag) && rank == 0) drain_loads<kStages>(stage, full);
+  } else if (kMode == kWeightGradient && warp == kClearWarp) {
+    uint32_t it = 0, turns = 0;  // a bit for each stage: the parity of its next cut
+    bool ok = true;
+    for (int t = block; ok && t < total; t += grid) {
+      const Tile x = tile_at(t);
+      it += static_cast<uint32_t>(x.depth);
+      if (x.depth == 0 || !is_cut(x, x.depth - 1)) continue;
+      const int at = static_cast<int>((it - 1) % kStages);
+      ok = __all_sync(0xffffffffu, wait_phase_inline(cut(at), turns >> at & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER));
+      if (!ok) break;
+      turns ^= 1u << at;
+      clear_after<kStageBytes / kChunkBytes>(smem + at * kStageBytes, x.rows % kDepth, lane);
+      ptx::fence_proxy_async_all();  // the tensor cores read it, on a pair the other CTA's too
+      __syncwarp();
+      if (lane == 0) {
+        if (rank == 0) ptx::mbar_arrive(full(at));
+        else ptx::mbar_arrive_cluster(ptx::mapa_shared(full(at), 0));
+      }
+    }
   } else if (warp == kProductWarp) {
     if (rank == 0) {
       // the forward's weights and all of the weights' gradient have k as their rows in shared memory
@@ -251,14 +257,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
           int steps = kDepth / 16;
           if constexpr (kMode == kWeightGradient) {
             const int left = x.rows - kb * kDepth;
-            if (left < kDepth) {
-              steps = (left + 15) / 16;
-              if (!kPair && left % 16 != 0) {
-                clear_after<kStageBytes / kChunkBytes>(smem + stage.at * kStageBytes, left, lane);
-                ptx::fence_proxy_async_smem();
-                __syncwarp();
-              }
-            }
+            if (left < kDepth) steps = (left + 15) / 16;
           }
           ptx::tc_fence_after_sync();
           const uint64_t a = a0 + static_cast<uint32_t>(stage.at * (kStageBytes / 16)), b = b0 + static_cast<uint32_t>(stage.at * (kStageBytes / 16));
@@ -368,13 +367,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
   if constexpr (kPair) {
     __syncwarp();
     ptx::cluster_sync();  // neither CTA ends while the other may still use its shared memory
-    if (*abort_flag) {    // after an abort, loads may still be landing
-      const uint64_t t0 = ptx::global_timer_ns();
-      while (ptx::global_timer_ns() - t0 < 200000ull) {
-      }
-    }
   } else {
     __syncthreads();
+  }
+  if (*abort_flag) {  // after an abort, loads may still be landing
+    const uint64_t t0 = ptx::global_timer_ns();
+    while (ptx::global_timer_ns() - t0 < 200000ull) {
+    }
   }
   if (warp == kProductWarp) {
     ptx::tc_fence_after_sync();
