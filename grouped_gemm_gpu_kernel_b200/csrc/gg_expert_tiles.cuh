@@ -22,13 +22,17 @@ namespace tiles {
 constexpr int kTileThreads = 384;
 constexpr int kEpilogueWarps = 8;
 constexpr int kProductWarp = 8;
-constexpr int kLoadWarp = 10;                  // and the next one, which take the stages in turn: a stage's loads take one thread 600 cycles
+constexpr int kLoadWarp = 10;                  // and the next one, which take the stages in turn: one warp takes 500 cycles for a stage's loads
 constexpr int kTileRows = 128;                 // rows of a tile: M of the products
 constexpr int kRowBytes = 128;                 // of a stage's row: 64 values of 16 bits or 128 of 8
 constexpr int kABytes = kTileRows * kRowBytes; // of a stage
 constexpr int kBoxRows = 16;                   // rows that one load of a part of a tile takes
 constexpr int kStagingBytes = 2048;            // of an epilogue warp: 32 rows of 64 bytes
 constexpr int kMaxExperts = 1024;
+// Limits that keep rows, columns and tiles, and what a role adds to them, within 32 bits.
+constexpr int kMostRows = 2147483647 - 65536;
+constexpr int kMostSize = 1 << 30;
+constexpr long long kMostTiles = 2147483647 - 65536;
 constexpr int kRaster = 16;                    // tile rows that are gone through before the next tile column
 
 // Shared memory after the stages: staging, what a kernel wants for itself, the experts' tables, barriers.
@@ -65,6 +69,10 @@ __device__ __forceinline__ void activate_all(float (&v)[N], int act) {
 
 // first_row[e], first_tile[e] for e = 0..experts (totals at the end), by one warp. `per_row_tile`: tiles of one stretch of kStretch
 // rows of an expert. Counts that are negative or sum to more than `capacity` leave no rows, and -1 as the total of tiles.
+template <int kStretch>
+__device__ __forceinline__ int stretches_of(int rows) {
+  return rows / kStretch + (rows % kStretch != 0);
+}
 template <int kStretch = kTileRows>
 __device__ __forceinline__ void expert_table(const int* rows, int experts, int capacity, int per_row_tile, int* first_row, int* first_tile,
                                              int* status, int lane) {
@@ -74,7 +82,7 @@ __device__ __forceinline__ void expert_table(const int* rows, int experts, int c
     if (lane == 0) {
       first_row[0] = first_tile[0] = 0;
       first_row[1] = capacity;
-      first_tile[1] = (capacity + kStretch - 1) / kStretch * per_row_tile;
+      first_tile[1] = stretches_of<kStretch>(capacity) * per_row_tile;
     }
     return;
   }
@@ -83,25 +91,25 @@ __device__ __forceinline__ void expert_table(const int* rows, int experts, int c
     const int r = next;
     if (e0 + 32 + lane < experts) next = rows[e0 + 32 + lane];
     else next = 0;
-    // a count above capacity - row, or a negative one, ends it, so no sum passes 32 bits: 32 counts of at most capacity
+    // sums of 32 counts of at most capacity take 64 bits; tiles are counted only where the rows fit
     bad = bad || __any_sync(0xffffffffu, r < 0 || r > capacity);
     if (bad) break;
     long long sum = r;
-    int t = (r + kStretch - 1) / kStretch * per_row_tile;
+    unsigned t = static_cast<unsigned>(stretches_of<kStretch>(r)) * static_cast<unsigned>(per_row_tile);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long s = __shfl_up_sync(0xffffffffu, sum, o);
-      const int u = __shfl_up_sync(0xffffffffu, t, o);
+      const unsigned u = __shfl_up_sync(0xffffffffu, t, o);
       if (lane >= o) sum += s, t += u;
     }
     bad = __any_sync(0xffffffffu, sum + row > capacity);
     if (bad) break;
     if (e0 + lane < experts) {
       first_row[e0 + lane + 1] = row + static_cast<int>(sum);
-      first_tile[e0 + lane + 1] = tile + t;
+      first_tile[e0 + lane + 1] = tile + static_cast<int>(t);
     }
     row += static_cast<int>(__shfl_sync(0xffffffffu, sum, 31));
-    tile += __shfl_sync(0xffffffffu, t, 31);
+    tile += static_cast<int>(__shfl_sync(0xffffffffu, t, 31));
   }
   if (bad) {
     for (int e = lane; e <= experts; e += 32) first_row[e] = 0, first_tile[e] = e < experts ? 0 : -1;

@@ -12,9 +12,9 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <memory>
 #include <new>
 #include <type_traits>
-#include <vector>
 
 #include "gg_expert_tiles.cuh"
 #include "gg_internal.h"
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
     x.e = expert_of(first_tile, p.experts, t);
     const int count = first_row[x.e + 1] - first_row[x.e];
     int m;
-    place(t - first_tile[x.e], (count + kTileRows - 1) / kTileRows, p.tiles_n, m, x.n);
+    place(t - first_tile[x.e], stretches_of<kTileRows>(count), p.tiles_n, m, x.n);
     x.row = first_row[x.e] + m * kTileRows;
     x.rows = min(kTileRows, count - m * kTileRows);
     return x;
@@ -448,7 +448,7 @@ int gg_f8_plan_create(const gg_f8_problem* problem, gg_f8_plan** out) {
   const gg_f8_problem& q = *problem;
   const bool gated = q.up != nullptr, eight = q.output_type > GG_OUTPUT_BF16;
   const auto off16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 != 0; };
-  if (q.experts < 1 || q.experts > GG_F8_MAX_EXPERTS || q.n < 1 || q.k < 1 || q.ldb < q.k || q.ldb % 16 != 0 || !q.b || !q.b_scales ||
+  if (q.experts < 1 || q.experts > GG_F8_MAX_EXPERTS || q.n < 1 || q.n > gg::tiles::kMostSize || q.k < 1 || q.k > gg::tiles::kMostSize || q.ldb < q.k || q.ldb % 16 != 0 || !q.b || !q.b_scales ||
       (gated != (q.up_scales != nullptr)) || (gated && q.bias) || (q.input_type != GG_INPUT_E4M3 && q.input_type != GG_INPUT_E5M2) ||
       q.output_type < GG_OUTPUT_F32 || q.output_type > GG_OUTPUT_E5M2 || (eight && !gated) || q.activation < GG_ACT_NONE ||
       q.activation > GG_ACT_SILU)
@@ -460,9 +460,16 @@ int gg_f8_plan_create(const gg_f8_problem* problem, gg_f8_plan** out) {
   if (!plan) return cudaErrorMemoryAllocation;
   const size_t E = static_cast<size_t>(q.experts);
   const size_t map_bytes = 2 * E * sizeof(CUtensorMap), tables_at = gg::kShapes * map_bytes, status_at = tables_at + 3 * E * sizeof(void*);
-  std::vector<unsigned char> host(status_at + sizeof(int), 0);
-  const auto maps = [&](int shape) { return reinterpret_cast<CUtensorMap*>(host.data() + shape * map_bytes); };
-  const float** tables = reinterpret_cast<const float**>(host.data() + tables_at);
+  const size_t host_bytes = status_at + sizeof(int);
+  // aligned as tensor maps want it
+  const std::unique_ptr<CUtensorMap[]> host(new (std::nothrow) CUtensorMap[(host_bytes - 1) / sizeof(CUtensorMap) + 1]());
+  if (!host) {
+    delete plan;
+    return cudaErrorMemoryAllocation;
+  }
+  unsigned char* base = reinterpret_cast<unsigned char*>(host.get());
+  const auto maps = [&](int shape) { return reinterpret_cast<CUtensorMap*>(base + shape * map_bytes); };
+  const float** tables = reinterpret_cast<const float**>(base + tables_at);
   cudaError_t st = cudaGetDevice(&plan->device);
   if (st == cudaSuccess) st = cudaDeviceGetAttribute(&plan->sms, cudaDevAttrMultiProcessorCount, plan->device);
   for (int e = 0; e < q.experts && st == cudaSuccess; ++e) {
@@ -486,8 +493,8 @@ int gg_f8_plan_create(const gg_f8_problem* problem, gg_f8_plan** out) {
       if (st == cudaSuccess) st = cudaFuncSetAttribute(gg::f8_kernel<bn(), g()>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 gg::tiles::layout(S::kStages * S::kStageBytes, gg::tiles::kMaxExperts, S::kBars, gg::kScaleSlots * gg::kScaleBytes).bytes);
     });
-  if (st == cudaSuccess) st = cudaMalloc(reinterpret_cast<void**>(&plan->block), host.size());
-  if (st == cudaSuccess) st = cudaMemcpy(plan->block, host.data(), host.size(), cudaMemcpyHostToDevice);
+  if (st == cudaSuccess) st = cudaMalloc(reinterpret_cast<void**>(&plan->block), host_bytes);
+  if (st == cudaSuccess) st = cudaMemcpy(plan->block, host.get(), host_bytes, cudaMemcpyHostToDevice);
   if (st == cudaSuccess) st = cudaDeviceSynchronize();
   if (st != cudaSuccess) {
     if (plan->block) cudaFree(plan->block);
@@ -519,7 +526,7 @@ int gg_f8_plan_run(gg_f8_plan* plan, const void* a, int lda, const float* a_scal
   const gg_f8_problem& q = plan->problem;
   gg::F8Params p = plan->params;
   const bool gated = q.up != nullptr, eight = q.output_type > GG_OUTPUT_BF16;
-  if (capacity_rows < 0 || (!rows && q.experts != 1)) return cudaErrorInvalidValue;
+  if (capacity_rows < 0 || capacity_rows > gg::tiles::kMostRows || (!rows && q.experts != 1)) return cudaErrorInvalidValue;
   if (capacity_rows == 0 && !rows) return cudaSuccess;
   if (capacity_rows > 0 && (!a || !a_scales || !d || lda < q.k || lda % 16 != 0 || reinterpret_cast<uintptr_t>(a) % 16 != 0 || ldas < p.k_blocks ||
                             ldd < q.n || (eight && (!d_scales || ldds < (q.n - 1) / GG_SCALE_BLOCK + 1))))
@@ -551,7 +558,7 @@ int gg_f8_plan_run(gg_f8_plan* plan, const void* a, int lda, const float* a_scal
     if (gg::expected_us(s, likely, tiles_n(s), p.k_blocks, q.experts, plan->sms) < gg::expected_us(shape, likely, tiles_n(shape), p.k_blocks, q.experts, plan->sms))
       shape = s;
   const int64_t most = stretches * tiles_n(shape);
-  if (most > INT32_MAX) return cudaErrorInvalidValue;
+  if (most > gg::tiles::kMostTiles) return cudaErrorInvalidValue;
   p.tiles_n = static_cast<int>(tiles_n(shape));
   p.maps = plan->maps[shape];
   const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(plan->sms, most)));

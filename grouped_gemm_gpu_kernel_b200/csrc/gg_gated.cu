@@ -20,8 +20,8 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <memory>
 #include <new>
-#include <vector>
 
 #include "gg_expert_tiles.cuh"
 #include "gg_internal.h"
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
     } else {
       x.e = expert_of(first_tile, p.experts, t);
       const int count = first_row[x.e + 1] - first_row[x.e];
-      place(t - first_tile[x.e], (count + S::kStretch - 1) / S::kStretch, p.tiles_n, x.m, x.n);
+      place(t - first_tile[x.e], stretches_of<S::kStretch>(count), p.tiles_n, x.m, x.n);
       x.row = first_row[x.e] + x.m * S::kStretch + rank * kTileRows;
       x.rows = min(kTileRows, count - x.m * S::kStretch - rank * kTileRows);  // none for the second CTA of a pair: not positive
       x.depth = (kMode == kRowGradient ? 2 : 1) * ((p.inner + kDepth - 1) / kDepth);
@@ -527,19 +527,7 @@ cudaError_t prepare(gg_gated_plan* plan) {
   const int smem = gg::GatedShape<kPair>::smem(gg::tiles::kMaxExperts);
   cudaError_t st = cudaFuncSetAttribute(gg::gated_kernel<kMode, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (!kPair || st != cudaSuccess) return st;
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim = {2, 1, 1};
-  cfg.gridDim = dim3(2);
-  cfg.blockDim = dim3(gg::tiles::kTileThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  int pairs = 0;
-  st = cudaOccupancyMaxActiveClusters(&pairs, gg::gated_kernel<kMode, kPair>, &cfg);
-  plan->pairs = std::max(1, pairs);
-  return st;
+  return gg::resident_pairs(gg::gated_kernel<kMode, kPair>, gg::tiles::kTileThreads, static_cast<size_t>(smem), &plan->pairs);
 }
 
 // The maps of packed rows for RowLoads: whole tiles and boxes.
@@ -567,7 +555,7 @@ int gg_gated_plan_create(const gg_gated_problem* problem, gg_gated_plan** out) {
   if (!problem) return cudaErrorInvalidValue;
   const gg_gated_problem& q = *problem;
   const auto off16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 != 0; };
-  if (q.experts < 1 || q.experts > GG_GATED_MAX_EXPERTS || q.n < 1 || q.k < 1 || q.ldw < q.n || q.ldw % 8 != 0 || !q.gate || !q.up ||
+  if (q.experts < 1 || q.experts > GG_GATED_MAX_EXPERTS || q.n < 1 || q.n > gg::tiles::kMostSize || q.k < 1 || q.k > gg::tiles::kMostSize || q.ldw < q.n || q.ldw % 8 != 0 || !q.gate || !q.up ||
       (q.type != GG_INPUT_F16 && q.type != GG_INPUT_BF16) || q.activation < GG_ACT_NONE || q.activation > GG_ACT_SILU)
     return cudaErrorInvalidValue;
   for (int e = 0; e < q.experts; ++e)
@@ -576,8 +564,14 @@ int gg_gated_plan_create(const gg_gated_problem* problem, gg_gated_plan** out) {
   gg_gated_plan* plan = new (std::nothrow) gg_gated_plan();
   if (!plan) return cudaErrorMemoryAllocation;
   const size_t E = static_cast<size_t>(q.experts), map_bytes = 2 * E * sizeof(CUtensorMap), status_at = 2 * map_bytes;
-  std::vector<unsigned char> host(status_at + sizeof(int), 0);
-  CUtensorMap* forward = reinterpret_cast<CUtensorMap*>(host.data());
+  const size_t host_bytes = status_at + sizeof(int);
+  // aligned as tensor maps want it
+  const std::unique_ptr<CUtensorMap[]> host(new (std::nothrow) CUtensorMap[(host_bytes - 1) / sizeof(CUtensorMap) + 1]());
+  if (!host) {
+    delete plan;
+    return cudaErrorMemoryAllocation;
+  }
+  CUtensorMap* forward = host.get();
   CUtensorMap* rows = forward + 2 * E;
   const int kind = q.type == GG_INPUT_F16 ? 2 : 3;
   const int64_t pitch = static_cast<int64_t>(q.ldw) * 2;
@@ -596,8 +590,8 @@ int gg_gated_plan_create(const gg_gated_problem* problem, gg_gated_plan** out) {
   if (st == cudaSuccess) st = prepare<gg::kForward, true>(plan);
   if (st == cudaSuccess) st = prepare<gg::kRowGradient, true>(plan);
   if (st == cudaSuccess) st = prepare<gg::kWeightGradient, true>(plan);
-  if (st == cudaSuccess) st = cudaMalloc(reinterpret_cast<void**>(&plan->block), host.size());
-  if (st == cudaSuccess) st = cudaMemcpy(plan->block, host.data(), host.size(), cudaMemcpyHostToDevice);
+  if (st == cudaSuccess) st = cudaMalloc(reinterpret_cast<void**>(&plan->block), host_bytes);
+  if (st == cudaSuccess) st = cudaMemcpy(plan->block, host.get(), host_bytes, cudaMemcpyHostToDevice);
   if (st == cudaSuccess) st = cudaDeviceSynchronize();
   if (st != cudaSuccess) {
     if (plan->block) cudaFree(plan->block);
@@ -615,7 +609,7 @@ int gg_gated_plan_create(const gg_gated_problem* problem, gg_gated_plan** out) {
 int gg_gated_plan_run(gg_gated_plan* plan, const gg_gated* call, void* stream) {
   if (!plan || !plan->block) return cudaErrorInvalidDevicePointer;
   const gg_gated_problem& q = plan->problem;
-  if (!call || call->capacity_rows < 0 || (!call->rows && q.experts != 1)) return cudaErrorInvalidValue;
+  if (!call || call->capacity_rows < 0 || call->capacity_rows > gg::tiles::kMostRows || (!call->rows && q.experts != 1)) return cudaErrorInvalidValue;
   const gg_gated& c = *call;
   if (c.capacity_rows == 0 && !c.rows) return cudaSuccess;
   if (c.capacity_rows > 0 && (!c.x || !c.h || c.ldx < q.k || !gg::on16(c.x, static_cast<int64_t>(c.ldx) * 2) || c.ldh < q.n ||
@@ -634,7 +628,7 @@ int gg_gated_plan_run(gg_gated_plan* plan, const gg_gated* call, void* stream) {
   if (c.capacity_rows > 0 && !encode_both(&p.in[0], q.type, c.x, q.k, c.capacity_rows, c.ldx)) return cudaErrorInvalidValue;
   const bool pair = rows_in_pairs(plan, c.capacity_rows);
   const int64_t most = stretches(plan, c.capacity_rows, pair) * p.tiles_n;
-  if (most > INT32_MAX) return cudaErrorInvalidValue;
+  if (most > gg::tiles::kMostTiles) return cudaErrorInvalidValue;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return pair ? launch<gg::kForward, true>(plan, p, most, s) : launch<gg::kForward, false>(plan, p, most, s);
 }
@@ -642,7 +636,7 @@ int gg_gated_plan_run(gg_gated_plan* plan, const gg_gated* call, void* stream) {
 int gg_gated_plan_backward(gg_gated_plan* plan, const gg_gated_gradient* gradient, void* stream) {
   if (!plan || !plan->block) return cudaErrorInvalidDevicePointer;
   const gg_gated_problem& q = plan->problem;
-  if (!gradient || gradient->capacity_rows < 0 || (!gradient->rows && q.experts != 1)) return cudaErrorInvalidValue;
+  if (!gradient || gradient->capacity_rows < 0 || gradient->capacity_rows > gg::tiles::kMostRows || (!gradient->rows && q.experts != 1)) return cudaErrorInvalidValue;
   const gg_gated_gradient& c = *gradient;
   const int type16 = q.type == GG_INPUT_F16 ? GG_OUTPUT_F16 : GG_OUTPUT_BF16;
   if ((!c.grad_wg != !c.grad_wu) || (c.grad_wg && ((c.weight_grad_type != GG_OUTPUT_F32 && c.weight_grad_type != type16) || c.ldgw < q.n ||
@@ -694,7 +688,7 @@ int gg_gated_plan_backward(gg_gated_plan* plan, const gg_gated_gradient* gradien
   }
   const int64_t most_x = px.maps ? stretches(plan, c.capacity_rows, pair_x) * px.tiles_n : 0;
   const int64_t most_w = pw.maps ? static_cast<int64_t>(q.experts) * pw.tiles_m * pw.tiles_n : 0;
-  if (most_x > INT32_MAX || most_w > INT32_MAX) return cudaErrorInvalidValue;
+  if (most_x > gg::tiles::kMostTiles || most_w > gg::tiles::kMostTiles) return cudaErrorInvalidValue;
 
   if (c.capacity_rows > 0) {
     gg::GateGradientParams g{c.gate, c.up, c.grad_h, c.grad_gate, c.grad_up, c.rows, c.ldg, c.ldgh, c.ldgg, q.experts, q.n, c.capacity_rows, q.activation};

@@ -25,6 +25,23 @@ inline cudaError_t expect_device(int device) {
   return st != cudaSuccess ? st : now == device ? cudaSuccess : cudaErrorInvalidDevice;
 }
 
+// Clusters of two blocks of a kernel that the GPU holds at a time.
+template <typename... Params>
+cudaError_t resident_pairs(void (*kernel)(Params...), unsigned threads, size_t smem, int* pairs) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {2, 1, 1};
+  cfg.gridDim = dim3(2);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t st = cudaOccupancyMaxActiveClusters(pairs, kernel, &cfg);
+  if (*pairs < 1) *pairs = 1;
+  return st;
+}
+
 // cluster > 1: blocks of the grid's clusters.
 template <typename... Params, typename... Args>
 cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, unsigned cluster,

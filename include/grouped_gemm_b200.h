@@ -546,9 +546,11 @@ void gg_q4_plan_destroy(gg_q4_plan* plan);
  *   rstd(r) = 1 / sqrt(mean over c of h(r, c)^2 + eps)
  *   y(r, c) = h(r, c) * rstd(r) * weight(c)
  *   8 bits: scale(r, b) = the largest |y| of columns 128 b to 128 b + 127, over the largest finite number of the
- *   type (448 or 57344); q = y / scale(r, b), rounded to nearest even; y is not rounded in between. A block whose largest |y|
- *   is below 2^-100 has scale 0 and q 0; one that holds an infinity or a NaN has a scale that is not finite.
- * Everything but what is stored is FP32. The sums are taken in a fixed order: the same call gives the same bits. */
+ *   type (448 or 57344); q = y times the inverse of scale(r, b), rounded to nearest even; y is not rounded in between. A
+ *   block whose largest |y| is below 2^-100 has scale 0 and q 0; one that holds an infinity or a NaN has a scale that is
+ *   not finite.
+ * Everything but what is stored is FP32, the sum of a row's squares too: past 3.4e38 rstd is 0. The sums are taken in a fixed
+ * order: the same call gives the same bits. */
 #define GG_NORM_MAX_WIDTH 32768
 typedef struct gg_norm_config {
   int width;       /* 1..GG_NORM_MAX_WIDTH */
@@ -618,8 +620,8 @@ typedef struct gg_f8_problem {
   const float* const* up_scales;    /* with up: like b_scales */
   const float* const* bias;         /* optional, not with up: host array of device pointers (NULL entries: none): n FP32 values */
   int experts;                      /* 1..GG_F8_MAX_EXPERTS */
-  int n;                            /* outputs, >= 1 */
-  int k;                            /* inputs, >= 1 */
+  int n;                            /* outputs, 1..2^30 */
+  int k;                            /* inputs, 1..2^30 */
   int ldb;                          /* a multiple of 16, >= k */
   int input_type;                   /* GG_INPUT_E4M3 or GG_INPUT_E5M2: A and the weights */
   int output_type;                  /* GG_OUTPUT_F32, F16 or BF16; with up also GG_OUTPUT_E4M3 or E5M2 */
@@ -631,7 +633,7 @@ typedef struct gg_f8_plan gg_f8_plan;
  * device once, to write its tables. Errors: sizes or types out of range, null pointers, weights or a pitch off a 16-byte
  * boundary -> cudaErrorInvalidValue before any device work; CUDA errors passed through. */
 int gg_f8_plan_create(const gg_f8_problem* problem, gg_f8_plan** out);
-/* a: capacity_rows x k, pitch lda (a multiple of 16, >= k), 16-byte aligned; a_scales: capacity_rows x ceil(k / 128),
+/* capacity_rows: at most 2^31 - 65537. a: capacity_rows x k, pitch lda (a multiple of 16, >= k), 16-byte aligned; a_scales: capacity_rows x ceil(k / 128),
  * pitch ldas. rows: `experts` counts in device memory; NULL with experts == 1: all capacity_rows rows.
  * d: capacity_rows x n of the output type, pitch ldd (>= n), any alignment; d_scales (8-bit D): capacity_rows x
  * ceil(n / 128), pitch ldds. Rows past the counts' sum are not written. One launch on `stream`. Counts that are negative or
@@ -657,15 +659,15 @@ typedef struct gg_gated_problem {
   const void* const* gate;  /* host array of `experts` device pointers: Wg, k x n, row pitch ldw */
   const void* const* up;    /* the same for Wu */
   int experts;              /* 1..GG_GATED_MAX_EXPERTS */
-  int n;                    /* inner size, >= 1 */
-  int k;                    /* outer size, >= 1 */
+  int n;                    /* inner size, 1..2^30 */
+  int k;                    /* outer size, 1..2^30 */
   int ldw;                  /* a multiple of 8, >= n */
   int type;                 /* GG_INPUT_F16 or GG_INPUT_BF16: all 16-bit matrices */
   int activation;           /* GG_ACT_* (ReLU of a NaN is 0 and its gradient at 0 is 0, GELU in its tanh form) */
 } gg_gated_problem;
 #define GG_GATED_MAX_EXPERTS 1024
 
-/* One forward pass; capacity_rows rows are allocated. */
+/* One forward pass; capacity_rows rows (at most 2^31 - 65537) are allocated. h, gate and up do not overlap one another or x. */
 typedef struct gg_gated {
   const void* x;       /* rows x k, pitch ldx (a multiple of 8) */
   const int* rows;     /* `experts` counts in device memory; NULL with experts == 1: all capacity_rows rows */

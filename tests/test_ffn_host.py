@@ -48,7 +48,7 @@ def test_norms_out_of_range_are_refused(change):
 F8 = dict(experts=2, n=16, k=64, ldb=64, input_type=capi.GG_INPUT_E4M3, output_type=0, activation=0)
 
 
-@pytest.mark.parametrize("change", [dict(experts=0), dict(experts=1025), dict(n=0), dict(k=0), dict(k=-1), dict(ldb=63), dict(ldb=72), dict(ldb=48),
+@pytest.mark.parametrize("change", [dict(experts=0), dict(experts=1025), dict(n=0), dict(n=2 ** 30 + 1), dict(k=0), dict(k=-1), dict(k=2 ** 30 + 1, ldb=2 ** 30 + 16), dict(ldb=63), dict(ldb=72), dict(ldb=48),
                                     dict(input_type=0), dict(input_type=1), dict(input_type=4), dict(output_type=-1), dict(output_type=5),
                                     dict(output_type=capi.GG_OUTPUT_E4M3), dict(output_type=capi.GG_OUTPUT_E5M2), dict(activation=4),
                                     dict(activation=-1), dict(b=0), dict(b=PTR + 8), dict(b_scales=0), dict(up=0), dict(up=PTR + 1),
@@ -70,7 +70,7 @@ def test_f8_problems_out_of_range_are_refused(change):
 GATED = dict(experts=2, n=16, k=64, ldw=16, type=0, activation=0)
 
 
-@pytest.mark.parametrize("change", [dict(experts=0), dict(experts=1025), dict(n=0), dict(k=0), dict(ldw=15), dict(ldw=20), dict(type=2), dict(type=-1),
+@pytest.mark.parametrize("change", [dict(experts=0), dict(experts=1025), dict(n=0), dict(n=2 ** 30 + 1, ldw=2 ** 30 + 8), dict(k=0), dict(k=2 ** 30 + 1), dict(ldw=15), dict(ldw=20), dict(type=2), dict(type=-1),
                                     dict(activation=4), dict(activation=-1), dict(gate=0), dict(gate=PTR + 2), dict(up=0), dict(up=PTR + 8)])
 def test_gated_problems_out_of_range_are_refused(change):
     f = GATED | {n: v for n, v in change.items() if n in GATED}

@@ -149,6 +149,16 @@ def test_tile_widths(cuda, n, rows):
     c.check()
 
 
+@pytest.mark.parametrize("counts", [[513], [300, 724], [0, 1000, 257], [256, 512, 1, 255]])
+@pytest.mark.parametrize("n,k,out,gated", [(9472, 260, "bf16", False), (9477, 128, "f32", False), (4736, 700, "bf16", True), (4800, 390, "e4m3", True),
+                                           (4737, 1000, "e5m2", True)])
+def test_many_rows(cuda, counts, n, k, out, gated):
+    """Several tiles of rows of an expert, of the widest kind, and more of them than SMs."""
+    c = Case(counts, n, k, out=out, gated=gated, act="silu" if gated else "none", ldd=-(-n // 32) * 32 if out != "f32" else None)
+    assert c.run() == 0
+    c.check()
+
+
 @pytest.mark.parametrize("out", ["f32", "f16", "bf16", "e4m3", "e5m2"])
 @pytest.mark.parametrize("counts,n,k", [([5, 0, 130, 1, 64], 300, 384), ([1], 128, 128), ([40] * 8, 4736, 200), ([2] * 3, 1, 7), ([200], 127, 33)])
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
@@ -277,7 +287,7 @@ def test_refusals(cuda):
     lib = capi.load()
     call = lambda **f: lib.gg_f8_plan_run(c.plan._h, *[(dict(a=c.a.data_ptr(), lda=64, s=c.sa.data_ptr(), lds=3, rows=c.rows.data_ptr(), d=c.d.data_ptr(),  # noqa: E731
                                                              ldd=64, ds=None, ldds=0, cap=11) | f)[n] for n in ("a", "lda", "s", "lds", "rows", "d", "ldd", "ds", "ldds", "cap")], None)
-    for bad in (dict(a=None), dict(s=None), dict(d=None), dict(lda=48), dict(lds=0), dict(ldd=63), dict(cap=-1)):
+    for bad in (dict(a=None), dict(s=None), dict(d=None), dict(lda=48), dict(lds=0), dict(ldd=63), dict(cap=-1), dict(cap=2 ** 31 - 65536)):
         assert call(**bad) == invalid
     g = Case([4, 4], 64, 64, out="e4m3", gated=True, act="silu")
     with pytest.raises(ValueError):

@@ -277,9 +277,11 @@ def test_not_finite_stays_with_its_expert(cuda):
         assert torch.equal(c.gwg[e], clean[2][e]) and torch.equal(c.gwu[e], clean[3][e])
 
 
-def test_same_bits_captured_on_streams_and_with_new_counts(cuda):
+@pytest.mark.parametrize("counts,n,k", [([20, 30, 0, 77], 500, 200), ([700, 30, 0, 1400], 200, 300)])
+def test_same_bits_captured_on_streams_and_with_new_counts(cuda, counts, n, k):
     import torch
-    c = Case([20, 30, 0, 77], 500, 200)
+    c = Case(counts, n, k)
+    total = sum(counts)
     assert c.forward() == 0 and c.backward() == 0
     c.check_forward()
     c.check_backward()
@@ -291,7 +293,7 @@ def test_same_bits_captured_on_streams_and_with_new_counts(cuda):
         assert c.plan.run(c.x, c.rows, c.h, stream=streams[0]) == 0
         assert c.plan.run(c.x, c.rows, other, stream=streams[1]) == 0
     torch.cuda.synchronize()
-    assert torch.equal(c.h[:127], want[0][:127]) and torch.equal(other[:127], want[0][:127])
+    assert torch.equal(c.h[:total], want[0][:total]) and torch.equal(other[:total], want[0][:total])
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=streams[0]):
         st = torch.cuda.current_stream()
@@ -302,7 +304,7 @@ def test_same_bits_captured_on_streams_and_with_new_counts(cuda):
     torch.cuda.synchronize()
     for a, b in zip((c.h, c.gx, c.gwg, c.gwu), want):
         assert torch.equal(a, b)
-    c.counts = [60, 0, 60, 7]
+    c.counts, c.total = [60, 0, total - 67, 7], total
     c.rows.copy_(torch.tensor(c.counts, dtype=torch.int32))
     for t in (c.h, c.gx, c.gwg, c.gwu):
         t.fill_(7)

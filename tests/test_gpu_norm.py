@@ -127,7 +127,7 @@ def test_eight_bits(cuda, kind):
     x[3] *= 1e15
     x[4, 300] = float("inf")
     x[5, 10] = float("nan")
-    norm = gg.RmsNorm(width, eps=0.0 if False else 1e-6)
+    norm = gg.RmsNorm(width, eps=1e-6)
     q = torch.zeros(rows, width, device="cuda", dtype=dtypes()[kind])
     s, y = torch.zeros(rows, 5, device="cuda"), torch.zeros(rows, width, device="cuda")
     assert norm.run(x, y=y, q=q, scales=s) == 0
@@ -162,6 +162,11 @@ def test_optional_parts(cuda):
     assert norm.backward(x, None, rstd, gy, gx) == 0
     assert norm.backward(x, torch.ones(300, device="cuda"), rstd, gy, full, grad_weight=gw, grad_h=torch.zeros_like(x)) == 0
     assert torch.equal(gx, full)
+    h = torch.empty_like(x)
+    assert norm.run(x, residual_out=h) == 0 and torch.equal(h, x)  # no residual: x
+    q, s = torch.empty(9, 300, device="cuda", dtype=dtypes()["e5m2"]), torch.empty(9, 3, device="cuda")
+    assert norm.run(x, q=q, scales=s) == 0
+    check("q", q.double() * s.double().repeat_interleave(128, 1)[:, :300], want, want.abs() * (2.0 ** -3 + 1e-4) + 1e-6)
     none = torch.empty(0, 300, device="cuda")
     gw.fill_(3.0)
     assert norm.run(none, y=none) == 0
