@@ -6,12 +6,18 @@
 //   grad_weight = sum over rows of grad_y * xhat
 //
 // Memory bounds it: a row is read once, stays in registers through the sum over it, and is written once. A row
-// belongs to a team of 1 to 16 warps (more than one: a whole block), each of which holds a span of 256 of its values, 8 a thread, or
-// with wider rows than the block has warps for 2 to 8 spans. In a span a thread has 8 values in a piece where rows are
+// belongs to a team of 1 to 16 warps (more than one: a whole block), each of which holds 1 to 8 spans of 256 of its values, 8 of
+// each a thread (team_of). In a span a thread has 8 values in a piece where rows are
 // aligned (16 bytes of 16-bit values), so that 16 lanes hold a block of 128 columns, and else every 32nd of 256, so that a
 // warp's loads of single values are whole lines, and 4 of a lane's 8 are of one block. The teams that fit the GPU go through the rows,
-// and a team asks for its next row before it adds this one up. h is rounded to its type first and the norm is of
+// and a team asks for its next row before it adds this one up (asks_ahead). h is rounded to its type first and the norm is of
 // what is stored, as the gradient finds it.
+//
+// 16384 rows of 4096 in BF16, with the residual: forward 91 us, 5.9 TB/s; gradient with the residual's and the weight's 101 us,
+// 5.3 TB/s, 6 us of it the last sum over the blocks' parts. FP32: 170 us and 174, 6.3 and 6.2 TB/s. A copy has 6.55. Rows that are
+// not aligned to 16 bytes go value by value: 67041 rows of 1001 in BF16 182 us and 208. Wide rows hold fewer blocks an SM: 2048
+// rows of 32768 in BF16 154 us and 379 (the gradient keeps two rows and the weight's sums, 8 spans of each, and spills).
+// 4 rows of 4096 with 8-bit results: 5 us, a launch and the latency of one row.
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
@@ -32,8 +38,10 @@ namespace {
 constexpr int kSpan = 256;  // values that a warp takes in one piece
 
 constexpr int kMostWarps = 16;  // of a row, which leaves a thread 128 registers
-// Whether the next row's values fit beside this one's.
-__host__ __device__ constexpr bool asks_ahead(int spans) { return spans <= 2; }
+// Whether the next row's values fit beside this one's: 16384 wide rows of 16 bits take 192 us where they are not asked for ahead
+// and 96 where they are, of FP32, with 4 spans a warp, 187 and 241.
+__host__ __device__ constexpr bool asks_ahead(int type, int spans) { return spans <= (type == GG_OUTPUT_F32 ? 2 : 8); }
+__host__ __device__ constexpr bool gradient_asks_ahead(int spans) { return spans <= 2; }
 
 struct NormParams {
   const void* x;
@@ -95,38 +103,33 @@ struct Eight {
       }
     }
   }
+  __device__ __forceinline__ void store(void* base, int64_t at, int span, int lane, int width) const {
+    const int c0 = column<kVec>(span, lane, 0);
+    if (kVec && c0 + 8 <= width) {
+      uint4* p = reinterpret_cast<uint4*>(static_cast<char*>(base) + (at + c0) * OutFormat<F>::kBytes);
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) p[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = column<kVec>(span, lane, j);
+      if (c < width) {
+        if constexpr (F == kOutF32) static_cast<uint32_t*>(base)[at + c] = w[j];
+        else static_cast<unsigned short*>(base)[at + c] = static_cast<unsigned short>(w[j / 2] >> (16 * (j % 2)));
+      }
+    }
+  }
+  // Rounded to the type.
+  __device__ __forceinline__ void set(int pair, float x, float y) {
+    if constexpr (F == kOutF32) w[2 * pair] = __float_as_uint(x), w[2 * pair + 1] = __float_as_uint(y);
+    else w[pair] = pack2<F>(x, y);
+  }
   __device__ __forceinline__ float value(int j) const {
     if constexpr (F == kOutF32) return __uint_as_float(w[j]);
     else return widen16<F>(static_cast<unsigned short>(w[j / 2] >> (16 * (j % 2))));
   }
 };
-
-template <int F, bool kVec>
-__device__ __forceinline__ void store8(void* base, int64_t at, int span, int lane, int width, const float (&v)[8]) {
-  const int c0 = column<kVec>(span, lane, 0);
-  if (kVec && c0 + 8 <= width) {
-    char* p = static_cast<char*>(base) + (at + c0) * OutFormat<F>::kBytes;
-    if constexpr (F == kOutF32) {
-      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(p + 16) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      *reinterpret_cast<uint4*>(p) = make_uint4(pack2<F>(v[0], v[1]), pack2<F>(v[2], v[3]), pack2<F>(v[4], v[5]), pack2<F>(v[6], v[7]));
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int c = column<kVec>(span, lane, j);
-    if (c < width) store_out<F>(base, at + c, v[j]);
-  }
-}
-
-template <int F>
-__device__ __forceinline__ float rounded(float v) {
-  if constexpr (F == kOutF32) return v;
-  else if constexpr (F == kOutF16) return __half2float(__float2half_rn(v));
-  else return __bfloat162float(__float2bfloat16_rn(v));
-}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -202,7 +205,7 @@ __device__ __forceinline__ void store_8bit(const NormParams& p, int64_t row, int
 
 // F: type of the rows; W: of the weight; kSpans: spans that a warp holds; kVec: rows aligned.
 template <int F, int W, int kSpans, bool kVec>
-__global__ void __launch_bounds__(32 * kMostWarps) norm_kernel(const NormParams p, int warps) {
+__global__ void __launch_bounds__(32 * kMostWarps, kSpans == 1 ? 2 : 1) norm_kernel(const NormParams p, int warps) {
   __shared__ float sums[64];
   const int lane = threadIdx.x % 32;
   const Place at(warps);
@@ -217,23 +220,43 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_kernel(const NormParams 
       for (int i = 0; i < kSpans; ++i) r[i].load(p.residual, row * p.ldr, at.member + i * warps, lane, p.width);
     }
   };
-  if constexpr (asks_ahead(kSpans)) ask(at.row);
+  constexpr bool kAhead = asks_ahead(F, kSpans);
+  if constexpr (kAhead) ask(at.row);
   int turn = 0;
   for (int64_t row = at.row; row < p.rows; row += at.step, ++turn) {  // whole teams
-    if constexpr (!asks_ahead(kSpans)) ask(row);
-    float h[kSpans][8];
+    if constexpr (!kAhead) ask(row);
+    Eight<F, kVec> h[kSpans];
     float sum = 0.0f;
+    const auto account = [&](int i) {
+      if (p.residual_out) h[i].store(p.residual_out, row * p.ldro, at.member + i * warps, lane, p.width);
 #pragma unroll
-    for (int i = 0; i < kSpans; ++i)
+      for (int j = 0; j < 8; ++j) sum = fmaf(h[i].value(j), h[i].value(j), sum);
+    };
+    // Span by span where the values were asked for a row ago, which leaves the most room for the next row's (16384 wide rows of
+    // 16 bits: 95 us, and 132 as below). Values just asked for are all taken before the first branch, which would have each span
+    // wait for its own (FP32: 188 us, and 270 as above).
+    if constexpr (kAhead) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] = p.residual ? rounded<F>(x[i].value(j) + r[i].value(j)) : x[i].value(j);
+      for (int i = 0; i < kSpans; ++i) {
+        h[i] = x[i];
+        if (p.residual) {
 #pragma unroll
-    for (int i = 0; i < kSpans; ++i) {
-      if (p.residual_out) store8<F, kVec>(p.residual_out, row * p.ldro, at.member + i * warps, lane, p.width, h[i]);
+          for (int j = 0; j < 8; j += 2) h[i].set(j / 2, x[i].value(j) + r[i].value(j), x[i].value(j + 1) + r[i].value(j + 1));
+        }
+        account(i);
+      }
+    } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
+      for (int i = 0; i < kSpans; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          h[i].set(j / 2, p.residual ? x[i].value(j) + r[i].value(j) : x[i].value(j),
+                   p.residual ? x[i].value(j + 1) + r[i].value(j + 1) : x[i].value(j + 1));
+        }
+#pragma unroll
+      for (int i = 0; i < kSpans; ++i) account(i);
     }
-    if constexpr (asks_ahead(kSpans)) ask(row + at.step);
+    if constexpr (kAhead) ask(row + at.step);
     sum = team_sum(sum, warps, sums, turn);
     // both steps are correctly rounded
     const float rstd = __frcp_rn(__fsqrt_rn(sum / static_cast<float>(p.width) + p.eps));
@@ -248,12 +271,17 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_kernel(const NormParams 
         Eight<W, kVec> w;
         w.load(p.weight, 0, span, lane, p.width);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = h[i][j] * rstd * w.value(j);
+        for (int j = 0; j < 8; ++j) y[j] = h[i].value(j) * rstd * w.value(j);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = h[i][j] * rstd;
+        for (int j = 0; j < 8; ++j) y[j] = h[i].value(j) * rstd;
       }
-      if (p.y) store8<F, kVec>(p.y, row * p.ldy, span, lane, p.width, y);
+      if (p.y) {
+        Eight<F, kVec> out;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) out.set(j / 2, y[j], y[j + 1]);
+        out.store(p.y, row * p.ldy, span, lane, p.width);
+      }
       if (p.q) store_8bit<kVec>(p, row, span, lane, y);
     }
   }
@@ -271,6 +299,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, kSpans == 1 && F != kOutF32 ?
   for (int i = 0; i < kSpans; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) gw[i][j] = 0.0f;
+  constexpr bool kAhead = gradient_asks_ahead(kSpans);
   Eight<F, kVec> rh[kSpans], rg[kSpans], rp[kSpans];
   float rstd_next = 0.0f;
   const auto ask = [&](int64_t row) {
@@ -279,14 +308,14 @@ __global__ void __launch_bounds__(32 * kMostWarps, kSpans == 1 && F != kOutF32 ?
     for (int i = 0; i < kSpans; ++i) {
       rh[i].load(p.h, row * p.ldh, at.member + i * warps, lane, p.width);
       rg[i].load(p.grad_y, row * p.ldgy, at.member + i * warps, lane, p.width);
-      if (asks_ahead(kSpans) && p.grad_h) rp[i].load(p.grad_h, row * p.ldgh, at.member + i * warps, lane, p.width);
+      if (kAhead && p.grad_h) rp[i].load(p.grad_h, row * p.ldgh, at.member + i * warps, lane, p.width);
     }
     rstd_next = p.rstd[row];
   };
-  if constexpr (asks_ahead(kSpans)) ask(at.row);
+  if constexpr (kAhead) ask(at.row);
   int turn = 0;
   for (int64_t row = at.row; row < p.rows; row += at.step, ++turn) {
-    if constexpr (!asks_ahead(kSpans)) ask(row);
+    if constexpr (!kAhead) ask(row);
     const float rstd = rstd_next;
     float h[kSpans][8], g[kSpans][8];
     Eight<F, kVec> past[kSpans];
@@ -302,24 +331,27 @@ __global__ void __launch_bounds__(32 * kMostWarps, kSpans == 1 && F != kOutF32 ?
         g[i][j] = p.weight ? rg[i].value(j) * w.value(j) : rg[i].value(j);
         sum = fmaf(g[i][j], h[i][j], sum);
       }
-      if constexpr (asks_ahead(kSpans)) past[i] = rp[i];
+      if constexpr (kAhead) past[i] = rp[i];
     }
-    if constexpr (asks_ahead(kSpans)) ask(row + at.step);
+    if constexpr (kAhead) ask(row + at.step);
     const float mean = team_sum(sum, warps, sums, turn) / static_cast<float>(p.width);
 #pragma unroll
     for (int i = 0; i < kSpans; ++i) {
       const int span = at.member + i * warps;
-      if constexpr (!asks_ahead(kSpans)) {
+      if constexpr (!kAhead) {
         if (p.grad_h) past[i].load(p.grad_h, row * p.ldgh, span, lane, p.width);
       }
       float gx[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) gx[j] = fmaf(rstd, fmaf(-h[i][j], mean, g[i][j]), p.grad_h ? past[i].value(j) : 0.0f);
-      store8<F, kVec>(p.grad_x, row * p.ldgx, span, lane, p.width, gx);
+      Eight<F, kVec> out;
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) out.set(j / 2, gx[j], gx[j + 1]);
+      out.store(p.grad_x, row * p.ldgx, span, lane, p.width);
     }
   }
   if (!p.partial) return;
-  if (warps == 1) {  // a block of several teams: their sum, in order
+  if (warps == 1) {  // a block of several teams, each of which is one warp with one span (team_of): their sum, in order
     __shared__ float part[kMostWarps][kSpan];
 #pragma unroll
     for (int j = 0; j < 8; ++j) part[threadIdx.x / 32][column<kVec>(0, lane, j)] = gw[0][j];
@@ -357,14 +389,17 @@ __global__ void __launch_bounds__(32 * kSumWarps) norm_weight_sum_kernel(const f
   if (lane == 0 && blockIdx.x * 32 + warp < width) out[blockIdx.x * 32 + warp] = s;
 }
 
-// The warps that hold a row, the spans that each of them does (as few as the warps allow: 16384 rows of 4096 in BF16 take 101,
-// 111 and 118 us with 1, 2 and 4, and the gradient 142, 218 and 249), and the threads of a block.
+// The warps that hold a row, the spans that each of them does, and the threads of a block. Rows of FP32: as few spans as the warps
+// allow (16384 rows of 4096: 170 us with 1 and 188 with 2, the gradient 174 and 191). Of 16 bits: 1 as long as the warps allow
+// (91 us with 1, 100 with 2), then 4 (8192 rows of 8192: 102 us with 2, 95 with 4; 13421 of 5000: 150 and 109, since a block of 10
+// warps leaves no room for a second); the gradient 2 from 4 spans on (16384 rows of 4096: 123 us with 1, 101 with 2).
 struct Team {
   int warps, spans, threads;
 };
-Team team_of(int width, bool gradient) {
+Team team_of(int width, int type, bool gradient) {
   const int spans = (width - 1) / kSpan + 1;
   int each = 1;
+  if (type != GG_OUTPUT_F32) each = gradient ? (spans >= 4 ? 2 : 1) : (spans > kMostWarps ? 4 : 1);
   while ((spans + each - 1) / each > kMostWarps) each *= 2;
   const int warps = (spans + each - 1) / each;
   return {warps, each, 32 * (warps > 1 ? warps : gradient ? 16 : 4)};
@@ -426,8 +461,8 @@ int gg_norm_create(const gg_norm_config* config, gg_norm_plan** out) {
   cudaError_t st = cudaGetDevice(&plan->device);
   int sms = 0;
   if (st == cudaSuccess) st = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, plan->device);
-  plan->team = gg::team_of(config->width, false);
-  plan->gradient_team = gg::team_of(config->width, true);
+  plan->team = gg::team_of(config->width, config->type, false);
+  plan->gradient_team = gg::team_of(config->width, config->type, true);
   gg::with_types(config->type, config->weight_type, [&](auto f, auto wt) {
     for (int vec = 0; vec < 2; ++vec) {
       const auto count = [&](auto kernel, int threads, int* blocks) {
