@@ -13,8 +13,8 @@
 // and a team asks for its next row before it adds this one up (asks_ahead). h is rounded to its type first and the norm is of
 // what is stored, as the gradient finds it.
 //
-// 16384 rows of 4096 in BF16, with the residual: forward 91 us, 5.9 TB/s; gradient with the residual's and the weight's 101 us,
-// 5.3 TB/s, 6 us of it the last sum over the blocks' parts. FP32: 170 us and 174, 6.3 and 6.2 TB/s. A copy has 6.55. Rows that are
+// 16384 rows of 4096 in BF16, with the residual: forward 93 us, 5.8 TB/s; gradient with the residual's and the weight's 101 us,
+// 5.3 TB/s, 6 us of it the last sum over the blocks' parts. FP32: 166 us and 174, 6.5 and 6.2 TB/s. 32768 rows into 16 and 8 bits: 230 us, 5.3. A copy has 6.55. Rows that are
 // not aligned to 16 bytes go value by value: 67041 rows of 1001 in BF16 182 us and 208. Wide rows hold fewer blocks an SM: 2048
 // rows of 32768 in BF16 154 us and 379 (the gradient keeps two rows and the weight's sums, 8 spans of each, and spills).
 // 4 rows of 4096 with 8-bit results: 5 us, a launch and the latency of one row.
@@ -39,7 +39,7 @@ constexpr int kSpan = 256;  // values that a warp takes in one piece
 
 constexpr int kMostWarps = 16;  // of a row, which leaves a thread 128 registers
 // Whether the next row's values fit beside this one's: 16384 wide rows of 16 bits take 192 us where they are not asked for ahead
-// and 96 where they are, of FP32, with 4 spans a warp, 187 and 241.
+// and 96 where they are; of FP32, with 4 spans a warp, a quarter more than where they are not.
 __host__ __device__ constexpr bool asks_ahead(int type, int spans) { return spans <= (type == GG_OUTPUT_F32 ? 2 : 8); }
 __host__ __device__ constexpr bool gradient_asks_ahead(int spans) { return spans <= 2; }
 
@@ -54,7 +54,7 @@ struct NormParams {
   float* rstd;
   int64_t ldx, ldr, ldro, ldy, ldq, lds;
   int rows, width;
-  float eps, largest;  // largest: of the 8-bit type
+  float eps;
   bool e5m2;
 };
 
@@ -161,19 +161,19 @@ struct Place {
   }
 };
 
-// y in 8 bits: a span's part of this lane.
+// y = t * factor in 8 bits: a span's part of this lane.
 template <bool kVec>
-__device__ __forceinline__ void store_8bit(const NormParams& p, int64_t row, int span, int lane, const float (&y)[8]) {
+__device__ __forceinline__ void store_8bit(const NormParams& p, int64_t row, int span, int lane, const float (&t)[8], float factor) {
   if constexpr (kVec) {
     const int c0 = column<kVec>(span, lane, 0);
     uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, magnitude(y[j]));
+    for (int j = 0; j < 8; ++j) top = max(top, magnitude(t[j]));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const Scale8 s(top, p.largest);
-    if (lane % 16 == 0 && c0 < p.width) p.scales[row * p.lds + c0 / GG_SCALE_BLOCK] = s.scale;
-    const uint2 b = make_uint2(s.four(y[0], y[1], y[2], y[3], p.e5m2), s.four(y[4], y[5], y[6], y[7], p.e5m2));
+    const ExactScale8 s(top, factor, p.e5m2);
+    if (lane % 16 == 0 && c0 < p.width) p.scales[row * p.lds + c0 / GG_SCALE_BLOCK] = s.scale(factor, p.e5m2);
+    const uint2 b = make_uint2(s.four(t[0], t[1], t[2], t[3], p.e5m2), s.four(t[4], t[5], t[6], t[7], p.e5m2));
     unsigned char* q = p.q + row * p.ldq + c0;
     if (c0 + 8 <= p.width) {
       *reinterpret_cast<uint2*>(q) = b;
@@ -187,13 +187,13 @@ __device__ __forceinline__ void store_8bit(const NormParams& p, int64_t row, int
     for (int half = 0; half < 2; ++half) {
       uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) top = max(top, magnitude(y[4 * half + j]));
+      for (int j = 0; j < 4; ++j) top = max(top, magnitude(t[4 * half + j]));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const Scale8 s(top, p.largest);
+      const ExactScale8 s(top, factor, p.e5m2);
       const int b0 = span * kSpan + half * GG_SCALE_BLOCK;
-      if (lane == 0 && b0 < p.width) p.scales[row * p.lds + b0 / GG_SCALE_BLOCK] = s.scale;
-      const uint32_t b = s.four(y[4 * half], y[4 * half + 1], y[4 * half + 2], y[4 * half + 3], p.e5m2);
+      if (lane == 0 && b0 < p.width) p.scales[row * p.lds + b0 / GG_SCALE_BLOCK] = s.scale(factor, p.e5m2);
+      const uint32_t b = s.four(t[4 * half], t[4 * half + 1], t[4 * half + 2], t[4 * half + 3], p.e5m2);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int c = b0 + j * 32 + lane;
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, kSpans == 1 ? 2 : 1) norm_ker
     };
     // Span by span where the values were asked for a row ago, which leaves the most room for the next row's (16384 wide rows of
     // 16 bits: 95 us, and 132 as below). Values just asked for are all taken before the first branch, which would have each span
-    // wait for its own (FP32: 188 us, and 270 as above).
+    // wait for its own (FP32: 188 us then, and 270 as above).
     if constexpr (kAhead) {
 #pragma unroll
       for (int i = 0; i < kSpans; ++i) {
@@ -262,27 +262,34 @@ __global__ void __launch_bounds__(32 * kMostWarps, kSpans == 1 ? 2 : 1) norm_ker
     const float rstd = __frcp_rn(__fsqrt_rn(sum / static_cast<float>(p.width) + p.eps));
     if (p.rstd && at.member == 0 && lane == 0) p.rstd[row] = rstd;
     if (!p.y && !p.q) continue;
+    // For 8 bits rstd = power * factor, a power of two and a number from 2 to 4: h * power * weight is exact with 16-bit rows and
+    // weights, and stays below y.
+    float factor = 1.0f, power = rstd;
+    if (p.q) {
+      factor = __uint_as_float((__float_as_uint(rstd) & 0x007fffffu) | 0x40000000u);
+      if (rstd == rstd) power = 0.5f * __uint_as_float(__float_as_uint(rstd) & 0x7f800000u);
+    }
 #pragma unroll
     for (int i = 0; i < kSpans; ++i) {
       const int span = at.member + i * warps;
       if (span * kSpan >= p.width) break;
-      float y[8];
+      float t[8];  // y over `factor`
       if (p.weight) {
         Eight<W, kVec> w;
         w.load(p.weight, 0, span, lane, p.width);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = h[i].value(j) * rstd * w.value(j);
+        for (int j = 0; j < 8; ++j) t[j] = h[i].value(j) * power * w.value(j);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = h[i].value(j) * rstd;
+        for (int j = 0; j < 8; ++j) t[j] = h[i].value(j) * power;
       }
       if (p.y) {
         Eight<F, kVec> out;
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) out.set(j / 2, y[j], y[j + 1]);
+        for (int j = 0; j < 8; j += 2) out.set(j / 2, t[j] * factor, t[j + 1] * factor);
         out.store(p.y, row * p.ldy, span, lane, p.width);
       }
-      if (p.q) store_8bit<kVec>(p, row, span, lane, y);
+      if (p.q) store_8bit<kVec>(p, row, span, lane, t, factor);
     }
   }
 }
@@ -506,7 +513,6 @@ int gg_norm_run(const gg_norm_plan* plan, const gg_norm* call, void* stream) {
   p.ldx = q.ldx, p.ldr = q.ldr, p.ldro = q.ldro, p.ldy = q.ldy, p.ldq = q.ldq, p.lds = q.lds;
   p.rows = q.rows, p.width = w, p.eps = plan->config.eps;
   p.e5m2 = q.q_type == GG_OUTPUT_E5M2;
-  p.largest = p.e5m2 ? 57344.0f : 448.0f;
   const bool vec = gg::rows_on(q.x, q.ldx, b, 16) && gg::rows_on(q.residual, q.ldr, b, 16) && gg::rows_on(q.residual_out, q.ldro, b, 16) &&
                    gg::rows_on(q.y, q.ldy, b, 16) && gg::rows_on(q.q, q.ldq, 1, 8) && gg::rows_on(q.weight, 0, 1, 16);
   const gg::Team& t = plan->team;

@@ -546,7 +546,8 @@ void gg_q4_plan_destroy(gg_q4_plan* plan);
  *   rstd(r) = 1 / sqrt(mean over c of h(r, c)^2 + eps)
  *   y(r, c) = h(r, c) * rstd(r) * weight(c)
  *   8 bits: scale(r, b) = the largest |y| of columns 128 b to 128 b + 127, over the largest finite number of the
- *   type (448 or 57344); q = y times the inverse of scale(r, b), rounded to nearest even; y is not rounded in between. A
+ *   type (448 or 57344); q = y over scale(r, b), rounded to nearest even; y is not rounded in between. With x and weight in
+ *   BF16 every q is the nearest one to the exact quotient, ties to even; with others a tie can go to either side. A
  *   block whose largest |y| is below 2^-100 has scale 0 and q 0; one that holds an infinity or a NaN has a scale that is
  *   not finite.
  * Everything but what is stored is FP32, the sum of a row's squares too: past 3.4e38 rstd is 0. The sums are taken in a fixed

@@ -145,6 +145,28 @@ def test_eight_bits(cuda, kind):
     assert not bool(torch.isfinite(s[4, 2])) and not bool(torch.isfinite(s[5]).any())
 
 
+@pytest.mark.parametrize("kind", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("width,aligned", [(4096, True), (1000, True), (387, False)])
+def test_eight_bits_of_ties(cuda, kind, width, aligned):
+    """With rows and weights in BF16 every 8-bit value is the nearest one, ties to even: rstd falls out of y over the block's
+    largest, which leaves a quotient 7 a / b times a power of two, a and b whole numbers below 2^16. One that is no tie is at least
+    1 / (b c) away from the tie c, of 5 bits, relative to it: 2^-21, and the kernel's quotient is within 2^-23, the 64-bit one's
+    rounding to FP32, which restores ties, within 2^-24."""
+    import torch
+    gen = torch.Generator("cuda").manual_seed(width)
+    rows = 300
+    x = torch.randn(rows, width + (0 if aligned else 2), device="cuda", generator=gen).bfloat16()[:, :width]
+    w = (1 + 0.1 * torch.randn(width, device="cuda", generator=gen)).bfloat16()
+    norm = gg.RmsNorm(width, dtype=gg.OutputType.kBF16)
+    q = torch.empty(rows, width, device="cuda", dtype=dtypes()[kind])
+    s = torch.empty(rows, -(-width // 128), device="cuda")
+    assert norm.run(x, w, q=q, scales=s) == 0
+    t = torch.nn.functional.pad(x.double() * w.double(), (0, -width % 128)).view(rows, -1, 128)
+    top = 448.0 if kind == "e4m3" else 57344.0
+    want = (t * top / t.abs().amax(2, keepdim=True)).float().to(dtypes()[kind]).view(rows, -1)[:, :width]
+    assert torch.equal(q.float(), want.float())
+
+
 def test_optional_parts(cuda):
     """Without weight, residual and 8 bits; without the gradients that are not asked for; no rows at all."""
     import torch
