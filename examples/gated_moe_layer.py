@@ -6,7 +6,7 @@ weights that have a scale for each block of 128.
 Training runs norm -> router -> dispatch -> gated block (GatedPlan) -> way down (MoePlan) -> combine, and back. Row counts
 stay on the device but for the gradient of Wd, whose inner dimension they are. Serving runs norm (rows in 16 bits for the router
 and in 8 for the experts) -> router -> dispatch of rows and scales -> gated 8-bit product, into 8 bits -> 8-bit product
--> combine: eight launches a step.
+-> combine: eight launches a step beside the logits' product, all on one stream, so that a step can be captured in a graph.
 
     python examples/gated_moe_layer.py
 """
@@ -140,21 +140,26 @@ class GatedMoeServer:
         self.down = gg.F8Plan(experts, hidden, inner, _ptrs(qd), inner, _ptrs(sd))
         self.h, self.n, self.q, self.s = b16(tokens, hidden), b16(tokens, hidden), e4m3(tokens, hidden), f32(tokens, blocks(hidden))
         self.indices, self.positions, self.rows = i32(tokens, top_k), i32(tokens, top_k), i32(experts)
-        self.weights, self.losses = f32(tokens, top_k), f32(3)
+        self.weights, self.losses, self.logits = f32(tokens, top_k), f32(3), f32(tokens, experts)
         self.packed, self.packed_s = e4m3(rows, hidden), f32(rows, blocks(hidden))
         self.mid, self.mid_s, self.out = e4m3(rows, inner), f32(rows, blocks(inner)), b16(rows, hidden)
 
     def step(self, x, residual, logits=None, y=None, stream=None):
-        """(tokens, hidden) BF16 -> (h, y). logits: where a captured step finds them (None: computed here)."""
-        _done(self.norm.run(x, self.norm_weight, y=self.n, residual=residual, residual_out=self.h, q=self.q, scales=self.s, stream=stream))
-        logits = self.n.float() @ self.gate.t() if logits is None else logits
-        _done(self.router.run(logits, self.indices, self.weights, self.positions, self.rows, self.losses, stream=stream))
-        _done(gg.moe_dispatch(self.q, self.positions, self.packed, stream))
-        _done(gg.moe_dispatch(self.s, self.positions, self.packed_s, stream))
-        _done(self.gate_up.run(self.packed, self.packed_s, self.rows, self.mid, d_scales=self.mid_s, stream=stream))
-        _done(self.down.run(self.mid, self.mid_s, self.rows, self.out, stream=stream))
-        y = torch.empty_like(x) if y is None else y
-        _done(gg.moe_combine(self.out, self.positions, y, self.weights, stream))
+        """(tokens, hidden) BF16 -> (h, y). logits: (tokens, experts) FP32, where the step puts the router's logits (None: a buffer of
+        the server's); y: where it puts y. stream: a torch stream (None: torch's current one). Everything runs on it, the
+        logits' product too, so that a captured step routes what its inputs hold when it is replayed."""
+        stream = torch.cuda.current_stream() if stream is None else stream
+        with torch.cuda.stream(stream):
+            logits = self.logits if logits is None else logits
+            _done(self.norm.run(x, self.norm_weight, y=self.n, residual=residual, residual_out=self.h, q=self.q, scales=self.s, stream=stream))
+            torch.mm(self.n.float(), self.gate.t(), out=logits)
+            _done(self.router.run(logits, self.indices, self.weights, self.positions, self.rows, self.losses, stream=stream))
+            _done(gg.moe_dispatch(self.q, self.positions, self.packed, stream))
+            _done(gg.moe_dispatch(self.s, self.positions, self.packed_s, stream))
+            _done(self.gate_up.run(self.packed, self.packed_s, self.rows, self.mid, d_scales=self.mid_s, stream=stream))
+            _done(self.down.run(self.mid, self.mid_s, self.rows, self.out, stream=stream))
+            y = torch.empty_like(x) if y is None else y
+            _done(gg.moe_combine(self.out, self.positions, y, self.weights, stream))
         return self.h, y
 
 

@@ -99,3 +99,53 @@ def test_serving_step(cuda, module, tokens, hidden, inner):
     assert torch.equal(out, first)
     assert server.gate_up.status() == 0 and server.down.status() == 0
     del graph
+
+
+@pytest.mark.parametrize("tokens,hidden,inner", [(1, 256, 512), (64, 1024, 640)])
+def test_captured_serving_step_routes_its_own_rows(cuda, module, tokens, hidden, inner):
+    """A captured step, replayed on rows that it was not captured with, gives what a step on them gives, bit for bit: the logits are
+    those of the rows of the replay. With logits of the server's and with the caller's."""
+    import torch
+    w = module.weights(8, hidden, inner, seed=5)
+    server = module.GatedMoeServer(*w, top_k=2, tokens=tokens)
+    g = torch.Generator(device=cuda).manual_seed(tokens)
+    make = lambda: torch.randn(tokens, hidden, device=cuda, generator=g).bfloat16()  # noqa: E731
+    x, r, out = make(), make(), torch.zeros(tokens, hidden, device=cuda, dtype=torch.bfloat16)
+    for logits in (None, torch.full((tokens, 8), float("nan"), device=cuda)):
+        s, graph = torch.cuda.Stream(cuda), torch.cuda.CUDAGraph()
+        server.step(x, r)  # what a first call sets up
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=s):
+            server.step(x, r, logits=logits, y=out, stream=torch.cuda.current_stream())
+        for _ in range(3):
+            x.copy_(make()), r.copy_(make())
+            h, y = server.step(x, r)
+            h, y, indices, kept = h.clone(), y.clone(), server.indices.clone(), server.logits.clone()
+            for t in (server.h, server.n, server.out, server.mid_s, server.packed_s, server.logits):
+                t.fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(server.logits if logits is None else logits, kept) and torch.equal(server.indices, indices)
+            assert torch.equal(server.h, h) and torch.equal(out, y)
+        del graph
+    assert server.gate_up.status() == 0 and server.down.status() == 0
+
+
+def test_serving_step_on_a_stream(cuda, module):
+    """Without logits from outside, on a stream that is neither torch's current one nor the default, behind work that takes a while:
+    the same bits as on the default stream."""
+    import torch
+    server = module.GatedMoeServer(*module.weights(8, 256, 512, seed=6), top_k=2, tokens=16)
+    g = torch.Generator(device=cuda).manual_seed(6)
+    x, r = [torch.randn(16, 256, device=cuda, generator=g).bfloat16() for _ in range(2)]
+    h, y = [t.clone() for t in server.step(x, r)]
+    late_x, late_r = torch.zeros_like(x), torch.zeros_like(r)
+    server.step(late_x, late_r)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream(cuda)
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(50_000_000)
+        late_x.copy_(x), late_r.copy_(r)
+    got = server.step(late_x, late_r, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], h) and torch.equal(got[1], y)
