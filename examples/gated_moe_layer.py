@@ -30,6 +30,11 @@ def _done(status: int) -> None:
         raise RuntimeError(f"status {status}")
 
 
+def _stream():
+    """The stream that torch's own operations between the calls run on."""
+    return torch.cuda.current_stream()
+
+
 def _ptrs(t):
     return [x.data_ptr() for x in t]
 
@@ -66,32 +71,32 @@ class GatedMoeLayer:
 
     def forward(self, x, residual):
         """(tokens, hidden) BF16 -> (h, y)"""
-        _done(self.norm.run(x, self.norm_weight, y=self.n, residual=residual, residual_out=self.h, rstd=self.rstd))
+        _done(self.norm.run(x, self.norm_weight, y=self.n, residual=residual, residual_out=self.h, rstd=self.rstd, stream=_stream()))
         self.logits = self.n.float() @ self.gate.t()
-        _done(self.router.run(self.logits, self.indices, self.weights, self.positions, self.rows, self.losses, lse=self.lse))
-        _done(gg.moe_dispatch(self.n, self.positions, self.packed))
-        _done(self.block.run(self.packed, self.rows, self.mid, gate=self.gate_out, up=self.up_out))
-        _done(self.down.run(self.rows))
+        _done(self.router.run(self.logits, self.indices, self.weights, self.positions, self.rows, self.losses, lse=self.lse, stream=_stream()))
+        _done(gg.moe_dispatch(self.n, self.positions, self.packed, stream=_stream()))
+        _done(self.block.run(self.packed, self.rows, self.mid, gate=self.gate_out, up=self.up_out, stream=_stream()))
+        _done(self.down.run(self.rows, stream=_stream()))
         y = torch.empty_like(x)
-        _done(gg.moe_combine(self.out, self.positions, y, self.weights))
+        _done(gg.moe_combine(self.out, self.positions, y, self.weights, stream=_stream()))
         return self.h, y
 
     def backward(self, grad_h, grad_y):
         """Gradients (x, norm weight, gate, wg, wu, wd) of <grad_h, h> + <grad_y, y> + balance * losses[0] + z * losses[1]; the
         residual's is x's."""
-        _done(gg.moe_combine_backward(grad_y, self.out, self.positions, self.weights, self.out, self.grad_weights))
-        _done(self.down_back.run(self.rows))
+        _done(gg.moe_combine_backward(grad_y, self.out, self.positions, self.weights, self.out, self.grad_weights, stream=_stream()))
+        _done(self.down_back.run(self.rows, stream=_stream()))
         grad_wg, grad_wu = torch.empty_like(self.wg), torch.empty_like(self.wu)
         # grad_gate and grad_up take the places of gate and up
         _done(self.block.backward(self.packed, self.gate_out, self.up_out, self.grad_mid, self.rows, self.gate_out, self.up_out,
-                                  grad_x=self.grad_packed, grad_gate_w=grad_wg, grad_up_w=grad_wu))
+                                  grad_x=self.grad_packed, grad_gate_w=grad_wg, grad_up_w=grad_wu, stream=_stream()))
         _done(self.router.backward(self.logits, self.indices, self.weights, self.rows, self.losses, self.lse, self.grad_weights,
-                                   self.grad_losses, self.grad_logits))
+                                   self.grad_losses, self.grad_logits, stream=_stream()))
         grad_n = torch.empty_like(self.n)
-        _done(gg.moe_combine(self.grad_packed, self.positions, grad_n))
+        _done(gg.moe_combine(self.grad_packed, self.positions, grad_n, stream=_stream()))
         grad_n = (grad_n.float() + self.grad_logits @ self.gate).bfloat16()
         grad_x, grad_norm = torch.empty_like(self.h), torch.empty(self.hidden, device=self.h.device)
-        _done(self.norm.backward(self.h, self.norm_weight, self.rstd, grad_n, grad_x, grad_weight=grad_norm, grad_h=grad_h))
+        _done(self.norm.backward(self.h, self.norm_weight, self.rstd, grad_n, grad_x, grad_weight=grad_norm, grad_h=grad_h, stream=_stream()))
         return grad_x, grad_norm, self.grad_logits.t() @ self.n.float(), grad_wg, grad_wu, self._down_gradient()
 
     def _down_gradient(self):
@@ -104,7 +109,7 @@ class GatedMoeLayer:
                                                d[e].data_ptr(), self.inner, self.hidden, self.hidden, self.hidden))
             at += r
         cfg = gg.KernelConfig(128, 128, 64, input_type=gg.InputType.kBF16, a_layout=gg.Layout.kColMajor)
-        _done(gg.run_grouped_gemm_once(problems, gg.SortMode.kByTiles, cfg))
+        _done(gg.run_grouped_gemm_once(problems, gg.SortMode.kByTiles, cfg, stream=_stream()))
         return d
 
 
@@ -148,7 +153,7 @@ class GatedMoeServer:
         """(tokens, hidden) BF16 -> (h, y). logits: (tokens, experts) FP32, where the step puts the router's logits (None: a buffer of
         the server's); y: where it puts y. stream: a torch stream (None: torch's current one). Everything runs on it, the
         logits' product too, so that a captured step routes what its inputs hold when it is replayed."""
-        stream = torch.cuda.current_stream() if stream is None else stream
+        stream = _stream() if stream is None else stream
         with torch.cuda.stream(stream):
             logits = self.logits if logits is None else logits
             _done(self.norm.run(x, self.norm_weight, y=self.n, residual=residual, residual_out=self.h, q=self.q, scales=self.s, stream=stream))

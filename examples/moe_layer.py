@@ -27,6 +27,11 @@ def _done(status: int) -> None:
         raise RuntimeError(f"status {status}")
 
 
+def _stream():
+    """The stream that torch's own operations between the calls run on."""
+    return torch.cuda.current_stream()
+
+
 class MoeLayer:
     """FP16 experts up (experts, hidden, inner) and down (experts, inner, hidden), FP32 gate (experts, hidden)."""
 
@@ -60,25 +65,25 @@ class MoeLayer:
         """x (tokens, hidden) FP16 -> y; mask: tokens to leave out (0)."""
         self.x, self.logits = x, x.float() @ self.gate.t()
         _done(self.router.run(self.logits, self.indices, self.weights, self.positions, self.rows, self.losses, lse=self.lse,
-                              prob_mean=self.prob_mean, token_mask=mask))
-        _done(gg.moe_dispatch(x, self.positions, self.packed))
-        _done(self.up_plan.run(self.rows))
-        _done(self.down_plan.run(self.rows))
+                              prob_mean=self.prob_mean, token_mask=mask, stream=_stream()))
+        _done(gg.moe_dispatch(x, self.positions, self.packed, stream=_stream()))
+        _done(self.up_plan.run(self.rows, stream=_stream()))
+        _done(self.down_plan.run(self.rows, stream=_stream()))
         y = torch.empty_like(x)
-        _done(gg.moe_combine(self.out, self.positions, y, self.weights))
+        _done(gg.moe_combine(self.out, self.positions, y, self.weights, stream=_stream()))
         return y
 
     def backward(self, grad_y):
         """Gradients (x, gate, up, down) of <grad_y, y> + balance * losses[0] + z * losses[1]."""
         # the gradient of the experts' rows takes the place of their values
-        _done(gg.moe_combine_backward(grad_y, self.out, self.positions, self.weights, self.out, self.grad_weights))
-        _done(self.down_back.run(self.rows))
+        _done(gg.moe_combine_backward(grad_y, self.out, self.positions, self.weights, self.out, self.grad_weights, stream=_stream()))
+        _done(self.down_back.run(self.rows, stream=_stream()))
         self.grad_h.mul_(self.h > 0)
-        _done(self.up_back.run(self.rows))
+        _done(self.up_back.run(self.rows, stream=_stream()))
         _done(self.router.backward(self.logits, self.indices, self.weights, self.rows, self.losses, self.lse, self.grad_weights,
-                                   self.grad_losses, self.grad_logits))
+                                   self.grad_losses, self.grad_logits, stream=_stream()))
         grad_x = torch.empty_like(self.x)
-        _done(gg.moe_combine(self.grad_packed, self.positions, grad_x))
+        _done(gg.moe_combine(self.grad_packed, self.positions, grad_x, stream=_stream()))
         grad_x = (grad_x.float() + self.grad_logits @ self.gate).half()
         counts = self.rows.tolist()
         return (grad_x, self.grad_logits.t() @ self.x.float(), self._weight_gradient(self.packed, self.grad_h, counts),
@@ -94,7 +99,7 @@ class MoeLayer:
                                                d[e].data_ptr(), a.shape[1], g.shape[1], g.shape[1], g.shape[1]))
             at += r
         cfg = gg.KernelConfig(128, 128, 64, a_layout=gg.Layout.kColMajor)
-        _done(gg.run_grouped_gemm_once(problems, gg.SortMode.kByTiles, cfg))
+        _done(gg.run_grouped_gemm_once(problems, gg.SortMode.kByTiles, cfg, stream=_stream()))
         return d
 
 
@@ -128,11 +133,11 @@ class MoeDecoder:
 
     def step(self, x):
         logits = x.float() @ self.gate.t()
-        _done(self.router.run(logits, self.indices, self.weights, self.positions, self.rows, self.losses, row_tokens=self.row_tokens))
-        _done(self.plans[0].run(x, self.rows, self.h, row_tokens=self.row_tokens))
-        _done(self.plans[1].run(self.h, self.rows, self.out))
+        _done(self.router.run(logits, self.indices, self.weights, self.positions, self.rows, self.losses, row_tokens=self.row_tokens, stream=_stream()))
+        _done(self.plans[0].run(x, self.rows, self.h, row_tokens=self.row_tokens, stream=_stream()))
+        _done(self.plans[1].run(self.h, self.rows, self.out, stream=_stream()))
         y = torch.empty_like(x)
-        _done(gg.moe_combine(self.out, self.positions, y, self.weights))
+        _done(gg.moe_combine(self.out, self.positions, y, self.weights, stream=_stream()))
         return y
 
 
