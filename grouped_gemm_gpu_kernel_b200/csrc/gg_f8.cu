@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
         most = max(most, __float_as_uint(top[done & 1u][half ^ 1][row]));
         if (mine) {
           const bool e5m2 = p.output_type == GG_OUTPUT_E5M2;
-          const Scale8 s(most, e5m2 ? 57344.0f : 448.0f);
+          const Scale8 s(most, e5m2);
           if (half == 0 && row < x.rows) p.d_scales[static_cast<int64_t>(x.row + row) * p.ldds + x.n] = s.scale;
           const auto put = [&](auto kind) {
             uint32_t w[kMine / 4];

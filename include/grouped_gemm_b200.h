@@ -613,7 +613,7 @@ void gg_norm_destroy(gg_norm_plan* plan);
  * with U the same product with a second matrix of weights. Rows are packed as in gg_moe_plan_run (expert 0's rows
  * first) with the counts in device memory. The products are exact, their sums and the scales' products FP32; D is rounded
  * once, in the gated form also to 8 bits with a scale for each row and 128 outputs, by the rule of gg_norm_run: the
- * rows of the next product. With experts = 1 and no counts it is a plain matrix product. */
+ * rows of the next product (every 8-bit value is the nearest one to the quotient as FP32 holds it, ties to even). With experts = 1 and no counts it is a plain matrix product. */
 typedef struct gg_f8_problem {
   const void* const* b;             /* host array of `experts` device pointers: n rows of k bytes, pitch ldb, 16-byte aligned */
   const float* const* b_scales;     /* host array of device pointers: ceil(n / 128) x ceil(k / 128), packed */
