@@ -46,7 +46,7 @@ constexpr Layout layout(int stage_bytes, int experts, int bars, int own = 0) {
   l.table = l.own + own;
   l.bars = (l.table + 2 * (experts + 1) * 4 + 7) / 8 * 8;
   l.words = l.bars + 8 * bars;
-  l.bytes = l.words + 16 + 1024;  // slack: stages start on 1024 bytes
+  l.bytes = l.words + 16 + 1024;  // words: tensor memory's address, the abort flag, two of progress; slack: stages start on 1024 bytes
   return l;
 }
 

@@ -99,6 +99,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
   const auto cut = [&](int s) { return bar0 + 8u * (2 * kStages + 2 * kAcc + 1 + s); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + l.words);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + l.words + 4);
+  // Stages that each loading warp has asked for. Who waits for a whole tile, or for several, waits as long as these go on.
+  volatile uint32_t* progress = reinterpret_cast<volatile uint32_t*>(smem + l.words + 8);
 
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   const int rank = kPair ? static_cast<int>(ptx::cluster_ctarank()) : 0;
@@ -108,6 +110,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
     for (int b = 0; b < kAcc; ++b) ptx::mbar_init(ready(b), 1), ptx::mbar_init(taken(b), (kPair ? 2 : 1) * kEpilogueWarps);
     ptx::mbar_init(drained, 1);
     *abort_flag = 0;
+    progress[0] = progress[1] = 0;
     ptx::fence_mbar_init();
   }
   if constexpr (kPair) ptx::cluster_sync();  // the barriers are there before the other CTA uses them
@@ -164,6 +167,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
     Ring<kStages, 2> stage;
     stage.at = warp - kLoadWarp;
     int skip = stage.at;  // stages of 64 until this warp's next
+    uint32_t asked = 0;
     bool ok = true;
     for (int t = block; ok && t < total; t += grid) {
       const Tile x = tile_at(t);
@@ -213,6 +217,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
               load(b + i * kChunkBytes, &p.in[1 + (kPair ? rank : i / 2)], x.n * kWidth + i % 2 * kDepth, at);
           }
           if (kPair && !clear && rank != 0) ptx::mbar_arrive_cluster_relaxed(counted);  // counts; the bytes are tracked by themselves
+          progress[warp - kLoadWarp] = ++asked;
         }
         __syncwarp();
         stage.next();
@@ -228,7 +233,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
       it += static_cast<uint32_t>(x.depth);
       if (x.depth == 0 || !is_cut(x, x.depth - 1)) continue;
       const int at = static_cast<int>((it - 1) % kStages);
-      ok = __all_sync(0xffffffffu, wait_phase_inline(cut(at), turns >> at & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER));
+      // through all the tiles without a cut before this one
+      ok = __all_sync(0xffffffffu, wait_progress_inline(cut(at), turns >> at & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_PRODUCER, progress));
       if (!ok) break;
       turns ^= 1u << at;
       clear_after<kStageBytes / kChunkBytes>(smem + at * kStageBytes, x.rows % kDepth, lane);
@@ -309,7 +315,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
     for (int t = block; t < total; t += grid, ++done) {
       const Tile x = tile_at(t);
       const int buf = static_cast<int>(done % kAcc);
-      if (!__all_sync(0xffffffffu, wait_phase_inline(ready(buf), (done / kAcc) & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_EPILOGUE)))
+      if (!__all_sync(0xffffffffu, wait_progress_inline(ready(buf), (done / kAcc) & 1u, abort_flag, p.status, p.timeout_ns, GG_STATUS_TIMEOUT_EPILOGUE,
+                                                        progress)))
         break;
       ptx::tc_fence_after_sync();
       const uint32_t from = tmem + static_cast<uint32_t>(buf * kBN) + (static_cast<uint32_t>(quarter * 32) << 16);
