@@ -396,18 +396,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
   }
 }
 
-// act'(x) and act(x), in full precision: the pass is bound by memory.
+// act'(x) and act(x), with the forward pass's exponential and division.
 __device__ __forceinline__ void slope_of(float x, int act, float& slope, float& value) {
   if (act == GG_ACT_SILU) {
-    const float s = __fdividef(1.0f, 1.0f + __expf(fminf(-x, 80.0f)));
+    const float s = over_logistic(1.0f, x);
     value = x * s;
     slope = s * fmaf(x, 1.0f - s, 1.0f);
   } else if (act == GG_ACT_GELU) {
-    // 0.5 (1 + tanh(u)) = s with s = 1 / (1 + exp(-2u)), u = c (x + 0.044715 x^3); its derivative is 2 s (1 - s) u'
-    const float c = 1.5957691216057308f;  // 2 sqrt(2 / pi)
-    const float s = __fdividef(1.0f, 1.0f + __expf(fminf(-c * fmaf(0.044715f * x, x * x, x), 80.0f)));
+    // x s(z) with s the logistic function: its derivative is s + x s (1 - s) z'. Far out s is 0 or 1 and the second term 0, while z'
+    // leaves FP32 (past |x| = 5e19).
+    const float s = over_logistic(1.0f, gelu_exponent(x)), bend = x * s * (1.0f - s);
     value = x * s;
-    slope = fmaf(x * s * (1.0f - s), c * fmaf(3.0f * 0.044715f * x, x, 1.0f), s);
+    slope = bend == 0.0f ? s : fmaf(bend, 1.5957691216057308f * fmaf(3.0f * 0.044715f * x, x, 1.0f), s);
   } else if (act == GG_ACT_RELU) {
     value = fmaxf(x, 0.0f);
     slope = x > 0.0f ? 1.0f : 0.0f;
