@@ -426,6 +426,7 @@ struct GateGradientParams {
   const int* rows;
   int64_t ldg, ldgh, ldgg;
   int experts, n, capacity, activation;
+  int* status;
 };
 
 constexpr int kGateThreads = 256;
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(kGateThreads) gate_gradient_kernel(const GateG
   if (threadIdx.x == 0) s_rows = p.rows ? 0 : p.capacity, s_bad = 0;
   chained_begin();
   __syncthreads();
-  if (p.rows) {  // their sum; bad counts are reported by the products that follow
+  if (p.rows) {  // their sum
     long long sum = 0;
     bool bad = false;
     for (int e = threadIdx.x; e < p.experts; e += kGateThreads) {
@@ -450,7 +451,10 @@ __global__ void __launch_bounds__(kGateThreads) gate_gradient_kernel(const GateG
     if (bad) s_bad = 1;
   }
   __syncthreads();
-  if (s_bad || s_rows > p.capacity) return;
+  if (s_bad || s_rows > p.capacity) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(p.status, GG_STATUS_BAD_ROWS);
+    return;
+  }
   const int per_row = (p.n + 7) / 8;
   const int64_t pieces = s_rows * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kGateThreads + threadIdx.x; i < pieces; i += static_cast<int64_t>(gridDim.x) * kGateThreads) {
@@ -704,12 +708,12 @@ int gg_gated_plan_backward(gg_gated_plan* plan, const gg_gated_gradient* gradien
   const int64_t most_w = pw.maps ? static_cast<int64_t>(q.experts) * pw.tiles_m * pw.tiles_n : 0;
   if (most_x > gg::tiles::kMostTiles || most_w > gg::tiles::kMostTiles) return cudaErrorInvalidValue;
 
-  if (c.capacity_rows > 0) {
-    gg::GateGradientParams g{c.gate, c.up, c.grad_h, c.grad_gate, c.grad_up, c.rows, c.ldg, c.ldgh, c.ldgg, q.experts, q.n, c.capacity_rows, q.activation};
+  if (c.capacity_rows > 0 || c.rows) {  // without room for rows: for the counts' check
+    gg::GateGradientParams g{c.gate, c.up, c.grad_h, c.grad_gate, c.grad_up, c.rows, c.ldg, c.ldgh, c.ldgg, q.experts, q.n, c.capacity_rows, q.activation, plan->status};
     const bool vec = gg::on16(c.gate, static_cast<int64_t>(c.ldg) * 2) && gg::on16(c.up, static_cast<int64_t>(c.ldg) * 2) &&
                      gg::on16(c.grad_h, static_cast<int64_t>(c.ldgh) * 2);
     const int64_t want = (static_cast<int64_t>(c.capacity_rows) * ((q.n + 7) / 8) + gg::kGateThreads - 1) / gg::kGateThreads;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(want, static_cast<int64_t>(plan->sms) * 8)));
+    const dim3 grid(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(want, static_cast<int64_t>(plan->sms) * 8))));
     const auto go = [&](auto kernel) { st = gg::launch_chained(kernel, grid, gg::kGateThreads, 0, s, 1, g); };
     if (kind == 2) vec ? go(gg::gate_gradient_kernel<gg::kOutF16, true>) : go(gg::gate_gradient_kernel<gg::kOutF16, false>);
     else vec ? go(gg::gate_gradient_kernel<gg::kOutBF16, true>) : go(gg::gate_gradient_kernel<gg::kOutBF16, false>);

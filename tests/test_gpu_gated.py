@@ -363,3 +363,23 @@ def test_refusals(cuda):
     assert c.plan.backward(**(ok | dict(grad_gate=odd[0], grad_up=odd[1]))) == invalid
     c.plan.close()
     assert c.plan.run(c.x, c.rows, c.h) == capi.CUDA_ERROR_INVALID_DEVICE_POINTER
+
+
+@pytest.mark.parametrize("counts", [[5, -1, 3], [20, 20, 20], [2 ** 31 - 1, 2 ** 31 - 1, 2]])
+@pytest.mark.parametrize("spare", [3, None])
+def test_bad_counts_without_products(cuda, counts, spare):
+    """The gradients of gate and up alone, with room for some rows or (None) for none: bad counts are reported too."""
+    import torch
+    c = Case([10, 10, 9], 64, 64)
+    rows = slice(0, None if spare else 0)
+    c.rows.copy_(torch.tensor(counts, dtype=torch.int32))
+    call = lambda: c.plan.backward(*[t[rows] for t in (c.x, c.gate, c.up, c.grad_h)], c.rows, c.gg[rows], c.gu[rows])  # noqa: E731
+    assert call() == 0
+    torch.cuda.synchronize()
+    assert c.plan.status() == capi.GG_STATUS_BAD_ROWS
+    assert bool((c.gg == 7).all()) and bool((c.gu == 7).all())
+    assert c.plan.status() == 0
+    c.rows.zero_()
+    assert call() == 0
+    torch.cuda.synchronize()
+    assert c.plan.status() == 0
