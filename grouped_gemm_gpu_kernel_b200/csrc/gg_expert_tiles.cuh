@@ -358,8 +358,10 @@ __device__ __forceinline__ void clear_rows(uint8_t* smem) {
   ptx::fence_proxy_async_smem();
 }
 
-// After an abort: waits, bounded, for the loads of one loading warp's stages before the block ends: `stage` is the next it would have
-// filled, and one that it had not filled yet runs out its limit.
+// At the end of a loading warp: waits, bounded, for the loads of its stages, since a block must not end while they may still land in
+// its shared memory. The products wait for them too, unless another warp has given up, before this one's end or after it, so this
+// does not ask whether one has. `stage` is the next that the warp would have filled; one that it had not filled yet is passed at once,
+// and one that never completes runs out its limit.
 template <int kStages, typename FullBar>
 __device__ __forceinline__ void drain_loads(Ring<kStages, 2> stage, FullBar full) {
   for (int j = 0; j < kStages / 2; ++j) {

@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
       }
       skip = kb - p.k_blocks;
     }
-    if (!ok || *abort_flag) drain_loads<kStages>(stage, full);
+    drain_loads<kStages>(stage, full);
   } else if (warp == kScaleWarp) {
     const int last = (p.n - 1) / GG_SCALE_BLOCK;
     uint32_t slot = 0;

@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) gated_kernel(const __grid_con
       }
       skip = kb - x.depth;
     }
-    if ((!ok || *abort_flag) && rank == 0) drain_loads<kStages>(stage, full);
+    if (rank == 0) drain_loads<kStages>(stage, full);
   } else if (kMode == kWeightGradient && warp == kClearWarp) {
     uint32_t it = 0, turns = 0;  // a bit for each stage: the parity of its next cut
     bool ok = true;
