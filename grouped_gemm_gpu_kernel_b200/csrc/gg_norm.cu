@@ -422,12 +422,15 @@ void with_types(int type, int weight_type, Do go) {
   else go(integral_constant<int, kOutBF16>(), integral_constant<int, kOutF32>());
 }
 
-template <typename Do>
+// kTwo: a warp may hold 2 spans (a forward pass of 16 bits goes from 1 to 4).
+template <bool kTwo, typename Do>
 void with_spans(int spans, bool vec, Do go) {
   using std::integral_constant;
   const auto one = [&](auto v) {
+    if constexpr (kTwo) {
+      if (spans == 2) return go(integral_constant<int, 2>(), v);
+    }
     if (spans == 1) go(integral_constant<int, 1>(), v);
-    else if (spans == 2) go(integral_constant<int, 2>(), v);
     else if (spans == 4) go(integral_constant<int, 4>(), v);
     else go(integral_constant<int, 8>(), v);
   };
@@ -477,10 +480,10 @@ int gg_norm_create(const gg_norm_config* config, gg_norm_plan** out) {
         if (st == cudaSuccess) st = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0);
         *blocks = sms * std::max(1, per_sm);
       };
-      gg::with_spans(plan->team.spans, vec != 0, [&](auto n, auto v) {
+      gg::with_spans<f() == gg::kOutF32>(plan->team.spans, vec != 0, [&](auto n, auto v) {
         count(gg::norm_kernel<f(), wt(), n(), v()>, plan->team.threads, &plan->blocks[vec]);
       });
-      gg::with_spans(plan->gradient_team.spans, vec != 0, [&](auto n, auto v) {
+      gg::with_spans<true>(plan->gradient_team.spans, vec != 0, [&](auto n, auto v) {
         count(gg::norm_gradient_kernel<f(), wt(), n(), v()>, plan->gradient_team.threads, &plan->gradient_blocks[vec]);
       });
     }
@@ -519,7 +522,7 @@ int gg_norm_run(const gg_norm_plan* plan, const gg_norm* call, void* stream) {
   const int teams = t.threads / (32 * t.warps);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(plan->blocks[vec], (static_cast<int64_t>(q.rows) + teams - 1) / teams));
   gg::with_types(plan->config.type, plan->config.weight_type, [&](auto f, auto wt) {
-    gg::with_spans(t.spans, vec, [&](auto n, auto v) {
+    gg::with_spans<f() == gg::kOutF32>(t.spans, vec, [&](auto n, auto v) {
       st = gg::launch_chained(gg::norm_kernel<f(), wt(), n(), v()>, dim3(grid), static_cast<unsigned>(t.threads), 0,
                               static_cast<cudaStream_t>(stream), 1, p, t.warps);
     });
@@ -549,7 +552,7 @@ int gg_norm_backward(gg_norm_plan* plan, const gg_norm_gradient* gradient, void*
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(plan->gradient_blocks[vec], (static_cast<int64_t>(q.rows) + teams - 1) / teams));
   if (q.rows > 0)
     gg::with_types(plan->config.type, plan->config.weight_type, [&](auto f, auto wt) {
-      gg::with_spans(t.spans, vec, [&](auto n, auto v) {
+      gg::with_spans<true>(t.spans, vec, [&](auto n, auto v) {
         st = gg::launch_chained(gg::norm_gradient_kernel<f(), wt(), n(), v()>, dim3(grid), static_cast<unsigned>(t.threads), 0, s,
                                 1, p, t.warps);
       });
