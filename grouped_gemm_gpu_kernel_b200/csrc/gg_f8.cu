@@ -319,6 +319,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
 #pragma unroll
       for (int j = 0; j < 4; ++j) sa[j] = p.a_scales + static_cast<int64_t>(x.row + min(j * 32 + lane, x.rows - 1)) * p.ldas;
       // A slot's scales are asked for two slots before they are written: their way from L2 takes longer than a slot lasts.
+      // The rows' by ordinary loads: the kernel before, which wrote them, may have run beside this one's beginning, and __ldg
+      // is for what nothing writes as long as the kernel lasts.
       struct Group {
         float a[4][kScaleBlocks], b;
       };
@@ -328,11 +330,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) f8_kernel(const __grid_consta
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (j * 32 < x.rows && four) {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(sa[j] + kb0));
+            const float4 v = *reinterpret_cast<const float4*>(sa[j] + kb0);
             g.a[j][0] = v.x, g.a[j][1] = v.y, g.a[j][2] = v.z, g.a[j][3] = v.w;
           } else {
 #pragma unroll
-            for (int i = 0; i < kScaleBlocks; ++i) g.a[j][i] = j * 32 < x.rows && kb0 + i < p.k_blocks ? __ldg(sa[j] + kb0 + i) : 0.0f;
+            for (int i = 0; i < kScaleBlocks; ++i) g.a[j][i] = j * 32 < x.rows && kb0 + i < p.k_blocks ? sa[j][kb0 + i] : 0.0f;
           }
         }
       };
