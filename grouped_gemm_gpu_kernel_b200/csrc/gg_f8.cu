@@ -9,12 +9,12 @@
 // sums in their registers, BN / 2 a thread, two at a time (fma.rn.f32x2). Meanwhile the tensor cores work on the next b.
 //
 // What bounds it: few rows an expert, the weights from memory (64 rows on 8 experts of 4096 x 14336: 86 us, 5.5 TB/s of the 6.55 of a
-// copy; gated, of two 14336 x 4096: 180 us, 5.2; one row on one
-// expert: 35 us, 128 tiles of 32 outputs, each with 112 blocks of k one after another). Many rows,
+// copy; gated, of two 14336 x 4096: 182 us, 5.2; one row on one
+// expert: 33 us, 128 tiles of 32 outputs, each with 112 blocks of k one after another). Many rows,
 // the way of each accumulator: 128 x 256 sums leave tensor memory for every 512 cycles' products, and its 512 columns
 // hold two of them, so that the products of the next but one wait for the sums' way out (the tensor pipe is 46 % busy with 4096 rows on 8
-// experts of 4096 x 4096, 92 us). 16384 rows on 64 experts, 14336 x 4096: 1345 us, 1.43 PFLOP/s; 16 experts of 1024 rows each 1044 us, 1.84,
-// where the product alone would be 2.8 (3.3 at full clock). Calls back to back are slowed by the card's power limit: 1610 us.
+// experts of 4096 x 4096, 92 us). 16384 rows on 64 experts, 14336 x 4096: 1345 us, 1.43 PFLOP/s; 16 experts of 1024 rows each 1044 us, 1.84; 4096 rows
+// on 8 experts, gated, into 8 bits: 520 us, 1.85, where the product alone would be 2.8 (3.3 at full clock). Calls back to back are slowed by the card's power limit: 1610 us.
 // Tried and slower: pairs of CTAs (2470 us: the sums' release crosses to the other CTA for every block), sums kept in tensor memory
 // (2280). No difference: other boxes, element types and L2 promotions of the loads, a k of its own to start with for each CTA.
 #include <cuda.h>

@@ -19,8 +19,9 @@
 // What bounds it: few rows, the weights from memory (16 rows on 8 experts of 2 x 14336 x 4096: 299 us, 6.3 TB/s of the 6.55 of a
 // copy). Many rows, the tensor cores and then the card's power limit. 8192 rows on one expert of 4096 x 4096: 1.56 PFLOP/s in all three
 // products. 8192 rows on 8 experts of 14336 x 4096 (1.92 TFLOP a product): forward 1400 us, 1.37 PFLOP/s, the pass before the
-// gradients 210 us, 5.6 TB/s, rows 1530 us, 1.26 PFLOP/s, weights 1900 us, 1.0: the card is at its power limit, and neither without its
-// stores nor without its loads does the last take less. Pairs against single CTAs, at 1024 rows an expert: forward 1430 us and
+// gradients 210 us, 5.6 TB/s, rows 1530 us, 1.26 PFLOP/s, weights 1900 us, 1.0. The card is at its power limit, which does not explain the
+// last: with 2048 rows on 2 experts of 4096 x 4096 its tensor pipe is 66 % busy, the others' 88 and 90, at about one clock (1.54 to 1.59 GHz);
+// neither without its stores nor without its loads does it take less. Pairs against single CTAs, at 1024 rows an expert: forward 1430 us and
 // 1520, rows 1590 and 1660; at 512 the same. Tile rows gone through 2, 4 or 8 at a time in place of 16: no less.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -509,7 +510,7 @@ struct gg_gated_plan {
 
 namespace {
 
-constexpr int kPairRows = 512;     // rows of an expert, in the mean, from which on its tiles are of 256
+constexpr int kPairRows = 512;     // rows of an expert that the capacity has, in the mean, from which on its tiles are of 256
 constexpr int kPairColumns = 256;  // k from which on the weights' gradients' are
 
 gg::GatedParams common(const gg_gated_plan* plan, const int* rows, int capacity) {

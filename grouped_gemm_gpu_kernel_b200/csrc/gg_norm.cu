@@ -14,7 +14,8 @@
 // what is stored, as the gradient finds it.
 //
 // 16384 rows of 4096 in BF16, with the residual: forward 93 us, 5.8 TB/s; gradient with the residual's and the weight's 101 us,
-// 5.3 TB/s, 6 us of it the last sum over the blocks' parts. FP32: 166 us and 174, 6.5 and 6.2 TB/s. 32768 rows into 16 and 8 bits: 230 us, 5.3. A copy has 6.55. Rows that are
+// 5.3 TB/s, 6 us of it the last sum over the blocks' parts. FP32: 166 us and 174, 6.5 and 6.2 TB/s. 32768 rows into 16 and 8 bits: 230 to
+// 240 us, 5.1 to 5.3; 16384 into 8 bits alone, without a residual, 97 us, by the instructions of the 8-bit form. A copy has 6.55. Rows that are
 // not aligned to 16 bytes go value by value: 67041 rows of 1001 in BF16 182 us and 208. Wide rows hold fewer blocks an SM: 2048
 // rows of 32768 in BF16 154 us and 379 (the gradient keeps two rows and the weight's sums, 8 spans of each, and spills).
 // 4 rows of 4096 with 8-bit results: 5 us, a launch and the latency of one row.

@@ -140,7 +140,8 @@ typedef struct gg_problem {
 #define GG_ACT_NONE 0
 #define GG_ACT_RELU 1
 #define GG_ACT_GELU 2
-/* x / (1 + exp(-x)). Only gg_f8_plan_create and gg_gated_plan_create take it. */
+/* x / (1 + exp(-x)). Only gg_f8_plan_create and gg_gated_plan_create take it. There it and GELU, and their slopes, are within 4e-5 of the
+ * value, and of a value below 1e-32 in magnitude within 1e-32. */
 #define GG_ACT_SILU 3
 #define GG_LAYOUT_ROW_MAJOR 0
 #define GG_LAYOUT_COL_MAJOR 1
@@ -634,7 +635,7 @@ typedef struct gg_f8_plan gg_f8_plan;
  * device once, to write its tables. Errors: sizes or types out of range, null pointers, weights or a pitch off a 16-byte
  * boundary -> cudaErrorInvalidValue before any device work; CUDA errors passed through. */
 int gg_f8_plan_create(const gg_f8_problem* problem, gg_f8_plan** out);
-/* capacity_rows: at most 2^31 - 65537. a: capacity_rows x k, pitch lda (a multiple of 16, >= k), 16-byte aligned; a_scales: capacity_rows x ceil(k / 128),
+/* capacity_rows: at most 2^31 - 65537; the tiles' width is chosen for so many rows. a: capacity_rows x k, pitch lda (a multiple of 16, >= k), 16-byte aligned; a_scales: capacity_rows x ceil(k / 128),
  * pitch ldas. rows: `experts` counts in device memory; NULL with experts == 1: all capacity_rows rows.
  * d: capacity_rows x n of the output type, pitch ldd (>= n), any alignment; d_scales (8-bit D): capacity_rows x
  * ceil(n / 128), pitch ldds. Rows past the counts' sum are not written. One launch on `stream`. Counts that are negative or
@@ -668,7 +669,8 @@ typedef struct gg_gated_problem {
 } gg_gated_problem;
 #define GG_GATED_MAX_EXPERTS 1024
 
-/* One forward pass; capacity_rows rows (at most 2^31 - 65537) are allocated. h, gate and up do not overlap one another or x. */
+/* One forward pass; capacity_rows rows (at most 2^31 - 65537) are allocated. From 512 of them an expert on, tiles are of 256 rows: a capacity
+ * that the counts fill is fastest (1024 rows on 8 experts: 312 us in 1024 rows, 448 in 16384). h, gate and up do not overlap one another or x. */
 typedef struct gg_gated {
   const void* x;       /* rows x k, pitch ldx (a multiple of 8) */
   const int* rows;     /* `experts` counts in device memory; NULL with experts == 1: all capacity_rows rows */
